@@ -406,6 +406,143 @@ int int8k_quantize_heads(const void* x, int dtype, int parts, int8_t* q0, float*
                          int8_t* q1, float* s1, int8_t* q2, float* s2, int B, int S, int H,
                          int head_dim, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Operators of a grouped-query serving step (no counterparts in the         */
+/* reference): the INT8 projection, the query and key norms with the position */
+/* rotation, attention over packed prompts, and a KV cache held in 4 bits.    */
+/* ------------------------------------------------------------------------ */
+
+/* INT8 linear layer:
+ *   out[t, n] = T( (f32(acc) * scale_x[t]) * scale_W[n] (+ bias[n]) ),
+ *   acc = sum_k x[t, k] * W[k, n], exact int32; T rounds the fp32 value once to
+ *   `dtype` (int8k_dtype).
+ * x int8 [T, K]; W int8 [K, N], or [N, K] with INT8K_LINEAR_WEIGHT_PREPACKED; out
+ * [T, N]; scale_x [T] or [1], scale_W [N] or [1] (n_scale_* gives the length);
+ * bias fp32 [N] or NULL.  K and N multiples of 16, K below 131072 (the int32 sum
+ * cannot overflow); x and W below 4 GiB (else INT8K_ERR_UNSUPPORTED).  x, W, out and
+ * workspace 16-byte aligned.
+ * int8k_linear_workspace_bytes: what a call of exactly T rows needs (0: none). */
+#define INT8K_LINEAR_WEIGHT_PREPACKED 1
+
+size_t int8k_linear_workspace_bytes(int T, int K, int N, int flags);
+
+int int8k_linear(const int8_t* x, const int8_t* W, void* out, int dtype, const float* scale_x,
+                 int n_scale_x, const float* scale_W, int n_scale_W, const float* bias, int T,
+                 int K, int N, int flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Query and key norms per head and the position rotation, in one pass.
+ * x [B, S, (heads + 2 kv_heads) * head_dim] of `dtype` is a fused QKV projection's
+ * output; in fp32, for each token and each query or key head:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (q_weight / k_weight fp32 [head_dim];
+ *                                             NULL: that part has no norm)
+ *   (a, b) -> (a c - b s, b c + a s) for the pairs (y[i], y[i + rot_dim/2]), i <
+ *     rot_dim/2, or (y[2i], y[2i+1]) with INT8K_ROPE_INTERLEAVED,
+ *     c = cos[pos][i], s = sin[pos][i], pos = positions[b*S + t];
+ * dims from rot_dim on are not rotated, values are neither normed nor rotated.
+ * cos, sin fp32 [max_positions, rot_dim/2]; positions int32 [B*S]; a position
+ * outside [0, max_positions) takes the nearest row and is counted
+ * (int8k_rope_bad_positions, per device since the library was loaded;
+ * synchronises).  Outputs, rounded to `dtype` once: q [B, heads, S, head_dim], k and v
+ * [B, kv_heads, S, head_dim].  The _quantize form emits int8 rows and fp32 scales
+ * [B, heads or kv_heads, S] instead: int8k_quantize_per_token of those rounded rows,
+ * byte for byte.  head_dim a multiple of 16 up to 256, rot_dim even, 2 .. head_dim.
+ * x and the outputs 16-byte aligned (scales 4, codes 8). */
+#define INT8K_ROPE_INTERLEAVED 1
+
+int int8k_qk_norm_rope(const void* x, int dtype, const float* cos, const float* sin,
+                       int max_positions, int rot_dim, const int32_t* positions,
+                       const float* q_weight, const float* k_weight, float eps, void* q, void* k,
+                       void* v, int B, int S, int heads, int kv_heads, int head_dim, int flags,
+                       void* stream);
+
+int int8k_qk_norm_rope_quantize(const void* x, int dtype, const float* cos, const float* sin,
+                                int max_positions, int rot_dim, const int32_t* positions,
+                                const float* q_weight, const float* k_weight, float eps,
+                                int8_t* q, float* scale_q, int8_t* k, float* scale_k, int8_t* v,
+                                float* scale_v, int B, int S, int heads, int kv_heads,
+                                int head_dim, int flags, void* stream);
+
+int int8k_rope_bad_positions(unsigned int* count);
+
+/* INT8 prefill attention over packed sequences with grouped heads:
+ *   Q int8 [heads, total_tokens, D], K, V int8 [kv_heads, total_tokens, D], per-token
+ *   scales fp32 [heads or kv_heads, total_tokens]; heads a multiple of kv_heads, query
+ *   head h reads key head h / (heads / kv_heads)
+ *   cu_seqlens int32 [num_seqs + 1] (device): sequence i is the tokens cu_seqlens[i] ..
+ *   cu_seqlens[i+1]-1; empty sequences are fine.  Bounds outside [0, total_tokens] or
+ *   falling ones are cut to the tensors.
+ *   out fp16 [heads, total_tokens, D], or [total_tokens, heads, D] with
+ *   INT8K_ATTN_OUT_THD (the row order the output projection reads)
+ * Each query attends to the keys of its sequence, with INT8K_ATTN_CAUSAL to those up to
+ * itself; the math is int8k_attention_forward's.  Rows of tokens that no sequence holds
+ * (padding behind the last one) are left as they were, or written as zeros with
+ * INT8K_ATTN_ZERO_REST.  head_dim a multiple of 16 up to 256.  Q, K, V 16-byte, out
+ * 8-byte aligned. */
+#define INT8K_ATTN_OUT_THD 2
+#define INT8K_ATTN_ZERO_REST 4
+
+int int8k_attention_forward_packed(const int8_t* Q, const int8_t* K, const int8_t* V,
+                                   uint16_t* out, const float* scale_Q, const float* scale_K,
+                                   const float* scale_V, const int32_t* cu_seqlens, int num_seqs,
+                                   int total_tokens, int heads, int kv_heads, int head_dim,
+                                   int flags, void* stream);
+
+/* A paged KV cache held in 4 bits.  A row (one token of one key head) is head_dim
+ * codes, two a byte (element 2i in the low half of byte i), stored as code + 8, and
+ * one fp32 scale:
+ *   s = max(|row|, 1e-8) / 7, code = rn(clamp(x / s, -8, 7)), x ~= code * s.
+ *   K_pages / V_pages uint8 [num_pages, kv_heads, page_size, head_dim / 2]
+ *   sK_pages / sV_pages fp32 [num_pages, kv_heads, page_size]
+ * head_dim 64 or 128; page_size a power of two in [16, 1024]; num_pages * page_size
+ * below 2^31.  Pages 16-byte aligned. */
+
+/* Quantizes T tokens into rows slots[t] = page * page_size + offset (int32, device) of
+ * every key head.  k_new / v_new [T, kv_heads, head_dim] of `dtype`, head_dim contiguous,
+ * the other two with strides in elements (multiples of 16 bytes; 16-byte aligned).  A
+ * negative slot skips its token (padding); slots past the cache are skipped and counted
+ * (int8k_kv4_bad_ids).  The slots of one call must be distinct: of two tokens on one slot
+ * either may win, code by code.  A row with a NaN gets a NaN scale. */
+int int8k_kv4_cache_append(const void* k_new, const void* v_new, int dtype,
+                           long long k_token_stride, long long k_head_stride,
+                           long long v_token_stride, long long v_head_stride, uint8_t* K_pages,
+                           uint8_t* V_pages, float* sK_pages, float* sV_pages,
+                           const int32_t* slots, int T, int kv_heads, int head_dim,
+                           int num_pages, int page_size, void* stream);
+
+/* The rows at `slots` of one side of the cache as numbers: out [T, kv_heads, head_dim] of
+ * `dtype`, T(f32(code) * scale).  Slots outside the cache read as zeros.  out 16-byte
+ * aligned. */
+int int8k_kv4_cache_read(const uint8_t* pages, const float* scales, const int32_t* slots,
+                         void* out, int dtype, int T, int kv_heads, int head_dim, int num_pages,
+                         int page_size, void* stream);
+
+/* Decode attention over that cache with grouped heads:
+ *   Q int8 [B, heads, D], scale_Q fp32 [B*heads]; heads a multiple of kv_heads
+ *   block_tables int32 [B, max_pages_per_seq], context_lens int32 [B]: as
+ *   int8k_decode_attention_forward_paged's (a length of 0 gives a zero row; longer ones
+ *   than max_context are cut to it)
+ *   out fp16 [B, heads, D]
+ *   out = sum_j softmax_j(q . k_j sQ sK_j / sqrt(D)) v_j sV_j, q . k exact int32.
+ * A page id outside [0, num_pages) reads page num_pages-1 and is counted
+ * (int8k_kv4_bad_ids).  Entries past a sequence's length are never read.  The workspace
+ * holds partial states; the query for the longest max_context serves shorter ones of the
+ * same B and heads. */
+size_t int8k_decode_attention_kv4_paged_workspace_bytes(int B, int heads, int kv_heads,
+                                                        int max_context, int head_dim);
+
+int int8k_decode_attention_forward_kv4_paged(
+    const int8_t* Q, const uint8_t* K_pages, const uint8_t* V_pages, uint16_t* out,
+    const float* scale_Q, const float* sK_pages, const float* sV_pages,
+    const int32_t* block_tables, const int32_t* context_lens, int B, int heads, int kv_heads,
+    int head_dim, int num_pages, int page_size, int max_pages_per_seq, int max_context,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Diagnostics of the 4-bit cache: *count receives, for the current device since the
+ * library was loaded, the tokens appended to slots past the cache plus the work units of
+ * decodes that met a page id outside [0, num_pages) among the entries their positions
+ * use.  Synchronises with the device. */
+int int8k_kv4_bad_ids(unsigned int* count);
+
 #ifdef __cplusplus
 }
 #endif

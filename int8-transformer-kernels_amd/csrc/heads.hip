@@ -1,0 +1,351 @@
+// heads.hip — norms of queries and keys per head and the position rotation in one pass, gfx950.
+//
+// x [B, S, (heads + 2 kv_heads) * D] is a fused QKV projection's output.  For each token and
+// each query or key head, with fp32 arithmetic throughout:
+//   y_d = x_d / sqrt(mean_d x_d^2 + eps) * w_d              (where the part has weights)
+//   (a, b) -> (a cos - b sin, b cos + a sin)                for the rot_dim / 2 pairs (a, b),
+//   (y_t, y_{t + rot_dim/2}), or (y_2t, y_2t+1) interleaved, by cos[pos][t], sin[pos][t];
+// dims from rot_dim on and the value heads pass through.  The result is rounded to x's dtype
+// once and stored as heads [B, H, S, D], or quantized per row as int8k_quantize_per_token
+// quantizes those rounded rows.
+//
+// Memory-bound: x is read once and the heads are written once.  A lane holds both elements of
+// its 8 pairs, 16 elements of a row (D / 16 lanes per row), so the rotation needs no exchange
+// between lanes, and a wave holds 64 / (D / 16) consecutive tokens and walks a range of
+// heads: the angles of a token, twice the bytes of one of its rows, are read once for all of
+// them and the rows that a wave writes for a head are consecutive in memory.
+#include <algorithm>
+#include <cmath>
+
+#include "rows.h"
+
+namespace int8k {
+namespace {
+
+__device__ unsigned int g_rope_bad_positions;
+
+struct HeadsArgs {
+    const void* x;
+    const float *cos, *sin;
+    const int32_t* pos;
+    const float* w[2];  // norm weights of queries and keys, or null
+    float eps;
+    void* y[3];       // [B, H_p, S, D] in x's dtype, or
+    int8_t* q[3];     // the codes and
+    float* s[3];      // their row scales
+    long long tokens;
+    int S, heads, kv_heads, D, max_pos, half;  // half = rot_dim / 2
+    int lg;           // 1 << lg lanes per row
+    int heads_per_wave;
+};
+
+// How the 8 pairs of lane item c lie in a row.
+enum PairLayout {
+    kSplit = 0,        // a, b = 8 elements at 8 c and half + 8 c (half a multiple of 8)
+    kInterleaved = 1,  // the 16 elements from 16 c
+    kSplitAny = 2      // as kSplit for any half: element by element
+};
+
+// Element indices of pair t of a row: the rotated pairs first, then neighbours.
+__device__ __forceinline__ void pair_at(int t, int half, int& a, int& b) {
+    a = t < half ? t : 2 * t;  // 2 half + 2 (t - half)
+    b = t < half ? t + half : 2 * t + 1;
+}
+
+template <int DT>
+__device__ __forceinline__ float load_one(const void* x, size_t i) {
+    if constexpr (DT == INT8K_DTYPE_F32) return static_cast<const float*>(x)[i];
+    const uint16_t u = static_cast<const uint16_t*>(x)[i];
+    if constexpr (DT == INT8K_DTYPE_F16) return __half2float(__ushort_as_half(u));
+    return __uint_as_float((uint32_t)u << 16);
+}
+
+// v as a number of the dtype (round to nearest even).
+template <int DT>
+__device__ __forceinline__ float round_to(float v) {
+    if constexpr (DT == INT8K_DTYPE_F16) return __half2float(f16_of_f32(v));
+    if constexpr (DT == INT8K_DTYPE_BF16) {
+        const uint32_t u = __float_as_uint(v);
+        const uint32_t r = u + 0x7fffu + ((u >> 16) & 1u);
+        return __uint_as_float((v != v ? u | 0x400000u : r) & 0xffff0000u);
+    }
+    return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void store_one(void* y, size_t i, float v) {
+    if constexpr (DT == INT8K_DTYPE_F32) static_cast<float*>(y)[i] = v;
+    else if constexpr (DT == INT8K_DTYPE_F16)
+        static_cast<uint16_t*>(y)[i] = f32_to_f16_bits(v);
+    else static_cast<uint16_t*>(y)[i] = (uint16_t)(__float_as_uint(v) >> 16);
+}
+
+// 8 consecutive elements.
+template <int DT>
+__device__ __forceinline__ void load8(const void* x, size_t i, float (&v)[8]) {
+    if constexpr (DT == INT8K_DTYPE_F32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
+        const float4 a = p[0], b = p[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        unpack_chunk<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i), v);
+    }
+}
+// 8 values that are numbers of the dtype.
+template <int DT>
+__device__ __forceinline__ void store8(void* y, size_t i, const float (&v)[8]) {
+    if constexpr (DT == INT8K_DTYPE_F32) {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(y) + i);
+        p[0] = make_float4(v[0], v[1], v[2], v[3]);
+        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == INT8K_DTYPE_F16)
+                w[k] = f32_to_f16_bits(v[2 * k]) | ((uint32_t)f32_to_f16_bits(v[2 * k + 1]) << 16);
+            else
+                w[k] = (__float_as_uint(v[2 * k]) >> 16) | (__float_as_uint(v[2 * k + 1]) & 0xffff0000u);
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int DT, bool QUANT, int LAYOUT>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadsArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & ((1 << p.lg) - 1);
+    const bool has = 16 * c < p.D;
+    const int per_wave = 64 >> p.lg;
+    const long long t_raw = ((long long)blockIdx.x * 4 + wave) * per_wave + (lane >> p.lg);
+    const bool ok = t_raw < p.tokens && has;
+    const long long t = min(t_raw, p.tokens - 1);
+    const int cc = has ? c : 0;  // idle lanes of a row read its first item and store nothing
+
+    const int raw_pos = p.pos[t];
+    const int pos = min(max(raw_pos, 0), p.max_pos - 1);
+    if (blockIdx.y == 0) {
+        const uint64_t bad = __ballot(raw_pos != pos && c == 0 && t_raw < p.tokens);
+        if (bad != 0 && lane == 0) atomicAdd(&g_rope_bad_positions, (unsigned)__popcll(bad));
+    }
+    const float* cs = p.cos + (size_t)pos * p.half;
+    const float* sn = p.sin + (size_t)pos * p.half;
+    float co[8], si[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int k = 8 * cc + i;
+        const bool turns = k < p.half;
+        co[i] = turns ? cs[k] : 1.f;
+        si[i] = turns ? sn[k] : 0.f;
+    }
+    // where this item's chunks lie in a row (kSplit, kInterleaved)
+    int ia = 16 * cc, ib = 16 * cc + 8;
+    if (LAYOUT == kSplit && 8 * cc < p.half) ia = 8 * cc, ib = p.half + 8 * cc;
+
+    const int total = p.heads + 2 * p.kv_heads;
+    const size_t width = (size_t)total * p.D;
+    const int h0 = blockIdx.y * p.heads_per_wave, h1 = min(h0 + p.heads_per_wave, total);
+    const long long b = t / p.S;
+    const long long s = t - b * p.S;
+    for (int hh = h0; hh < h1; ++hh) {
+        const int part = hh < p.heads ? 0 : hh < p.heads + p.kv_heads ? 1 : 2;
+        const int ph = part == 0 ? p.heads : p.kv_heads;
+        const int h = hh - (part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads);
+        const size_t in = (size_t)t * width + (size_t)hh * p.D;
+        const size_t row = ((size_t)b * ph + h) * p.S + s;
+        float a[8], v[8];
+        if constexpr (LAYOUT == kSplitAny) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                int ka, kb;
+                pair_at(8 * cc + i, p.half, ka, kb);
+                a[i] = load_one<DT>(p.x, in + ka);
+                v[i] = load_one<DT>(p.x, in + kb);
+            }
+        } else {
+            float lo[8], hi[8];
+            load8<DT>(p.x, in + ia, lo);
+            load8<DT>(p.x, in + ib, hi);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (LAYOUT == kSplit) a[i] = lo[i], v[i] = hi[i];
+                else {
+                    a[i] = i < 4 ? lo[2 * (i & 3)] : hi[2 * (i & 3)];
+                    v[i] = i < 4 ? lo[2 * (i & 3) + 1] : hi[2 * (i & 3) + 1];
+                }
+            }
+        }
+        if (part < 2) {
+            const float* w = p.w[part];
+            if (w != nullptr) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(v[i], v[i], ss));
+                ss = row_reduce(has ? ss : 0.f, p.lg, [](float m, float n) { return m + n; });
+                const float inv = 1.f / sqrtf(ss / (float)p.D + p.eps);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    int ka, kb;
+                    if constexpr (LAYOUT == kSplitAny) pair_at(8 * cc + i, p.half, ka, kb);
+                    else if constexpr (LAYOUT == kSplit) ka = ia + i, kb = ib + i;
+                    else ka = 16 * cc + 2 * i, kb = ka + 1;
+                    a[i] = a[i] * inv * w[ka];
+                    v[i] = v[i] * inv * w[kb];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (8 * cc + i < p.half) {
+                    const float ra = a[i] * co[i] - v[i] * si[i];
+                    const float rb = v[i] * co[i] + a[i] * si[i];
+                    a[i] = ra, v[i] = rb;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = round_to<DT>(a[i]), v[i] = round_to<DT>(v[i]);
+        }
+        // back to memory order
+        float lo[8], hi[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (LAYOUT == kInterleaved) {
+                lo[i] = (i & 1) ? v[i / 2] : a[i / 2];
+                hi[i] = (i & 1) ? v[4 + i / 2] : a[4 + i / 2];
+            } else {
+                lo[i] = a[i], hi[i] = v[i];
+            }
+        }
+        const size_t out = row * p.D;
+        if constexpr (QUANT) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(v[i])));
+            m = row_reduce(has ? m : 0.f, p.lg, [](float x, float y) { return fmaxf(x, y); });
+            const float sc = fmaxf(m, 1e-8f) / 127.f;
+            const float rinv = 1.f / sc;
+            if (ok) {
+                if constexpr (LAYOUT == kSplitAny) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        int ka, kb;
+                        pair_at(8 * cc + i, p.half, ka, kb);
+                        p.q[part][out + ka] = (int8_t)quant_code(a[i], sc);
+                        p.q[part][out + kb] = (int8_t)quant_code(v[i], sc);
+                    }
+                } else {
+                    store_codes<8>(lo, sc, rinv, p.q[part] + out + ia);
+                    store_codes<8>(hi, sc, rinv, p.q[part] + out + ib);
+                }
+                if (c == 0) p.s[part][row] = sc;
+            }
+        } else if (ok) {
+            if constexpr (LAYOUT == kSplitAny) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    int ka, kb;
+                    pair_at(8 * cc + i, p.half, ka, kb);
+                    store_one<DT>(p.y[part], out + ka, a[i]);
+                    store_one<DT>(p.y[part], out + kb, v[i]);
+                }
+            } else {
+                store8<DT>(p.y[part], out + ia, lo);
+                store8<DT>(p.y[part], out + ib, hi);
+            }
+        }
+    }
+}
+
+template <bool QUANT>
+int launch_heads(HeadsArgs p, int dtype, bool interleaved, hipStream_t stream) {
+    const int items = p.D / 16;
+    while ((1 << p.lg) < items) ++p.lg;
+    const int total = p.heads + 2 * p.kv_heads;
+    const long long blocks = ceil_div(p.tokens, 4LL * (64 >> p.lg));
+    // one head per wave until the grid holds 8 waves per SIMD, then more
+    p.heads_per_wave = (int)std::max<long long>(1, std::min<long long>(total, blocks * total / 2048));
+    const long long gy = ceil_div(total, p.heads_per_wave);
+    if (blocks >= (1LL << 24) || gy > 65535) return INT8K_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)blocks, (unsigned)gy);
+    const int layout = interleaved ? kInterleaved : p.half % 8 == 0 ? kSplit : kSplitAny;
+    with_dtype(dtype, [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (layout == kSplit) qk_norm_rope_kernel<DT, QUANT, kSplit><<<grid, 256, 0, stream>>>(p);
+        else if (layout == kInterleaved)
+            qk_norm_rope_kernel<DT, QUANT, kInterleaved><<<grid, 256, 0, stream>>>(p);
+        else qk_norm_rope_kernel<DT, QUANT, kSplitAny><<<grid, 256, 0, stream>>>(p);
+    });
+    return check_launch("qk_norm_rope_kernel");
+}
+
+template <bool QUANT>
+int heads_entry(const void* x, int dtype, const float* cos, const float* sin, int max_positions,
+                int rot_dim, const int32_t* positions, const float* q_weight,
+                const float* k_weight, float eps, void* const (&y)[3], int8_t* const (&q)[3],
+                float* const (&s)[3], int B, int S, int heads, int kv_heads, int head_dim,
+                int flags, void* stream) {
+    clear_last_error();
+    if (!x || !cos || !sin || !positions) return INT8K_ERR_INVALID_ARGUMENT;
+    for (int i = 0; i < 3; ++i)
+        if (QUANT ? !q[i] || !s[i] : !y[i]) return INT8K_ERR_INVALID_ARGUMENT;
+    if (flags & ~INT8K_ROPE_INTERLEAVED) return INT8K_ERR_INVALID_ARGUMENT;
+    if (dtype < INT8K_DTYPE_F16 || dtype > INT8K_DTYPE_F32) return INT8K_ERR_INVALID_ARGUMENT;
+    if (B <= 0 || S <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_positions <= 0 ||
+        rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim || heads > 65535 || kv_heads > 65535)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (head_dim % 16 || head_dim > 256) return INT8K_ERR_UNSUPPORTED;
+    if (!aligned_to(x, 16) || !aligned_to(cos, 4) || !aligned_to(sin, 4) ||
+        !aligned_to(positions, 4) || !aligned_to(q_weight, 4) || !aligned_to(k_weight, 4))
+        return INT8K_ERR_MISALIGNED;
+    for (int i = 0; i < 3; ++i)
+        if (QUANT ? !aligned_to(q[i], 8) || !aligned_to(s[i], 4) : !aligned_to(y[i], 16))
+            return INT8K_ERR_MISALIGNED;
+    HeadsArgs p{};
+    p.x = x, p.cos = cos, p.sin = sin, p.pos = positions;
+    p.w[0] = q_weight, p.w[1] = k_weight, p.eps = eps;
+    for (int i = 0; i < 3; ++i) p.y[i] = y[i], p.q[i] = q[i], p.s[i] = s[i];
+    p.tokens = (long long)B * S;
+    p.S = S, p.heads = heads, p.kv_heads = kv_heads, p.D = head_dim;
+    p.max_pos = max_positions, p.half = rot_dim / 2;
+    return launch_heads<QUANT>(p, dtype, (flags & INT8K_ROPE_INTERLEAVED) != 0, as_stream(stream));
+}
+
+}  // namespace
+}  // namespace int8k
+
+using namespace int8k;
+
+extern "C" int int8k_qk_norm_rope(const void* x, int dtype, const float* cos, const float* sin,
+                                  int max_positions, int rot_dim, const int32_t* positions,
+                                  const float* q_weight, const float* k_weight, float eps,
+                                  void* q, void* k, void* v, int B, int S, int heads,
+                                  int kv_heads, int head_dim, int flags, void* stream) {
+    return heads_entry<false>(x, dtype, cos, sin, max_positions, rot_dim, positions, q_weight,
+                              k_weight, eps, {q, k, v}, {nullptr, nullptr, nullptr},
+                              {nullptr, nullptr, nullptr}, B, S, heads, kv_heads, head_dim, flags,
+                              stream);
+}
+
+extern "C" int int8k_qk_norm_rope_quantize(
+    const void* x, int dtype, const float* cos, const float* sin, int max_positions, int rot_dim,
+    const int32_t* positions, const float* q_weight, const float* k_weight, float eps, int8_t* q,
+    float* scale_q, int8_t* k, float* scale_k, int8_t* v, float* scale_v, int B, int S, int heads,
+    int kv_heads, int head_dim, int flags, void* stream) {
+    return heads_entry<true>(x, dtype, cos, sin, max_positions, rot_dim, positions, q_weight,
+                             k_weight, eps, {nullptr, nullptr, nullptr}, {q, k, v},
+                             {scale_q, scale_k, scale_v}, B, S, heads, kv_heads, head_dim, flags,
+                             stream);
+}
+
+extern "C" int int8k_rope_bad_positions(unsigned int* count) {
+    clear_last_error();
+    if (!count) return INT8K_ERR_INVALID_ARGUMENT;
+    const hipError_t e = hipMemcpyFromSymbol(count, HIP_SYMBOL(g_rope_bad_positions),
+                                             sizeof(unsigned int), 0, hipMemcpyDeviceToHost);
+    if (e != hipSuccess) {
+        set_last_error("hipMemcpyFromSymbol(g_rope_bad_positions)", e);
+        return INT8K_ERR_HIP;
+    }
+    return INT8K_OK;
+}

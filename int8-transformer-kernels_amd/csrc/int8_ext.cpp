@@ -769,6 +769,355 @@ std::tuple<torch::Tensor, torch::Tensor> int8_decode_attention_forward_paged_qua
     return {r[0], r[1]};
 }
 
+// ── grouped-query serving (new ops; no reference counterparts) ─────────────
+
+namespace {
+
+// A contiguous tensor whose data the kernels can read 16 bytes at a time.
+torch::Tensor dense16(const torch::Tensor& t) {
+    auto c = t.contiguous();
+    return aligned16(c) ? c : c.clone();
+}
+
+void check_on(const torch::Tensor& t, const torch::Tensor& with, const char* name) {
+    TORCH_CHECK(t.device() == with.device(), name, " must be on the device of the other inputs");
+}
+
+void check_float32(const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.dtype() == torch::kFloat32, name, " must be float32");
+}
+
+void check_int32(const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.dtype() == torch::kInt32, name, " must be int32");
+}
+
+// Arguments of the C ABI are ints.
+int as_int(int64_t v, const char* name) {
+    TORCH_CHECK(v >= 0 && v <= INT32_MAX, name, " out of range");
+    return (int)v;
+}
+
+}  // namespace
+
+// y = x . W with a scale per token and per output channel (and an optional bias): x int8
+// (..., K); W int8 (K, N), or (N, K) with prepacked; scale_x and scale_W fp32 with one
+// element per row of x / channel, or one.  Returns (..., N) of dtype (default fp16).
+torch::Tensor int8_linear_torch(torch::Tensor x, torch::Tensor W, torch::Tensor scale_x,
+                                torch::Tensor scale_W, c10::optional<torch::Tensor> bias,
+                                bool prepacked, c10::optional<at::ScalarType> dtype) {
+    TORCH_CHECK(x.device().is_cuda(), "x must be a CUDA tensor");
+    TORCH_CHECK(x.dtype() == torch::kInt8 && W.dtype() == torch::kInt8, "x, W must be int8");
+    TORCH_CHECK(x.dim() >= 1 && x.numel() > 0, "x must be a non-empty tensor");
+    TORCH_CHECK(W.dim() == 2 && W.numel() > 0,
+                prepacked ? "W must be 2-D (N, K)" : "W must be 2-D (K, N)");
+    check_on(W, x, "W");
+    const int64_t K = x.size(-1), T = x.numel() / K, N = prepacked ? W.size(0) : W.size(1);
+    TORCH_CHECK((prepacked ? W.size(1) : W.size(0)) == K, "W shape mismatch (K rows expected)");
+    TORCH_CHECK(K % 16 == 0 && N % 16 == 0, "int8_linear needs K and N to be multiples of 16");
+    check_scale(scale_x, T, "scale_x", x.device());
+    check_scale(scale_W, N, "scale_W", x.device());
+    torch::Tensor b;
+    if (bias.has_value() && bias->defined()) {
+        check_float32(*bias, "bias");
+        check_on(*bias, x, "bias");
+        TORCH_CHECK(bias->numel() == N, "bias must have N elements");
+        b = bias->contiguous();
+    }
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    auto xc = dense16(x), wc = dense16(W);
+    auto sx = scale_x.contiguous(), sw = scale_W.contiguous();
+    auto shape = x.sizes().vec();
+    shape.back() = N;
+    auto y = torch::empty(shape, torch::TensorOptions()
+                                     .dtype(dtype.has_value() ? *dtype : torch::kFloat16)
+                                     .device(x.device()));
+    const int code = dtype_code(y), flags = prepacked ? INT8K_LINEAR_WEIGHT_PREPACKED : 0;
+    const int t = as_int(T, "rows of x"), k = as_int(K, "K"), n = as_int(N, "N");
+    const size_t ws_bytes = int8k_linear_workspace_bytes(t, k, n, flags);
+    auto ws = workspace(ws_bytes, x.device());
+    check_status(int8k_linear(xc.data_ptr<int8_t>(), wc.data_ptr<int8_t>(), y.data_ptr(), code,
+                              sx.data_ptr<float>(), (int)sx.numel(), sw.data_ptr<float>(),
+                              (int)sw.numel(), b.defined() ? b.data_ptr<float>() : nullptr, t, k,
+                              n, flags, ws.data(), ws_bytes, current_stream(x)),
+                 "int8_linear");
+    return y;
+}
+
+// x (B, S, (heads + 2 kv_heads) * D) or (T, ...) -> heads (B, H, S, D) or (H, T, D) of q, k, v:
+// norms of queries and keys where weights are given, rotation by cos/sin (P, rot_dim / 2) at
+// `positions` int32 (one per token); in x's dtype, or as per-token int8 with fp32 scales.
+static std::vector<torch::Tensor> qk_norm_rope_impl(
+    torch::Tensor x, int64_t heads, int64_t kv_heads, torch::Tensor cos, torch::Tensor sin,
+    torch::Tensor positions, c10::optional<torch::Tensor> q_weight,
+    c10::optional<torch::Tensor> k_weight, double eps, bool interleaved, bool quant) {
+    TORCH_CHECK(x.device().is_cuda(), "x must be a CUDA tensor");
+    TORCH_CHECK((x.dim() == 2 || x.dim() == 3) && x.numel() > 0,
+                "x must be a non-empty (batch, seq, width) or (tokens, width) tensor");
+    TORCH_CHECK(heads >= 1 && kv_heads >= 1 && heads <= 65535 && kv_heads <= 65535,
+                "heads and kv_heads must be positive");
+    const int64_t parts = heads + 2 * kv_heads;
+    TORCH_CHECK(x.size(-1) % parts == 0, "last dim must be (heads + 2 * kv_heads) * head_dim");
+    const int64_t D = x.size(-1) / parts;
+    const int64_t B = x.dim() == 3 ? x.size(0) : 1, S = x.size(-2);
+    TORCH_CHECK(D % 16 == 0 && D <= 256, "head_dim must be a multiple of 16 up to 256");
+    check_float32(cos, "cos");
+    check_float32(sin, "sin");
+    check_int32(positions, "positions");
+    TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(0) >= 1,
+                "cos and sin must be (positions, rot_dim / 2) of one shape");
+    TORCH_CHECK(cos.size(1) >= 1 && 2 * cos.size(1) <= D, "rot_dim must be in [2, head_dim]");
+    TORCH_CHECK(positions.numel() == B * S, "positions must have one element per token");
+    for (const auto* t : {&cos, &sin, &positions}) check_on(*t, x, "cos, sin and positions");
+    torch::Tensor w[2];
+    const c10::optional<torch::Tensor>* given[2] = {&q_weight, &k_weight};
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    for (int i = 0; i < 2; ++i) {
+        if (!given[i]->has_value() || !(*given[i])->defined()) continue;
+        TORCH_CHECK((*given[i])->numel() == D, "norm weights must have head_dim elements");
+        w[i] = (*given[i])->to(x.device(), torch::kFloat32).contiguous();
+    }
+    const int code = dtype_code(x);
+    auto xc = dense16(x);
+    auto cc = cos.contiguous(), sc = sin.contiguous(), pc = positions.contiguous();
+    std::vector<torch::Tensor> outs;
+    for (const int64_t n : {heads, kv_heads, kv_heads}) {
+        std::vector<int64_t> rows = {B, n, S};
+        if (x.dim() == 2) rows.erase(rows.begin());
+        auto shape = rows;
+        shape.push_back(D);
+        outs.push_back(torch::empty(shape, torch::TensorOptions()
+                                               .dtype(quant ? torch::kInt8 : x.scalar_type())
+                                               .device(x.device())));
+        if (quant)
+            outs.push_back(torch::empty(
+                rows, torch::TensorOptions().dtype(torch::kFloat32).device(x.device())));
+    }
+    const int flags = interleaved ? INT8K_ROPE_INTERLEAVED : 0;
+    const int rot = 2 * (int)cos.size(1), top = as_int(cos.size(0), "rows of cos");
+    const float *wq = w[0].defined() ? w[0].data_ptr<float>() : nullptr,
+                *wk = w[1].defined() ? w[1].data_ptr<float>() : nullptr;
+    const int b = as_int(B, "batch"), s = as_int(S, "seq");
+    if (quant) {
+        auto q = [&](int i) { return outs[2 * i].data_ptr<int8_t>(); };
+        auto sp = [&](int i) { return outs[2 * i + 1].data_ptr<float>(); };
+        check_status(int8k_qk_norm_rope_quantize(
+                         xc.data_ptr(), code, cc.data_ptr<float>(), sc.data_ptr<float>(), top, rot,
+                         pc.data_ptr<int32_t>(), wq, wk, (float)eps, q(0), sp(0), q(1), sp(1),
+                         q(2), sp(2), b, s, (int)heads, (int)kv_heads, (int)D, flags,
+                         current_stream(x)),
+                     "qk_norm_rope_quantize");
+    } else {
+        check_status(int8k_qk_norm_rope(xc.data_ptr(), code, cc.data_ptr<float>(),
+                                        sc.data_ptr<float>(), top, rot, pc.data_ptr<int32_t>(),
+                                        wq, wk, (float)eps, outs[0].data_ptr(),
+                                        outs[1].data_ptr(), outs[2].data_ptr(), b, s, (int)heads,
+                                        (int)kv_heads, (int)D, flags, current_stream(x)),
+                     "qk_norm_rope");
+    }
+    return outs;
+}
+
+std::vector<torch::Tensor> qk_norm_rope_torch(
+    torch::Tensor x, int64_t heads, int64_t kv_heads, torch::Tensor cos, torch::Tensor sin,
+    torch::Tensor positions, c10::optional<torch::Tensor> q_weight,
+    c10::optional<torch::Tensor> k_weight, double eps, bool interleaved) {
+    return qk_norm_rope_impl(x, heads, kv_heads, cos, sin, positions, q_weight, k_weight, eps,
+                             interleaved, false);
+}
+
+std::vector<torch::Tensor> qk_norm_rope_quantize_torch(
+    torch::Tensor x, int64_t heads, int64_t kv_heads, torch::Tensor cos, torch::Tensor sin,
+    torch::Tensor positions, c10::optional<torch::Tensor> q_weight,
+    c10::optional<torch::Tensor> k_weight, double eps, bool interleaved) {
+    return qk_norm_rope_impl(x, heads, kv_heads, cos, sin, positions, q_weight, k_weight, eps,
+                             interleaved, true);
+}
+
+// Attention over packed sequences: Q int8 (H, T, D), K, V int8 (Hkv, T, D), scales fp32 with
+// H*T / Hkv*T elements, cu_seqlens int32 (n + 1,).  Returns fp16 (H, T, D), or (T, H, D) with
+// out_thd; rows of no sequence are zeros.
+torch::Tensor int8_attention_forward_packed_torch(torch::Tensor Q, torch::Tensor K,
+                                                  torch::Tensor V, torch::Tensor scale_Q,
+                                                  torch::Tensor scale_K, torch::Tensor scale_V,
+                                                  torch::Tensor cu_seqlens, bool is_causal,
+                                                  bool out_thd) {
+    TORCH_CHECK(Q.device().is_cuda(), "Q must be a CUDA tensor");
+    TORCH_CHECK(Q.dtype() == torch::kInt8 && K.dtype() == torch::kInt8 &&
+                    V.dtype() == torch::kInt8,
+                "Q/K/V must be int8");
+    TORCH_CHECK(Q.dim() == 3 && K.dim() == 3 && K.sizes() == V.sizes(),
+                "expected Q (heads, tokens, head_dim), K and V (kv_heads, tokens, head_dim)");
+    const int64_t H = Q.size(0), T = Q.size(1), D = Q.size(2), Hkv = K.size(0);
+    TORCH_CHECK(Q.numel() > 0 && K.numel() > 0, "Q/K/V must not be empty");
+    TORCH_CHECK(K.size(1) == T && K.size(2) == D, "Q/K token or head_dim mismatch");
+    TORCH_CHECK(H % Hkv == 0, "heads must be a multiple of kv_heads");
+    TORCH_CHECK(D % 16 == 0 && D <= 256,
+                "packed attention supports head_dim a multiple of 16 up to 256");
+    check_float32(scale_Q, "scale_Q");
+    check_float32(scale_K, "scale_K");
+    check_float32(scale_V, "scale_V");
+    check_int32(cu_seqlens, "cu_seqlens");
+    TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.numel() >= 2,
+                "cu_seqlens must be (num_seqs + 1,)");
+    for (const auto* t : {&K, &V, &scale_Q, &scale_K, &scale_V, &cu_seqlens})
+        check_on(*t, Q, "every input");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(Q.device());
+    auto sQ = flat_scale(scale_Q, H * T, "scale_Q");
+    auto sK = flat_scale(scale_K, Hkv * T, "scale_K");
+    auto sV = flat_scale(scale_V, Hkv * T, "scale_V");
+    auto q = dense16(Q), k = dense16(K), v = dense16(V);
+    auto cu = cu_seqlens.contiguous();
+    auto out = torch::empty(out_thd ? std::vector<int64_t>{T, H, D} : std::vector<int64_t>{H, T, D},
+                            torch::TensorOptions().dtype(torch::kFloat16).device(Q.device()));
+    const int flags = INT8K_ATTN_ZERO_REST | (is_causal ? INT8K_ATTN_CAUSAL : 0) |
+                      (out_thd ? INT8K_ATTN_OUT_THD : 0);
+    check_status(int8k_attention_forward_packed(
+                     q.data_ptr<int8_t>(), k.data_ptr<int8_t>(), v.data_ptr<int8_t>(),
+                     reinterpret_cast<uint16_t*>(out.data_ptr<at::Half>()), sQ.data_ptr<float>(),
+                     sK.data_ptr<float>(), sV.data_ptr<float>(), cu.data_ptr<int32_t>(),
+                     as_int(cu.numel() - 1, "num_seqs"), as_int(T, "tokens"), as_int(H, "heads"),
+                     as_int(Hkv, "kv_heads"), (int)D, flags, current_stream(Q)),
+                 "int8_attention_forward_packed");
+    return out;
+}
+
+namespace {
+
+struct Kv4Dims {
+    int num_pages, kv_heads, page, head_dim;
+};
+
+// One side of a 4-bit cache: pages uint8 (num_pages, kv_heads, page, head_dim / 2), scales fp32
+// (num_pages, kv_heads, page).
+Kv4Dims check_kv4(const torch::Tensor& pages, const torch::Tensor& scales, const char* name) {
+    TORCH_CHECK(pages.device().is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(pages.dtype() == torch::kUInt8, name, " must be uint8");
+    TORCH_CHECK(pages.dim() == 4 && pages.numel() > 0, name,
+                " must be (num_pages, kv_heads, page, head_dim / 2)");
+    TORCH_CHECK(pages.is_contiguous() && scales.is_contiguous(), name,
+                " and its scales must be contiguous");
+    TORCH_CHECK(aligned16(pages), name, " must be 16-byte aligned");
+    check_float32(scales, "cache scales");
+    check_on(scales, pages, "cache scales");
+    TORCH_CHECK(scales.numel() == pages.size(0) * pages.size(1) * pages.size(2),
+                "cache scales must have num_pages * kv_heads * page elements");
+    const int64_t D = 2 * pages.size(3), P = pages.size(2);
+    TORCH_CHECK(D == 64 || D == 128, "the 4-bit cache supports head_dim 64 or 128");
+    TORCH_CHECK(P >= 16 && P <= 1024 && (P & (P - 1)) == 0,
+                "page must be a power of two in [16, 1024]");
+    return {as_int(pages.size(0), "num_pages"), as_int(pages.size(1), "kv_heads"), (int)P, (int)D};
+}
+
+void check_slots(const torch::Tensor& slots, const torch::Tensor& pages) {
+    check_int32(slots, "slots");
+    check_on(slots, pages, "slots");
+    TORCH_CHECK(slots.dim() == 1 && slots.numel() > 0, "slots must be a non-empty (tokens,)");
+}
+
+// new tokens (T, kv_heads, D) whose rows the kernel can read where they are
+torch::Tensor token_rows(const torch::Tensor& t) {
+    const int64_t w = 16 / t.element_size();
+    const bool fits = aligned16(t) && t.stride(2) == 1 && t.stride(0) % w == 0 && t.stride(1) % w == 0;
+    return fits ? t : dense16(t);
+}
+
+}  // namespace
+
+// Quantize k_new/v_new (tokens, kv_heads, head_dim), any strides, into rows `slots` int32
+// (tokens,) of the 4-bit pages.  In place; negative slots are skipped.
+void kv4_cache_append_torch(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor K_pages,
+                            torch::Tensor V_pages, torch::Tensor sK_pages, torch::Tensor sV_pages,
+                            torch::Tensor slots) {
+    const Kv4Dims d = check_kv4(K_pages, sK_pages, "K_pages");
+    check_kv4(V_pages, sV_pages, "V_pages");
+    TORCH_CHECK(K_pages.sizes() == V_pages.sizes(), "K_pages/V_pages shape mismatch");
+    check_slots(slots, K_pages);
+    TORCH_CHECK(k_new.dim() == 3 && k_new.sizes() == v_new.sizes() && k_new.dtype() == v_new.dtype(),
+                "k_new/v_new must be (tokens, kv_heads, head_dim) of one shape and dtype");
+    TORCH_CHECK(k_new.size(0) == slots.numel() && k_new.size(1) == d.kv_heads &&
+                    k_new.size(2) == d.head_dim,
+                "cache/new-token shape mismatch");
+    for (const auto* t : {&k_new, &v_new, &V_pages}) check_on(*t, K_pages, "every input");
+    const int code = dtype_code(k_new);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(K_pages.device());
+    auto k = token_rows(k_new), v = token_rows(v_new);
+    auto sl = slots.contiguous();
+    check_status(int8k_kv4_cache_append(
+                     k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0),
+                     v.stride(1), K_pages.data_ptr<uint8_t>(), V_pages.data_ptr<uint8_t>(),
+                     sK_pages.data_ptr<float>(), sV_pages.data_ptr<float>(),
+                     sl.data_ptr<int32_t>(), as_int(sl.numel(), "tokens"), d.kv_heads, d.head_dim,
+                     d.num_pages, d.page, current_stream(K_pages)),
+                 "kv4_cache_append");
+}
+
+// Rows `slots` of one side of the cache as (tokens, kv_heads, head_dim) of dtype (default fp16).
+torch::Tensor kv4_cache_read_torch(torch::Tensor pages, torch::Tensor scales, torch::Tensor slots,
+                                   c10::optional<at::ScalarType> dtype) {
+    const Kv4Dims d = check_kv4(pages, scales, "pages");
+    check_slots(slots, pages);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(pages.device());
+    auto out = torch::empty({slots.numel(), d.kv_heads, d.head_dim},
+                            torch::TensorOptions()
+                                .dtype(dtype.has_value() ? *dtype : torch::kFloat16)
+                                .device(pages.device()));
+    const int code = dtype_code(out);
+    auto sl = slots.contiguous();
+    check_status(int8k_kv4_cache_read(pages.data_ptr<uint8_t>(), scales.data_ptr<float>(),
+                                      sl.data_ptr<int32_t>(), out.data_ptr(), code,
+                                      as_int(sl.numel(), "tokens"), d.kv_heads, d.head_dim,
+                                      d.num_pages, d.page, current_stream(pages)),
+                 "kv4_cache_read");
+    return out;
+}
+
+// Decode over a paged 4-bit cache: Q int8 (B, H, D), pages as above with kv_heads dividing H,
+// block_tables (B, max_pages) int32, context_lens (B,) int32.  Returns fp16 (B, H, D).
+torch::Tensor int8_decode_attention_forward_kv4_paged_torch(
+    torch::Tensor Q, torch::Tensor K_pages, torch::Tensor V_pages, torch::Tensor scale_Q,
+    torch::Tensor sK_pages, torch::Tensor sV_pages, torch::Tensor block_tables,
+    torch::Tensor context_lens, int64_t max_context) {
+    const Kv4Dims d = check_kv4(K_pages, sK_pages, "K_pages");
+    check_kv4(V_pages, sV_pages, "V_pages");
+    TORCH_CHECK(K_pages.sizes() == V_pages.sizes(), "K_pages/V_pages shape mismatch");
+    TORCH_CHECK(Q.dtype() == torch::kInt8, "Q must be int8");
+    TORCH_CHECK(Q.dim() == 3 && Q.numel() > 0, "expected Q (batch, heads, head_dim)");
+    const int64_t B = Q.size(0), H = Q.size(1), D = Q.size(2);
+    TORCH_CHECK(D == d.head_dim, "Q/K head_dim mismatch");
+    TORCH_CHECK(H % d.kv_heads == 0, "heads must be a multiple of kv_heads");
+    check_float32(scale_Q, "scale_Q");
+    check_int32(block_tables, "block_tables");
+    check_int32(context_lens, "context_lens");
+    TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == B && context_lens.numel() == B,
+                "block_tables (batch, max_pages) / context_lens (batch,) shape mismatch");
+    for (const auto* t : {&Q, &V_pages, &scale_Q, &block_tables, &context_lens})
+        check_on(*t, K_pages, "every input");
+    const int64_t max_pages = block_tables.size(1);
+    TORCH_CHECK(max_context >= 1 && max_context <= max_pages * d.page,
+                "max_context must be in [1, max_pages * page]");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(K_pages.device());
+    auto q = dense16(Q);
+    auto sQ = flat_scale(scale_Q, B * H, "scale_Q");
+    auto bt = block_tables.contiguous(), cl = context_lens.contiguous();
+    auto out = torch::empty({B, H, D},
+                            torch::TensorOptions().dtype(torch::kFloat16).device(Q.device()));
+    const int b = as_int(B, "batch"), h = as_int(H, "heads"),
+              top = as_int(max_context, "max_context");
+    const size_t ws_bytes =
+        int8k_decode_attention_kv4_paged_workspace_bytes(b, h, d.kv_heads, top, d.head_dim);
+    auto ws = workspace(ws_bytes, Q.device());
+    check_status(int8k_decode_attention_forward_kv4_paged(
+                     q.data_ptr<int8_t>(), K_pages.data_ptr<uint8_t>(),
+                     V_pages.data_ptr<uint8_t>(),
+                     reinterpret_cast<uint16_t*>(out.data_ptr<at::Half>()), sQ.data_ptr<float>(),
+                     sK_pages.data_ptr<float>(), sV_pages.data_ptr<float>(),
+                     bt.data_ptr<int32_t>(), cl.data_ptr<int32_t>(), b, h, d.kv_heads, d.head_dim,
+                     d.num_pages, d.page, as_int(max_pages, "max_pages"), top, ws.data(),
+                     ws_bytes, current_stream(Q)),
+                 "int8_decode_attention_forward_kv4_paged");
+    return out;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("int8_attention_forward", &int8_attention_forward_torch,
           "INT8 attention with per-token quantization — returns FP16 (optional is_causal; "
@@ -834,5 +1183,40 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("int8_decode_attention_forward_paged_quant",
           &int8_decode_attention_forward_paged_quant_torch,
           "INT8 paged decode emitting per-token int8 — returns (int8, fp32 scales)");
+    // Grouped-query serving (not in the reference's module).
+    m.def("int8_linear", &int8_linear_torch,
+          "INT8 linear with per-token and per-channel scales and an optional bias — returns "
+          "(..., N) of dtype (default fp16)",
+          py::arg("x"), py::arg("W"), py::arg("scale_x"), py::arg("scale_W"),
+          py::arg("bias") = py::none(), py::arg("prepacked") = false,
+          py::arg("dtype") = py::none());
+    m.def("qk_norm_rope", &qk_norm_rope_torch,
+          "Split a fused QKV projection into heads with per-head query/key norms and the "
+          "position rotation — returns [q, k, v]",
+          py::arg("x"), py::arg("heads"), py::arg("kv_heads"), py::arg("cos"), py::arg("sin"),
+          py::arg("positions"), py::arg("q_weight") = py::none(),
+          py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6,
+          py::arg("interleaved") = false);
+    m.def("qk_norm_rope_quantize", &qk_norm_rope_quantize_torch,
+          "qk_norm_rope emitting per-token int8 — returns [q, s_q, k, s_k, v, s_v]",
+          py::arg("x"), py::arg("heads"), py::arg("kv_heads"), py::arg("cos"), py::arg("sin"),
+          py::arg("positions"), py::arg("q_weight") = py::none(),
+          py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6,
+          py::arg("interleaved") = false);
+    m.def("int8_attention_forward_packed", &int8_attention_forward_packed_torch,
+          "INT8 attention over packed sequences with grouped heads — returns FP16 (H, T, D), or "
+          "(T, H, D) with out_thd",
+          py::arg("Q"), py::arg("K"), py::arg("V"), py::arg("scale_Q"), py::arg("scale_K"),
+          py::arg("scale_V"), py::arg("cu_seqlens"), py::arg("is_causal") = false,
+          py::arg("out_thd") = false);
+    m.def("kv4_cache_append", &kv4_cache_append_torch,
+          "Quantize new K/V tokens into rows `slots` of a paged 4-bit KV cache (in place)");
+    m.def("kv4_cache_read", &kv4_cache_read_torch,
+          "Rows `slots` of one side of a 4-bit KV cache as (tokens, kv_heads, head_dim) of dtype",
+          py::arg("pages"), py::arg("scales"), py::arg("slots"), py::arg("dtype") = py::none());
+    m.def("int8_decode_attention_forward_kv4_paged",
+          &int8_decode_attention_forward_kv4_paged_torch,
+          "INT8 query decode attention over a paged 4-bit KV cache with grouped heads — returns "
+          "FP16");
     m.attr("abi_version") = int8k_abi_version();
 }

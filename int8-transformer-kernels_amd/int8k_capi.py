@@ -66,6 +66,18 @@ _SIGNATURES = {
     "int8k_decode_attention_forward_noalloc": (_I, [_P] * 7 + [_I] * 4 + [_P]),
     "int8k_mlp_sync_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint)]),
     "int8k_decode_paged_bad_page_ids": (_I, [ctypes.POINTER(ctypes.c_uint)]),
+    "int8k_linear_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "int8k_linear": (_I, [_P, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _SZ, _P]),
+    "int8k_qk_norm_rope": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P, _F, _P, _P, _P] + [_I] * 6 + [_P]),
+    "int8k_qk_norm_rope_quantize": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P, _F] + [_P] * 6 +
+                                    [_I] * 6 + [_P]),
+    "int8k_rope_bad_positions": (_I, [ctypes.POINTER(ctypes.c_uint)]),
+    "int8k_attention_forward_packed": (_I, [_P] * 8 + [_I] * 6 + [_P]),
+    "int8k_kv4_cache_append": (_I, [_P, _P, _I, _LL, _LL, _LL, _LL] + [_P] * 5 + [_I] * 5 + [_P]),
+    "int8k_kv4_cache_read": (_I, [_P] * 4 + [_I] * 6 + [_P]),
+    "int8k_decode_attention_kv4_paged_workspace_bytes": (_SZ, [_I] * 5),
+    "int8k_decode_attention_forward_kv4_paged": (_I, [_P] * 9 + [_I] * 8 + [_P, _SZ, _P]),
+    "int8k_kv4_bad_ids": (_I, [ctypes.POINTER(ctypes.c_uint)]),
 }
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
@@ -520,3 +532,140 @@ def quantize_heads(x, heads, parts=3):
                                      _stream(x))
     check("int8k_quantize_heads", st)
     return outs
+
+
+# --------------------------------------------------------------------------
+# grouped-query serving: linear, head norms + rotation, packed prompts, 4-bit cache
+# --------------------------------------------------------------------------
+
+LINEAR_WEIGHT_PREPACKED = 1  # INT8K_LINEAR_WEIGHT_PREPACKED
+ROPE_INTERLEAVED = 1         # INT8K_ROPE_INTERLEAVED
+ATTN_OUT_THD = 2             # INT8K_ATTN_OUT_THD
+ATTN_ZERO_REST = 4           # INT8K_ATTN_ZERO_REST
+
+
+def linear_workspace_bytes(T, K, N, flags=0):
+    return load().int8k_linear_workspace_bytes(T, K, N, flags)
+
+
+def linear(x, W, scale_x, scale_W, bias=None, flags=0, dtype=None, out=None, workspace=None):
+    """x [T, K] int8; W int8 [K, N] ([N, K] with LINEAR_WEIGHT_PREPACKED); fp32 scales of
+    length 1 or T / N.  Returns [T, N] of dtype (fp16)."""
+    import torch
+
+    T, K = x.shape
+    N = W.shape[0] if flags & LINEAR_WEIGHT_PREPACKED else W.shape[1]
+    if out is None:
+        out = torch.empty((T, N), dtype=dtype or torch.float16, device=x.device)
+    if workspace is None:
+        workspace = torch.empty(max(linear_workspace_bytes(T, K, N, flags), 1), dtype=torch.uint8,
+                                device=x.device)
+    check("int8k_linear", load().int8k_linear(
+        _ptr(x), _ptr(W), _ptr(out), _dtype_code(out), _ptr(scale_x), scale_x.numel(),
+        _ptr(scale_W), scale_W.numel(), _ptr(bias), T, K, N, flags, _ptr(workspace),
+        workspace.numel(), _stream(x)))
+    return out
+
+
+def qk_norm_rope(x, heads, kv_heads, cos, sin, positions, q_weight=None, k_weight=None,
+                 eps=1e-6, flags=0, quantize=False):
+    """x [B, S, (heads + 2 kv_heads) * D] -> [q, k, v] heads [B, H, S, D] of x's dtype, or
+    [q, sq, k, sk, v, sv] int8 and fp32 scales."""
+    import torch
+
+    B, S, width = x.shape
+    D = width // (heads + 2 * kv_heads)
+    outs = []
+    for n in (heads, kv_heads, kv_heads):
+        outs.append(torch.empty((B, n, S, D), dtype=torch.int8 if quantize else x.dtype,
+                                device=x.device))
+        if quantize:
+            outs.append(torch.empty((B, n, S), dtype=torch.float32, device=x.device))
+    f = load().int8k_qk_norm_rope_quantize if quantize else load().int8k_qk_norm_rope
+    check("int8k_qk_norm_rope", f(
+        _ptr(x), _dtype_code(x), _ptr(cos), _ptr(sin), cos.shape[0], 2 * cos.shape[1],
+        _ptr(positions), _ptr(q_weight), _ptr(k_weight), float(eps), *(_ptr(o) for o in outs),
+        B, S, heads, kv_heads, D, flags, _stream(x)))
+    return outs
+
+
+def rope_bad_positions() -> int:
+    """Tokens whose position lay outside the angle tables, on the current device since load."""
+    n = ctypes.c_uint(0)
+    check("int8k_rope_bad_positions", load().int8k_rope_bad_positions(ctypes.byref(n)))
+    return int(n.value)
+
+
+def attention_forward_packed(Qi, Ki, Vi, sQ, sK, sV, cu_seqlens, causal=False, out_thd=False,
+                             zero_rest=False, out=None):
+    """Qi [H, T, D], Ki/Vi [Hkv, T, D] int8, scales [H or Hkv, T], cu_seqlens int32 [n+1]
+    (device) -> fp16 [H, T, D] ([T, H, D] with out_thd)."""
+    import torch
+
+    H, T, D = Qi.shape
+    if out is None:
+        out = torch.empty((T, H, D) if out_thd else (H, T, D), dtype=torch.float16,
+                          device=Qi.device)
+    flags = ((ATTN_CAUSAL if causal else 0) | (ATTN_OUT_THD if out_thd else 0) |
+             (ATTN_ZERO_REST if zero_rest else 0))
+    check("int8k_attention_forward_packed", load().int8k_attention_forward_packed(
+        _ptr(Qi), _ptr(Ki), _ptr(Vi), _ptr(out), _ptr(sQ), _ptr(sK), _ptr(sV), _ptr(cu_seqlens),
+        cu_seqlens.numel() - 1, T, H, Ki.shape[0], D, flags, _stream(Qi)))
+    return out
+
+
+def kv4_cache_append(k_new, v_new, K_pages, V_pages, sK_pages, sV_pages, slots):
+    """k_new/v_new [T, Hkv, D] (D contiguous) into rows `slots` int32 [T] of the 4-bit pages."""
+    T, H, D = k_new.shape
+    check("int8k_kv4_cache_append", load().int8k_kv4_cache_append(
+        _ptr(k_new), _ptr(v_new), _dtype_code(k_new), k_new.stride(0), k_new.stride(1),
+        v_new.stride(0), v_new.stride(1), _ptr(K_pages), _ptr(V_pages), _ptr(sK_pages),
+        _ptr(sV_pages), _ptr(slots), T, H, D, K_pages.shape[0], K_pages.shape[2],
+        _stream(k_new)))
+
+
+def kv4_cache_read(pages, scales, slots, dtype=None):
+    """Rows `slots` of one side of the 4-bit cache: [T, Hkv, D] of dtype (fp16)."""
+    import torch
+
+    NP, H, P, half = pages.shape
+    out = torch.empty((slots.numel(), H, 2 * half), dtype=dtype or torch.float16,
+                      device=pages.device)
+    check("int8k_kv4_cache_read", load().int8k_kv4_cache_read(
+        _ptr(pages), _ptr(scales), _ptr(slots), _ptr(out), _dtype_code(out), slots.numel(), H,
+        2 * half, NP, P, _stream(pages)))
+    return out
+
+
+def decode_kv4_paged_workspace_bytes(B, heads, kv_heads, max_context, D):
+    return load().int8k_decode_attention_kv4_paged_workspace_bytes(B, heads, kv_heads,
+                                                                   max_context, D)
+
+
+def decode_attention_kv4_paged(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, block_tables,
+                               context_lens, max_context, out=None, workspace=None):
+    """Qi int8 [B, H, D] against 4-bit pages [num_pages, Hkv, page, D/2] -> fp16 [B, H, D]."""
+    import torch
+
+    B, H, D = Qi.shape
+    NP, Hkv, P, _ = K_pages.shape
+    if out is None:
+        out = torch.empty((B, H, D), dtype=torch.float16, device=Qi.device)
+    if workspace is None:
+        n = decode_kv4_paged_workspace_bytes(B, H, Hkv, max_context, D)
+        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=Qi.device)
+    check("int8k_decode_attention_forward_kv4_paged",
+          load().int8k_decode_attention_forward_kv4_paged(
+              _ptr(Qi), _ptr(K_pages), _ptr(V_pages), _ptr(out), _ptr(sQ), _ptr(sK_pages),
+              _ptr(sV_pages), _ptr(block_tables), _ptr(context_lens), B, H, Hkv, D, NP, P,
+              block_tables.shape[1], max_context, _ptr(workspace), workspace.numel(),
+              _stream(Qi)))
+    return out
+
+
+def kv4_bad_ids() -> int:
+    """Appends past the cache plus decode units that met a bad page id, on the current device
+    since load."""
+    n = ctypes.c_uint(0)
+    check("int8k_kv4_bad_ids", load().int8k_kv4_bad_ids(ctypes.byref(n)))
+    return int(n.value)
