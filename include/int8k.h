@@ -490,7 +490,7 @@ int int8k_attention_forward_packed(const int8_t* Q, const int8_t* K, const int8_
 /* A paged KV cache held in 4 bits.  A row (one token of one key head) is head_dim
  * codes, two a byte (element 2i in the low half of byte i), stored as code + 8, and
  * one fp32 scale:
- *   s = max(|row|, 1e-8) / 7, code = rn(clamp(x / s, -8, 7)), x ~= code * s.
+ *   s = max(|row|, 1e-8) * fl(1/7), code = rn(clamp(x / s, -8, 7)), x ~= code * s.
  *   K_pages / V_pages uint8 [num_pages, kv_heads, page_size, head_dim / 2]
  *   sK_pages / sV_pages fp32 [num_pages, kv_heads, page_size]
  * head_dim 64 or 128; page_size a power of two in [16, 1024]; num_pages * page_size

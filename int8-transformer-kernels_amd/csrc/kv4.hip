@@ -3,9 +3,12 @@
 //
 // A cache row is one token of one key head: D codes of 4 bits, two a byte (element 2i in the
 // low half of byte i, 2i + 1 in the high half), each stored as code + 8, and one fp32 scale:
-//   s = max(|row|, 1e-8) / 7,  code = rn(clamp(x / s, -8, 7)),  x ~= code * s
+//   s = max(|row|, 1e-8) * fl(1/7),  code = rn(clamp(x / s, -8, 7)),  x ~= code * s
+// (the product with the rounded reciprocal is what `amax / 7` is on the device in PyTorch, whose
+// division by a host number multiplies)
 // K_pages and V_pages uint8 [num_pages, kv_heads, page, D/2], scales fp32 [num_pages,
 // kv_heads, page].  A NaN in a row makes its scale NaN (as amax does in PyTorch).
+#include <algorithm>
 #include <cmath>
 
 #include "rows.h"
@@ -22,7 +25,7 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 
 __device__ __forceinline__ float kv4_scale(uint32_t amax_bits) {
     const float m = __uint_as_float(amax_bits);
-    return (m < 1e-8f ? 1e-8f : m) / 7.f;  // NaN stays NaN
+    return (m < 1e-8f ? 1e-8f : m) * (1.f / 7.f);  // NaN stays NaN
 }
 
 __device__ __forceinline__ uint32_t kv4_code(float x, float s) {
@@ -132,66 +135,391 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict
 }
 
 // ------------------------------------------------------------------ decode
-// One block per (sequence, query head): each group of D/8 lanes takes a position at a time,
-// keeps a running maximum and sum of its own, and the groups' states are joined in LDS.
+// The scores and the weighted values of up to 16 query heads that share a key head are one
+// MFMA tile, so a wave reads every cache row once for all of them: tiles of 32 positions,
+//   S^T[32 keys x 16 q] = K . Q^T    v_mfma_i32_16x16x64_i8, exact int32: the codes enter as
+//                                    0..15 (one AND, one shift), -8 sum(q) as the initial sum
+//   O^T[D x 16 q]      += V^T . P^T  v_mfma_f32_16x16x32_f16, the codes as exact fp16
+// In the accumulator layout lane l holds query l % 16 and rows 4 (l / 16) + r.  Rows are keys
+// in the order 4 (m % 4) + m / 4, so lane group g = l / 16 ends up with the scores of keys
+// 4 j + g, j = 0..7, as the B operand of the second product wants them: P never changes lanes.
+// The A operand of that product is 8 keys of one dim per lane: lane l reads word l % 16 (8
+// dims) of those 8 rows and picks a byte of two keys at a time (v_perm), each half of which
+// becomes two fp16 codes with an AND, an OR and one packed operation.  No LDS in the loop.
+//
+// Positions are uniform over the wave, so pages and addresses are scalar.  A wave holds the
+// next tile's loads in registers while it computes one (4.3 KiB at D = 128).
+//
+// m is a reference for the exponentials, not necessarily the running maximum: a tile whose
+// scores stay below m + 8 (powers of two) and whose weights p * sV * f stay in fp16's range
+// takes the short path, with no exchange between lanes and no rescaling.  f is a power of
+// two per query that keeps the fp16 weights near 1 whatever the size of the value scales; it
+// follows the largest p * sV whenever m moves.  l sums p in fp32; O is fp32.
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+constexpr int kTile = 32;       // keys per tile
+constexpr int kMaxRows = 16;    // query heads per block
+constexpr float kLead = 8.f;    // how far (log2) a score may lie above m
+constexpr float kMaxWeight = 60000.f;
+
+struct Kv4Decode {
+    const int8_t* Q;
+    const uint8_t *K, *V;
+    const float *sQ, *sK, *sV;
+    const int32_t *tables, *lens;
+    uint16_t* out;
+    float *part_ml, *part_acc;  // [B * Hq][nsplit][2] and [..][D] (nsplit > 1)
+    int Hq, Hkv, num_pages, log2_page, max_pages, max_context;
+    int groups, rows, nsplit;   // blocks of query heads per key head, heads in each
+    float qk;
+};
+
+// Value of lane N of each row of 16 lanes (DPP row_newbcast).
+template <int N>
+__device__ __forceinline__ float bcast16(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xF, 0xF, false));
+}
+
+// max or sum over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float max_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return max_xor32(fmaxf(__int_as_float(a[0]), __int_as_float(a[1])));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return sum_xor32(__int_as_float(a[0]) + __int_as_float(a[1]));
+}
+
 template <int D>
-__global__ __launch_bounds__(256) void kv4_decode_kernel(
-    const int8_t* __restrict__ Q, const uint8_t* __restrict__ Kp, const uint8_t* __restrict__ Vp,
-    const float* __restrict__ sQ, const float* __restrict__ sKp, const float* __restrict__ sVp,
-    const int32_t* __restrict__ tables, const int32_t* __restrict__ lens,
-    uint16_t* __restrict__ out, int Hq, int Hkv, int num_pages, int log2_page, int max_pages,
-    int max_context, float qk) {
-    constexpr int L = D / 8, kGroups = 256 / L;
-    __shared__ float s_m[kGroups], s_l[kGroups], s_acc[kGroups][D];
-    const int b = blockIdx.x / Hq, h = blockIdx.x % Hq, kvh = h / (Hq / Hkv);
-    const int c = threadIdx.x & (L - 1), g = threadIdx.x / L;
-    const int len = min(max(lens[b], 0), max_context);
-    const int32_t* table = tables + (size_t)b * max_pages;
-    float q[8];
+struct Kv4Tile {
+    static constexpr int kW = D / 32;  // 4-byte words of a K row per lane
+    uint32_t k[2][kW];                 // rows 4 (m % 4) + m / 4 (+ 16): bytes 4 kW g ..
+    uint32_t v[8];                     // word of key 4 j + g
+    float sk, sv;                      // lane n of a row of lanes: key 4 (n % 8) + g
+};
+
+template <int D>
+__global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
+    constexpr int kRow = D / 2;         // bytes per cache row
+    constexpr int NF = D / 16;          // fragments of O^T
+    constexpr int kW = Kv4Tile<D>::kW;
+    constexpr int kORow = D + 4;        // floats per row of O in LDS
+    extern __shared__ __align__(16) float s_merge[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nw = blockDim.x >> 6;
+    const int g = lane >> 4, m16 = lane & 15;
+
+    // block -> (sequence, key head, heads of it, split)
+    int x = blockIdx.x;
+    const int grp = x % p.groups;
+    x /= p.groups;
+    const int split = x % p.nsplit;
+    x /= p.nsplit;
+    const int kvh = x % p.Hkv, b = x / p.Hkv;
+    const int per_kv = p.Hq / p.Hkv;
+    const int rows = min(p.rows, per_kv - grp * p.rows);
+    const int head0 = kvh * per_kv + grp * p.rows;  // first query head
+    const int len = min(max(__builtin_amdgcn_readfirstlane(p.lens[b]), 0), p.max_context);
+    const int tiles = (len + kTile - 1) / kTile;
+    const int per_split = (tiles + p.nsplit - 1) / p.nsplit;
+    const int t_begin = min(split * per_split, tiles), t_end = min(t_begin + per_split, tiles);
+    const int32_t* __restrict__ table = p.tables + (size_t)b * p.max_pages;
+    const int pmask = (1 << p.log2_page) - 1;
+
+    // this lane's query row (lanes past the rows hold zeros) and -8 sum(q)
+    const bool qok = m16 < rows;
+    const size_t qrow = (size_t)b * p.Hq + head0 + min(m16, rows - 1);
+    uint32_t qlo[kW], qhi[kW];  // even and odd elements of 8 kW consecutive ones
+    int qsum = 0;
+    {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(p.Q + qrow * D) + 2 * kW * g;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = (float)Q[(size_t)blockIdx.x * D + 8 * c + i];
-    const float qs = sQ[blockIdx.x] * qk;
-    float m = -INFINITY, l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    unsigned bad = 0;
-    for (int j = g; j < len; j += kGroups) {
-        int page = table[j >> log2_page];
-        if ((unsigned)page >= (unsigned)num_pages) page = num_pages - 1, bad = 1;
-        const size_t r = (((size_t)page * Hkv + kvh) << log2_page) + (j & ((1 << log2_page) - 1));
-        const uint32_t kw = reinterpret_cast<const uint32_t*>(Kp + r * (D / 2))[c];
-        const uint32_t vw = reinterpret_cast<const uint32_t*>(Vp + r * (D / 2))[c];
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dot = fmaf((float)((int)((kw >> (4 * i)) & 15u) - 8), q[i], dot);
-        dot = row_reduce(dot, D == 64 ? 3 : 4, [](float x, float y) { return x + y; });
-        const float s = dot * qs * sKp[r];
-        const float m_new = fmaxf(m, s);
-        const float corr = fast_exp2(m - m_new), p = fast_exp2(s - m_new);
-        l = l * corr + p;
-        const float w = p * sVp[r];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            acc[i] = fmaf(w, (float)((int)((vw >> (4 * i)) & 15u) - 8), acc[i] * corr);
-        m = m_new;
+        for (int w = 0; w < kW; ++w) {
+            const uint32_t a = qok ? q[2 * w] : 0u, c = qok ? q[2 * w + 1] : 0u;
+            qlo[w] = __builtin_amdgcn_perm(c, a, 0x06040200u);
+            qhi[w] = __builtin_amdgcn_perm(c, a, 0x07050301u);
+            qsum = __builtin_amdgcn_sdot4((int)a, 0x01010101, qsum, false);
+            qsum = __builtin_amdgcn_sdot4((int)c, 0x01010101, qsum, false);
+        }
+        const auto s16 = __builtin_amdgcn_permlane16_swap(qsum, qsum, false, false);
+        qsum = (int)(s16[0] + s16[1]);
+        const auto s32 = __builtin_amdgcn_permlane32_swap(qsum, qsum, false, false);
+        qsum = -8 * (int)(s32[0] + s32[1]);
     }
-    if (__ballot(bad != 0) != 0 && (threadIdx.x & 63) == 0) atomicAdd(&g_kv4_bad_ids, 1u);
-    if (c == 0) s_m[g] = m, s_l[g] = l;
+    const float qs = qok ? p.sQ[qrow] * p.qk : 0.f;
+
+    // lane offsets inside 16 rows
+    const uint32_t k_off = (uint32_t)(4 * (m16 & 3) + (m16 >> 2)) * kRow + 4 * kW * g;
+    const uint32_t v_off = (uint32_t)g * kRow + 4 * (D == 128 ? m16 : m16 & 7);
+    const int s_off = 4 * (m16 & 3) + g;        // row of this lane's scales inside its 16
+    const bool s_upper = (m16 & 4) != 0;        // they lie in the second 16 keys
+    bool bad = false;
+
+    // the two runs of 16 rows of tile t (a page holds whole runs): first row of each
+    auto run_row = [&](int key) -> size_t {
+        const int idx = min(key, len - 1) >> p.log2_page;  // entries past the length are not read
+        const int raw = __builtin_amdgcn_readfirstlane(table[idx]);
+        const int page = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
+        bad = bad || page != raw;
+        return (((size_t)page * p.Hkv + kvh) << p.log2_page) + (size_t)(key & pmask);
+    };
+    auto load = [&](Kv4Tile<D>& r, size_t row0, size_t row1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s_acc[g][8 * c + i] = acc[i];
-    __syncthreads();
-    if (threadIdx.x < D) {
-        float mm = -INFINITY, ll = 0.f, a = 0.f;
-        for (int i = 0; i < kGroups; ++i) mm = fmaxf(mm, s_m[i]);
-        if (len > 0) {
-            for (int i = 0; i < kGroups; ++i) {
-                if (i >= len) break;  // groups without a position
-                const float f = fast_exp2(s_m[i] - mm);
-                ll += s_l[i] * f;
-                a += s_acc[i][threadIdx.x] * f;
+        for (int h = 0; h < 2; ++h) {
+            const size_t row = h == 0 ? row0 : row1;
+            const uint8_t* kb = p.K + row * kRow + k_off;
+            if constexpr (kW == 4) {
+                const uint4 w = *reinterpret_cast<const uint4*>(kb);
+                r.k[h][0] = w.x, r.k[h][1] = w.y, r.k[h][2] = w.z, r.k[h][3] = w.w;
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(kb);
+                r.k[h][0] = w.x, r.k[h][1] = w.y;
+            }
+            const uint8_t* vb = p.V + row * kRow + v_off;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                r.v[4 * h + j] = *reinterpret_cast<const uint32_t*>(vb + 4 * j * kRow);
+        }
+        const size_t srow = (s_upper ? row1 : row0) + s_off;
+        r.sk = p.sK[srow];
+        r.sv = p.sV[srow];
+    };
+
+    v4f o[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f, fsc = 1.f;
+
+    // bytes of two keys' words: b0/b1 are this lane's byte pair at D = 64 (dims 4..7 of the
+    // word for the upper 8 rows of the fragment)
+    uint32_t sel[D == 128 ? 4 : 2];
+#pragma unroll
+    for (int i = 0; i < (D == 128 ? 4 : 2); ++i) {
+        const uint32_t byte = D == 128 ? i : i + (m16 & 8 ? 2 : 0);
+        sel[i] = byte | 0x0c000c00u | ((4u + byte) << 16);
+    }
+
+    auto compute = [&](const Kv4Tile<D>& r, int t) {
+        v4i sa[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sa[h] = v4i{qsum, qsum, qsum, qsum};
+            if constexpr (D == 128) {
+                v4i lo, hi, ql, qh;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    lo[w] = (int)(r.k[h][w] & 0x0f0f0f0fu);
+                    hi[w] = (int)((r.k[h][w] >> 4) & 0x0f0f0f0fu);
+                    ql[w] = (int)qlo[w];
+                    qh[w] = (int)qhi[w];
+                }
+                sa[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, ql, sa[h], 0, 0, 0);
+                sa[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, qh, sa[h], 0, 0, 0);
+            } else {
+                const v4i a = {(int)(r.k[h][0] & 0x0f0f0f0fu), (int)(r.k[h][1] & 0x0f0f0f0fu),
+                               (int)((r.k[h][0] >> 4) & 0x0f0f0f0fu),
+                               (int)((r.k[h][1] >> 4) & 0x0f0f0f0fu)};
+                const v4i q = {(int)qlo[0], (int)qlo[1], (int)qhi[0], (int)qhi[1]};
+                sa[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, q, sa[h], 0, 0, 0);
             }
         }
-        out[(size_t)blockIdx.x * D + threadIdx.x] =
-            len > 0 ? __half_as_ushort(f16_of_f32(a / ll)) : (uint16_t)0;
+        // u_j = q . k_j sK_j of key 4 j + g
+        const float skj[8] = {bcast16<0>(r.sk), bcast16<1>(r.sk), bcast16<2>(r.sk), bcast16<3>(r.sk),
+                              bcast16<4>(r.sk), bcast16<5>(r.sk), bcast16<6>(r.sk), bcast16<7>(r.sk)};
+        const float svj[8] = {bcast16<0>(r.sv), bcast16<1>(r.sv), bcast16<2>(r.sv), bcast16<3>(r.sv),
+                              bcast16<4>(r.sv), bcast16<5>(r.sv), bcast16<6>(r.sv), bcast16<7>(r.sv)};
+        float u[8], w[8], pj[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = static_cast<float>(sa[j >> 2][j & 3]) * skj[j];
+        bool slow = t * kTile + kTile > len;  // wave-uniform
+        if (!slow) {
+            float e[8], top = -INFINITY, wide = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                e[j] = fmaf(u[j], qs, -m);
+                top = fmaxf(top, e[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                pj[j] = fast_exp2(e[j]);
+                w[j] = pj[j] * fsc * svj[j];
+                wide = fmaxf(wide, fabsf(w[j]));
+            }
+            slow = __ballot(!(top <= kLead && wide <= kMaxWeight)) != 0;
+        }
+        if (slow) {
+            float s[8], top = -INFINITY, pm = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool seen = t * kTile + 4 * j + g < len;
+                s[j] = seen ? u[j] * qs : -INFINITY;
+                top = fmaxf(top, s[j]);
+            }
+            const float m_new = fmaxf(m, max_groups(top));
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = fast_exp2(m - m_use);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool seen = t * kTile + 4 * j + g < len;
+                pj[j] = fast_exp2(s[j] - m_use);
+                w[j] = seen ? pj[j] * svj[j] : 0.f;
+                pm = fmaxf(pm, fabsf(w[j]));
+            }
+            pm = max_groups(pm);
+            float f_new = fsc;
+            if (pm > 0.f && pm < INFINITY) {
+                int e;
+                frexpf(pm, &e);
+                const float f_pm = __builtin_ldexpf(1.f, -min(max(e, -60), 60));
+                f_new = m_new > m ? f_pm : fminf(fsc, f_pm);
+            }
+            const float ratio = alpha * (f_new / fsc);
+            l *= alpha;
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[f][i] *= ratio;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] *= f_new;
+            m = m_new, fsc = f_new;
+        }
+        l += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+        // fp16 weights: one rounding of p sV f
+        const v8h pw = {(_Float16)w[0], (_Float16)w[1], (_Float16)w[2], (_Float16)w[3],
+                        (_Float16)w[4], (_Float16)w[5], (_Float16)w[6], (_Float16)w[7]};
+        // codes of a byte of two keys: 0x6400 | n is 1024 + n in fp16 and 0x6400 | 16 n is
+        // 1024 + 16 n, both exact, as are the sums below
+        const h2 low_bias = {(_Float16)-1032.f, (_Float16)-1032.f};
+        const h2 high_scale = {(_Float16)0.0625f, (_Float16)0.0625f};
+        const h2 high_bias = {(_Float16)-72.f, (_Float16)-72.f};
+#pragma unroll
+        for (int i = 0; i < NF / 2; ++i) {
+            v8h lo, hi;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t c = __builtin_amdgcn_perm(r.v[2 * j + 1], r.v[2 * j], sel[i]);
+                const h2 a = __builtin_bit_cast(h2, (c & 0x000f000fu) | 0x64006400u) + low_bias;
+                const h2 d = __builtin_elementwise_fma(
+                    __builtin_bit_cast(h2, (c & 0x00f000f0u) | 0x64006400u), high_scale, high_bias);
+                lo[2 * j] = a.x, lo[2 * j + 1] = a.y;
+                hi[2 * j] = d.x, hi[2 * j + 1] = d.y;
+            }
+            o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pw, o[2 * i], 0, 0, 0);
+            o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pw, o[2 * i + 1], 0, 0, 0);
+        }
+    };
+
+    {
+        int t = t_begin + wave;
+        Kv4Tile<D> ra, rb;
+        size_t n0 = 0, n1 = 0;  // rows of the tile after next
+        auto rows_of = [&](int tt) {
+            if (tt < t_end) n0 = run_row(tt * kTile), n1 = run_row(tt * kTile + 16);
+        };
+        rows_of(t);
+        if (t < t_end) load(ra, n0, n1);
+        rows_of(t + nw);
+        while (t < t_end) {
+            if (t + nw < t_end) load(rb, n0, n1);
+            rows_of(t + 2 * nw);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(ra, t);
+            t += nw;
+            if (t >= t_end) break;
+            if (t + nw < t_end) load(ra, n0, n1);
+            rows_of(t + 2 * nw);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(rb, t);
+            t += nw;
+        }
     }
+    if (bad && lane == 0) atomicAdd(&g_kv4_bad_ids, 1u);
+
+    // Join the waves: m, l, f and O of each row go to LDS, then element by element.
+    // Layout: [wave][m, l, f of 16 rows][rows][kORow].
+    l = sum_groups(l);
+    const int wave_words = 3 * kMaxRows + p.rows * kORow;
+    float* mine = s_merge + wave * wave_words;
+    if (qok) {
+        if (g == 0) mine[m16] = m, mine[kMaxRows + m16] = l, mine[2 * kMaxRows + m16] = fsc;
+        float* orow = mine + 3 * kMaxRows + m16 * kORow;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int mr = 4 * g + i;  // row of the fragment: dims d0 ..
+            const int d0 = D == 128 ? 8 * mr : 8 * (mr & 7) + 4 * (mr >> 3);
+#pragma unroll
+            for (int f = 0; f < NF; f += 4)
+                *reinterpret_cast<float4*>(orow + d0 + f) =
+                    make_float4(o[f][i], o[f + 1][i], o[f + 2][i], o[f + 3][i]);
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * D; e += blockDim.x) {
+        const int row = e / D, d = e % D;
+        float top = -INFINITY, sum = 0.f, acc = 0.f;
+        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_merge[w * wave_words + row]);
+        const float use = top == -INFINITY ? 0.f : top;
+        for (int w = 0; w < nw; ++w) {
+            const float* q = s_merge + w * wave_words;
+            const float a = fast_exp2(q[row] - use);
+            sum += q[kMaxRows + row] * a;
+            acc += q[3 * kMaxRows + row * kORow + d] * (a / q[2 * kMaxRows + row]);
+        }
+        const size_t orow = (size_t)b * p.Hq + head0 + row;
+        if (p.nsplit == 1) {
+            p.out[orow * D + d] = len > 0 ? __half_as_ushort(f16_of_f32(acc / sum)) : (uint16_t)0;
+        } else {
+            const size_t part = orow * p.nsplit + split;
+            if (d == 0) p.part_ml[2 * part] = top, p.part_ml[2 * part + 1] = sum;
+            p.part_acc[part * D + d] = acc;
+        }
+    }
+}
+
+// Joins the splits of each row.
+template <int D>
+__global__ __launch_bounds__(D) void kv4_combine_kernel(const float* __restrict__ ml,
+                                                        const float* __restrict__ acc,
+                                                        const int32_t* __restrict__ lens,
+                                                        uint16_t* __restrict__ out, int Hq,
+                                                        int nsplit) {
+    const size_t row = blockIdx.x;
+    const int d = threadIdx.x;
+    const float* r = ml + row * nsplit * 2;
+    float top = -INFINITY, sum = 0.f, a = 0.f;
+    for (int i = 0; i < nsplit; ++i) top = fmaxf(top, r[2 * i]);
+    const float use = top == -INFINITY ? 0.f : top;
+    for (int i = 0; i < nsplit; ++i) {
+        const float f = fast_exp2(r[2 * i] - use);
+        sum += r[2 * i + 1] * f;
+        a += acc[(row * nsplit + i) * D + d] * f;
+    }
+    out[row * D + d] = lens[blockIdx.x / Hq] > 0 ? __half_as_ushort(f16_of_f32(a / sum)) : (uint16_t)0;
+}
+
+struct Kv4Plan {
+    int groups, rows, waves, nsplit;
+    size_t lds(int D) const { return (size_t)waves * (3 * kMaxRows + rows * (D + 4)) * 4; }
+};
+
+Kv4Plan kv4_plan(int B, int Hq, int Hkv, int max_context) {
+    Kv4Plan pl{};
+    const int per_kv = Hq / Hkv;
+    pl.groups = (per_kv + kMaxRows - 1) / kMaxRows;
+    pl.rows = (per_kv + pl.groups - 1) / pl.groups;
+    pl.groups = (per_kv + pl.rows - 1) / pl.rows;
+    const long long units = (long long)B * Hkv * pl.groups;
+    const long long tiles = ceil_div(max_context, kTile);
+    pl.waves = 4;
+    pl.nsplit = (int)std::max<long long>(
+        1, std::min<long long>(ceil_div(2048, units), ceil_div(tiles, 8)));
+    if (tiles <= 32) pl.nsplit = 1, pl.waves = tiles <= 4 ? 4 : 8;
+    return pl;
 }
 
 int log2_of(int page) {
@@ -206,6 +534,16 @@ template <typename F>
 void with_head_dim(int D, F&& f) {
     if (D == 64) f(std::integral_constant<int, 64>{});
     else f(std::integral_constant<int, 128>{});
+}
+
+struct Kv4Partials {
+    size_t ml_bytes, bytes;
+};
+Kv4Partials kv4_partials(int B, int Hq, const Kv4Plan& pl, int D) {
+    if (pl.nsplit == 1) return {0, 0};
+    const size_t parts = (size_t)B * Hq * pl.nsplit;
+    const size_t ml = round_up(parts * 2 * sizeof(float), kWorkspaceAlign);
+    return {ml, ml + round_up(parts * D * sizeof(float), kWorkspaceAlign)};
 }
 
 // Shared checks of the cache's shape: INT8K_OK or the status to return.
@@ -284,8 +622,10 @@ extern "C" int int8k_kv4_cache_read(const uint8_t* pages, const float* scales,
 
 extern "C" size_t int8k_decode_attention_kv4_paged_workspace_bytes(int B, int heads, int kv_heads,
                                                                    int max_context, int head_dim) {
-    (void)B, (void)heads, (void)kv_heads, (void)max_context, (void)head_dim;
-    return 0;
+    if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 ||
+        (head_dim != 64 && head_dim != 128))
+        return 0;
+    return kv4_partials(B, heads, kv4_plan(B, heads, kv_heads, max_context), head_dim).bytes;
 }
 
 extern "C" int int8k_decode_attention_forward_kv4_paged(
@@ -307,15 +647,45 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
         !aligned_to(scale_Q, 4) || !aligned_to(sK_pages, 4) || !aligned_to(sV_pages, 4) ||
         !aligned_to(block_tables, 4) || !aligned_to(context_lens, 4) || !aligned_to(out, 8))
         return INT8K_ERR_MISALIGNED;
-    if ((long long)B * heads >= (1LL << 24)) return INT8K_ERR_UNSUPPORTED;
-    (void)workspace, (void)workspace_bytes;
-    const float qk = (1.0f / std::sqrt((float)head_dim)) * kLog2e;
+    if ((long long)B * heads >= (1LL << 22)) return INT8K_ERR_UNSUPPORTED;
+    const Kv4Plan pl = kv4_plan(B, heads, kv_heads, max_context);
+    const Kv4Partials part = kv4_partials(B, heads, pl, head_dim);
+    if (part.bytes > 0) {
+        if (!workspace || workspace_bytes < part.bytes) return INT8K_ERR_WORKSPACE;
+        if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
+    }
+    const long long blocks = (long long)B * kv_heads * pl.groups * pl.nsplit;
+    if (blocks * pl.waves >= (1LL << 26)) return INT8K_ERR_UNSUPPORTED;  // work-items below 2^32
+    Kv4Decode p{};
+    p.Q = Q, p.K = K_pages, p.V = V_pages, p.sQ = scale_Q, p.sK = sK_pages, p.sV = sV_pages;
+    p.tables = block_tables, p.lens = context_lens, p.out = out;
+    p.part_ml = static_cast<float*>(workspace);
+    p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + part.ml_bytes);
+    p.Hq = heads, p.Hkv = kv_heads, p.num_pages = num_pages, p.log2_page = log2_of(page_size);
+    p.max_pages = max_pages_per_seq, p.max_context = max_context;
+    p.groups = pl.groups, p.rows = pl.rows, p.nsplit = pl.nsplit;
+    p.qk = (1.0f / std::sqrt((float)head_dim)) * kLog2e;
+    int st = INT8K_OK;
     with_head_dim(head_dim, [&](auto d) {
-        kv4_decode_kernel<decltype(d)::value><<<(unsigned)(B * heads), 256, 0, as_stream(stream)>>>(
-            Q, K_pages, V_pages, scale_Q, sK_pages, sV_pages, block_tables, context_lens, out,
-            heads, kv_heads, num_pages, log2_of(page_size), max_pages_per_seq, max_context, qk);
+        constexpr int D = decltype(d)::value;
+        static PerDeviceOnce once;
+        st = once.run([] {
+            const hipError_t e = hipFuncSetAttribute(
+                reinterpret_cast<const void*>(&kv4_decode_kernel<D>),
+                hipFuncAttributeMaxDynamicSharedMemorySize, 8 * (3 * kMaxRows + kMaxRows * (D + 4)) * 4);
+            if (e == hipSuccess) return (int)INT8K_OK;
+            set_last_error("hipFuncSetAttribute", e);
+            return (int)INT8K_ERR_HIP;
+        });
+        if (st != INT8K_OK) return;
+        kv4_decode_kernel<D><<<(unsigned)blocks, 64 * pl.waves, pl.lds(D), as_stream(stream)>>>(p);
+        st = check_launch("kv4_decode_kernel");
+        if (st != INT8K_OK || pl.nsplit == 1) return;
+        kv4_combine_kernel<D><<<(unsigned)(B * heads), D, 0, as_stream(stream)>>>(
+            p.part_ml, p.part_acc, context_lens, out, heads, pl.nsplit);
+        st = check_launch("kv4_combine_kernel");
     });
-    return check_launch("kv4_decode_kernel");
+    return st;
 }
 
 extern "C" int int8k_kv4_bad_ids(unsigned int* count) {

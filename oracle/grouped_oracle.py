@@ -79,7 +79,7 @@ def kv4_quantize(x):
     x = x.astype(F32)
     with np.errstate(invalid="ignore", over="ignore"):
         amax = np.abs(x).max(-1)
-        s = (np.where(amax < F32(1e-8), F32(1e-8), amax) / F32(7)).astype(F32)
+        s = (np.where(amax < F32(1e-8), F32(1e-8), amax) * (F32(1) / F32(7))).astype(F32)
         q = (x / s[..., None]).astype(F32)
         q = np.where(np.isnan(q), F32(-8), np.clip(q, F32(-8), F32(7)))
     return np.rint(q).astype(np.int8), s
