@@ -148,22 +148,27 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict
 // becomes two fp16 codes with an AND, an OR and one packed operation.  No LDS in the loop.
 //
 // Positions are uniform over the wave, so pages and addresses are scalar.  A wave holds the
-// next tile's loads in registers while it computes one (4.3 KiB at D = 128).
+// next tile's loads in registers while it computes one (4.3 KiB at D = 128).  Every load
+// instruction covers whole lines and is non-temporal (B32, 8 key heads of 128, up to 16K
+// positions: 80 -> 71 us; the loads alone 75 -> 66).
 //
-// m is a reference for the exponentials, not necessarily the running maximum: a tile whose
-// scores stay below m + 8 (powers of two) and whose weights p * sV * f stay in fp16's range
-// takes the short path, with no exchange between lanes and no rescaling.  f is a power of
-// two per query that keeps the fp16 weights near 1 whatever the size of the value scales; it
-// follows the largest p * sV whenever m moves.  l sums p in fp32; O is fp32.
+// p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
+// that the largest weight p sV of the tile that set it lies in [0.5, 1), whatever the size of
+// the value scales, and a tile whose weights stay in fp16's range under the current m takes
+// the short path, with no exchange between lanes and no rescaling.  l sums p and O the
+// weighted codes, both in fp32 and both relative to m.
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32;       // keys per tile
 constexpr int kMaxRows = 16;    // query heads per block
-constexpr float kLead = 8.f;    // how far (log2) a score may lie above m
-constexpr float kMaxWeight = 60000.f;
+constexpr float kMaxWeight = 60000.f;  // fp16 weights stay below it
+constexpr float kMaxSum = 0x1p60f;      // and the sum of a lane's 8 p below this
+constexpr int kMaxShift = 60;           // |m - running maximum| where m is set
 
 struct Kv4Decode {
     const int8_t* Q;
@@ -172,7 +177,7 @@ struct Kv4Decode {
     const int32_t *tables, *lens;
     uint16_t* out;
     float *part_ml, *part_acc;  // [B * Hq][nsplit][2] and [..][D] (nsplit > 1)
-    int Hq, Hkv, num_pages, log2_page, max_pages, max_context;
+    int B, Hq, Hkv, num_pages, log2_page, max_pages, max_context;
     int groups, rows, nsplit;   // blocks of query heads per key head, heads in each
     float qk;
 };
@@ -181,7 +186,7 @@ struct Kv4Decode {
 template <int N>
 __device__ __forceinline__ float bcast16(float v) {
     return __int_as_float(
-        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xF, 0xF, false));
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xF, 0xF, true));
 }
 
 // max or sum over the lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -214,13 +219,16 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
     const int nw = blockDim.x >> 6;
     const int g = lane >> 4, m16 = lane & 15;
 
-    // block -> (sequence, key head, heads of it, split)
-    int x = blockIdx.x;
-    const int grp = x % p.groups;
-    x /= p.groups;
-    const int split = x % p.nsplit;
-    x /= p.nsplit;
-    const int kvh = x % p.Hkv, b = x / p.Hkv;
+    // Block -> (sequence, split), key head and heads of it.  Blocks go to the 8 XCDs in turn;
+    // the key heads of one piece of a sequence, whose pages lie side by side in memory, run one
+    // after the other on one XCD (B = 1, 8 heads, 1000 positions: 9.0 us in 4 splits dealt out
+    // head by head, 7.3 in 8, where that falls so by itself).
+    const int heads_here = p.Hkv * p.groups;
+    const int local = (int)blockIdx.x / 8;
+    const int piece = local / heads_here * 8 + (int)blockIdx.x % 8;
+    if (piece >= p.B * p.nsplit) return;
+    const int b = piece / p.nsplit, split = piece % p.nsplit;
+    const int kvh = local % heads_here / p.groups, grp = local % p.groups;
     const int per_kv = p.Hq / p.Hkv;
     const int rows = min(p.rows, per_kv - grp * p.rows);
     const int head0 = kvh * per_kv + grp * p.rows;  // first query head
@@ -260,40 +268,57 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
     const bool s_upper = (m16 & 4) != 0;        // they lie in the second 16 keys
     bool bad = false;
 
-    // the two runs of 16 rows of tile t (a page holds whole runs): first row of each
-    auto run_row = [&](int key) -> size_t {
-        const int idx = min(key, len - 1) >> p.log2_page;  // entries past the length are not read
-        const int raw = __builtin_amdgcn_readfirstlane(table[idx]);
-        const int page = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
-        bad = bad || page != raw;
-        return (((size_t)page * p.Hkv + kvh) << p.log2_page) + (size_t)(key & pmask);
+    // The two runs of 16 rows of tile t: their page ids (a page holds whole runs; entries past
+    // the length are not read), and from those the first row of each.  The ids are read a tile
+    // before the rows are needed, which is a tile before the data is: nothing waits on them.
+    const bool two_pages = p.log2_page == 4;
+    int id0 = 0, id1 = 0;
+    auto fetch_ids = [&](int t) {
+        if (t >= t_end) return;
+        id0 = table[(t * kTile) >> p.log2_page];
+        if (two_pages) id1 = table[min(t * kTile + 16, len - 1) >> p.log2_page];
     };
-    auto load = [&](Kv4Tile<D>& r, size_t row0, size_t row1) {
+    size_t row0 = 0, row1 = 0;
+    auto rows_of_ids = [&](int t) {
+        if (t >= t_end) return;
+        auto first = [&](int raw, int key) {
+            const int page = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
+            bad = bad || page != raw;
+            return (((size_t)page * p.Hkv + kvh) << p.log2_page) + (size_t)(key & pmask);
+        };
+        const int raw0 = __builtin_amdgcn_readfirstlane(id0);
+        row0 = first(raw0, t * kTile);
+        row1 = row0 + 16;
+        if (two_pages) row1 = first(__builtin_amdgcn_readfirstlane(id1), t * kTile + 16);
+    };
+    auto load = [&](Kv4Tile<D>& r) {
+        const size_t first = row0, second = row1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const size_t row = h == 0 ? row0 : row1;
+            const size_t row = h == 0 ? first : second;
             const uint8_t* kb = p.K + row * kRow + k_off;
             if constexpr (kW == 4) {
-                const uint4 w = *reinterpret_cast<const uint4*>(kb);
+                const v4u w = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(kb));
                 r.k[h][0] = w.x, r.k[h][1] = w.y, r.k[h][2] = w.z, r.k[h][3] = w.w;
             } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(kb);
+                const v2u w = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(kb));
                 r.k[h][0] = w.x, r.k[h][1] = w.y;
             }
             const uint8_t* vb = p.V + row * kRow + v_off;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                r.v[4 * h + j] = *reinterpret_cast<const uint32_t*>(vb + 4 * j * kRow);
+                r.v[4 * h + j] =
+                    __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb + 4 * j * kRow));
         }
-        const size_t srow = (s_upper ? row1 : row0) + s_off;
-        r.sk = p.sK[srow];
-        r.sv = p.sV[srow];
+        const size_t srow = (s_upper ? second : first) + s_off;
+        r.sk = __builtin_nontemporal_load(p.sK + srow);
+        r.sv = __builtin_nontemporal_load(p.sV + srow);
     };
 
     v4f o[NF];
 #pragma unroll
     for (int f = 0; f < NF; ++f) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f, fsc = 1.f;
+    float m = -INFINITY, l = 0.f;
 
     // bytes of two keys' words: b0/b1 are this lane's byte pair at D = 64 (dims 4..7 of the
     // word for the upper 8 rows of the fragment)
@@ -336,64 +361,67 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
         float u[8], w[8], pj[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) u[j] = static_cast<float>(sa[j >> 2][j & 3]) * skj[j];
-        bool slow = t * kTile + kTile > len;  // wave-uniform
-        if (!slow) {
-            float e[8], top = -INFINITY, wide = 0.f;
+        auto weights = [&]() {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                e[j] = fmaf(u[j], qs, -m);
-                top = fmaxf(top, e[j]);
+                pj[j] = fast_exp2(fmaf(u[j], qs, -m));
+                w[j] = pj[j] * svj[j];
             }
+        };
+        auto sum8 = [&]() {
+            return ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+        };
+        const bool partial = t * kTile + kTile > len;  // wave-uniform
+        float psum = 0.f;
+        bool slow = partial;
+        if (!partial) {
+            weights();
+            psum = sum8();
+            float wide = fmaxf(fabsf(w[0]), fabsf(w[1]));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                pj[j] = fast_exp2(e[j]);
-                w[j] = pj[j] * fsc * svj[j];
-                wide = fmaxf(wide, fabsf(w[j]));
-            }
-            slow = __ballot(!(top <= kLead && wide <= kMaxWeight)) != 0;
+            for (int j = 2; j < 8; j += 2) wide = fmaxf(wide, fmaxf(fabsf(w[j]), fabsf(w[j + 1])));
+            // (the first tile, whose m is -inf, has an infinite sum)
+            slow = __ballot(fmaxf(wide, psum * (kMaxWeight / kMaxSum)) > kMaxWeight) != 0;
         }
         if (slow) {
-            float s[8], top = -INFINITY, pm = 0.f;
+            // the exact maximum, then the largest weight under it
+            float top = -INFINITY, pm = 0.f;
+            bool seen[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const bool seen = t * kTile + 4 * j + g < len;
-                s[j] = seen ? u[j] * qs : -INFINITY;
-                top = fmaxf(top, s[j]);
+                seen[j] = t * kTile + 4 * j + g < len;
+                if (seen[j]) top = fmaxf(top, u[j] * qs);
             }
-            const float m_new = fmaxf(m, max_groups(top));
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = fast_exp2(m - m_use);
+            top = max_groups(top);
+            const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool seen = t * kTile + 4 * j + g < len;
-                pj[j] = fast_exp2(s[j] - m_use);
-                w[j] = seen ? pj[j] * svj[j] : 0.f;
-                pm = fmaxf(pm, fabsf(w[j]));
-            }
+            for (int j = 0; j < 8; ++j)
+                if (seen[j]) pm = fmaxf(pm, fabsf(fast_exp2(fmaf(u[j], qs, -base)) * svj[j]));
             pm = max_groups(pm);
-            float f_new = fsc;
-            if (pm > 0.f && pm < INFINITY) {
-                int e;
-                frexpf(pm, &e);
-                const float f_pm = __builtin_ldexpf(1.f, -min(max(e, -60), 60));
-                f_new = m_new > m ? f_pm : fminf(fsc, f_pm);
-            }
-            const float ratio = alpha * (f_new / fsc);
+            int e = 0;
+            if (pm > 0.f && pm < INFINITY) frexpf(pm, &e);
+            const float m_new = fmaxf(m, top + (float)min(max(e, -kMaxShift), kMaxShift));
+            const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
+            m = m_new;
             l *= alpha;
 #pragma unroll
             for (int f = 0; f < NF; ++f)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[f][i] *= ratio;
+                for (int i = 0; i < 4; ++i) o[f][i] *= alpha;
+            weights();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] *= f_new;
-            m = m_new, fsc = f_new;
+            for (int j = 0; j < 8; ++j)  // rows behind the length may hold anything
+                if (!seen[j]) pj[j] = w[j] = 0.f;
+            psum = sum8();
         }
-        l += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
-        // fp16 weights: one rounding of p sV f
+        l += psum;
+        // fp16 weights: one rounding of p sV
         const v8h pw = {(_Float16)w[0], (_Float16)w[1], (_Float16)w[2], (_Float16)w[3],
                         (_Float16)w[4], (_Float16)w[5], (_Float16)w[6], (_Float16)w[7]};
         // codes of a byte of two keys: 0x6400 | n is 1024 + n in fp16 and 0x6400 | 16 n is
         // 1024 + 16 n, both exact, as are the sums below
+        uint32_t magic = 0x64006400u;
+        asm("" : "+v"(magic));  // in a register: with a literal mask, v_and_or_b32 takes no second literal
         const h2 low_bias = {(_Float16)-1032.f, (_Float16)-1032.f};
         const h2 high_scale = {(_Float16)0.0625f, (_Float16)0.0625f};
         const h2 high_bias = {(_Float16)-72.f, (_Float16)-72.f};
@@ -403,9 +431,9 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t c = __builtin_amdgcn_perm(r.v[2 * j + 1], r.v[2 * j], sel[i]);
-                const h2 a = __builtin_bit_cast(h2, (c & 0x000f000fu) | 0x64006400u) + low_bias;
+                const h2 a = __builtin_bit_cast(h2, (c & 0x000f000fu) | magic) + low_bias;
                 const h2 d = __builtin_elementwise_fma(
-                    __builtin_bit_cast(h2, (c & 0x00f000f0u) | 0x64006400u), high_scale, high_bias);
+                    __builtin_bit_cast(h2, (c & 0x00f000f0u) | magic), high_scale, high_bias);
                 lo[2 * j] = a.x, lo[2 * j + 1] = a.y;
                 hi[2 * j] = d.x, hi[2 * j + 1] = d.y;
             }
@@ -417,22 +445,26 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
     {
         int t = t_begin + wave;
         Kv4Tile<D> ra, rb;
-        size_t n0 = 0, n1 = 0;  // rows of the tile after next
-        auto rows_of = [&](int tt) {
-            if (tt < t_end) n0 = run_row(tt * kTile), n1 = run_row(tt * kTile + 16);
-        };
-        rows_of(t);
-        if (t < t_end) load(ra, n0, n1);
-        rows_of(t + nw);
+        // Data of tile t in ra, rows of tile t + nw, ids of tile t + 2 nw.  The loads are not
+        // conditional: past the last tile they repeat its rows (in a branch, the wait for
+        // this tile's data would have to cover the next one's as well).
+        fetch_ids(t);
+        rows_of_ids(t);
+        fetch_ids(t + nw);
+        if (t < t_end) load(ra);
+        rows_of_ids(t + nw);
+        fetch_ids(t + 2 * nw);
         while (t < t_end) {
-            if (t + nw < t_end) load(rb, n0, n1);
-            rows_of(t + 2 * nw);
+            load(rb);
+            rows_of_ids(t + 2 * nw);
+            fetch_ids(t + 3 * nw);
             __builtin_amdgcn_sched_barrier(0);
             compute(ra, t);
             t += nw;
             if (t >= t_end) break;
-            if (t + nw < t_end) load(ra, n0, n1);
-            rows_of(t + 2 * nw);
+            load(ra);
+            rows_of_ids(t + 2 * nw);
+            fetch_ids(t + 3 * nw);
             __builtin_amdgcn_sched_barrier(0);
             compute(rb, t);
             t += nw;
@@ -440,14 +472,14 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
     }
     if (bad && lane == 0) atomicAdd(&g_kv4_bad_ids, 1u);
 
-    // Join the waves: m, l, f and O of each row go to LDS, then element by element.
-    // Layout: [wave][m, l, f of 16 rows][rows][kORow].
+    // Join the waves: m, l and O of each row go to LDS, then element by element.
+    // Layout: [wave][m, l of 16 rows][rows][kORow].
     l = sum_groups(l);
-    const int wave_words = 3 * kMaxRows + p.rows * kORow;
+    const int wave_words = 2 * kMaxRows + p.rows * kORow;
     float* mine = s_merge + wave * wave_words;
     if (qok) {
-        if (g == 0) mine[m16] = m, mine[kMaxRows + m16] = l, mine[2 * kMaxRows + m16] = fsc;
-        float* orow = mine + 3 * kMaxRows + m16 * kORow;
+        if (g == 0) mine[m16] = m, mine[kMaxRows + m16] = l;
+        float* orow = mine + 2 * kMaxRows + m16 * kORow;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int mr = 4 * g + i;  // row of the fragment: dims d0 ..
@@ -468,7 +500,7 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
             const float* q = s_merge + w * wave_words;
             const float a = fast_exp2(q[row] - use);
             sum += q[kMaxRows + row] * a;
-            acc += q[3 * kMaxRows + row * kORow + d] * (a / q[2 * kMaxRows + row]);
+            acc += q[2 * kMaxRows + row * kORow + d] * a;
         }
         const size_t orow = (size_t)b * p.Hq + head0 + row;
         if (p.nsplit == 1) {
@@ -481,7 +513,9 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
     }
 }
 
-// Joins the splits of each row.
+// Joins the splits of each row, one thread per dim: eight partials in flight at a time (slots
+// past the last repeat it with weight zero; one at a time, six splits took 2 us more than
+// eight).
 template <int D>
 __global__ __launch_bounds__(D) void kv4_combine_kernel(const float* __restrict__ ml,
                                                         const float* __restrict__ acc,
@@ -490,23 +524,53 @@ __global__ __launch_bounds__(D) void kv4_combine_kernel(const float* __restrict_
                                                         int nsplit) {
     const size_t row = blockIdx.x;
     const int d = threadIdx.x;
-    const float* r = ml + row * nsplit * 2;
-    float top = -INFINITY, sum = 0.f, a = 0.f;
-    for (int i = 0; i < nsplit; ++i) top = fmaxf(top, r[2 * i]);
-    const float use = top == -INFINITY ? 0.f : top;
-    for (int i = 0; i < nsplit; ++i) {
-        const float f = fast_exp2(r[2 * i] - use);
-        sum += r[2 * i + 1] * f;
-        a += acc[(row * nsplit + i) * D + d] * f;
+    const float2* r = reinterpret_cast<const float2*>(ml) + row * nsplit;
+    const float* x = acc + row * nsplit * D + d;
+    const int len = lens[blockIdx.x / Hq];
+    float m = -INFINITY, sum = 0.f, a = 0.f;
+    for (int i0 = 0; i0 < nsplit; i0 += 8) {
+        float2 s[8];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = min(i0 + k, nsplit - 1);
+            s[k] = r[i];
+            v[k] = x[(size_t)i * D];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
+        const float use = top == -INFINITY ? 0.f : top;
+        const float keep = fast_exp2(m - use);
+        sum *= keep;
+        a *= keep;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = i0 + k < nsplit ? fast_exp2(s[k].x - use) : 0.f;
+            // (a repeated slot must not turn an infinite partial into NaN)
+            sum += i0 + k < nsplit ? s[k].y * f : 0.f;
+            a += i0 + k < nsplit ? v[k] * f : 0.f;
+        }
+        m = top;
     }
-    out[row * D + d] = lens[blockIdx.x / Hq] > 0 ? __half_as_ushort(f16_of_f32(a / sum)) : (uint16_t)0;
+    out[row * D + d] = len > 0 ? __half_as_ushort(f16_of_f32(a / sum)) : (uint16_t)0;
 }
 
 struct Kv4Plan {
     int groups, rows, waves, nsplit;
-    size_t lds(int D) const { return (size_t)waves * (3 * kMaxRows + rows * (D + 4)) * 4; }
+    int max_split;  // most splits of any context: sizes the workspace
+    size_t lds(int D) const { return (size_t)waves * (2 * kMaxRows + rows * (D + 4)) * 4; }
 };
 
+// Waves per block and splits of a sequence with the least estimated time (0.01 us) for
+// sequences of max_context.  A wave takes 0.63 us per tile alone on its SIMD and 0.12 us per
+// wave resident on the CU where they share it (16: the rate of memory); a round of blocks
+// costs 2 us of first loads and merging, a second kernel 1 us, 0.05 per split and the partials' traffic.
+// Few blocks per CU end unevenly when the sequences differ in length (12% / blocks).
+// Estimated / measured, us: B32, 8 key heads of 128, 16K positions, 4 splits of 4 waves
+// 70 / 68, 8 of 4 72 / 72; B1 32K, 32 of 8 12 / 14, 16 of 8 16 / 16, one of 8 128 / 123; B8 8K,
+// 4 of 8 16 / 16; B64 2K, one of 4 22 / 22, 2 of 4 24 / 25; B64 300, one of 4 9.4 / 9.2, of 8
+// 10.3 / 10.3.
 Kv4Plan kv4_plan(int B, int Hq, int Hkv, int max_context) {
     Kv4Plan pl{};
     const int per_kv = Hq / Hkv;
@@ -515,10 +579,24 @@ Kv4Plan kv4_plan(int B, int Hq, int Hkv, int max_context) {
     pl.groups = (per_kv + pl.rows - 1) / pl.rows;
     const long long units = (long long)B * Hkv * pl.groups;
     const long long tiles = ceil_div(max_context, kTile);
-    pl.waves = 4;
-    pl.nsplit = (int)std::max<long long>(
-        1, std::min<long long>(ceil_div(2048, units), ceil_div(tiles, 8)));
-    if (tiles <= 32) pl.nsplit = 1, pl.waves = tiles <= 4 ? 4 : 8;
+    constexpr int kCus = 256, kResident = 16;  // waves per CU
+    pl.max_split = (int)std::min<long long>(64, std::max<long long>(1, 1024 / units));
+    pl.nsplit = 1, pl.waves = 4;
+    long long best = -1;
+    for (int s : {1, 2, 3, 4, 5, 6, 8, 11, 16, 24, 32, 48, 64}) {
+        if (s > pl.max_split || s > tiles) break;
+        for (int w : {4, 8}) {
+            const long long blocks = units * s;
+            const long long waves = ceil_div(blocks, kCus) * w;  // per CU
+            const long long resident = std::min<long long>(waves, kResident);
+            const long long rounds = ceil_div(waves, kResident);
+            const long long tile = std::max<long long>(63, 12 * resident);
+            long long time = rounds * (200 + ceil_div(ceil_div(tiles, s), w) * tile);
+            if (blocks >= kCus) time += time * 12 * kCus / (100 * blocks);
+            if (s > 1) time += 100 + 5 * s + blocks / 10;
+            if (best < 0 || time < best) best = time, pl.nsplit = s, pl.waves = w;
+        }
+    }
     return pl;
 }
 
@@ -539,9 +617,9 @@ void with_head_dim(int D, F&& f) {
 struct Kv4Partials {
     size_t ml_bytes, bytes;
 };
-Kv4Partials kv4_partials(int B, int Hq, const Kv4Plan& pl, int D) {
-    if (pl.nsplit == 1) return {0, 0};
-    const size_t parts = (size_t)B * Hq * pl.nsplit;
+Kv4Partials kv4_partials(int B, int Hq, int nsplit, int D) {
+    if (nsplit == 1) return {0, 0};
+    const size_t parts = (size_t)B * Hq * nsplit;
     const size_t ml = round_up(parts * 2 * sizeof(float), kWorkspaceAlign);
     return {ml, ml + round_up(parts * D * sizeof(float), kWorkspaceAlign)};
 }
@@ -625,7 +703,7 @@ extern "C" size_t int8k_decode_attention_kv4_paged_workspace_bytes(int B, int he
     if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    return kv4_partials(B, heads, kv4_plan(B, heads, kv_heads, max_context), head_dim).bytes;
+    return kv4_partials(B, heads, kv4_plan(B, heads, kv_heads, max_context).max_split, head_dim).bytes;
 }
 
 extern "C" int int8k_decode_attention_forward_kv4_paged(
@@ -649,19 +727,19 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
         return INT8K_ERR_MISALIGNED;
     if ((long long)B * heads >= (1LL << 22)) return INT8K_ERR_UNSUPPORTED;
     const Kv4Plan pl = kv4_plan(B, heads, kv_heads, max_context);
-    const Kv4Partials part = kv4_partials(B, heads, pl, head_dim);
+    const Kv4Partials part = kv4_partials(B, heads, pl.nsplit, head_dim);
     if (part.bytes > 0) {
         if (!workspace || workspace_bytes < part.bytes) return INT8K_ERR_WORKSPACE;
         if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
     }
-    const long long blocks = (long long)B * kv_heads * pl.groups * pl.nsplit;
+    const long long blocks = ceil_div((long long)B * pl.nsplit, 8) * 8 * kv_heads * pl.groups;
     if (blocks * pl.waves >= (1LL << 26)) return INT8K_ERR_UNSUPPORTED;  // work-items below 2^32
     Kv4Decode p{};
     p.Q = Q, p.K = K_pages, p.V = V_pages, p.sQ = scale_Q, p.sK = sK_pages, p.sV = sV_pages;
     p.tables = block_tables, p.lens = context_lens, p.out = out;
     p.part_ml = static_cast<float*>(workspace);
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + part.ml_bytes);
-    p.Hq = heads, p.Hkv = kv_heads, p.num_pages = num_pages, p.log2_page = log2_of(page_size);
+    p.B = B, p.Hq = heads, p.Hkv = kv_heads, p.num_pages = num_pages, p.log2_page = log2_of(page_size);
     p.max_pages = max_pages_per_seq, p.max_context = max_context;
     p.groups = pl.groups, p.rows = pl.rows, p.nsplit = pl.nsplit;
     p.qk = (1.0f / std::sqrt((float)head_dim)) * kLog2e;
@@ -672,7 +750,7 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
         st = once.run([] {
             const hipError_t e = hipFuncSetAttribute(
                 reinterpret_cast<const void*>(&kv4_decode_kernel<D>),
-                hipFuncAttributeMaxDynamicSharedMemorySize, 8 * (3 * kMaxRows + kMaxRows * (D + 4)) * 4);
+                hipFuncAttributeMaxDynamicSharedMemorySize, 8 * (2 * kMaxRows + kMaxRows * (D + 4)) * 4);
             if (e == hipSuccess) return (int)INT8K_OK;
             set_last_error("hipFuncSetAttribute", e);
             return (int)INT8K_ERR_HIP;
