@@ -3,37 +3,136 @@
 //   y[t, n] = T( (f32(acc) * sx[t]) * sw[n] (+ b[n]) ),  acc = sum_k x[t, k] w[k, n], exact int32
 //
 // x int8 [T, K]; w int8 [K, N] as stored, or [N, K] packed; y fp16, bf16 or fp32, rounded once
-// from the fp32 value.  The products run on the GEMM core of gemm_i8.h.
-#include "gemm_i8.h"
+// from the fp32 value.  The products run on the loops of the MLP's GEMMs (gemm_i8.h,
+// gemm_i8_paths.h); the routes differ in how the result leaves:
+//   skinny   32 x 32 tiles, K over the waves of a block (few tokens, small packed weights)
+//   stream   the weights streamed once over all CUs, exact int32 partials, then rows
+//   small    64 x 64 tiles, four blocks per CU
+//   mid      128 x 128 tiles, two blocks per CU; K split into partials where CUs would idle
+//   tiled    256 x 256 tiles
+// The tiles are computed transposed (SWAP), so a lane holds 4 adjacent columns of one row: 32
+// rows at a time go through the wave's own piece of LDS and leave as whole lines.
+#include "gemm_i8_paths.h"
 #include "rows.h"
 
 namespace int8k {
 namespace {
 
-using namespace gemm;
-
 struct LinearArgs {
     const int8_t *x, *w;
     void* y;
+    int32_t* part;  // [splits][M][N]
     const float *sx, *sw, *bias;
     int sx_stride, sw_stride;  // 0: one scale for all
     int M, N, K;
 };
 
 template <int DT>
-__device__ __forceinline__ void store_value(void* y, size_t i, float v) {
-    if constexpr (DT == INT8K_DTYPE_F32) {
-        static_cast<float*>(y)[i] = v;
-    } else if constexpr (DT == INT8K_DTYPE_F16) {
-        static_cast<uint16_t*>(y)[i] = __half_as_ushort(f16_of_f32(v));
+constexpr int kOutBytes = DT == INT8K_DTYPE_F32 ? 4 : 2;
+
+// The value of a sum; the same expression on every route.
+__device__ __forceinline__ float linear_value(int acc, float sx, float sw, float b) {
+    return static_cast<float>(acc) * sx * sw + b;
+}
+
+// Two values as numbers of a 16-bit dtype.
+template <int DT>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    if constexpr (DT == INT8K_DTYPE_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
     } else {
-        const uint32_t u = __float_as_uint(v);
-        static_cast<uint16_t*>(y)[i] =
-            (uint16_t)(v != v ? (u >> 16) | 0x40u : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
     }
 }
 
-// 256 x 256 tiles.
+// 4 consecutive values to dst (8 or 16 bytes).
+template <int DT>
+__device__ __forceinline__ void store_four(void* dst, const float (&v)[4]) {
+    if constexpr (DT == INT8K_DTYPE_F32)
+        *static_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+        *static_cast<uint2*>(dst) = make_uint2(pack_pair<DT>(v[0], v[1]), pack_pair<DT>(v[2], v[3]));
+}
+
+// The row and column scales and the bias of a tile of B x B outputs, loaded before the main
+// loop (clamped, unconditional) by threads t < B and parked in LDS behind it.
+struct TileScales {
+    float sx, sw, b;
+};
+template <int B>
+__device__ __forceinline__ TileScales load_scales(const LinearArgs& p, int m0, int n0) {
+    const int t = threadIdx.x & (B - 1);
+    TileScales s;
+    s.sx = p.sx[(size_t)min(m0 + t, p.M - 1) * p.sx_stride];
+    s.sw = p.sw[(size_t)min(n0 + t, p.N - 1) * p.sw_stride];
+    s.b = p.bias != nullptr ? p.bias[min(n0 + t, p.N - 1)] : 0.f;
+    return s;
+}
+
+// The outputs of a wave's (32 TM_) x (32 TN_) sub-tile at (row0, col0) of the matrix, (rl, cl)
+// of the tile.  stage: this wave's LDS, 32 rows of kEpiRow bytes; scales: [sx B][sw B][bias B].
+template <int DT, int TN_>
+constexpr int kEpiRow = TN_ * 32 * kOutBytes<DT> + 16;
+template <int DT, int TM_, int TN_, int B>
+__device__ __forceinline__ void epilogue_rows(const v16i (&acc)[TM_][TN_], const LinearArgs& p,
+                                              int m0, int n0, int rl, int cl, char* stage,
+                                              const float* scales) {
+    constexpr int E = kOutBytes<DT>, kRow = kEpiRow<DT, TN_>;
+    constexpr int kLanes = TN_ * 32 * E / 16;  // 16-byte pieces of a row
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const float* ssw = scales + B + cl + 4 * half;
+    const float* sb = ssw + B;
+    const int piece = lane % kLanes, first = lane / kLanes;
+    const int col = n0 + cl + piece * (16 / E);
+#pragma unroll
+    for (int i = 0; i < TM_; ++i) {
+        const float sx = scales[rl + 32 * i + (lane & 31)];
+        char* mine = stage + (lane & 31) * kRow + 4 * half * E;
+#pragma unroll
+        for (int j = 0; j < TN_; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 w4 = *reinterpret_cast<const float4*>(ssw + 32 * j + 8 * q);
+                const float4 b4 = *reinterpret_cast<const float4*>(sb + 32 * j + 8 * q);
+                const float v[4] = {linear_value(acc[i][j][4 * q], sx, w4.x, b4.x),
+                                    linear_value(acc[i][j][4 * q + 1], sx, w4.y, b4.y),
+                                    linear_value(acc[i][j][4 * q + 2], sx, w4.z, b4.z),
+                                    linear_value(acc[i][j][4 * q + 3], sx, w4.w, b4.w)};
+                store_four<DT>(mine + (32 * j + 8 * q) * E, v);
+            }
+        // lanes read what other lanes of the wave wrote (its LDS operations complete in order)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += 64 / kLanes) {
+            const int row = m0 + rl + 32 * i + r + first;
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + (r + first) * kRow + piece * 16);
+            // N is a multiple of 16: a piece is wholly in or out
+            if (row < p.M && col < p.N)
+                *reinterpret_cast<uint4*>(static_cast<char*>(p.y) + ((size_t)row * p.N + col) * E) = w;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int B>
+__device__ __forceinline__ void park_scales(const TileScales& s, float* scales) {
+    if (B == kThreads || (int)threadIdx.x < B) {
+        scales[threadIdx.x] = s.sx;
+        scales[B + threadIdx.x] = s.sw;
+        scales[2 * B + threadIdx.x] = s.b;
+    }
+    __syncthreads();  // every wave is done with the operand stages, too
+}
+
+// ------------------------------------------------------------------ 256 x 256 tiles
+constexpr int kTiledLds = LDS_BYTES + 3 * BM * 4;
+
 template <int DT, bool BKN>
 __global__ __launch_bounds__(kThreads, 1) void linear_tiled_kernel(LinearArgs p, int tiles_m,
                                                                    int tiles_n) {
@@ -41,49 +140,447 @@ __global__ __launch_bounds__(kThreads, 1) void linear_tiled_kernel(LinearArgs p,
     int tm, tn;
     tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
+    const TileScales s = load_scales<BM>(p, m0, n0);
     v16i acc[TM][TN];
     const int ldb = BKN ? p.N : p.K;
     if (m0 + BM <= p.M && n0 + BN <= p.N && p.K % BK == 0)
-        mainloop<false, false, BKN>(acc, p.x, p.w, p.M, p.N, p.K, p.K, ldb, m0, n0, lds);
+        mainloop<false, true, BKN>(acc, p.x, p.w, p.M, p.N, p.K, p.K, ldb, m0, n0, lds);
     else
-        mainloop<true, false, BKN>(acc, p.x, p.w, p.M, p.N, p.K, p.K, ldb, m0, n0, lds);
+        mainloop<true, true, BKN>(acc, p.x, p.w, p.M, p.N, p.K, p.K, ldb, m0, n0, lds);
+    float* scales = reinterpret_cast<float*>(lds + LDS_BYTES);
+    park_scales<BM>(s, scales);
+    const int wave = threadIdx.x >> 6;
+    static_assert(4 * 32 * kEpiRow<INT8K_DTYPE_F32, TN> <= LDS_BYTES, "the waves' pieces fit");
+    epilogue_rows<DT, TM, TN, BM>(acc, p, m0, n0, (wave >> 1) * WM, (wave & 1) * WN,
+                                  lds + wave * 32 * kEpiRow<DT, TN>, scales);
+}
+
+// ------------------------------------------------------------------ 128 x 128 tiles
+template <bool BKN>
+constexpr int kMidScales = 2 * MidLds<BKN>::kStage;
+static_assert(4 * 32 * kEpiRow<INT8K_DTYPE_F32, kMidT> <= 2 * MidLds<false>::kStage, "fits");
+
+template <int DT, bool BKN>
+__global__ __launch_bounds__(kThreads, 2) void linear_mid_kernel(LinearArgs p, int tiles_m,
+                                                                 int tiles_n) {
+    extern __shared__ __align__(16) char lds[];
+    int tm, tn;
+    tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * kMidB, n0 = tn * kMidB;
+    const TileScales s = load_scales<kMidB>(p, m0, n0);
+    v16i acc[kMidT][kMidT];
+    if (m0 + kMidB <= p.M && n0 + kMidB <= p.N && p.K % BK == 0)
+        mid_mainloop<false, BKN, true>(acc, p.x, p.w, p.M, p.N, p.K, 0, p.K, m0, n0, lds);
+    else
+        mid_mainloop<true, BKN, true>(acc, p.x, p.w, p.M, p.N, p.K, 0, p.K, m0, n0, lds);
+    float* scales = reinterpret_cast<float*>(lds + kMidScales<BKN>);
+    park_scales<kMidB>(s, scales);
+    const int wave = threadIdx.x >> 6;
+    epilogue_rows<DT, kMidT, kMidT, kMidB>(acc, p, m0, n0, (wave >> 1) * kMidW,
+                                           (wave & 1) * kMidW, lds + wave * 32 * kEpiRow<DT, kMidT>,
+                                           scales);
+}
+
+// A K range per blockIdx.y, exact int32 partials.
+template <bool BKN>
+__global__ __launch_bounds__(kThreads, 2) void linear_mid_split_kernel(LinearArgs p, int tiles_m,
+                                                                       int tiles_n,
+                                                                       int k_per_split) {
+    extern __shared__ __align__(16) char lds[];
+    int tm, tn;
+    tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * kMidB, n0 = tn * kMidB;
+    const int kb = (int)blockIdx.y * k_per_split, ke = min(p.K - kb, k_per_split) + kb;
+    v16i acc[kMidT][kMidT];
+    if (m0 + kMidB <= p.M && n0 + kMidB <= p.N && (ke - kb) % BK == 0)
+        mid_mainloop<false, BKN, true>(acc, p.x, p.w, p.M, p.N, p.K, kb, ke, m0, n0, lds);
+    else
+        mid_mainloop<true, BKN, true>(acc, p.x, p.w, p.M, p.N, p.K, kb, ke, m0, n0, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int rbase = m0 + (wave >> 1) * WM, cbase = n0 + (wave & 1) * WN + (lane & 31);
+    const int row0 = m0 + (wave >> 1) * kMidW + (lane & 31);
+    const int col0 = n0 + (wave & 1) * kMidW + 4 * (lane >> 5);
+    int32_t* c = p.part + (size_t)blockIdx.y * p.M * p.N;
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int col = cbase + j * 32;
-        if (col >= p.N) continue;
-        const float sb = p.sw[(size_t)col * p.sw_stride];
-        const float bi = p.bias != nullptr ? p.bias[col] : 0.f;
+    for (int i = 0; i < kMidT; ++i) {
+        const int row = row0 + 32 * i;
+        if (row >= p.M) continue;
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int j = 0; j < kMidT; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = rbase + i * 32 + acc_row(r, lane);
-                if (row >= p.M) continue;
-                const float v = static_cast<float>(acc[i][j][r]) * p.sx[(size_t)row * p.sx_stride] * sb + bi;
-                store_value<DT>(p.y, (size_t)row * p.N + col, v);
+            for (int q = 0; q < 4; ++q) {
+                const int col = col0 + 32 * j + 8 * q;
+                if (col < p.N)
+                    *reinterpret_cast<v4i*>(c + (size_t)row * p.N + col) =
+                        v4i{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                            acc[i][j][4 * q + 3]};
             }
     }
 }
 
-template <int DT, bool BKN>
-int launch_linear_tiled(const LinearArgs& p, hipStream_t stream) {
-    static PerDeviceOnce lds_once;
-    const int st = lds_once.run([] {
-        const hipError_t e = hipFuncSetAttribute(
-            reinterpret_cast<const void*>(&linear_tiled_kernel<DT, BKN>),
-            hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES);
-        if (e != hipSuccess) {
-            set_last_error("hipFuncSetAttribute", e);
-            return (int)INT8K_ERR_HIP;
+// ------------------------------------------------------------------ 64 x 64 tiles
+// 64 x 64 tiles for the sizes between: a wave owns 32 x 32 and a block 37 KiB of LDS, so four
+// blocks share a CU and hide each other's barriers and LDS round trips.  A 128 x 128 tile alone
+// on its CU takes 0.70-0.86 us a step, bound by those (loading its operands a step earlier
+// changed nothing).  Operands are loaded two steps ahead into registers.
+constexpr int kSmB = 64;
+template <bool BKN>
+struct SmallLds {
+    // rows of a [K][N] stage lie 96 bytes apart: the 8 rows of a transposing read start 32
+    // bytes apart in the banks
+    static constexpr int kBStride = BKN ? kSmB + 32 : LDS_STRIDE;
+    static constexpr int kA = kSmB * LDS_STRIDE;
+    static constexpr int kStage = kA + (BKN ? BK : kSmB) * kBStride;
+    static constexpr int kScales = 2 * kStage;
+    static constexpr int kBytes = kScales + 3 * kSmB * 4;
+};
+
+template <bool EDGE, bool BKN>
+__device__ __forceinline__ void small_mainloop(v16i& acc, const LinearArgs& p, int kb, int ke,
+                                               int m0, int n0, char* lds) {
+    using L = SmallLds<BKN>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0;
+    const int nk = (ke - kb + BK - 1) / BK;
+    const int a_off = (wm * 32 + (lane & 31)) * LDS_STRIDE + (lane >> 5) * 16;
+    const int g16 = lane >> 4, s16 = lane & 15;
+    const int b_off = L::kA + (BKN ? (16 * (g16 >> 1) + (s16 >> 1)) * L::kBStride + wn * 32 +
+                                         16 * (g16 & 1) + 8 * (s16 & 1)
+                                   : (wn * 32 + (lane & 31)) * L::kBStride + (lane >> 5) * 16);
+    struct Step {
+        int4 a[2], b[2];
+    };
+    Step f0, f1;  // even and odd steps on their way
+    // A (and a packed B): chunk c = t + 256 i, row c / 8, bytes (c % 8) * 16 of the step; B as
+    // stored: k row c / 4, bytes (c % 4) * 16 of the tile's 64 columns.  Chunks past the matrix
+    // load clamped addresses and are zeroed on EDGE.
+    auto load = [&](Step& f, int kt) {
+        const int k0 = kb + kt * BK;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = threadIdx.x + i * kThreads;
+            const int row = c / kChunksPerRow, gk = min(k0 + (c % kChunksPerRow) * 16, p.K - 16);
+            f.a[i] = *reinterpret_cast<const int4*>(p.x + (size_t)min(m0 + row, p.M - 1) * p.K + gk);
+            if constexpr (BKN)
+                f.b[i] = *reinterpret_cast<const int4*>(
+                    p.w + (size_t)min(k0 + (c >> 2), p.K - 1) * p.N + min(n0 + (c & 3) * 16, p.N - 16));
+            else
+                f.b[i] = *reinterpret_cast<const int4*>(p.w + (size_t)min(n0 + row, p.N - 1) * p.K + gk);
         }
-        return (int)INT8K_OK;
+    };
+    auto store = [&](const Step& f, char* stage, int kt) {
+        const int k0 = kb + kt * BK;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = threadIdx.x + i * kThreads;
+            const int row = c / kChunksPerRow, kc = (c % kChunksPerRow) * 16;
+            const int br = BKN ? c >> 2 : row, bc = BKN ? (c & 3) * 16 : kc;
+            int4 va = f.a[i], vb = f.b[i];
+            if constexpr (EDGE) {
+                if (!(k0 + kc < ke && m0 + row < p.M)) va = make_int4(0, 0, 0, 0);
+                const bool bok = BKN ? k0 + br < ke && n0 + bc < p.N : k0 + bc < ke && n0 + br < p.N;
+                if (!bok) vb = make_int4(0, 0, 0, 0);
+            }
+            *reinterpret_cast<int4*>(stage + row * LDS_STRIDE + kc) = va;
+            *reinterpret_cast<int4*>(stage + L::kA + br * L::kBStride + bc) = vb;
+        }
+    };
+    auto read = [&](v4i& a, v4i& b, const char* stage, int s) {
+        a = *reinterpret_cast<const v4i*>(stage + a_off + s * 32);
+        if constexpr (BKN) {
+            typedef int v2i __attribute__((ext_vector_type(2)));
+            typedef __attribute__((address_space(3))) v2i lds_v2i;
+            const char* q = stage + b_off + s * 32 * L::kBStride;
+            const v2i lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(q));
+            const v2i hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(q + 8 * L::kBStride));
+            b = v4i{lo.x, lo.y, hi.x, hi.y};
+        } else {
+            b = *reinterpret_cast<const v4i*>(stage + b_off + s * 32);
+        }
+    };
+    // Step kt reads buffer kt & 1; f holds step kt + 1, which goes to the other buffer (its last
+    // reads, step kt - 1's, finished before that step's barrier) and is refilled with step
+    // kt + 3.  Loads past the end of K repeat its last bytes and are not used.
+    auto step = [&](Step& f, int kt) {
+        const char* cur = lds + (kt & 1) * L::kStage;
+        v4i a[4], b[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) read(a[s], b[s], cur, s);
+        store(f, lds + ((kt + 1) & 1) * L::kStage, kt + 1);
+        load(f, kt + 3);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc = mfma_ab<true>(a[s], b[s], acc);
+        __syncthreads();
+    };
+    load(f0, 0);
+    load(f1, 1);
+    store(f0, lds, 0);
+    load(f0, 2);
+    __syncthreads();
+    for (int kt = 0; kt < nk; kt += 2) {
+        step(f1, kt);
+        if (kt + 1 >= nk) break;
+        step(f0, kt + 1);
+    }
+}
+
+static_assert(4 * 32 * kEpiRow<INT8K_DTYPE_F32, 1> <= 2 * SmallLds<false>::kStage, "fits");
+
+template <int DT, bool BKN>
+__global__ __launch_bounds__(kThreads, 4) void linear_small_kernel(LinearArgs p, int tiles_m,
+                                                                   int tiles_n) {
+    extern __shared__ __align__(16) char lds[];
+    int tm, tn;
+    tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * kSmB, n0 = tn * kSmB;
+    const TileScales s = load_scales<kSmB>(p, m0, n0);
+    v16i acc[1][1];
+    if (m0 + kSmB <= p.M && n0 + kSmB <= p.N && p.K % BK == 0)
+        small_mainloop<false, BKN>(acc[0][0], p, 0, p.K, m0, n0, lds);
+    else
+        small_mainloop<true, BKN>(acc[0][0], p, 0, p.K, m0, n0, lds);
+    float* scales = reinterpret_cast<float*>(lds + SmallLds<BKN>::kScales);
+    park_scales<kSmB>(s, scales);
+    const int wave = threadIdx.x >> 6;
+    epilogue_rows<DT, 1, 1, kSmB>(acc, p, m0, n0, (wave >> 1) * 32, (wave & 1) * 32,
+                                  lds + wave * 32 * kEpiRow<DT, 1>, scales);
+}
+
+// ------------------------------------------------------------------ partials to rows
+// 4 columns per thread: the splits' sums, eight loads in flight, then the value.
+template <int DT>
+__global__ __launch_bounds__(256) void linear_rows_kernel(LinearArgs p, int splits) {
+    const int groups = p.N / 4;
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= (long long)p.M * groups) return;
+    const int row = (int)(e / groups), n = 4 * (int)(e - (long long)row * groups);
+    const float sx = p.sx[(size_t)row * p.sx_stride];
+    float sw[4], b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        sw[k] = p.sw[(size_t)(n + k) * p.sw_stride];
+        b[k] = p.bias != nullptr ? p.bias[n + k] : 0.f;
+    }
+    const int32_t* src = p.part + (size_t)row * p.N + n;
+    const size_t plane = (size_t)p.M * p.N;
+    v4i sum = {0, 0, 0, 0};
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+        v4i x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            x[k] = *reinterpret_cast<const v4i*>(src + min(s0 + k, splits - 1) * plane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (s0 + k < splits) sum += x[k];
+    }
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = linear_value(sum[k], sx, sw[k], b[k]);
+    store_four<DT>(static_cast<char*>(p.y) + ((size_t)row * p.N + n) * kOutBytes<DT>, v);
+}
+
+// ------------------------------------------------------------------ few tokens, small weights
+// A block owns a 32 x 32 output tile; its 8 waves take every 8th 128-deep step of K
+// straight from global memory (packed weights), two steps in flight, and meet in LDS.
+constexpr int kSkinnyWaves = 8;  // (4 and 16: 2-10% slower from T = 1 to 512)
+
+template <int DT>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void linear_skinny_kernel(LinearArgs p) {
+    constexpr int kCol = 36, nw = kSkinnyWaves;
+    __shared__ __align__(16) int part[nw * 32 * kCol];  // [wave][32 columns][32 rows + 4]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32;
+    const size_t koff = (size_t)(lane >> 5) * 16;
+    const int8_t* arow = p.x + (size_t)min(m0 + (lane & 31), p.M - 1) * p.K + koff;
+    const int8_t* brow = p.w + (size_t)min(n0 + (lane & 31), p.N - 1) * p.K + koff;
+    v16i acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0;
+    const int step = 128 * nw;
+    v4i b0[4], a0[4], b1[4], a1[4];
+    int k = 128 * wave;
+    if (k < p.K) skinny_load(b0, a0, arow, brow, k);
+    for (; k < p.K; k += 2 * step) {
+        if (k + step < p.K) skinny_load(b1, a1, arow, brow, k + step);
+        skinny_mfma(acc, b0, a0);
+        if (k + step >= p.K) break;
+        if (k + 2 * step < p.K) skinny_load(b0, a0, arow, brow, k + 2 * step);
+        skinny_mfma(acc, b1, a1);
+    }
+    // lane: column lane % 32, rows 8 q + 4 (lane / 32) ..
+    int* mine = part + (wave * 32 + (lane & 31)) * kCol + 4 * (lane >> 5);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<v4i*>(mine + 8 * q) =
+            v4i{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    __syncthreads();
+    // 4 columns of a row per thread
+    for (int e = threadIdx.x; e < 256; e += blockDim.x) {
+        const int row = e >> 3, c = (e & 7) * 4;
+        const int m = m0 + row, n = n0 + c;
+        if (m >= p.M || n >= p.N) continue;
+        const float sx = p.sx[(size_t)m * p.sx_stride];
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < nw; ++w) sum += part[(w * 32 + c + i) * kCol + row];
+            v[i] = linear_value(sum, sx, p.sw[(size_t)(n + i) * p.sw_stride],
+                                p.bias != nullptr ? p.bias[n + i] : 0.f);
+        }
+        store_four<DT>(static_cast<char*>(p.y) + ((size_t)m * p.N + n) * kOutBytes<DT>, v);
+    }
+}
+
+// ------------------------------------------------------------------ plan, launch
+
+enum class LinearRoute { kSkinny, kStream, kSmall, kMid, kTiled };
+
+struct LinearPlan {
+    LinearRoute route;
+    StreamPlan st;
+    MidPlan mid;
+    int splits;      // int32 partials, 0: none
+    size_t bytes(int M, int N) const { return (size_t)splits * M * N * 4; }
+};
+
+// The route with the least estimated time (0.01 us; `steps` of 128 deep).  Fits of each route
+// timed at T = 1 .. 4096 and 512 -> 768 .. 4096 -> 6144, estimated / measured (us):
+//  - skinny: 3 us and, per 1024 of K and round of 256 blocks, 1.85 us, less for few rows, whose
+//    lanes load the same lines (T = 1, 1024 -> 1024 4.2 / 3.8; T = 32, 4096 -> 4096 10.4 / 10.3;
+//    T = 128, 2048 -> 2560 10.4 / 10.5; T = 512, 1024 -> 1024 6.7 / 6.8);
+//  - stream: a read of the weights per 32 or 64 rows behind a start and a second kernel (T = 1,
+//    4096 -> 6144 9.8 / 9.6; T = 64 14.6 / 14.6);
+//  - small: 0.34 us a step to 256 blocks, 0.24 per 256 beyond (T = 333, 2048 -> 2560 8.4 / 8.9,
+//    16.6 on 128 x 128 tiles; T = 512, 4096 -> 4096 18.4 / 18.7, 24.6; T = 1000 33.7 / 34.1, 30.8);
+//  - mid: 0.78 us a step for a block alone on its CU, 1.33 for two; split over K, the partials'
+//    traffic and a second kernel (T = 512, 4096 -> 4096 27.5 / 24.6; T = 128, 4096 -> 6144 in 4
+//    splits 16.3 / 16.2);
+//  - tiled: 1.25 us a step and round, 0.55 more where the grid fills the GPU and the clock
+//    falls with the power (T = 4096, 4096 -> 4096 67 / 66, 4096 -> 6144 115 / 112).
+LinearPlan linear_plan(int M, int K, int N, bool packed) {
+    LinearPlan pl{};
+    const long long steps = ceil_div(K, BK);
+    long long best = -1;
+    auto better = [&](long long time, LinearRoute route) {
+        if (best >= 0 && time >= best) return false;
+        best = time, pl.route = route, pl.splits = 0;
+        return true;
+    };
+    {
+        const long long tiles = ceil_div(M, BM) * ceil_div(N, BN), rounds = ceil_div(tiles, 256);
+        better(900 + steps * (125 * rounds + 55 * tiles / 256), LinearRoute::kTiled);
+    }
+    const long long mid_tiles = ceil_div(M, kMidB) * ceil_div(N, kMidB);
+    for (long long sp = 1; sp <= std::min(16LL, steps); ++sp) {
+        const long long st = ceil_div(steps, sp), n = ceil_div(steps, st);
+        if (n != sp) continue;  // the same plan as fewer splits
+        const long long blocks = mid_tiles * n, rest = blocks % 512;
+        const long long gemm = st * (133 * (blocks / 512) + (rest > 256 ? 133 : rest > 0 ? 78 : 0));
+        const long long rows = n > 1 ? 200 + 8 * n * (long long)M * N / 45000 : 0;
+        if (better(250 + gemm + rows + (long long)N * K / 100000, LinearRoute::kMid)) {
+            pl.mid = MidPlan{(int)ceil_div(M, kMidB), (int)ceil_div(N, kMidB), (int)n, (int)(st * BK)};
+            pl.splits = n > 1 ? (int)n : 0;
+        }
+    }
+    {
+        const long long rounds = ceil_div(ceil_div(M, kSmB) * ceil_div(N, kSmB), 256);
+        better(300 + steps * (rounds == 1 ? 34 : 24 * rounds), LinearRoute::kSmall);
+    }
+    const long long nk = (long long)N * K;
+    if (M <= 512) {
+        const StreamPlan sp = stream_plan(M, N, K);
+        if (better(sp.mt == 1 ? 650 + nk * 13 / 1000000 : 930 + nk * 21 / 1000000 * sp.tiles_m,
+                   LinearRoute::kStream)) {
+            pl.st = sp;
+            pl.splits = sp.splits;
+        }
+    }
+    if (packed && K % 128 == 0) {
+        const long long rounds = ceil_div(ceil_div(N, 32) * ceil_div(M, 32), 256);
+        better(300 + (115 + 22 * std::min(M, 32) / 10) * rounds * K / 1024, LinearRoute::kSkinny);
+    }
+    return pl;
+}
+
+int set_lds(PerDeviceOnce& once, const void* kernel, int bytes) {
+    return once.run([=] {
+        const hipError_t e =
+            hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess) return (int)INT8K_OK;
+        set_last_error("hipFuncSetAttribute", e);
+        return (int)INT8K_ERR_HIP;
     });
-    if (st != INT8K_OK) return st;
-    const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
-    linear_tiled_kernel<DT, BKN><<<tiles_m * tiles_n, kThreads, LDS_BYTES, stream>>>(p, tiles_m, tiles_n);
-    return check_launch("linear_tiled_kernel");
+}
+
+template <int DT>
+int launch_rows(const LinearArgs& p, int splits, hipStream_t stream) {
+    const long long threads = (long long)p.M * (p.N / 4);
+    linear_rows_kernel<DT><<<(unsigned)ceil_div(threads, 256), 256, 0, stream>>>(p, splits);
+    return check_launch("linear_rows_kernel");
+}
+
+template <int DT, bool BKN>
+int launch_linear(const LinearArgs& p, const LinearPlan& pl, hipStream_t stream) {
+    switch (pl.route) {
+        case LinearRoute::kSkinny: {
+            const dim3 grid((unsigned)ceil_div(p.N, 32), (unsigned)ceil_div(p.M, 32));
+            linear_skinny_kernel<DT><<<grid, 64 * kSkinnyWaves, 0, stream>>>(p);
+            return check_launch("linear_skinny_kernel");
+        }
+        case LinearRoute::kStream: {
+            static PerDeviceOnce once1, once2;
+            constexpr int kMax = kStMaxWaves * StreamTile<BKN>::kBytes;
+            if (const int st = pl.st.mt == 1
+                                   ? set_lds(once1, (const void*)gemm_i8_stream_kernel<1, BKN>, kMax)
+                                   : set_lds(once2, (const void*)gemm_i8_stream_kernel<2, BKN>, kMax))
+                return st;
+            if (const int st = launch_gemm_stream<BKN>(p.x, p.w, p.M, p.N, p.K, pl.st, p.part, stream))
+                return st;
+            return launch_rows<DT>(p, pl.splits, stream);
+        }
+        case LinearRoute::kSmall: {
+            static PerDeviceOnce once;
+            const int tiles_m = (int)ceil_div(p.M, kSmB), tiles_n = (int)ceil_div(p.N, kSmB);
+            if (const int st = set_lds(once, (const void*)linear_small_kernel<DT, BKN>,
+                                       SmallLds<BKN>::kBytes))
+                return st;
+            linear_small_kernel<DT, BKN>
+                <<<tiles_m * tiles_n, kThreads, SmallLds<BKN>::kBytes, stream>>>(p, tiles_m, tiles_n);
+            return check_launch("linear_small_kernel");
+        }
+        case LinearRoute::kMid: {
+            static PerDeviceOnce once, once_split;
+            const int tiles = pl.mid.tiles_m * pl.mid.tiles_n;
+            if (pl.splits > 0) {
+                if (const int st = set_lds(once_split, (const void*)linear_mid_split_kernel<BKN>,
+                                           MidLds<BKN>::kBytes))
+                    return st;
+                linear_mid_split_kernel<BKN>
+                    <<<dim3(tiles, pl.splits), kThreads, MidLds<BKN>::kBytes, stream>>>(
+                        p, pl.mid.tiles_m, pl.mid.tiles_n, pl.mid.k_per_split);
+                if (const int st = check_launch("linear_mid_split_kernel")) return st;
+                return launch_rows<DT>(p, pl.splits, stream);
+            }
+            if (const int st = set_lds(once, (const void*)linear_mid_kernel<DT, BKN>,
+                                       MidLds<BKN>::kBytes))
+                return st;
+            linear_mid_kernel<DT, BKN><<<tiles, kThreads, MidLds<BKN>::kBytes, stream>>>(
+                p, pl.mid.tiles_m, pl.mid.tiles_n);
+            return check_launch("linear_mid_kernel");
+        }
+        default: {
+            static PerDeviceOnce once;
+            if (const int st = set_lds(once, (const void*)linear_tiled_kernel<DT, BKN>, kTiledLds))
+                return st;
+            const int tiles_m = (int)ceil_div(p.M, BM), tiles_n = (int)ceil_div(p.N, BN);
+            linear_tiled_kernel<DT, BKN>
+                <<<tiles_m * tiles_n, kThreads, kTiledLds, stream>>>(p, tiles_m, tiles_n);
+            return check_launch("linear_tiled_kernel");
+        }
+    }
 }
 
 // |x w| <= 2^14 and K products: below 2^17 of them the int32 sum cannot overflow.
@@ -94,9 +591,17 @@ constexpr int kMaxK = (1 << 17) - 16;
 
 using namespace int8k;
 
+static bool linear_shape_ok(int T, int K, int N) {
+    return T > 0 && K > 0 && N > 0 && K % 16 == 0 && N % 16 == 0 && K <= kMaxK &&
+           // operands are read through 32-bit buffer offsets
+           (long long)T * K < (1LL << 32) && (long long)N * K < (1LL << 32) &&
+           ceil_div(T, kMidB) * ceil_div(N, kMidB) < (1LL << 22) &&
+           (long long)T * N < (1LL << 36);
+}
+
 extern "C" size_t int8k_linear_workspace_bytes(int T, int K, int N, int flags) {
-    (void)T, (void)K, (void)N, (void)flags;
-    return 0;
+    if (!linear_shape_ok(T, K, N)) return 0;
+    return linear_plan(T, K, N, (flags & INT8K_LINEAR_WEIGHT_PREPACKED) != 0).bytes(T, N);
 }
 
 extern "C" int int8k_linear(const int8_t* x, const int8_t* W, void* out, int dtype,
@@ -110,23 +615,23 @@ extern "C" int int8k_linear(const int8_t* x, const int8_t* W, void* out, int dty
         return INT8K_ERR_INVALID_ARGUMENT;
     if ((n_scale_x != 1 && n_scale_x != T) || (n_scale_W != 1 && n_scale_W != N))
         return INT8K_ERR_INVALID_ARGUMENT;
-    if (K % 16 || N % 16 || K > kMaxK) return INT8K_ERR_UNSUPPORTED;
-    // operands are read through 32-bit buffer offsets
-    if ((long long)T * K >= (1LL << 32) || (long long)N * K >= (1LL << 32))
-        return INT8K_ERR_UNSUPPORTED;
-    if (ceil_div(T, BM) * ceil_div(N, BN) >= (1LL << 24)) return INT8K_ERR_UNSUPPORTED;
+    if (!linear_shape_ok(T, K, N)) return INT8K_ERR_UNSUPPORTED;
     if (!aligned_to(x, 16) || !aligned_to(W, 16) || !aligned_to(out, 16) ||
         !aligned_to(scale_x, 4) || !aligned_to(scale_W, 4) || !aligned_to(bias, 4))
         return INT8K_ERR_MISALIGNED;
-    (void)workspace, (void)workspace_bytes;
-    const LinearArgs p{x, W, out, scale_x, scale_W, bias, n_scale_x == 1 ? 0 : 1,
-                       n_scale_W == 1 ? 0 : 1, T, N, K};
     const bool packed = (flags & INT8K_LINEAR_WEIGHT_PREPACKED) != 0;
+    const LinearPlan pl = linear_plan(T, K, N, packed);
+    if (const size_t need = pl.bytes(T, N)) {
+        if (!workspace || workspace_bytes < need) return INT8K_ERR_WORKSPACE;
+        if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
+    }
+    const LinearArgs p{x, W, out, static_cast<int32_t*>(workspace), scale_x, scale_W, bias,
+                       n_scale_x == 1 ? 0 : 1, n_scale_W == 1 ? 0 : 1, T, N, K};
     int st = INT8K_OK;
     with_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        st = packed ? launch_linear_tiled<DT, false>(p, as_stream(stream))
-                    : launch_linear_tiled<DT, true>(p, as_stream(stream));
+        st = packed ? launch_linear<DT, false>(p, pl, as_stream(stream))
+                    : launch_linear<DT, true>(p, pl, as_stream(stream));
     });
     return st;
 }
