@@ -60,16 +60,35 @@ __device__ __forceinline__ float load_one(const void* x, size_t i) {
     return __uint_as_float((uint32_t)u << 16);
 }
 
-// v as a number of the dtype (round to nearest even).
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+
+// Two values rounded to numbers of a 16-bit dtype (to nearest even), packed.
 template <int DT>
-__device__ __forceinline__ float round_to(float v) {
-    if constexpr (DT == INT8K_DTYPE_F16) return __half2float(f16_of_f32(v));
-    if constexpr (DT == INT8K_DTYPE_BF16) {
-        const uint32_t u = __float_as_uint(v);
-        const uint32_t r = u + 0x7fffu + ((u >> 16) & 1u);
-        return __uint_as_float((v != v ? u | 0x400000u : r) & 0xffff0000u);
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    if constexpr (DT == INT8K_DTYPE_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
+    } else {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
     }
-    return v;
+}
+
+// Values as numbers of the dtype.
+template <int DT>
+__device__ __forceinline__ void round_all(float (&v)[8]) {
+    if constexpr (DT == INT8K_DTYPE_F32) return;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint32_t w = pack_pair<DT>(v[i], v[i + 1]);
+        if constexpr (DT == INT8K_DTYPE_F16) {
+            v[i] = __half2float(__ushort_as_half((unsigned short)(w & 0xffffu)));
+            v[i + 1] = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+        } else {
+            v[i] = __uint_as_float(w << 16);
+            v[i + 1] = __uint_as_float(w & 0xffff0000u);
+        }
+    }
 }
 
 template <int DT>
@@ -80,16 +99,31 @@ __device__ __forceinline__ void store_one(void* y, size_t i, float v) {
     else static_cast<uint16_t*>(y)[i] = (uint16_t)(__float_as_uint(v) >> 16);
 }
 
-// 8 consecutive elements.
+// 8 consecutive elements as loaded.
 template <int DT>
-__device__ __forceinline__ void load8(const void* x, size_t i, float (&v)[8]) {
+struct Raw8 {
+    uint4 w[DT == INT8K_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const void* x, size_t i) {
+    Raw8<DT> r;
     if constexpr (DT == INT8K_DTYPE_F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
-        const float4 a = p[0], b = p[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + i);
+        r.w[0] = p[0], r.w[1] = p[1];
     } else {
-        unpack_chunk<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i), v);
+        r.w[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ void unpack8(const Raw8<DT>& r, float (&v)[8]) {
+    if constexpr (DT == INT8K_DTYPE_F32) {
+        const uint32_t d[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w,
+                               r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(d[k]);
+    } else {
+        unpack_chunk<DT>(r.w[0], v);
     }
 }
 // 8 values that are numbers of the dtype.
@@ -100,15 +134,164 @@ __device__ __forceinline__ void store8(void* y, size_t i, const float (&v)[8]) {
         p[0] = make_float4(v[0], v[1], v[2], v[3]);
         p[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        uint32_t w[4];
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + i) =
+            make_uint4(pack_pair<DT>(v[0], v[1]), pack_pair<DT>(v[2], v[3]),
+                       pack_pair<DT>(v[4], v[5]), pack_pair<DT>(v[6], v[7]));
+    }
+}
+
+// The codes that store_codes (rows.h) stores, with the rounding and the packing in one step:
+// adding 1.5 * 2^23 rounds half to even and leaves the code in the low byte.
+__device__ __forceinline__ void store_codes8(const float (&v)[8], float s, float inv, int8_t* dst) {
+    uint32_t b[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if constexpr (DT == INT8K_DTYPE_F16)
-                w[k] = f32_to_f16_bits(v[2 * k]) | ((uint32_t)f32_to_f16_bits(v[2 * k + 1]) << 16);
-            else
-                w[k] = (__float_as_uint(v[2 * k]) >> 16) | (__float_as_uint(v[2 * k + 1]) & 0xffff0000u);
+    for (int j = 0; j < 2; ++j) {
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            c[i] = __float_as_uint(fminf(fmaxf(quotient(v[4 * j + i], s, inv), -128.f), 127.f) +
+                                   12582912.0f);
+        b[j] = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u) |
+               __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+    }
+    *reinterpret_cast<uint2*>(dst) = make_uint2(b[0], b[1]);
+}
+
+// The heads [h0, h1) of one part (0 queries, 1 keys, 2 values) for this lane's token.
+template <int DT, bool QUANT, int LAYOUT>
+__device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0, int h1, size_t in,
+                                           size_t row, int cc, bool has, bool ok, int ia, int ib,
+                                           const float (&co)[8], const float (&si)[8]) {
+    // element indices of the pairs of this item
+    auto pair = [&](int i, int& ka, int& kb) {
+        if constexpr (LAYOUT == kSplitAny) pair_at(8 * cc + i, p.half, ka, kb);
+        else if constexpr (LAYOUT == kSplit) ka = ia + i, kb = ib + i;
+        else ka = ia + 2 * i, kb = ka + 1;
+    };
+    const float* wp = part < 2 ? p.w[part] : nullptr;
+    // (a, b) -> (a ca - b sb, b cb + a sa) / rms: the norm's weights go into the angles.  Pairs
+    // past the rotation have cos 1 and sin 0.
+    float ca[8], cb[8], sa[8], sb[8];
+    if (part < 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            int ka, kb;
+            pair(i, ka, kb);
+            const float wa = wp != nullptr ? wp[ka] : 1.f, wb = wp != nullptr ? wp[kb] : 1.f;
+            ca[i] = wa * co[i], sb[i] = wb * si[i];
+            cb[i] = wb * co[i], sa[i] = wa * si[i];
         }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    const size_t row_step = (size_t)p.S;
+    auto heads = [&](Raw8<DT> lo, Raw8<DT> hi, float (&ga)[8], float (&gv)[8], size_t r) {
+        float a[8], v[8];
+        if constexpr (LAYOUT == kSplitAny) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = ga[i], v[i] = gv[i];
+        } else {
+            float l[8], h[8];
+            unpack8<DT>(lo, l);
+            unpack8<DT>(hi, h);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (LAYOUT == kSplit) a[i] = l[i], v[i] = h[i];
+                else {
+                    a[i] = i < 4 ? l[2 * (i & 3)] : h[2 * (i & 3)];
+                    v[i] = i < 4 ? l[2 * (i & 3) + 1] : h[2 * (i & 3) + 1];
+                }
+            }
+        }
+        if (part < 2) {
+            float inv = 1.f;
+            if (wp != nullptr) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(v[i], v[i], ss));
+                ss = row_reduce(has ? ss : 0.f, p.lg, [](float m, float n) { return m + n; });
+                inv = 1.f / sqrtf(ss / (float)p.D + p.eps);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // normed first: squares in range do not promise products in range
+                const float na = a[i] * inv, nv = v[i] * inv;
+                a[i] = na * ca[i] - nv * sb[i];
+                v[i] = nv * cb[i] + na * sa[i];
+            }
+            round_all<DT>(a);
+            round_all<DT>(v);
+        }
+        // back to memory order
+        float l[8], h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (LAYOUT == kInterleaved) {
+                l[i] = (i & 1) ? v[i / 2] : a[i / 2];
+                h[i] = (i & 1) ? v[4 + i / 2] : a[4 + i / 2];
+            } else {
+                l[i] = a[i], h[i] = v[i];
+            }
+        }
+        const size_t out = r * p.D;
+        if constexpr (QUANT) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(v[i])));
+            m = row_reduce(has ? m : 0.f, p.lg, [](float x, float y) { return fmaxf(x, y); });
+            const float sc = fmaxf(m, 1e-8f) / 127.f;
+            const float rinv = 1.f / sc;
+            if (ok) {
+                if constexpr (LAYOUT == kSplitAny) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        int ka, kb;
+                        pair(i, ka, kb);
+                        p.q[part][out + ka] = (int8_t)quant_code(a[i], sc);
+                        p.q[part][out + kb] = (int8_t)quant_code(v[i], sc);
+                    }
+                } else {
+                    store_codes8(l, sc, rinv, p.q[part] + out + ia);
+                    store_codes8(h, sc, rinv, p.q[part] + out + ib);
+                }
+                if (cc == 0) p.s[part][r] = sc;
+            }
+        } else if (ok) {
+            if constexpr (LAYOUT == kSplitAny) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    int ka, kb;
+                    pair(i, ka, kb);
+                    store_one<DT>(p.y[part], out + ka, a[i]);
+                    store_one<DT>(p.y[part], out + kb, v[i]);
+                }
+            } else {
+                store8<DT>(p.y[part], out + ia, l);
+                store8<DT>(p.y[part], out + ib, h);
+            }
+        }
+    };
+    if constexpr (LAYOUT == kSplitAny) {
+        for (int h = h0; h < h1; ++h, in += p.D, row += row_step) {
+            float a[8], v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                int ka, kb;
+                pair(i, ka, kb);
+                a[i] = load_one<DT>(p.x, in + ka);
+                v[i] = load_one<DT>(p.x, in + kb);
+            }
+            heads({}, {}, a, v, row);
+        }
+    } else {
+        // the next head's elements are on their way while one is computed (past the last
+        // head they repeat it)
+        float none[8];
+        Raw8<DT> lo = load8<DT>(p.x, in + ia), hi = load8<DT>(p.x, in + ib);
+        for (int h = h0; h < h1; ++h, row += row_step) {
+            in += h + 1 < h1 ? p.D : 0;
+            const Raw8<DT> nl = load8<DT>(p.x, in + ia), nh = load8<DT>(p.x, in + ib);
+            heads(lo, hi, none, none, row);
+            lo = nl, hi = nh;
+        }
     }
 }
 
@@ -145,115 +328,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadsArgs p) {
     if (LAYOUT == kSplit && 8 * cc < p.half) ia = 8 * cc, ib = p.half + 8 * cc;
 
     const int total = p.heads + 2 * p.kv_heads;
-    const size_t width = (size_t)total * p.D;
     const int h0 = blockIdx.y * p.heads_per_wave, h1 = min(h0 + p.heads_per_wave, total);
     const long long b = t / p.S;
     const long long s = t - b * p.S;
-    for (int hh = h0; hh < h1; ++hh) {
-        const int part = hh < p.heads ? 0 : hh < p.heads + p.kv_heads ? 1 : 2;
-        const int ph = part == 0 ? p.heads : p.kv_heads;
-        const int h = hh - (part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads);
-        const size_t in = (size_t)t * width + (size_t)hh * p.D;
-        const size_t row = ((size_t)b * ph + h) * p.S + s;
-        float a[8], v[8];
-        if constexpr (LAYOUT == kSplitAny) {
+    const size_t in = (size_t)t * total * p.D;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                int ka, kb;
-                pair_at(8 * cc + i, p.half, ka, kb);
-                a[i] = load_one<DT>(p.x, in + ka);
-                v[i] = load_one<DT>(p.x, in + kb);
-            }
-        } else {
-            float lo[8], hi[8];
-            load8<DT>(p.x, in + ia, lo);
-            load8<DT>(p.x, in + ib, hi);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (LAYOUT == kSplit) a[i] = lo[i], v[i] = hi[i];
-                else {
-                    a[i] = i < 4 ? lo[2 * (i & 3)] : hi[2 * (i & 3)];
-                    v[i] = i < 4 ? lo[2 * (i & 3) + 1] : hi[2 * (i & 3) + 1];
-                }
-            }
-        }
-        if (part < 2) {
-            const float* w = p.w[part];
-            if (w != nullptr) {
-                float ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(v[i], v[i], ss));
-                ss = row_reduce(has ? ss : 0.f, p.lg, [](float m, float n) { return m + n; });
-                const float inv = 1.f / sqrtf(ss / (float)p.D + p.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    int ka, kb;
-                    if constexpr (LAYOUT == kSplitAny) pair_at(8 * cc + i, p.half, ka, kb);
-                    else if constexpr (LAYOUT == kSplit) ka = ia + i, kb = ib + i;
-                    else ka = 16 * cc + 2 * i, kb = ka + 1;
-                    a[i] = a[i] * inv * w[ka];
-                    v[i] = v[i] * inv * w[kb];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (8 * cc + i < p.half) {
-                    const float ra = a[i] * co[i] - v[i] * si[i];
-                    const float rb = v[i] * co[i] + a[i] * si[i];
-                    a[i] = ra, v[i] = rb;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = round_to<DT>(a[i]), v[i] = round_to<DT>(v[i]);
-        }
-        // back to memory order
-        float lo[8], hi[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (LAYOUT == kInterleaved) {
-                lo[i] = (i & 1) ? v[i / 2] : a[i / 2];
-                hi[i] = (i & 1) ? v[4 + i / 2] : a[4 + i / 2];
-            } else {
-                lo[i] = a[i], hi[i] = v[i];
-            }
-        }
-        const size_t out = row * p.D;
-        if constexpr (QUANT) {
-            float m = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(v[i])));
-            m = row_reduce(has ? m : 0.f, p.lg, [](float x, float y) { return fmaxf(x, y); });
-            const float sc = fmaxf(m, 1e-8f) / 127.f;
-            const float rinv = 1.f / sc;
-            if (ok) {
-                if constexpr (LAYOUT == kSplitAny) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        int ka, kb;
-                        pair_at(8 * cc + i, p.half, ka, kb);
-                        p.q[part][out + ka] = (int8_t)quant_code(a[i], sc);
-                        p.q[part][out + kb] = (int8_t)quant_code(v[i], sc);
-                    }
-                } else {
-                    store_codes<8>(lo, sc, rinv, p.q[part] + out + ia);
-                    store_codes<8>(hi, sc, rinv, p.q[part] + out + ib);
-                }
-                if (c == 0) p.s[part][row] = sc;
-            }
-        } else if (ok) {
-            if constexpr (LAYOUT == kSplitAny) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    int ka, kb;
-                    pair_at(8 * cc + i, p.half, ka, kb);
-                    store_one<DT>(p.y[part], out + ka, a[i]);
-                    store_one<DT>(p.y[part], out + kb, v[i]);
-                }
-            } else {
-                store8<DT>(p.y[part], out + ia, lo);
-                store8<DT>(p.y[part], out + ib, hi);
-            }
-        }
+    for (int part = 0; part < 3; ++part) {
+        const int first = part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads;
+        const int count = part == 0 ? p.heads : p.kv_heads;
+        const int a = max(h0, first), e = min(h1, first + count);
+        if (a < e)
+            part_heads<DT, QUANT, LAYOUT>(p, part, a, e, in + (size_t)a * p.D,
+                                          ((size_t)b * count + (a - first)) * p.S + s, cc, has, ok,
+                                          ia, ib, co, si);
     }
 }
 
