@@ -7,7 +7,31 @@
 //   int8_attention_forward's (prefill.hip):
 //     s_ij = (q_i . k_j) sQ_i sK_j / sqrt(D),  out_i = sum_j softmax_j(s_ij) v_j sV_j
 //
-// The block is prefill_block (prefill_core.h) on one query tile of one head of one sequence.
+// A block of 4 waves owns one tile of 128 queries of one head of one sequence, 32 per wave, and
+// walks the keys in tiles of 64 transposed, so that each lane owns one query:
+// S^T = K . Q^T on v_mfma_i32_32x32x32_i8, O^T += V^T . P^T on v_mfma_f32_32x32x16_f16.  Unlike
+// prefill.hip's blocks:
+//  - V enters as exact fp16 and its scale goes into the weights, P = fp16(p sV): one rounding per
+//    term.  (With V sV rounded beside P the error against 64 bits is 1.8 times that of the
+//    formula in fp32 with one fp16 rounding of P, with this 1.4.)  l sums p in fp32.  It costs a
+//    multiplication and an addition more per score, 5-12% on prompts past 4096 tokens.
+//  - Only a wave's first tile takes the exact step that finds a maximum; diagonal and ragged
+//    tiles run the ordinary step with a mask.  Prompts of 300 to 2000 tokens gain 6-20%.
+//
+// What bounds it: the issue of a wave's instructions.  At D = 128 a tile is 24 large MFMAs (768
+// cycles) and about 200 vector instructions, 32 of them exponentials (1000 cycles); two waves
+// share a SIMD and take 4100-4800 cycles for a tile each, where the two sums alone are 3600.
+// Measured: 225 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8
+// key heads of 128 (the masked product is 49.6 G multiply-adds per operand: 0.88 P
+// operations/s); 524 us for one prompt of 8192; 9 us for five requests of at most 70.  Tried:
+//  - the softmax of a tile next to the MFMAs of its neighbours in one block of instructions (the
+//    next scores and the last product with V): 226 and 528 us, with three K buffers and all
+//    256 registers;
+//  - 8 waves and 256 queries per block, half the staging per query: 237 and 524 us, and 51
+//    against 43 us for eight prompts of 512;
+//  - log2 sV in the exponent and l by an MFMA over 4 x 4 blocks, 2 vector instructions less per
+//    score: 225 and 525 us, each small MFMA waiting for the large ones.
+//
 // The lengths are on the device, so the grid is sized for the most tiles that T tokens of n
 // sequences can have (T / kQ + n) and each wave finds its tile from the lengths itself: a
 // plan kernel would cost a launch of its own.  Tiles are taken in the order of their index
@@ -92,10 +116,365 @@ __device__ __forceinline__ bool packed_tile(const int32_t* __restrict__ cu, int 
     return false;  // not reached: the ranks below `total` all have a sequence
 }
 
+// ------------------------------------------------------------------ the block
+
+// LDS of a block, all twice: a K tile (int8 rows, 16-byte padded), a V tile (fp16 [key][dim]),
+// the scales of its keys.
+template <int D>
+struct PackedLds {
+    static constexpr int kKStride = D + 16;
+    static constexpr int kKBytes = kKV * kKStride;
+    static constexpr int kVRow = D + 32;  // halfs: see VLayout
+    static constexpr int kVBytes = kKV * kVRow * 2;
+    static constexpr int kV = 2 * kKBytes;
+    static constexpr int kS = kV + 2 * kVBytes;
+    static constexpr int kSFloats = 2 * kKV + 4;  // sK, sV, the largest |sV|
+    static constexpr int kBytes = kS + 2 * kSFloats * 4;
+};
+
+constexpr int kPackedWaves = 4;              // per block, 32 queries each
+constexpr float kPackedMaxWeight = 60000.f;  // fp16 weights stay below it
+constexpr int kPackedMaxShift = 60;          // |m - running maximum| where m is set
+
+template <int D, bool CAUSAL, bool PAD, typename OutRow>
+__device__ __forceinline__ void packed_block(char* smem, const int8_t* __restrict__ Qh,
+                                             const int8_t* __restrict__ Kh,
+                                             const int8_t* __restrict__ Vh,
+                                             const float* __restrict__ sQh,
+                                             const float* __restrict__ sKh,
+                                             const float* __restrict__ sVh,
+                                             uint16_t* __restrict__ out, int S, int qt,
+                                             float qk_scale_log2, int d_mem, OutRow out_row) {
+    constexpr int QW = kPackedWaves;
+    constexpr int NS = D / 32;  // 32-wide d slices (QK k-steps) and O^T row tiles
+    constexpr int kQ = 32 * QW, kT = 64 * QW;
+    using L = PackedLds<D>;
+    using St = Stage<D, QW>;
+    using VL = VLayout<D, QW>;
+    const int dm = PAD ? d_mem : D;
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int h = lane >> 5;
+    const int qw0 = qt * kQ + wave * 32;  // first query of this wave
+    const int q = qw0 + (lane & 31);      // this lane's query
+    const bool qok = q < S;
+
+    // Q^T fragments (B operand of the QK MFMA): column q, 16 bytes of d-slice s.
+    v4i qf[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        qf[s] = (!PAD || 32 * s + 16 * h < dm)
+                    ? *reinterpret_cast<const v4i*>(Qh + (size_t)min(q, S - 1) * dm + 32 * s + 16 * h)
+                    : v4i{0, 0, 0, 0};
+    const float qscale = qok ? sQh[q] * qk_scale_log2 : 0.f;
+
+    // Step i of the walk is tile tile_of(i): first the nd tiles that some query of the block
+    // does not see whole (the diagonal, the last tile of a ragged sequence), which are masked,
+    // the last of them first, so a wave that skips some of them skips the first ones; then the
+    // whole ones.
+    const int kv_end = CAUSAL ? min(S, (qt + 1) * kQ) : S;
+    const int n = (kv_end + kKV - 1) / kKV;
+    const int kd = CAUSAL ? qt * kQ / kKV : S / kKV;  // whole tiles
+    const int nd = n - kd;
+    auto tile_of = [&](int i) {
+        i = min(i, n - 1);  // steps past the end repeat the last tile's loads
+        return i < nd ? n - 1 - i : i - nd;
+    };
+    const int q_wave_last = min(qw0 + 31, S - 1);
+    auto computes = [&](int i) { return qw0 < S && !(CAUSAL && tile_of(i) * kKV > q_wave_last); };
+
+    // ---- loads
+    const TileSrc src = make_tile_src<D, QW>(Kh, Vh, sKh, sVh, S, dm, t);
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    struct KeyLoads {
+        int4 k[St::kKChunks];
+    };
+    struct ScaleLoads {
+        float k, v;
+    };
+    uint2 pvr[St::kVItems][4];
+    auto fetch_k = [&](int i) {
+        KeyLoads l;
+        const int k0 = tile_of(i) * kKV;
+#pragma unroll
+        for (int c = 0; c < St::kKChunks; ++c) {
+            v4u w = {0, 0, 0, 0};
+            if (!PAD || src.kvalid)
+                w = __builtin_amdgcn_raw_buffer_load_b128(
+                    src.k, src.voff_k, k0 * dm + c * (PAD ? src.kstep : (uint32_t)(kT * 16)), 0);
+            l.k[c] = make_int4((int)w.x, (int)w.y, (int)w.z, (int)w.w);
+        }
+        return l;
+    };
+    auto fetch_v = [&](int i) {
+        const int k0 = tile_of(i) * kKV;
+#pragma unroll
+        for (int c = 0; c < St::kVItems; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                pvr[c][r] = make_uint2(0, 0);
+                if (!PAD || (src.vvalid >> c) & 1u)
+                    pvr[c][r] = load_v_f16x4(src.v, src.voff_v, (k0 + r) * dm + c * 4 * VL::kW);
+            }
+    };
+    // (every wave holds the scales, the first one stores them)
+    auto fetch_s = [&](int i) {
+        const int k0 = tile_of(i) * kKV;
+        return ScaleLoads{
+            __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.s, src.voff_s, k0 * 4, 0)),
+            __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.sv, src.voff_s, k0 * 4, 0))};
+    };
+    auto put_k = [&](char* buf, const KeyLoads& l) {
+#pragma unroll
+        for (int c = 0; c < St::kKChunks; ++c) {
+            const int e = t + c * kT;
+            *reinterpret_cast<int4*>(buf + e / (D / 16) * L::kKStride + e % (D / 16) * 16) = l.k[c];
+        }
+    };
+    auto put_v = [&](char* buf) {
+        _Float16* vs = reinterpret_cast<_Float16*>(buf) + (t / VL::kW) * 4 * L::kVRow + (t % VL::kW) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < St::kVItems; ++c)
+                *reinterpret_cast<uint2*>(vs + r * L::kVRow + c * 4 * VL::kW) = pvr[c][r];
+    };
+    auto put_s = [&](int i, const ScaleLoads& l) {
+        if (wave != 0) return;
+        float* s = reinterpret_cast<float*>(smem + L::kS) + (i & 1) * L::kSFloats;
+        s[lane] = l.k;
+        s[kKV + lane] = l.v;
+        const float top = row_reduce(fabsf(l.v), 6, [](float a, float b) { return fmaxf(a, b); });
+        if (lane == 0) s[2 * kKV] = top;
+    };
+
+    // ---- compute
+    v16f o[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    // S^T = K . Q^T of a tile, two 32-key halves
+    v16i sacc[2];
+    const int k_lane = (lane & 31) * L::kKStride + 16 * h;
+    auto scores = [&](const char* kbuf) {
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+            v4i kf[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                kf[s] = *reinterpret_cast<const v4i*>(kbuf + k_lane + T * 32 * L::kKStride + s * 32);
+#pragma unroll
+            for (int z = 0; z < 16; ++z) sacc[T][z] = 0;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                sacc[T] = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[s], qf[s], sacc[T], 0, 0, 0);
+        }
+    };
+    // O^T += V^T . P^T, the V^T fragments by transposing reads (see VLayout)
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s lds_v4s;
+    const int v_lane = (4 * h + ((lane & 15) >> 2)) * 2 * L::kVRow +
+                       2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+    auto product = [&](const char* vbuf, const v8h (&p)[4]) {
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                const char* a = vbuf + v_lane + ks * 32 * L::kVRow + j * 64;
+                const v4h lo = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)a));
+                const v4h hi = __builtin_bit_cast(
+                    v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(a + 16 * L::kVRow)));
+                const v8h v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[ks], o[j], 0, 0, 0);
+            }
+        // the fragments (two reads each) 4 MFMAs ahead of their use
+#pragma unroll
+        for (int i = 0; i < 4; ++i) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+        for (int i = 0; i < 4 * NS - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    };
+    // The weights of a lane's four keys of chunk ch, 32 (ch / 4) + 8 (ch % 4) + 4 h + 0..3, their
+    // scores being registers 4 (ch % 4) .. + 3 of half ch / 4: p = 2^(x - m), P = fp16(p sV).
+    // Returns the sum of p.  sQ sK comes from an MFMA over 4 x 4 blocks (lanes 4b .. 4b + 3, the
+    // outer product of a lane's own key scale with the lanes' query scales), which leaves one
+    // multiplication less per score than sK read as it is: 520 us against 529 at 8192 tokens, 32
+    // heads of 128.
+    typedef float v4f __attribute__((ext_vector_type(4)));
+    auto scale_qk = [&](int ch, const float* sc) {
+        return __builtin_amdgcn_mfma_f32_4x4x1f32(sc[32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + (lane & 3)], qscale,
+                                                  v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    };
+    auto scale_v = [&](int ch, const float* sc) {
+        return *reinterpret_cast<const v4f*>(sc + kKV + 32 * (ch >> 2) + 8 * (ch & 3) + 4 * h);
+    };
+    auto weights = [&](int ch, const float* sc, v8h (&p)[4], auto mask, auto seen) {
+        const int T = ch >> 2, g = ch & 3;
+        const v4f sqk = scale_qk(ch, sc), sv = scale_v(ch, sc);
+        float e[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            e[c] = fast_exp2(fmaf(static_cast<float>(sacc[T][4 * g + c]), sqk[c], -m));
+            float w = e[c] * sv[c];
+            if constexpr (decltype(mask)::value) {
+                const bool ok = seen(32 * T + 8 * g + 4 * h + c);
+                e[c] = ok ? e[c] : 0.f;
+                w = ok ? w : 0.f;
+            }
+            p[2 * T + (g >> 1)][4 * (g & 1) + c] = (_Float16)w;
+        }
+        return (e[0] + e[1]) + (e[2] + e[3]);
+    };
+    // The exact path: sets m so that the largest weight p sV of the tile lies in [0.5, 1) and
+    // rescales O and l.
+    auto slow = [&](int i, const float* sc, v8h (&p)[4]) {
+        const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
+        auto seen = [&](int key) { return key <= last; };
+        float top = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+            const v4f sqk = scale_qk(ch, sc);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float x = static_cast<float>(sacc[ch >> 2][4 * (ch & 3) + c]) * sqk[c];
+                top = fmaxf(top, seen(32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + c) ? x : -INFINITY);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        top = max_xor32(top);
+        const float base = top == -INFINITY ? 0.f : top;
+        float pm = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+            const v4f sqk = scale_qk(ch, sc), sv = scale_v(ch, sc);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float x = sv[c] * fast_exp2(fmaf(static_cast<float>(sacc[ch >> 2][4 * (ch & 3) + c]),
+                                                       sqk[c], -base));
+                pm = fmaxf(pm, seen(32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + c) ? fabsf(x) : 0.f);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        pm = max_xor32(pm);
+        int e = 0;
+        if (pm > 0.f && pm < INFINITY) frexpf(pm, &e);
+        const float m_new = fmaxf(m, top + (float)min(max(e, -kPackedMaxShift), kPackedMaxShift));
+        const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            l += weights(c, sc, p, std::true_type{}, seen);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto scales_of = [&](int i) {
+        return reinterpret_cast<const float*>(smem + L::kS) + (i & 1) * L::kSFloats;
+    };
+
+    // Step i reads buffer i & 1 while the registers hold tile i + 1, loaded during step i - 1;
+    // at its end that goes to the other buffer, the loads of tile i + 2 go out, and the step's
+    // one barrier follows.
+    auto k_buf = [&](int i) { return smem + (i & 1) * L::kKBytes; };
+    auto v_buf = [&](int i) { return smem + L::kV + (i & 1) * L::kVBytes; };
+    KeyLoads pk;
+    ScaleLoads ps;
+    auto fetch = [&](int i) {
+        pk = fetch_k(i);
+        fetch_v(i);
+        ps = fetch_s(i);
+    };
+    auto put = [&](int i) {
+        put_k(k_buf(i), pk);
+        put_v(v_buf(i));
+        put_s(i, ps);
+    };
+    fetch(0);
+    put(0);
+    fetch(1);
+    __syncthreads();
+    auto advance = [&](int i) {
+        put(i + 1);
+        fetch(i + 2);
+        __syncthreads();
+    };
+    // The steps up to `end` that keep m; false where step i, whose scores are in sacc, has
+    // weights that leave the range m gives them, before anything of it is in O.
+    int i = 0;
+    auto steps = [&](int end, auto mask) {
+        for (; i < end; ++i) {
+            const float* sc = scales_of(i);
+            const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
+            scores(k_buf(i));
+            v8h p[4];
+            float psum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                psum += weights(c, sc, p, mask, [&](int key) { return key <= last; });
+                // (keeps the scales of all chunks from being read first: 2-9% at D = 256)
+                if (c & 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            // every weight is at most the sum of p times the tile's largest |sV|
+            if (__ballot(!(psum * sc[2 * kKV] <= kPackedMaxWeight && psum <= 0x1p60f)) != 0) return false;
+            l += psum;
+            product(v_buf(i), p);
+            advance(i);
+        }
+        return true;
+    };
+    bool running = false;  // wave-uniform: an exact step has set m
+    while (i < n) {
+        if (running) {
+            if (steps(nd, std::true_type{}) && steps(n, std::false_type{})) break;
+        }
+        if (computes(i)) {
+            if (!running) scores(k_buf(i));
+            running = true;
+            v8h p[4];
+            slow(i, scales_of(i), p);
+            product(v_buf(i), p);
+        }
+        advance(i);
+        ++i;
+    }
+
+    const float Lsum = sum_xor32(l);
+    if (!qok) return;  // lanes l and l^32 share q, so both leave or both stay
+    const float inv = 1.f / Lsum;
+    uint16_t* orow = out + out_row(q) * dm;
+#pragma unroll
+    for (int j = 0; j < NS; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * j + 8 * g + 4 * h;
+            if (PAD && d >= dm) continue;
+            uint32_t w[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                w[c] = __half_as_ushort(f16_of_f32(o[j][4 * g + 2 * c] * inv)) |
+                       ((uint32_t)__half_as_ushort(f16_of_f32(o[j][4 * g + 2 * c + 1] * inv)) << 16);
+            *reinterpret_cast<uint2*>(orow + d) = make_uint2(w[0], w[1]);
+        }
+}
+
 // zero_rest: the rows of out that no sequence holds are written as zeros by the blocks that
 // have no tile (the grid has one rank more than there can be tiles).
-template <int D, int QW, int KG, bool CAUSAL, bool PAD>
-__global__ __launch_bounds__((Shape<D, QW, KG>::kThreads), (Shape<D, QW, KG>::kMinBlocks)) void packed_kernel(
+// Heads: every XCD takes workgroups in turn, so where 8 divides the heads XCD x gets heads
+// x heads / 8 .. and its L2 the K and V of their key heads alone (231 against 252 us for the
+// prompts above).
+template <int D, bool CAUSAL, bool PAD>
+__global__ __launch_bounds__(64 * kPackedWaves, D == 256 ? 1 : 2) void packed_kernel(
     const int8_t* __restrict__ Q, const int8_t* __restrict__ K, const int8_t* __restrict__ V,
     const float* __restrict__ sQ, const float* __restrict__ sK, const float* __restrict__ sV,
     uint16_t* __restrict__ out, const int32_t* __restrict__ cu, int n, int T, int heads,
@@ -104,10 +483,11 @@ __global__ __launch_bounds__((Shape<D, QW, KG>::kThreads), (Shape<D, QW, KG>::kM
     const int dm = PAD ? d_mem : D;
     int rank = (int)blockIdx.x / heads;
     const int ranks = (int)gridDim.x / heads;
-    const int h = (int)blockIdx.x % heads;
+    int h = (int)blockIdx.x % heads;
+    if (heads % 8 == 0) h = h % 8 * (heads / 8) + h / 8;
     PackedTile t;
     const int wanted = rank;
-    if (!packed_tile<Shape<D, QW, KG>::kQ>(cu, n, T, rank, t)) {
+    if (!packed_tile<32 * kPackedWaves>(cu, n, T, rank, t)) {
         if (!zero_rest) return;
         // rank is now this block's index among the idle ones of its head
         const int idle = ranks - (wanted - rank);
@@ -123,9 +503,9 @@ __global__ __launch_bounds__((Shape<D, QW, KG>::kThreads), (Shape<D, QW, KG>::kM
         return;
     }
     const size_t qrow = (size_t)h * T + t.start, krow = (size_t)(h / group) * T + t.start;
-    prefill_block<D, QW, KG, CAUSAL, PAD>(
+    packed_block<D, CAUSAL, PAD>(
         smem_all, Q + qrow * dm, K + krow * dm, V + krow * dm, sQ + qrow, sK + krow, sV + krow,
-        out, nullptr, nullptr, t.len, t.qt, qk_scale_log2, d_mem, [&](int q) {
+        out, t.len, t.qt, qk_scale_log2, d_mem, [&](int q) {
             return thd ? (size_t)(t.start + q) * heads + h : qrow + q;
         });
 }
@@ -139,21 +519,21 @@ struct PackedArgs {
     bool causal, thd, zero_rest;
 };
 
-template <int D, int QW, int KG>
-int launch_packed_shape(const PackedArgs& a, hipStream_t stream) {
-    constexpr int kQ = Shape<D, QW, KG>::kQ, kThreads = Shape<D, QW, KG>::kThreads;
+template <int D>
+int launch_packed(const PackedArgs& a, hipStream_t stream) {
+    constexpr int kQ = 32 * kPackedWaves, kThreads = 64 * kPackedWaves;
     const long long ranks = (long long)a.T / kQ + a.n + 1;
     const float qk = (1.0f / std::sqrt((float)a.dm)) * kLog2e;
-    const int lds = KG * 2 * Stage<D, QW>::kBytes;
+    constexpr int kLds = PackedLds<D>::kBytes;
     if (ranks * a.heads * kThreads >= (1LL << 32)) return INT8K_ERR_UNSUPPORTED;
     static PerDeviceOnce lds_once;
     const int st = set_lds_limit(
-        lds_once, lds, packed_kernel<D, QW, KG, true, false>, packed_kernel<D, QW, KG, false, false>,
-        packed_kernel<D, QW, KG, true, true>, packed_kernel<D, QW, KG, false, true>);
+        lds_once, kLds, packed_kernel<D, true, false>, packed_kernel<D, false, false>,
+        packed_kernel<D, true, true>, packed_kernel<D, false, true>);
     if (st != INT8K_OK) return st;
     const unsigned blocks = (unsigned)(ranks * a.heads);
 #define INT8K_PACKED_LAUNCH(C, P)                                                               \
-    packed_kernel<D, QW, KG, C, P><<<blocks, kThreads, lds, stream>>>(                          \
+    packed_kernel<D, C, P><<<blocks, kThreads, kLds, stream>>>(                             \
         a.Q, a.K, a.V, a.sQ, a.sK, a.sV, a.out, a.cu, a.n, a.T, a.heads, a.heads / a.kv_heads,  \
         qk, a.thd ? 1 : 0, a.zero_rest ? 1 : 0, a.dm)
     if (a.dm == D) {
@@ -165,14 +545,6 @@ int launch_packed_shape(const PackedArgs& a, hipStream_t stream) {
     }
 #undef INT8K_PACKED_LAUNCH
     return check_launch("packed_kernel");
-}
-
-template <int D>
-int launch_packed(const PackedArgs& a, hipStream_t stream) {
-#define INT8K_PACKED_SHAPE(I) \
-    return launch_packed_shape<D, kShapes<D>[I].qw, kShapes<D>[I].kg>(a, stream)
-    INT8K_PACKED_SHAPE(0);
-#undef INT8K_PACKED_SHAPE
 }
 
 }  // namespace

@@ -71,12 +71,10 @@ def test_packed_equals_the_batched_kernel_on_equal_lengths(ext, gpu):
     b = [c[k].view(4, 3, 256, -1).transpose(0, 1).contiguous() for k in ("Q", "K", "V")]
     s = [c[k].view(4, 3, 256).transpose(0, 1).contiguous() for k in ("sQ", "sK", "sV")]
     ref = ext.int8_attention_forward(*b, *s, True).transpose(0, 1).reshape(4, 768, 128)
-    # The same fp16 weights and values, whose fp32 sums may be taken in another order: a sum of
-    # 256 terms is off by at most 256 * 2^-24 of sum p|v| on either side (an output near zero
-    # keeps that error, not one relative to itself), then each side rounds once (2^-11 each).
-    _, mag = _oracle(c, True)
-    bound = 2.0 ** -10 * np.abs(np64(ref)) + 2 * 256 * 2.0 ** -24 * mag + 2.0 ** -24
-    assert_within(np64(out), np64(ref), bound)
+    # each side is within its bound of the oracle, so they are within twice that of each other
+    exact, mag = _oracle(c, True)
+    vmax = float((c["V"].float().abs().amax(-1) * c["sV"]).max())
+    assert_within(np64(out), np64(ref), 2 * attention_bound(exact, mag, 256, vmax))
 
 
 @pytest.mark.parametrize("front,tail", [(0, 1), (0, 300), (5, 0), (33, 700)])
