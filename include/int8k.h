@@ -469,8 +469,9 @@ int int8k_rope_bad_positions(unsigned int* count);
  *   scales fp32 [heads or kv_heads, total_tokens]; heads a multiple of kv_heads, query
  *   head h reads key head h / (heads / kv_heads)
  *   cu_seqlens int32 [num_seqs + 1] (device): sequence i is the tokens cu_seqlens[i] ..
- *   cu_seqlens[i+1]-1; empty sequences are fine.  Bounds outside [0, total_tokens] or
- *   falling ones are cut to the tensors.
+ *   cu_seqlens[i+1]-1; empty sequences are fine.  Bounds outside [0, total_tokens] are cut
+ *   to it.  The bounds must not fall: if they do, no access leaves the tensors, but which
+ *   rows are written, and from which sequence, is not defined.
  *   out fp16 [heads, total_tokens, D], or [total_tokens, heads, D] with
  *   INT8K_ATTN_OUT_THD (the row order the output projection reads)
  * Each query attends to the keys of its sequence, with INT8K_ATTN_CAUSAL to those up to

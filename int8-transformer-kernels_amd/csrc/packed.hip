@@ -21,7 +21,7 @@
 // What bounds it: the issue of a wave's instructions.  At D = 128 a tile is 24 large MFMAs (768
 // cycles) and about 200 vector instructions, 32 of them exponentials (1000 cycles); two waves
 // share a SIMD and take 4100-4800 cycles for a tile each, where the two sums alone are 3600.
-// Measured: 225 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8
+// Measured (3% apart from card to card): 225 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8
 // key heads of 128 (the masked product is 49.6 G multiply-adds per operand: 0.88 P
 // operations/s); 524 us for one prompt of 8192; 9 us for five requests of at most 70.  Tried:
 //  - the softmax of a tile next to the MFMAs of its neighbours in one block of instructions (the
@@ -29,6 +29,8 @@
 //    256 registers;
 //  - 8 waves and 256 queries per block, half the staging per query: 237 and 524 us, and 51
 //    against 43 us for eight prompts of 512;
+//  - steps of 32 keys, half the code and three quarters of the registers: 236 and 559 us, and 8.5
+//    against 9.1 us for the five short requests;
 //  - log2 sV in the exponent and l by an MFMA over 4 x 4 blocks, 2 vector instructions less per
 //    score: 225 and 525 us, each small MFMA waiting for the large ones.
 //
@@ -195,7 +197,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     uint2 pvr[St::kVItems][4];
     auto fetch_k = [&](int i) {
         KeyLoads l;
-        const int k0 = tile_of(i) * kKV;
+        const uint32_t k0 = tile_of(i) * kKV;  // (offsets below 2^32 by the entry's check)
 #pragma unroll
         for (int c = 0; c < St::kKChunks; ++c) {
             v4u w = {0, 0, 0, 0};
@@ -207,7 +209,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         return l;
     };
     auto fetch_v = [&](int i) {
-        const int k0 = tile_of(i) * kKV;
+        const uint32_t k0 = tile_of(i) * kKV;
 #pragma unroll
         for (int c = 0; c < St::kVItems; ++c)
 #pragma unroll
@@ -219,7 +221,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     };
     // (every wave holds the scales, the first one stores them)
     auto fetch_s = [&](int i) {
-        const int k0 = tile_of(i) * kKV;
+        const uint32_t k0 = tile_of(i) * kKV;
         return ScaleLoads{
             __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.s, src.voff_s, k0 * 4, 0)),
             __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(src.sv, src.voff_s, k0 * 4, 0))};
@@ -323,6 +325,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         for (int c = 0; c < 4; ++c) {
             e[c] = fast_exp2(fmaf(static_cast<float>(sacc[T][4 * g + c]), sqk[c], -m));
             float w = e[c] * sv[c];
+            asm("" : "+v"(w));  // rounded to fp32 first in every copy of this code
             if constexpr (decltype(mask)::value) {
                 const bool ok = seen(32 * T + 8 * g + 4 * h + c);
                 e[c] = ok ? e[c] : 0.f;
@@ -332,6 +335,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         }
         return (e[0] + e[1]) + (e[2] + e[3]);
     };
+    float over = 1.f;  // not 0: the query's weights leave the range of m
     // The exact path: sets m so that the largest weight p sV of the tile lies in [0.5, 1) and
     // rescales O and l.
     auto slow = [&](int i, const float* sc, v8h (&p)[4]) {
@@ -365,7 +369,9 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         pm = max_xor32(pm);
         int e = 0;
         if (pm > 0.f && pm < INFINITY) frexpf(pm, &e);
-        const float m_new = fmaxf(m, top + (float)min(max(e, -kPackedMaxShift), kPackedMaxShift));
+        // (a query whose weights fit keeps its m, whatever its neighbours in the wave hold)
+        const float raised = fmaxf(m, top + (float)min(max(e, -kPackedMaxShift), kPackedMaxShift));
+        const float m_new = max_xor32(over) != 0.f ? raised : m;
         const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
         m = m_new;
         l *= alpha;
@@ -373,11 +379,13 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         for (int j = 0; j < NS; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
+        float psum = 0.f;  // (summed as in a step that keeps m)
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            l += weights(c, sc, p, std::true_type{}, seen);
+            psum += weights(c, sc, p, std::true_type{}, seen);
             __builtin_amdgcn_sched_barrier(0);
         }
+        l += psum;
     };
     auto scales_of = [&](int i) {
         return reinterpret_cast<const float*>(smem + L::kS) + (i & 1) * L::kSFloats;
@@ -426,7 +434,8 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
                 if (c & 1) __builtin_amdgcn_sched_barrier(0);
             }
             // every weight is at most the sum of p times the tile's largest |sV|
-            if (__ballot(!(psum * sc[2 * kKV] <= kPackedMaxWeight && psum <= 0x1p60f)) != 0) return false;
+            over = psum * sc[2 * kKV] <= kPackedMaxWeight && psum <= 0x1p60f ? 0.f : 1.f;
+            if (__ballot(over != 0.f) != 0) return false;
             l += psum;
             product(v_buf(i), p);
             advance(i);

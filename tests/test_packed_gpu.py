@@ -144,3 +144,17 @@ def test_packed_graph_replay_with_other_lengths(ext, gpu):
         torch.cuda.synchronize()
         assert torch.equal(held, want), cu
         _check(c, want.transpose(0, 1), True, str(cu))
+
+
+def test_packed_rows_do_not_depend_on_their_neighbours(ext, gpu):
+    # a query whose scores grow late sets its own reference; the others of its wave keep theirs
+    c = _case([400], 2, 1, 128, gpu, seed=5)
+    want = ext.int8_attention_forward_packed(*_args(c))
+    assert torch.isfinite(want).all()
+    q = torch.tensor([3, 40, 100, 255, 399], device=gpu)
+    c["sQ"][:, q] *= 2.0 ** 10
+    out = ext.int8_attention_forward_packed(*_args(c))
+    rest = torch.ones(400, dtype=torch.bool, device=gpu)
+    rest[q] = False
+    assert torch.equal(out[:, rest], want[:, rest])
+    assert torch.isfinite(out).all()
