@@ -19,11 +19,12 @@
 //    tiles run the ordinary step with a mask.  Prompts of 300 to 2000 tokens gain 6-20%.
 //
 // What bounds it: the issue of a wave's instructions.  At D = 128 a tile is 24 large MFMAs (768
-// cycles) and about 200 vector instructions, 32 of them exponentials (1000 cycles); two waves
-// share a SIMD and take 4100-4800 cycles for a tile each, where the two sums alone are 3600.
-// Measured (3% apart from card to card): 225 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8
-// key heads of 128 (the masked product is 49.6 G multiply-adds per operand: 0.88 P
-// operations/s); 524 us for one prompt of 8192; 9 us for five requests of at most 70.  Tried:
+// cycles) and about 200 vector instructions, 32 of them exponentials of two slots each (930
+// cycles); two waves share a SIMD and take 4100-4800 cycles for a tile each, where the two sums
+// alone are 3400: they overlap little.  Measured (225-240 and 524-558 us from card to card):
+// 225 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8 key heads
+// of 128 (49.6 G multiply-adds under the mask in each product: 0.88 P operations/s); 524 us for
+// one prompt of 8192; 9 us for five requests of at most 70.  Tried:
 //  - the softmax of a tile next to the MFMAs of its neighbours in one block of instructions (the
 //    next scores and the last product with V): 226 and 528 us, with three K buffers and all
 //    256 registers;
@@ -39,7 +40,7 @@
 // plan kernel would cost a launch of its own.  Tiles are taken in the order of their index
 // inside their sequence, the highest first: under the causal mask that is heaviest first
 // over all sequences, so short ones fill the end of the grid.
-#include "prefill_core.h"
+#include "prefill_tiles.h"
 
 namespace int8k {
 namespace {
