@@ -9,6 +9,7 @@
 //   stream   the weights streamed once over all CUs, exact int32 partials, then rows
 //   small    64 x 64 tiles, four blocks per CU
 //   mid      128 x 128 tiles, two blocks per CU; K split into partials where CUs would idle
+//   wide     256 x 192 tiles, packed weights
 //   tiled    256 x 256 tiles
 // The tiles are computed transposed (SWAP), so a lane holds 4 adjacent columns of one row: 32
 // rows at a time go through the wave's own piece of LDS and leave as whole lines.
@@ -86,8 +87,6 @@ __device__ __forceinline__ void epilogue_rows(const v16i (&acc)[TM_][TN_], const
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const float* ssw = scales + B + cl + 4 * half;
     const float* sb = ssw + B;
-    const int piece = lane % kLanes, first = lane / kLanes;
-    const int col = n0 + cl + piece * (16 / E);
 #pragma unroll
     for (int i = 0; i < TM_; ++i) {
         const float sx = scales[rl + 32 * i + (lane & 31)];
@@ -108,9 +107,10 @@ __device__ __forceinline__ void epilogue_rows(const v16i (&acc)[TM_][TN_], const
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int r = 0; r < 32; r += 64 / kLanes) {
-            const int row = m0 + rl + 32 * i + r + first;
-            const uint4 w = *reinterpret_cast<const uint4*>(stage + (r + first) * kRow + piece * 16);
+        for (int e = lane; e < 32 * kLanes; e += 64) {
+            const int r = e / kLanes, piece = e % kLanes;
+            const int row = m0 + rl + 32 * i + r, col = n0 + cl + piece * (16 / E);
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + r * kRow + piece * 16);
             // N is a multiple of 16: a piece is wholly in or out
             if (row < p.M && col < p.N)
                 *reinterpret_cast<uint4*>(static_cast<char*>(p.y) + ((size_t)row * p.N + col) * E) = w;
@@ -153,6 +153,117 @@ __global__ __launch_bounds__(kThreads, 1) void linear_tiled_kernel(LinearArgs p,
     static_assert(4 * 32 * kEpiRow<INT8K_DTYPE_F32, TN> <= LDS_BYTES, "the waves' pieces fit");
     epilogue_rows<DT, TM, TN, BM>(acc, p, m0, n0, (wave >> 1) * WM, (wave & 1) * WN,
                                   lds + wave * 32 * kEpiRow<DT, TN>, scales);
+}
+
+// ------------------------------------------------------------------ 256 x 192 tiles
+// For packed weights whose 256 x 256 tiles leave the last round of CUs part empty: waves of
+// 128 x 96, on the schedule of the 256 x 256 loop (mainloop) with 12 MFMAs a slice.
+constexpr int kWideN = 192, kWideWN = kWideN / 2, kWideTN = kWideWN / 32;
+constexpr int kWideStage = A_STAGE + kWideN * LDS_STRIDE;
+constexpr int kWideLds = 2 * kWideStage + 3 * BM * 4;
+
+template <bool EDGE>
+__device__ __forceinline__ void wide_mainloop(v16i (&acc)[TM][kWideTN], const LinearArgs& p, int m0,
+                                              int n0, char* lds) {
+    constexpr int TN_ = kWideTN, kA = kChunks, kB = kWideN * kChunksPerRow / kThreads;
+    constexpr int kMfmas = TM * TN_, kReads = TM + TN_;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int a_off = ((wave >> 1) * WM + (lane & 31)) * LDS_STRIDE + (lane >> 5) * 16;
+    const int b_off = A_STAGE + ((wave & 1) * kWideWN + (lane & 31)) * LDS_STRIDE + (lane >> 5) * 16;
+    const OperandSrc srcA = operand_rowmajor(p.x, p.M, p.K, p.K, m0);
+    const OperandSrc srcB = operand_rowmajor(p.w, p.N, p.K, p.K, n0);
+    const int nk = (p.K + BK - 1) / BK;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN_; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    int4 f[kA + kB];  // chunks of A, then of B, of the stage after next
+    auto load = [&](int k0, int c) { f[c] = c < kA ? load_operand(srcA, k0, c) : load_operand(srcB, k0, c - kA); };
+    auto store = [&](char* stage, int k0, int c) {
+        if (c < kA) store_chunk<EDGE>(f[c], stage, p.M, p.K, m0, k0, c);
+        else store_chunk<EDGE>(f[c], stage + A_STAGE, p.N, p.K, n0, k0, c - kA);
+    };
+    v4i a[2][TM], b[2][TN_];
+    // fragment r of a slice: the A ones, then the B ones
+    auto read = [&](int to, const char* stage, int slice, int r) {
+        if (r < TM) a[to][r] = read_frag(stage, a_off, r, slice);
+        else b[to][r - TM] = read_frag(stage, b_off, r - TM, slice);
+    };
+    auto mfma = [&](int from, int g) {
+        const int i = g / TN_, j = g % TN_;
+        acc[i][j] = mfma_ab<true>(a[from][i], b[from][j], acc[i][j]);
+    };
+#pragma unroll
+    for (int c = 0; c < kA + kB; ++c) load(0, c);
+#pragma unroll
+    for (int c = 0; c < kA + kB; ++c) store(lds, 0, c);
+#pragma unroll
+    for (int c = 0; c < kA + kB; ++c) load(BK, c);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) read(0, lds, 0, r);
+    for (int kt = 0; kt < nk; ++kt) {
+        const char* cur = lds + (kt & 1) * kWideStage;
+        char* nxt = lds + ((kt + 1) & 1) * kWideStage;
+        // slices 0 and 1: the next slice's fragments between their MFMAs
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < kMfmas; ++g) {
+                if (g < kReads) read((s + 1) & 1, cur, s + 1, g);
+                mfma(s & 1, g);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // slice 2: slice 3's fragments, the next stage's chunks to LDS and their replacements
+#pragma unroll
+        for (int g = 0; g < kMfmas; ++g) {
+            if (g < kReads) read(1, cur, 3, g);
+#pragma unroll
+            for (int c = g * (kA + kB) / kMfmas; c < (g + 1) * (kA + kB) / kMfmas; ++c) {
+                store(nxt, (kt + 1) * BK, c);
+                load((kt + 2) * BK, c);
+            }
+            mfma(0, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // slice 3: half of its MFMAs cover the writes, the others the next slice 0
+#pragma unroll
+        for (int g = 0; g < kMfmas / 2; ++g) {
+            mfma(1, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int g = kMfmas / 2; g < kMfmas; ++g) {
+            const int u = g - kMfmas / 2;
+#pragma unroll
+            for (int r = u * kReads / (kMfmas / 2); r < (u + 1) * kReads / (kMfmas / 2); ++r) read(0, nxt, 0, r);
+            mfma(1, g);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads, 1) void linear_wide_kernel(LinearArgs p, int tiles_m, int tiles_n) {
+    extern __shared__ __align__(16) char lds[];
+    int tm, tn;
+    tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * kWideN;
+    const TileScales s = load_scales<BM>(p, m0, n0);
+    v16i acc[TM][kWideTN];
+    if (m0 + BM <= p.M && n0 + kWideN <= p.N && p.K % BK == 0) wide_mainloop<false>(acc, p, m0, n0, lds);
+    else wide_mainloop<true>(acc, p, m0, n0, lds);
+    float* scales = reinterpret_cast<float*>(lds + 2 * kWideStage);
+    park_scales<BM>(s, scales);
+    const int wave = threadIdx.x >> 6;
+    static_assert(4 * 32 * kEpiRow<INT8K_DTYPE_F32, kWideTN> <= 2 * kWideStage, "the waves' pieces fit");
+    epilogue_rows<DT, TM, kWideTN, BM>(acc, p, m0, n0, (wave >> 1) * WM, (wave & 1) * kWideWN,
+                                       lds + wave * 32 * kEpiRow<DT, kWideTN>, scales);
 }
 
 // ------------------------------------------------------------------ 128 x 128 tiles
@@ -436,7 +547,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void linear_skinny_kernel(Linear
 
 // ------------------------------------------------------------------ plan, launch
 
-enum class LinearRoute { kSkinny, kStream, kSmall, kMid, kTiled };
+enum class LinearRoute { kSkinny, kStream, kSmall, kMid, kWide, kTiled };
 
 struct LinearPlan {
     LinearRoute route;
@@ -455,11 +566,14 @@ struct LinearPlan {
 //    4096 -> 6144 9.8 / 9.6; T = 64 14.6 / 14.6);
 //  - small: 0.34 us a step to 256 blocks, 0.24 per 256 beyond (T = 333, 2048 -> 2560 8.4 / 8.9,
 //    16.6 on 128 x 128 tiles; T = 512, 4096 -> 4096 18.4 / 18.7, 24.6; T = 1000 33.7 / 34.1, 30.8);
-//  - mid: 0.78 us a step for a block alone on its CU, 1.33 for two; split over K, the partials'
-//    traffic and a second kernel (T = 512, 4096 -> 4096 27.5 / 24.6; T = 128, 4096 -> 6144 in 4
+//  - mid: 0.78 us a step for a block alone on its CU, 1.33 for two, 1.1 and up where some have
+//    two (T = 1000, 4096 -> 6144 44 / 40); split over K, the partials' traffic and a second
+//    kernel (T = 512, 4096 -> 4096 27.5 / 24.6; T = 128, 4096 -> 6144 in 4
 //    splits 16.3 / 16.2);
 //  - tiled: 1.25 us a step and round, 0.55 more where the grid fills the GPU and the clock
-//    falls with the power (T = 4096, 4096 -> 4096 67 / 66, 4096 -> 6144 115 / 112).
+//    falls with the power (T = 4096, 4096 -> 4096 67 / 66, 4096 -> 6144 115 / 112);
+//  - wide (packed weights): 0.98 us and 0.42 (T = 4096, 4096 -> 6144 99 / 102, where tiled takes
+//    115; T = 2048 54 / 53, tiled 59; T = 4096, 4096 -> 4096 99 / 91, tiled 67).
 LinearPlan linear_plan(int M, int K, int N, bool packed) {
     LinearPlan pl{};
     const long long steps = ceil_div(K, BK);
@@ -473,12 +587,17 @@ LinearPlan linear_plan(int M, int K, int N, bool packed) {
         const long long tiles = ceil_div(M, BM) * ceil_div(N, BN), rounds = ceil_div(tiles, 256);
         better(900 + steps * (125 * rounds + 55 * tiles / 256), LinearRoute::kTiled);
     }
+    if (packed) {
+        const long long tiles = ceil_div(M, BM) * ceil_div(N, kWideN), rounds = ceil_div(tiles, 256);
+        better(900 + steps * (98 * rounds + 42 * tiles / 256), LinearRoute::kWide);
+    }
     const long long mid_tiles = ceil_div(M, kMidB) * ceil_div(N, kMidB);
     for (long long sp = 1; sp <= std::min(16LL, steps); ++sp) {
         const long long st = ceil_div(steps, sp), n = ceil_div(steps, st);
         if (n != sp) continue;  // the same plan as fewer splits
         const long long blocks = mid_tiles * n, rest = blocks % 512;
-        const long long gemm = st * (133 * (blocks / 512) + (rest > 256 ? 133 : rest > 0 ? 78 : 0));
+        const long long last = rest > 256 ? 110 + 23 * (rest - 256) / 256 : rest > 0 ? 78 : 0;
+        const long long gemm = st * (133 * (blocks / 512) + last);
         const long long rows = n > 1 ? 200 + 8 * n * (long long)M * N / 45000 : 0;
         if (better(250 + gemm + rows + (long long)N * K / 100000, LinearRoute::kMid)) {
             pl.mid = MidPlan{(int)ceil_div(M, kMidB), (int)ceil_div(N, kMidB), (int)n, (int)(st * BK)};
@@ -570,6 +689,13 @@ int launch_linear(const LinearArgs& p, const LinearPlan& pl, hipStream_t stream)
             linear_mid_kernel<DT, BKN><<<tiles, kThreads, MidLds<BKN>::kBytes, stream>>>(
                 p, pl.mid.tiles_m, pl.mid.tiles_n);
             return check_launch("linear_mid_kernel");
+        }
+        case LinearRoute::kWide: {
+            static PerDeviceOnce once;
+            if (const int st = set_lds(once, (const void*)linear_wide_kernel<DT>, kWideLds)) return st;
+            const int tiles_m = (int)ceil_div(p.M, BM), tiles_n = (int)ceil_div(p.N, kWideN);
+            linear_wide_kernel<DT><<<tiles_m * tiles_n, kThreads, kWideLds, stream>>>(p, tiles_m, tiles_n);
+            return check_launch("linear_wide_kernel");
         }
         default: {
             static PerDeviceOnce once;

@@ -117,3 +117,10 @@ def test_linear_graph_replay_and_streams(ext, gpu, T):
         g2.replay()
         torch.cuda.synchronize()
         assert torch.equal(y1, eager) and torch.equal(y2, eager), i
+
+
+@pytest.mark.parametrize("T,K,N", [(2048, 2048, 6144), (1900, 1040, 6000), (2600, 1040, 3440)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_linear_tiles_that_fill_the_last_round(ext, gpu, T, K, N, dt):
+    # packed weights whose 256 x 192 tiles fit the CUs better than 256 x 256 ones, and ragged edges
+    _check(ext, gpu, T, K, N, dt, packed=True, bias=True)
