@@ -37,9 +37,13 @@
 //
 // The lengths are on the device, so the grid is sized for the most tiles that T tokens of n
 // sequences can have (T / kQ + n) and each wave finds its tile from the lengths itself: a
-// plan kernel would cost a launch of its own.  Tiles are taken in the order of their index
-// inside their sequence, the highest first: under the causal mask that is heaviest first
-// over all sequences, so short ones fill the end of the grid.
+// plan kernel would cost a launch of its own.  Up to 64 sequences, one per lane, tiles are taken
+// in the order of their index inside their sequence, the highest first: under the causal mask
+// that is heaviest first over all sequences, so short ones fill the end of the grid.  More are
+// walked 256 at a time, at most twice: the tiles of sequences of at least kLongTiles tiles come
+// first, sequence by sequence, then the others' (200 short prompts in 8192 tokens, 32 heads of
+// 128: 117 us, 188 with the order of fewer, whose search reads all lengths a dozen times; 1000
+// prompts 0.54 ms, 1.75).
 #include "prefill_tiles.h"
 
 namespace int8k {
@@ -55,6 +59,8 @@ __device__ __forceinline__ int wave_sum(int v) {
     return __builtin_amdgcn_readfirstlane((int)(b[0] + b[1]));
 }
 
+constexpr int kLongTiles = 8;
+
 // The query tile that rank `i` of the packed order is: sequence tokens [start, start + len),
 // tile qt of them.  False past the last tile; `i` is then the rank behind it.
 struct PackedTile {
@@ -64,59 +70,77 @@ template <int kQ>
 __device__ __forceinline__ bool packed_tile(const int32_t* __restrict__ cu, int n, int T, int& i,
                                             PackedTile& t) {
     const int lane = threadIdx.x & 63;
-    // start and length of this lane's sequence s0 + lane; lengths that would leave the T
-    // tokens are cut, so no offsets lead outside the tensors
-    auto bounds = [&](int s0, int& c0, int& len) {
-        const int s = min(s0 + lane, n - 1);
-        c0 = min(max(cu[s], 0), T);
-        len = s0 + lane < n ? min(max(cu[s + 1], c0), T) - c0 : 0;
+    // bounds that would leave the T tokens are cut, so none leads outside the tensors
+    auto bound = [&](int s) { return min(max(cu[min(s, n)], 0), T); };
+    auto tiles_in = [](int from, int to) { return (max(to - from, 0) + kQ - 1) / kQ; };
+    auto take = [&](int start, int end, int qt) {
+        t.start = start, t.len = end - start, t.qt = qt;
+        return true;
     };
-    int c0, len;
-    bounds(0, c0, len);
-    const int first = (len + kQ - 1) / kQ;  // tiles of the first 64 sequences, kept
-    auto tiles_of = [&](int s0) {
-        if (s0 == 0) return first;
-        int c, l;
-        bounds(s0, c, l);
-        return (l + kQ - 1) / kQ;
-    };
-    // tiles with index >= k
-    auto count = [&](int k) {
-        int c = 0;
-        for (int s0 = 0; s0 < n; s0 += 64) c += wave_sum(max(tiles_of(s0) - k, 0));
-        return c;
-    };
-    const int total = count(0);
-    if (i >= total) {
-        i -= total;
-        return false;
-    }
-    // the tile's index is the largest k with count(k) > i
-    int lo = 0, hi = (T + kQ - 1) / kQ;  // count(hi) == 0
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (count(mid) > i) lo = mid;
-        else hi = mid;
-    }
-    int j = i - count(lo + 1);  // the j-th sequence that has a tile of that index
-    for (int s0 = 0; s0 < n; s0 += 64) {
-        const bool has = tiles_of(s0) > lo;
-        const uint64_t mask = __ballot(has);
-        const int here = __popcll(mask);
-        if (j >= here) {
-            j -= here;
-            continue;
+    if (n <= 64) {
+        const int start = bound(lane), end = bound(lane + 1), tiles = tiles_in(start, end);
+        auto count = [&](int k) { return wave_sum(max(tiles - k, 0)); };  // tiles with index >= k
+        const int total = count(0);
+        if (i >= total) {
+            i -= total;
+            return false;
         }
+        // the tile's index is the largest k with count(k) > i
+        int lo = 0, hi = (T + kQ - 1) / kQ;  // count(hi) == 0
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (count(mid) > i) lo = mid;
+            else hi = mid;
+        }
+        // the j-th sequence that has a tile of that index
+        const int j = i - count(lo + 1);
+        const bool has = tiles > lo;
+        const uint64_t mask = __ballot(has);
         const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
         const int src = __builtin_ctzll(__ballot(has && rank == j));
-        if (s0 > 0) bounds(s0, c0, len);
-        t.start = __builtin_amdgcn_readlane(c0, src);
-        t.len = __builtin_amdgcn_readlane(len, src);
-        t.qt = lo;
-        return true;
+        return take(__builtin_amdgcn_readlane(start, src), __builtin_amdgcn_readlane(end, src), lo);
     }
-    return false;  // not reached: the ranks below `total` all have a sequence
+    int at[5];  // bounds of this lane's 4 sequences
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) at[k] = bound(s0 + 4 * lane + k);
+    };
+    load(0);
+    for (int pass = 0; pass < 2; ++pass) {
+        auto counted = [&](int from, int to) {  // the sequence's tiles if this pass takes them
+            const int tiles = tiles_in(from, to);
+            return (tiles >= kLongTiles) == (pass == 0) ? tiles : 0;
+        };
+        for (int s0 = 0; s0 < n; s0 += 256) {
+            if (n > 256 && (pass > 0 || s0 > 0)) load(s0);
+            int mine = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mine += counted(at[k], at[k + 1]);
+            const int here = wave_sum(mine);
+            if (i >= here) {
+                i -= here;
+                continue;
+            }
+            int upto = mine;  // inclusive sum over the lanes
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int below = __shfl_up(upto, d);
+                upto += lane >= d ? below : 0;
+            }
+            const int src = __builtin_ctzll(__ballot(upto > i));
+            int left = i - __builtin_amdgcn_readlane(upto - mine, src);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int start = __builtin_amdgcn_readlane(at[k], src);
+                const int end = __builtin_amdgcn_readlane(at[k + 1], src);
+                const int tiles = counted(start, end);
+                if (left < tiles) return take(start, end, tiles - 1 - left);
+                left -= tiles;
+            }
+        }
+    }
+    return false;
 }
 
 // ------------------------------------------------------------------ the block

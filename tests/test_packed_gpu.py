@@ -158,3 +158,12 @@ def test_packed_rows_do_not_depend_on_their_neighbours(ext, gpu):
     rest[q] = False
     assert torch.equal(out[:, rest], want[:, rest])
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("long_at", [0, 70, 149])
+def test_packed_long_sequences_among_many(ext, gpu, long_at):
+    # more than 64 sequences, some of them with 8 tiles and more, some empty
+    lens = [(7 * k) % 60 for k in range(150)]
+    lens[long_at], lens[(long_at + 64) % 150] = 1500, 1024
+    c = _case(lens, 2, 1, 64, gpu, tail=5)
+    _check(c, ext.int8_attention_forward_packed(*_args(c), is_causal=True), True)
