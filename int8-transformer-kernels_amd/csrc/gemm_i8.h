@@ -152,7 +152,7 @@ __device__ __forceinline__ void mfma_slice(v16i (&acc)[TM][TN], const v4i (&a)[T
 // are N-contiguous.  With BKN the main loop stages the B tile as it arrives, BK
 // rows of k with the tile's BN bytes of n each (rows padded to KN_STRIDE), and
 // forms each K-contiguous MFMA fragment with two transposing LDS reads
-// (ds_read_b64_tr_b8), so no weight transpose runs.  Measured on the box: in each
+// (ds_read_b64_tr_b8), so no weight transpose runs.  Measured: in each
 // group of 16 lanes, the instruction gives lane 8h + b byte b of the 8-byte rows
 // that lanes h, h+2, ..., h+14 address.  Lane s of group g therefore addresses
 // row 16 (g/2) + s/2 at columns 16 (g%2) + 8 (s%2): lane l then holds

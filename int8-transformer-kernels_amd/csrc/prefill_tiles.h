@@ -37,7 +37,7 @@ struct Shape {
 
 // V' is staged as it arrives, row-major fp16 [key][dim], and the PV MFMA's
 // V^T fragments are formed by transposing LDS reads (ds_read_b64_tr_b16).
-// Measured on the box: in each group of 16 lanes, the instruction gives lane
+// Measured: in each group of 16 lanes, the instruction gives lane
 // 4h + e half e of the 8-byte rows that lanes h, h+4, h+8, h+12 address.  So
 // lane 16G + 4k + h of a wave addresses key row 4 (G/2) + k and dims
 // 16 (G%2) + 4h of a 16-key slice, and lane l then holds dim l % 32 of keys
