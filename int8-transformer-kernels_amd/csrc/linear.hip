@@ -7,7 +7,7 @@
 // gemm_i8_paths.h); the routes differ in how the result leaves:
 //   skinny   32 x 32 tiles, K over the waves of a block (few tokens, small packed weights)
 //   stream   the weights streamed once over all CUs, exact int32 partials, then rows
-//   small    64 x 64 tiles, four blocks per CU
+//   small    64 x 64 tiles, four blocks per CU, or one of two wave groups that halve K
 //   mid      128 x 128 tiles, two blocks per CU; K split into partials where CUs would idle
 //   wide     256 x 192 tiles, packed weights
 //   tiled    256 x 256 tiles
@@ -341,19 +341,19 @@ struct SmallLds {
     static constexpr int kBStride = BKN ? kSmB + 32 : LDS_STRIDE;
     static constexpr int kA = kSmB * LDS_STRIDE;
     static constexpr int kStage = kA + (BKN ? BK : kSmB) * kBStride;
-    static constexpr int kScales = 2 * kStage;
-    static constexpr int kBytes = kScales + 3 * kSmB * 4;
+    static constexpr int scales(int groups) { return groups * 2 * kStage; }
+    static constexpr int bytes(int groups) { return scales(groups) + 3 * kSmB * 4; }
 };
 
+// nk steps of K from kb, the part of them below ke; t: thread within its group of 4 waves.
 template <bool EDGE, bool BKN>
-__device__ __forceinline__ void small_mainloop(v16i& acc, const LinearArgs& p, int kb, int ke,
-                                               int m0, int n0, char* lds) {
+__device__ __forceinline__ void small_mainloop(v16i& acc, const LinearArgs& p, int kb, int ke, int nk,
+                                               int m0, int n0, int t, char* lds) {
     using L = SmallLds<BKN>;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = t & 63, wave = t >> 6;
     const int wm = wave >> 1, wn = wave & 1;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0;
-    const int nk = (ke - kb + BK - 1) / BK;
     const int a_off = (wm * 32 + (lane & 31)) * LDS_STRIDE + (lane >> 5) * 16;
     const int g16 = lane >> 4, s16 = lane & 15;
     const int b_off = L::kA + (BKN ? (16 * (g16 >> 1) + (s16 >> 1)) * L::kBStride + wn * 32 +
@@ -370,7 +370,7 @@ __device__ __forceinline__ void small_mainloop(v16i& acc, const LinearArgs& p, i
         const int k0 = kb + kt * BK;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int c = threadIdx.x + i * kThreads;
+            const int c = t + i * kThreads;
             const int row = c / kChunksPerRow, gk = min(k0 + (c % kChunksPerRow) * 16, p.K - 16);
             f.a[i] = *reinterpret_cast<const int4*>(p.x + (size_t)min(m0 + row, p.M - 1) * p.K + gk);
             if constexpr (BKN)
@@ -384,7 +384,7 @@ __device__ __forceinline__ void small_mainloop(v16i& acc, const LinearArgs& p, i
         const int k0 = kb + kt * BK;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int c = threadIdx.x + i * kThreads;
+            const int c = t + i * kThreads;
             const int row = c / kChunksPerRow, kc = (c % kChunksPerRow) * 16;
             const int br = BKN ? c >> 2 : row, bc = BKN ? (c & 3) * 16 : kc;
             int4 va = f.a[i], vb = f.b[i];
@@ -438,22 +438,45 @@ __device__ __forceinline__ void small_mainloop(v16i& acc, const LinearArgs& p, i
 
 static_assert(4 * 32 * kEpiRow<INT8K_DTYPE_F32, 1> <= 2 * SmallLds<false>::kStage, "fits");
 
-template <int DT, bool BKN>
-__global__ __launch_bounds__(kThreads, 4) void linear_small_kernel(LinearArgs p, int tiles_m,
-                                                                   int tiles_n) {
+// KG groups of 4 waves take a KG-th of K each, with stages of their own; their sums meet in LDS.
+template <int DT, bool BKN, int KG>
+__global__ __launch_bounds__(kThreads * KG, 4 / KG) void linear_small_kernel(LinearArgs p, int tiles_m,
+                                                                             int tiles_n) {
+    using L = SmallLds<BKN>;
     extern __shared__ __align__(16) char lds[];
     int tm, tn;
     tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * kSmB, n0 = tn * kSmB;
     const TileScales s = load_scales<kSmB>(p, m0, n0);
+    const int t = threadIdx.x % kThreads, group = KG == 1 ? 0 : threadIdx.x / kThreads;
+    const int nk = (p.K + KG * BK - 1) / (KG * BK);
+    const int kb = group * nk * BK, ke = min(p.K, kb + nk * BK);
+    char* stages = lds + group * 2 * L::kStage;
     v16i acc[1][1];
-    if (m0 + kSmB <= p.M && n0 + kSmB <= p.N && p.K % BK == 0)
-        small_mainloop<false, BKN>(acc[0][0], p, 0, p.K, m0, n0, lds);
+    if (m0 + kSmB <= p.M && n0 + kSmB <= p.N && p.K % (KG * BK) == 0)
+        small_mainloop<false, BKN>(acc[0][0], p, kb, ke, nk, m0, n0, t, stages);
     else
-        small_mainloop<true, BKN>(acc[0][0], p, 0, p.K, m0, n0, lds);
-    float* scales = reinterpret_cast<float*>(lds + SmallLds<BKN>::kScales);
+        small_mainloop<true, BKN>(acc[0][0], p, kb, ke, nk, m0, n0, t, stages);
+    if constexpr (KG > 1) {
+        static_assert(KG == 2 && kThreads * 64 <= 2 * L::kStage, "the second group's sums fit its stages");
+        if (group > 0)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                reinterpret_cast<v4i*>(stages)[q * kThreads + t] =
+                    v4i{acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
+    }
+    float* scales = reinterpret_cast<float*>(lds + L::scales(KG));
     park_scales<kSmB>(s, scales);
-    const int wave = threadIdx.x >> 6;
+    if constexpr (KG > 1) {
+        if (group > 0) return;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const v4i x = reinterpret_cast<const v4i*>(lds + 2 * L::kStage)[q * kThreads + t];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[0][0][4 * q + k] += x[k];
+        }
+    }
+    const int wave = t >> 6;
     epilogue_rows<DT, 1, 1, kSmB>(acc, p, m0, n0, (wave >> 1) * 32, (wave & 1) * 32,
                                   lds + wave * 32 * kEpiRow<DT, 1>, scales);
 }
@@ -547,7 +570,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void linear_skinny_kernel(Linear
 
 // ------------------------------------------------------------------ plan, launch
 
-enum class LinearRoute { kSkinny, kStream, kSmall, kMid, kWide, kTiled };
+enum class LinearRoute { kSkinny, kStream, kSmall, kSmallTwo, kMid, kWide, kTiled };
 
 struct LinearPlan {
     LinearRoute route;
@@ -564,8 +587,10 @@ struct LinearPlan {
 //    T = 128, 2048 -> 2560 10.4 / 10.5; T = 512, 1024 -> 1024 6.7 / 6.8);
 //  - stream: a read of the weights per 32 or 64 rows behind a start and a second kernel (T = 1,
 //    4096 -> 6144 9.8 / 9.6; T = 64 14.6 / 14.6);
-//  - small: 0.34 us a step to 256 blocks, 0.24 per 256 beyond (T = 333, 2048 -> 2560 8.4 / 8.9,
-//    16.6 on 128 x 128 tiles; T = 512, 4096 -> 4096 18.4 / 18.7, 24.6; T = 1000 33.7 / 34.1, 30.8);
+//  - small: 0.34 us a step to 256 blocks, 0.24 per 256 beyond (T = 512, 4096 -> 4096 18.4 / 18.7,
+//    24.6 on 128 x 128 tiles; T = 1000 33.7 / 34.1, 30.8); to 256 blocks with K over two wave
+//    groups 0.46 us per two steps (T = 333, 2048 -> 2560 7.9 / 8.4, 9.3 with one group, 16.6 on
+//    128 x 128 tiles; T = 512, 4096 -> 2048 11.6 / 12.0, 14.8; T = 256, 1024 -> 4096 6.0 / 6.1, 5.9);
 //  - mid: 0.78 us a step for a block alone on its CU, 1.33 for two, 1.1 and up where some have
 //    two (T = 1000, 4096 -> 6144 44 / 40); split over K, the partials' traffic and a second
 //    kernel (T = 512, 4096 -> 4096 27.5 / 24.6; T = 128, 4096 -> 6144 in 4
@@ -607,6 +632,7 @@ LinearPlan linear_plan(int M, int K, int N, bool packed) {
     {
         const long long rounds = ceil_div(ceil_div(M, kSmB) * ceil_div(N, kSmB), 256);
         better(300 + steps * (rounds == 1 ? 34 : 24 * rounds), LinearRoute::kSmall);
+        if (rounds == 1) better(420 + ceil_div(steps, 2) * 46, LinearRoute::kSmallTwo);
     }
     const long long nk = (long long)N * K;
     if (M <= 512) {
@@ -641,6 +667,16 @@ int launch_rows(const LinearArgs& p, int splits, hipStream_t stream) {
     return check_launch("linear_rows_kernel");
 }
 
+template <int DT, bool BKN, int KG>
+int launch_small(const LinearArgs& p, hipStream_t stream) {
+    static PerDeviceOnce once;
+    constexpr int kBytes = SmallLds<BKN>::bytes(KG);
+    const int tiles_m = (int)ceil_div(p.M, kSmB), tiles_n = (int)ceil_div(p.N, kSmB);
+    if (const int st = set_lds(once, (const void*)linear_small_kernel<DT, BKN, KG>, kBytes)) return st;
+    linear_small_kernel<DT, BKN, KG><<<tiles_m * tiles_n, kThreads * KG, kBytes, stream>>>(p, tiles_m, tiles_n);
+    return check_launch("linear_small_kernel");
+}
+
 template <int DT, bool BKN>
 int launch_linear(const LinearArgs& p, const LinearPlan& pl, hipStream_t stream) {
     switch (pl.route) {
@@ -660,16 +696,10 @@ int launch_linear(const LinearArgs& p, const LinearPlan& pl, hipStream_t stream)
                 return st;
             return launch_rows<DT>(p, pl.splits, stream);
         }
-        case LinearRoute::kSmall: {
-            static PerDeviceOnce once;
-            const int tiles_m = (int)ceil_div(p.M, kSmB), tiles_n = (int)ceil_div(p.N, kSmB);
-            if (const int st = set_lds(once, (const void*)linear_small_kernel<DT, BKN>,
-                                       SmallLds<BKN>::kBytes))
-                return st;
-            linear_small_kernel<DT, BKN>
-                <<<tiles_m * tiles_n, kThreads, SmallLds<BKN>::kBytes, stream>>>(p, tiles_m, tiles_n);
-            return check_launch("linear_small_kernel");
-        }
+        case LinearRoute::kSmall:
+            return launch_small<DT, BKN, 1>(p, stream);
+        case LinearRoute::kSmallTwo:
+            return launch_small<DT, BKN, 2>(p, stream);
         case LinearRoute::kMid: {
             static PerDeviceOnce once, once_split;
             const int tiles = pl.mid.tiles_m * pl.mid.tiles_n;

@@ -124,3 +124,11 @@ def test_linear_graph_replay_and_streams(ext, gpu, T):
 def test_linear_tiles_that_fill_the_last_round(ext, gpu, T, K, N, dt):
     # packed weights whose 256 x 192 tiles fit the CUs better than 256 x 256 ones, and ragged edges
     _check(ext, gpu, T, K, N, dt, packed=True, bias=True)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("T,K,N", [(333, 2048, 2560), (300, 2064, 2576), (500, 4096, 2048), (130, 2176, 4112),
+                                   (256, 3840, 4096)])
+def test_linear_k_over_two_wave_groups(ext, gpu, T, K, N, packed):
+    # at most 256 tiles of 64 x 64 and a long K: whole and ragged halves of it
+    _check(ext, gpu, T, K, N, torch.bfloat16, packed, bias=True)
