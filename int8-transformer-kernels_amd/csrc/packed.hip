@@ -13,7 +13,7 @@
 // prefill.hip's blocks:
 //  - V enters as exact fp16 and its scale goes into the weights, P = fp16(p sV): one rounding per
 //    term.  (With V sV rounded beside P the error against 64 bits is 1.8 times that of the
-//    formula in fp32 with one fp16 rounding of P, with this 1.4.)  l sums p in fp32.  It costs a
+//    formula in fp32 with the output rounded once, with this 1.1-1.3.)  l sums p in fp32.  It costs a
 //    multiplication and an addition more per score, 5-12% on prompts past 4096 tokens.
 //  - Only a wave's first tile takes the exact step that finds a maximum; diagonal and ragged
 //    tiles run the ordinary step with a mask.  Prompts of 300 to 2000 tokens gain 6-20%.
@@ -161,7 +161,7 @@ struct PackedLds {
 
 constexpr int kPackedWaves = 4;              // per block, 32 queries each
 constexpr float kPackedMaxWeight = 60000.f;  // fp16 weights stay below it
-constexpr int kPackedMaxShift = 60;          // |m - running maximum| where m is set
+constexpr float kPackedMaxShift = 60.f;          // |m - running maximum| where m is set
 
 template <int D, bool CAUSAL, bool PAD, typename OutRow>
 __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restrict__ Qh,
@@ -361,8 +361,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         return (e[0] + e[1]) + (e[2] + e[3]);
     };
     float over = 1.f;  // not 0: the query's weights leave the range of m
-    // The exact path: sets m so that the largest weight p sV of the tile lies in [0.5, 1) and
-    // rescales O and l.
+    // The exact path: sets m so that the largest weight p sV of the tile is 1 and rescales O and l.
     auto slow = [&](int i, const float* sc, v8h (&p)[4]) {
         const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
         auto seen = [&](int key) { return key <= last; };
@@ -392,10 +391,11 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
             __builtin_amdgcn_sched_barrier(0);
         }
         pm = max_xor32(pm);
-        int e = 0;
-        if (pm > 0.f && pm < INFINITY) frexpf(pm, &e);
+        // the largest weight becomes 1, which fp16 holds exactly: a row of one key, or one that
+        // a key dominates, has no rounding error from it
+        const float shift = pm > 0.f && pm < INFINITY ? __builtin_amdgcn_logf(pm) : 0.f;
         // (a query whose weights fit keeps its m, whatever its neighbours in the wave hold)
-        const float raised = fmaxf(m, top + (float)min(max(e, -kPackedMaxShift), kPackedMaxShift));
+        const float raised = fmaxf(m, top + fminf(fmaxf(shift, -kPackedMaxShift), kPackedMaxShift));
         const float m_new = max_xor32(over) != 0.f ? raised : m;
         const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
         m = m_new;

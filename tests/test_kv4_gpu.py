@@ -280,3 +280,11 @@ def test_decode_offsets_past_32_bits(ext, gpu):
     small = dict(c, K=K[NP - 2:].clone(), V=V[NP - 2:].clone(), sK=sK[NP - 2:].clone(), sV=sV[NP - 2:].clone(),
                  tables=torch.tensor([[1, 0]], dtype=torch.int32, device=gpu))
     _check(small, out)
+
+
+def test_decode_of_one_position_rounds_only_its_output(ext, gpu):
+    # one key: the weight cancels but for its 22 bits (2^-22) and a few fp32 roundings (2^-21
+    # together), and the output rounds once (2^-11)
+    c = kv4_case(15, 6, 16, 4, 64, 16, [1] * 6, gpu)
+    ref, _ = G.kv4_decode(*(c[k].cpu().numpy() for k in ("Q", "K", "V", "sQ", "sK", "sV", "tables", "lens")))
+    assert_within(np64(_decode(ext, c)), ref, (2.0 ** -11 + 2.0 ** -20) * np.abs(ref) + 2.0 ** -25)

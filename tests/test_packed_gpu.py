@@ -167,3 +167,12 @@ def test_packed_long_sequences_among_many(ext, gpu, long_at):
     lens[long_at], lens[(long_at + 64) % 150] = 1500, 1024
     c = _case(lens, 2, 1, 64, gpu, tail=5)
     _check(c, ext.int8_attention_forward_packed(*_args(c), is_causal=True), True)
+
+
+def test_packed_prompts_of_one_token_round_only_their_output(ext, gpu):
+    # one key, whose weight is exactly 1 in fp16: a few fp32 roundings (2^-20 together) and the
+    # output's (2^-11)
+    c = _case([1] * 40, 4, 2, 64, gpu, seed=9)
+    ref, _ = _oracle(c, True)
+    out = ext.int8_attention_forward_packed(*_args(c), is_causal=True)
+    assert_within(np64(out), ref, (2.0 ** -11 + 2.0 ** -19) * np.abs(ref) + 2.0 ** -25)
