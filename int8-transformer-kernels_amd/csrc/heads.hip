@@ -198,7 +198,8 @@ __device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0,
     if constexpr (LAYOUT != kSplitAny) lo = load8<DT>(p.x, in + ia), hi = load8<DT>(p.x, in + ib);
     const float* wp = part < 2 ? p.w[part] : nullptr;
     // (a, b) -> (a ca - b sb, b cb + a sa) / rms: the norm's weights go into the angles.  Pairs
-    // past the rotation have cos 1 and sin 0.
+    // past the rotation have cos 1 and take nothing of the other element, not even its product
+    // with a sine of zero: an infinity or a NaN there is that element's own.
     float ca[8], cb[8], sa[8], sb[8];
     if (part < 2) {
         float wa[8], wb[8];
@@ -259,8 +260,10 @@ __device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0,
             for (int i = 0; i < 8; ++i) {
                 // normed first: squares in range do not promise products in range
                 const float na = a[i] * inv, nv = v[i] * inv;
-                a[i] = na * ca[i] - nv * sb[i];
-                v[i] = nv * cb[i] + na * sa[i];
+                const bool turned = LAYOUT == kSplit ? 8 * cc < p.half : 8 * cc + i < p.half;
+                const float ua = na * ca[i], uv = nv * cb[i];
+                a[i] = turned ? ua - nv * sb[i] : ua;
+                v[i] = turned ? uv + na * sa[i] : uv;
             }
             round_all<DT>(a);
             round_all<DT>(v);
