@@ -285,7 +285,8 @@ __device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0,
 #pragma unroll
             for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(v[i])));
             m = row_reduce(has ? m : 0.f, p.lg, [](float x, float y) { return fmaxf(x, y); });
-            const float sc = quotient(fmaxf(m, 1e-8f), 127.f, 1.f / 127.f);  // exactly the division
+            // exactly the division (whose correction step has no answer for an infinity)
+            const float sc = m < INFINITY ? quotient(fmaxf(m, 1e-8f), 127.f, 1.f / 127.f) : m;
             const float rinv = 1.f / sc;
             if (ok) {
                 if constexpr (LAYOUT == kSplitAny) {

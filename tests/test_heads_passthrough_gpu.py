@@ -65,3 +65,22 @@ def test_unrotated_infinity_under_a_norm(ext, gpu, D, rot, inter):
     assert torch.isnan(q[2, 5, -1]) and (q[2, 5, :-1] == 0).all()
     q[2, 5] = 0
     assert torch.isfinite(q).all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,rot,inter", LAYOUTS + [(64, 64, False), (128, 128, True), (80, 80, False)])
+def test_quantized_rows_of_non_finite_heads(ext, gpu, D, rot, inter, dt, bad):
+    # an infinity makes its row's scale infinite and every finite code 0, as the per-token
+    # quantizer has it, byte for byte
+    x, cos, sin, pos = _case(D, rot, dt)
+    for t in range(6):
+        x.view(40, 6, D)[6 * t + 1, t, (7 * t + D - 1) % D] = bad
+    args = _to(gpu, x, cos, sin, pos)
+    got = ext.qk_norm_rope(args[0], 4, 1, *args[1:], interleaved=inter)
+    q = ext.qk_norm_rope_quantize(args[0], 4, 1, *args[1:], interleaved=inter)
+    for i in range(3):
+        c, s = ext.quantize_per_token(got[i])
+        assert torch.equal(q[2 * i], c), "qkv"[i]
+        assert torch.equal(q[2 * i + 1].isnan(), s.isnan())
+        assert torch.equal(q[2 * i + 1].nan_to_num(), s.nan_to_num()), "qkv"[i]
