@@ -169,10 +169,13 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict
 // positions: 80 -> 71 us; the loads alone 75 -> 66).
 //
 // p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
-// that the largest weight p sV of the tile that set it lies in [0.5, 1), whatever the size of
+// that the largest weight p sV of the tile that set it lies in [2^9, 2^10), whatever the size of
 // the value scales, and a tile whose weights stay in fp16's range under the current m takes
 // the short path, with no exchange between lanes and no rescaling.  l sums p and O the
-// weighted codes, both in fp32 and both relative to m.
+// weighted codes, both in fp32 and both relative to m.  Below 2^-14 fp16 steps by 2^-24, so a
+// weight is off by at most 2^-25 beside a largest one of 2^9 or more: 65536 equal keys behind
+// one that outweighs them together by 2^8 still add up (with a largest weight below 1 they
+// vanish).  The factor of 60 up to kMaxWeight is the room before a tile takes the long path.
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -185,6 +188,7 @@ constexpr int kMaxRows = 16;    // query heads per block
 constexpr float kMaxWeight = 60000.f;  // fp16 weights stay below it
 constexpr float kMaxSum = 0x1p60f;      // and the sum of a lane's 8 p below this
 constexpr int kMaxShift = 60;           // |m - running maximum| where m is set
+constexpr int kTopExp = 10;             // the largest weight there: below 2^kTopExp
 
 struct Kv4Decode {
     const int8_t* Q;
@@ -416,7 +420,7 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
             pm = max_groups(pm);
             int e = 0;
             if (pm > 0.f && pm < INFINITY) frexpf(pm, &e);
-            const float m_new = fmaxf(m, top + (float)min(max(e, -kMaxShift), kMaxShift));
+            const float m_new = fmaxf(m, top + (float)min(max(e - kTopExp, -kMaxShift), kMaxShift));
             const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
             m = m_new;
             l *= alpha;
@@ -431,9 +435,9 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
             psum = sum8();
         }
         l += psum;
-        // p sV as two fp16, 22 bits of it: in one, the rounding of a row's largest weights
-        // outweighs that of the output (error against 64 bits 1.3 to 1.6 times the plain
-        // form's, 1.0 so; the matrix units have the time)
+        // p sV as two fp16, 22 bits of it down to 2^-3 (2^-12 of the largest): in one, the
+        // rounding of a row's largest weights outweighs that of the output (error against 64
+        // bits 1.3 to 1.6 times the plain form's, 1.0 so; the matrix units have the time)
         v8h pw, pr;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
