@@ -11,29 +11,33 @@
 // walks the keys in tiles of 64 transposed, so that each lane owns one query:
 // S^T = K . Q^T on v_mfma_i32_32x32x32_i8, O^T += V^T . P^T on v_mfma_f32_32x32x16_f16.  Unlike
 // prefill.hip's blocks:
-//  - V enters as exact fp16 and its scale goes into the weights, P = fp16(p sV): one rounding per
-//    term.  (With V sV rounded beside P the error against 64 bits is 1.8 times that of the
-//    formula in fp32 with the output rounded once, with this 1.1-1.3.)  l sums p in fp32.  It costs a
-//    multiplication and an addition more per score, 5-12% on prompts past 4096 tokens.
+//  - V enters as exact fp16 and its scale goes into the weights p sV, each carried in two fp16, its
+//    rounding and what that leaves (22 bits); l sums p in fp32.  The error against 64 bits is that
+//    of the formula in fp32 with the output rounded once (1.1-1.3 times it with one fp16 a
+//    weight, 1.8 with V sV rounded beside it).  The second product with V costs 36-40% more time
+//    at D = 128, 13% at 64 and 26% at 256: 325 us against 231 for the prompts below.
 //  - Only a wave's first tile takes the exact step that finds a maximum; diagonal and ragged
 //    tiles run the ordinary step with a mask.  Prompts of 300 to 2000 tokens gain 6-20%.
 //
-// What bounds it: the issue of a wave's instructions.  At D = 128 a tile is 24 large MFMAs (768
-// cycles) and about 200 vector instructions, 32 of them exponentials of two slots each (930
-// cycles); two waves share a SIMD and take 4100-4800 cycles for a tile each, where the two sums
-// alone are 3400: they overlap little.  Measured (225-240 and 524-558 us from card to card):
-// 225 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8 key heads
-// of 128 (49.6 G multiply-adds under the mask in each product: 0.88 P operations/s); 524 us for
-// one prompt of 8192; 9 us for five requests of at most 70.  Tried:
+// What bounds it: each wave's own chain of scores, softmax and product.  At D = 128 a tile is 40
+// large MFMAs (1340 cycles with the small ones) and 311 vector instructions, 32 of them
+// exponentials of two slots (1380 cycles); by the counters a wave takes 5500 cycles for it, 22% of
+// them waiting on LDS and the barrier and 40% to issue, two waves share a SIMD, and the clock
+// falls to 1.84 GHz under the load (2.4 at most).  Measured: 325 us for prompts of 333, 4096, 17,
+// 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8 key heads of 128 (49.6 G multiply-adds under
+// the mask in each product); 802-827 us for one prompt of 8192; 9.3 us for five requests of at most
+// 70.  Tried:
+//  - the product of one half of a tile among the softmax of the other: 850 us for the long prompt;
+//  - wave priorities around the products or the softmax: 827-834 us;
+//  and with one fp16 a weight (231 us, 590-600 and 9):
 //  - the softmax of a tile next to the MFMAs of its neighbours in one block of instructions (the
-//    next scores and the last product with V): 226 and 528 us, with three K buffers and all
-//    256 registers;
-//  - 8 waves and 256 queries per block, half the staging per query: 237 and 524 us, and 51
-//    against 43 us for eight prompts of 512;
-//  - steps of 32 keys, half the code and three quarters of the registers: 236 and 559 us, and 8.5
-//    against 9.1 us for the five short requests;
+//    next scores and the last product with V): no gain, with three K buffers and all 256 registers;
+//  - 8 waves and 256 queries per block, half the staging per query: no gain, and 51 against 43 us
+//    for eight prompts of 512;
+//  - steps of 32 keys, half the code and three quarters of the registers: 5% more for long prompts,
+//    8.5 against 9.1 us for the five short requests;
 //  - log2 sV in the exponent and l by an MFMA over 4 x 4 blocks, 2 vector instructions less per
-//    score: 225 and 525 us, each small MFMA waiting for the large ones.
+//    score: no gain, each small MFMA waiting for the large ones.
 //
 // The lengths are on the device, so the grid is sized for the most tiles that T tokens of n
 // sequences can have (T / kQ + n) and each wave finds its tile from the lengths itself: a
@@ -159,9 +163,22 @@ struct PackedLds {
     static constexpr int kBytes = kS + 2 * kSFloats * 4;
 };
 
+// w less half I of t, exactly where t is w rounded to fp16 (one instruction: the compiler widens
+// the half first).
+template <int I, typename H2>
+__device__ __forceinline__ float minus_half(float w, H2 t) {
+    float d;
+    if constexpr (I == 0)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(t), "v"(w));
+    else
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(t), "v"(w));
+    return d;
+}
+
 constexpr int kPackedWaves = 4;              // per block, 32 queries each
 constexpr float kPackedMaxWeight = 60000.f;  // fp16 weights stay below it
-constexpr float kPackedMaxShift = 60.f;          // |m - running maximum| where m is set
+constexpr float kPackedMaxShift = 60.f;      // |m - running maximum| where m is set
+constexpr float kPackedTopExp = 8.f;         // the largest weight there is 2^kPackedTopExp
 
 template <int D, bool CAUSAL, bool PAD, typename OutRow>
 __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restrict__ Qh,
@@ -283,22 +300,19 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    // S^T = K . Q^T of a tile, two 32-key halves
-    v16i sacc[2];
+    // S^T = K . Q^T of a tile's 32 keys from 32 T
     const int k_lane = (lane & 31) * L::kKStride + 16 * h;
-    auto scores = [&](const char* kbuf) {
+    auto scores = [&](const char* kbuf, int T) {
+        v4i kf[NS];
 #pragma unroll
-        for (int T = 0; T < 2; ++T) {
-            v4i kf[NS];
+        for (int s = 0; s < NS; ++s)
+            kf[s] = *reinterpret_cast<const v4i*>(kbuf + k_lane + T * 32 * L::kKStride + s * 32);
+        v16i a;
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
-                kf[s] = *reinterpret_cast<const v4i*>(kbuf + k_lane + T * 32 * L::kKStride + s * 32);
+        for (int z = 0; z < 16; ++z) a[z] = 0;
 #pragma unroll
-            for (int z = 0; z < 16; ++z) sacc[T][z] = 0;
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                sacc[T] = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[s], qf[s], sacc[T], 0, 0, 0);
-        }
+        for (int s = 0; s < NS; ++s) a = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[s], qf[s], a, 0, 0, 0);
+        return a;
     };
     // O^T += V^T . P^T, the V^T fragments by transposing reads (see VLayout)
     typedef _Float16 v4h __attribute__((ext_vector_type(4)));
@@ -306,7 +320,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     typedef __attribute__((address_space(3))) v4s lds_v4s;
     const int v_lane = (4 * h + ((lane & 15) >> 2)) * 2 * L::kVRow +
                        2 * (16 * ((lane >> 4) & 1) + 4 * (lane & 3));
-    auto product = [&](const char* vbuf, const v8h (&p)[4]) {
+    auto product = [&](const char* vbuf, const v8h (&p)[4], const v8h (&r)[4]) {
 #pragma unroll
         for (int j = 0; j < NS; ++j)
 #pragma unroll
@@ -317,23 +331,25 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
                     v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(a + 16 * L::kVRow)));
                 const v8h v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
                 o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[ks], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, r[ks], o[j], 0, 0, 0);
             }
-        // the fragments (two reads each) 4 MFMAs ahead of their use
+        // the fragments (two reads each) kAhead pairs of MFMAs ahead of their use
+        constexpr int kAhead = 2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        for (int i = 0; i < kAhead; ++i) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
-        for (int i = 0; i < 4 * NS - 4; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        for (int i = 0; i < 4 * NS - kAhead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * kAhead, 0);
     };
     // The weights of a lane's four keys of chunk ch, 32 (ch / 4) + 8 (ch % 4) + 4 h + 0..3, their
-    // scores being registers 4 (ch % 4) .. + 3 of half ch / 4: p = 2^(x - m), P = fp16(p sV).
-    // Returns the sum of p.  sQ sK comes from an MFMA over 4 x 4 blocks (lanes 4b .. 4b + 3, the
+    // scores being registers 4 (ch % 4) .. + 3 of its half's: p = 2^(x - m), P = p sV as
+    // P + R in fp16.  Returns the sum of e.  sQ sK comes from an MFMA over 4 x 4 blocks (lanes 4b .. 4b + 3, the
     // outer product of a lane's own key scale with the lanes' query scales), which leaves one
-    // multiplication less per score than sK read as it is: 520 us against 529 at 8192 tokens, 32
-    // heads of 128.
+    // multiplication less per score than sK read as it is (2% at 8192 tokens, 32 heads
+    // of 128).
     typedef float v4f __attribute__((ext_vector_type(4)));
     auto scale_qk = [&](int ch, const float* sc) {
         return __builtin_amdgcn_mfma_f32_4x4x1f32(sc[32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + (lane & 3)], qscale,
@@ -342,29 +358,40 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     auto scale_v = [&](int ch, const float* sc) {
         return *reinterpret_cast<const v4f*>(sc + kKV + 32 * (ch >> 2) + 8 * (ch & 3) + 4 * h);
     };
-    auto weights = [&](int ch, const float* sc, v8h (&p)[4], auto mask, auto seen) {
+    auto weights = [&](int ch, const v16i& s, const float* sc, v8h (&p)[4], v8h (&r)[4], auto mask, auto seen) {
         const int T = ch >> 2, g = ch & 3;
         const v4f sqk = scale_qk(ch, sc), sv = scale_v(ch, sc);
-        float e[4];
+        float e[4], w[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            e[c] = fast_exp2(fmaf(static_cast<float>(sacc[T][4 * g + c]), sqk[c], -m));
-            float w = e[c] * sv[c];
-            asm("" : "+v"(w));  // rounded to fp32 first in every copy of this code
+            e[c] = fast_exp2(fmaf(static_cast<float>(s[4 * g + c]), sqk[c], -m));
+            w[c] = e[c] * sv[c];
+            asm("" : "+v"(w[c]));  // rounded to fp32 first in every copy of this code
             if constexpr (decltype(mask)::value) {
                 const bool ok = seen(32 * T + 8 * g + 4 * h + c);
                 e[c] = ok ? e[c] : 0.f;
-                w = ok ? w : 0.f;
+                w[c] = ok ? w[c] : 0.f;
             }
-            p[2 * T + (g >> 1)][4 * (g & 1) + c] = (_Float16)w;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            const h2 top = __builtin_convertvector((f2){w[c], w[c + 1]}, h2);
+            const h2 rest = __builtin_convertvector((f2){minus_half<0>(w[c], top), minus_half<1>(w[c + 1], top)}, h2);
+            const int at = 4 * (g & 1) + c;
+            p[2 * T + (g >> 1)][at] = top.x, p[2 * T + (g >> 1)][at + 1] = top.y;
+            r[2 * T + (g >> 1)][at] = rest.x, r[2 * T + (g >> 1)][at + 1] = rest.y;
         }
         return (e[0] + e[1]) + (e[2] + e[3]);
     };
+    auto k_buf = [&](int i) { return smem + (i & 1) * L::kKBytes; };
     float over = 1.f;  // not 0: the query's weights leave the range of m
     // The exact path: sets m so that the largest weight p sV of the tile is 1 and rescales O and l.
-    auto slow = [&](int i, const float* sc, v8h (&p)[4]) {
+    auto slow = [&](int i, const float* sc, v8h (&p)[4], v8h (&r)[4]) {
         const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
         auto seen = [&](int key) { return key <= last; };
+        const v16i sacc[2] = {scores(k_buf(i), 0), scores(k_buf(i), 1)};
         float top = -INFINITY;
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch) {
@@ -391,11 +418,13 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
             __builtin_amdgcn_sched_barrier(0);
         }
         pm = max_xor32(pm);
-        // the largest weight becomes 1, which fp16 holds exactly: a row of one key, or one that
-        // a key dominates, has no rounding error from it
+        // The largest weight becomes 2^kPackedTopExp, which fp16 holds exactly.  Below 2^-14 fp16
+        // steps by 2^-24, so a weight is off by at most 2^-33 of the largest, and long flat
+        // tails add up; the factor of 234 up to kPackedMaxWeight is the room before a tile
+        // (the sum of its weights) takes this path again.
         const float shift = pm > 0.f && pm < INFINITY ? __builtin_amdgcn_logf(pm) : 0.f;
         // (a query whose weights fit keeps its m, whatever its neighbours in the wave hold)
-        const float raised = fmaxf(m, top + fminf(fmaxf(shift, -kPackedMaxShift), kPackedMaxShift));
+        const float raised = fmaxf(m, top + fminf(fmaxf(shift - kPackedTopExp, -kPackedMaxShift), kPackedMaxShift));
         const float m_new = max_xor32(over) != 0.f ? raised : m;
         const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
         m = m_new;
@@ -407,7 +436,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         float psum = 0.f;  // (summed as in a step that keeps m)
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            psum += weights(c, sc, p, std::true_type{}, seen);
+            psum += weights(c, sacc[c >> 2], sc, p, r, std::true_type{}, seen);
             __builtin_amdgcn_sched_barrier(0);
         }
         l += psum;
@@ -419,7 +448,6 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     // Step i reads buffer i & 1 while the registers hold tile i + 1, loaded during step i - 1;
     // at its end that goes to the other buffer, the loads of tile i + 2 go out, and the step's
     // one barrier follows.
-    auto k_buf = [&](int i) { return smem + (i & 1) * L::kKBytes; };
     auto v_buf = [&](int i) { return smem + L::kV + (i & 1) * L::kVBytes; };
     KeyLoads pk;
     ScaleLoads ps;
@@ -442,19 +470,19 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         fetch(i + 2);
         __syncthreads();
     };
-    // The steps up to `end` that keep m; false where step i, whose scores are in sacc, has
-    // weights that leave the range m gives them, before anything of it is in O.
+    // The steps up to `end` that keep m; false where step i has weights that leave the range m
+    // gives them, before anything of it is in O.
     int i = 0;
     auto steps = [&](int end, auto mask) {
         for (; i < end; ++i) {
             const float* sc = scales_of(i);
             const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
-            scores(k_buf(i));
-            v8h p[4];
+            v8h p[4], r[4];
             float psum = 0.f;
+            const v16i sacc[2] = {scores(k_buf(i), 0), scores(k_buf(i), 1)};
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                psum += weights(c, sc, p, mask, [&](int key) { return key <= last; });
+                psum += weights(c, sacc[c >> 2], sc, p, r, mask, [&](int key) { return key <= last; });
                 // (keeps the scales of all chunks from being read first: 2-9% at D = 256)
                 if (c & 1) __builtin_amdgcn_sched_barrier(0);
             }
@@ -462,7 +490,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
             over = psum * sc[2 * kKV] <= kPackedMaxWeight && psum <= 0x1p60f ? 0.f : 1.f;
             if (__ballot(over != 0.f) != 0) return false;
             l += psum;
-            product(v_buf(i), p);
+            product(v_buf(i), p, r);
             advance(i);
         }
         return true;
@@ -473,11 +501,10 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
             if (steps(nd, std::true_type{}) && steps(n, std::false_type{})) break;
         }
         if (computes(i)) {
-            if (!running) scores(k_buf(i));
             running = true;
-            v8h p[4];
-            slow(i, scales_of(i), p);
-            product(v_buf(i), p);
+            v8h p[4], r[4];
+            slow(i, scales_of(i), p, r);
+            product(v_buf(i), p, r);
         }
         advance(i);
         ++i;

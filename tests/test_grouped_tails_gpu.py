@@ -60,3 +60,32 @@ def test_decode_flat_tail(ext, gpu, B, n, D, at):
         want = _expected(n - 1, gap, 1.0)
         err = (got[:, h] - want).abs().max().item()
         assert err <= _bound(want, n, gap, 1.0, n // 32), (h, gap, got[0, h, 0].item(), want)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,causal", [(8192, True), (8192, False), (65536, True)])
+@pytest.mark.parametrize("at", ["first", "middle", "last"])
+def test_packed_flat_tail(ext, gpu, n, D, causal, at):
+    if n > 8192 and D > 64:
+        pytest.skip("the long row once, at the smallest head")
+    H = len(GAPS)
+    where = {"first": 0, "middle": n // 2 + 5, "last": n - 40}[at]
+    q = torch.zeros(H, n, D, dtype=torch.int8, device=gpu)
+    q[:, -30:] = 100  # the queries that are looked at, all behind the dominant key
+    k = torch.zeros(1, n, D, dtype=torch.int8, device=gpu)
+    k[0, where] = 7
+    v = torch.full((1, n, D), 10, dtype=torch.int8, device=gpu)
+    v[0, where] = 70
+    v[0, where, : D // 2] = 0
+    sq = torch.tensor([g * math.log(2) * math.sqrt(D) / (700 * D) for g in GAPS], device=gpu)
+    sq = sq.unsqueeze(1).expand(H, n).contiguous()
+    one = torch.ones(1, n, device=gpu)
+    out = ext.int8_attention_forward_packed(
+        q, k, v, sq, one, one * 0.1, torch.tensor([0, n], dtype=torch.int32, device=gpu), is_causal=causal)
+    got = out[:, -30:, : D // 2].double().cpu()
+    for h, gap in enumerate(GAPS):
+        for i in range(30):
+            seen = n - 29 + i if causal else n
+            want = _expected(seen - 1, gap, 1.0)
+            err = (got[h, i] - want).abs().max().item()
+            assert err <= _bound(want, n, gap, 1.0, n // 16) + 2.0 ** -22 * want, (h, i, gap, got[h, i, 0].item(), want)
