@@ -580,72 +580,97 @@ struct LinearPlan {
     size_t bytes(int M, int N) const { return (size_t)splits * M * N * 4; }
 };
 
-// The route with the least estimated time (0.01 us; `steps` of 128 deep).  Fits of each route
-// timed at T = 1 .. 4096 and 512 -> 768 .. 4096 -> 6144, estimated / measured (us):
-//  - skinny: 3 us and, per 1024 of K and round of 256 blocks, 1.85 us, less for few rows, whose
-//    lanes load the same lines (T = 1, 1024 -> 1024 4.2 / 3.8; T = 32, 4096 -> 4096 10.4 / 10.3;
-//    T = 128, 2048 -> 2560 10.4 / 10.5; T = 512, 1024 -> 1024 6.7 / 6.8);
+// The route with the least estimated time (us).  Fitted to every route timed at 318 sizes: T = 1 to
+// 4096, K = 16 to 131056, N = 16 to 128256, weights that come from memory wherever they do not fit
+// its cache.  No estimate is below the time to read the weights: 5.9 TB/s is the most that any
+// route reached (525 MB in 89 us), and the routes that reach less have their own rate.  `steps`
+// are 128 deep; `cold` is 1 for weights of 16 MiB and more, whose loads take longer than those of
+// small ones.
+//  - small: a step of a block takes a load's latency, or from 256 blocks on its share of the
+//    CU (T = 512, 4096 -> 4096: 21 packed, 26 as stored).  As stored it reads 64 bytes a row:
+//    5.0 TB/s, 3.7 where rows lie a multiple of 4096 bytes apart (28672 columns 35.5 us, 28736 28.8);
+//  - two: up to 256 tiles, a step for each group (T = 64, 4096 -> 6144: 14.5 and 22.7);
+//  - mid: a block alone on its CU, or two; split over K, the partials' traffic and a second kernel
+//    (T = 16, 14336 -> 4096 in 16 splits 16.9, streamed 19.6; T = 128, 4096 -> 28672 whole 35.6);
+//  - wide (packed weights), tiled: the share of rounds and the clock that falls as the GPU fills
+//    (T = 4096, 4096 -> 6144: 100 and 115);
 //  - stream: a read of the weights per 32 or 64 rows behind a start and a second kernel (T = 1,
-//    4096 -> 6144 9.8 / 9.6; T = 64 14.6 / 14.6);
-//  - small: 0.34 us a step to 256 blocks, 0.24 per 256 beyond (T = 512, 4096 -> 4096 18.4 / 18.7,
-//    24.6 on 128 x 128 tiles; T = 1000 33.7 / 34.1, 30.8); to 256 blocks with K over two wave
-//    groups 0.46 us per two steps (T = 333, 2048 -> 2560 7.9 / 8.4, 9.3 with one group, 16.6 on
-//    128 x 128 tiles; T = 512, 4096 -> 2048 11.6 / 12.0, 14.8; T = 256, 1024 -> 4096 6.0 / 6.1, 5.9);
-//  - mid: 0.78 us a step for a block alone on its CU, 1.33 for two, 1.1 and up where some have
-//    two (T = 1000, 4096 -> 6144 44 / 40); split over K, the partials' traffic and a second
-//    kernel (T = 512, 4096 -> 4096 27.5 / 24.6; T = 128, 4096 -> 6144 in 4
-//    splits 16.3 / 16.2);
-//  - tiled: 1.25 us a step and round, 0.55 more where the grid fills the GPU and the clock
-//    falls with the power (T = 4096, 4096 -> 4096 67 / 66, 4096 -> 6144 115 / 112);
-//  - wide (packed weights): 0.98 us and 0.42 (T = 4096, 4096 -> 6144 99 / 102, where tiled takes
-//    115; T = 2048 54 / 53, tiled 59; T = 4096, 4096 -> 4096 99 / 91, tiled 67).
+//    4096 -> 128256 96 us; as stored in rows of whole 128 bytes, or half as much again);
+//  - skinny (packed weights): per 1024 of K and round of 256 blocks, less for few rows, whose lanes
+//    load the same lines (T = 1, 4096 -> 6144 8.6, 4096 -> 128256 92).
+// Chosen / fastest over those sizes: 1.01 in the mean, 1.23 at worst.
+constexpr double kReadRate = 5.9;  // TB/s
+
 LinearPlan linear_plan(int M, int K, int N, bool packed) {
     LinearPlan pl{};
-    const long long steps = ceil_div(K, BK);
-    long long best = -1;
-    auto better = [&](long long time, LinearRoute route) {
+    const double steps = (double)ceil_div(K, BK);
+    const double mb = (double)N * K * 1e-6, out = (double)M * N * 1e-6;  // MB of weights, M outputs
+    const double cold = std::min((double)N * K, 16777216.0) / 16777216.0;
+    const bool ragged = !packed && N % 128 != 0;  // rows as stored are no whole lines
+    double best = -1;
+    auto better = [&](double time, LinearRoute route) {
         if (best >= 0 && time >= best) return false;
         best = time, pl.route = route, pl.splits = 0;
         return true;
     };
     {
-        const long long tiles = ceil_div(M, BM) * ceil_div(N, BN), rounds = ceil_div(tiles, 256);
-        better(900 + steps * (125 * rounds + 55 * tiles / 256), LinearRoute::kTiled);
+        const long long tiles = ceil_div(M, BM) * ceil_div(N, BN);
+        const double rounds = (double)ceil_div(tiles, 256), share = tiles / 256.0;
+        better(packed ? 6.4 + std::max(steps * (0.89 * rounds + 0.93 * share), mb / kReadRate) + 0.35 * out
+                      : 4.9 + std::max(steps * (1.02 * rounds + 0.80 * share), mb / kReadRate) + 0.42 * out,
+               LinearRoute::kTiled);
     }
     if (packed) {
-        const long long tiles = ceil_div(M, BM) * ceil_div(N, kWideN), rounds = ceil_div(tiles, 256);
-        better(900 + steps * (98 * rounds + 42 * tiles / 256), LinearRoute::kWide);
+        const long long tiles = ceil_div(M, BM) * ceil_div(N, kWideN);
+        const double rounds = (double)ceil_div(tiles, 256), share = tiles / 256.0;
+        better(5.0 + std::max(steps * (0.83 * rounds + 0.52 * share), mb / kReadRate) + 0.52 * out,
+               LinearRoute::kWide);
     }
     const long long mid_tiles = ceil_div(M, kMidB) * ceil_div(N, kMidB);
-    for (long long sp = 1; sp <= std::min(16LL, steps); ++sp) {
-        const long long st = ceil_div(steps, sp), n = ceil_div(steps, st);
+    // split where the blocks of whole K leave CUs without their two
+    const long long most = mid_tiles <= 512 ? std::min(16LL, (long long)steps) : 1;
+    for (long long sp = 1; sp <= most; ++sp) {
+        const long long st = ceil_div((long long)steps, sp), n = ceil_div((long long)steps, st);
         if (n != sp) continue;  // the same plan as fewer splits
         const long long blocks = mid_tiles * n, rest = blocks % 512;
-        const long long last = rest > 256 ? 110 + 23 * (rest - 256) / 256 : rest > 0 ? 78 : 0;
-        const long long gemm = st * (133 * (blocks / 512) + last);
-        const long long rows = n > 1 ? 200 + 8 * n * (long long)M * N / 45000 : 0;
-        if (better(250 + gemm + rows + (long long)N * K / 100000, LinearRoute::kMid)) {
+        const double alone = packed ? 0.59 + 0.22 * cold : 0.66 + 0.28 * cold;
+        const double both = packed ? 1.01 : 1.19, more = packed ? 0.16 : 0.09;
+        const double last = rest > 256 ? both + more * (rest - 256) / 256.0 : rest > 0 ? alone : 0.0;
+        const double gemm = st * ((both + more) * (double)(blocks / 512) + last);
+        const double rate = ragged ? 4.0 : n > 1 ? kReadRate : packed ? 4.4 : 5.4;
+        const double rows = n > 1 ? (packed ? 3.65 : 3.23) + 1.56 * n * out : 0.5 * out;
+        if (better(3.3 + std::max(gemm, mb / rate) + rows, LinearRoute::kMid)) {
             pl.mid = MidPlan{(int)ceil_div(M, kMidB), (int)ceil_div(N, kMidB), (int)n, (int)(st * BK)};
             pl.splits = n > 1 ? (int)n : 0;
         }
     }
     {
-        const long long rounds = ceil_div(ceil_div(M, kSmB) * ceil_div(N, kSmB), 256);
-        better(300 + steps * (rounds == 1 ? 34 : 24 * rounds), LinearRoute::kSmall);
-        if (rounds == 1) better(420 + ceil_div(steps, 2) * 46, LinearRoute::kSmallTwo);
+        const long long tiles = ceil_div(M, kSmB) * ceil_div(N, kSmB);
+        const double share = tiles / 256.0;
+        const double step = packed ? std::max(0.24 + 0.256 * cold, 0.08 + 0.224 * share)
+                                   : std::max(0.225 + 0.37 * cold, 0.284 * share);
+        const double rate = packed || N % 4096 != 0 ? 5.0 : 3.7;
+        better((packed ? 3.05 : 3.35) + std::max(steps * step, mb / rate) + 0.5 * out, LinearRoute::kSmall);
+        if (tiles <= 256) {
+            const double two = (double)ceil_div((long long)steps, 2) * (packed ? 0.31 + 0.32 * cold : 0.33 + 0.65 * cold);
+            better((packed ? 3.8 : 4.05) + std::max(two, mb / kReadRate) + 0.5 * out, LinearRoute::kSmallTwo);
+        }
     }
-    const long long nk = (long long)N * K;
     if (M <= 512) {
         const StreamPlan sp = stream_plan(M, N, K);
-        if (better(sp.mt == 1 ? 650 + nk * 13 / 1000000 : 930 + nk * 21 / 1000000 * sp.tiles_m,
-                   LinearRoute::kStream)) {
+        const double rate = packed || (!ragged && N % 4096 != 0) ? kReadRate : ragged ? 3.6 : 4.9;
+        const double start = sp.mt == 1 ? (packed ? 5.7 : 6.4) : (packed ? 8.1 : 8.9);
+        const double rows = sp.mt == 1 ? 0.0 : (0.22 + 0.115 * (sp.tiles_m - 1)) * (ragged ? 1.5 : 1.0);
+        const double join = (packed ? 0.88 : 0.51) * (double)ceil_div(sp.splits, 8) + (packed ? 1.43 : 1.0) * sp.splits * out;
+        if (better(start + std::max(mb * rows, mb / rate) + join, LinearRoute::kStream)) {
             pl.st = sp;
             pl.splits = sp.splits;
         }
     }
     if (packed && K % 128 == 0) {
-        const long long rounds = ceil_div(ceil_div(N, 32) * ceil_div(M, 32), 256);
-        better(300 + (115 + 22 * std::min(M, 32) / 10) * rounds * K / 1024, LinearRoute::kSkinny);
+        const double rounds = (double)ceil_div(ceil_div(N, 32) * ceil_div(M, 32), 256);
+        better(2.7 + std::max((1.3 + 0.021 * std::min(M, 32)) * rounds * K / 1024.0, mb / kReadRate),
+               LinearRoute::kSkinny);
     }
     return pl;
 }
