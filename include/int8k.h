@@ -421,10 +421,14 @@ int int8k_quantize_heads(const void* x, int dtype, int parts, int8_t* q0, float*
  * bias fp32 [N] or NULL.  K and N multiples of 16, K below 131072 (the int32 sum
  * cannot overflow); x and W below 4 GiB (else INT8K_ERR_UNSUPPORTED).  x, W, out and
  * workspace 16-byte aligned.
- * int8k_linear_workspace_bytes: what a call of exactly T rows needs (0: none). */
+ * int8k_linear_workspace_bytes: a workspace of this size serves every call of up to T rows
+ * with the same K, N and flags (fewer rows may need more: their K is split into partials).
+ * int8k_linear_call_workspace_bytes: what a call of exactly T rows needs (0: none), for
+ * callers that allocate per call. */
 #define INT8K_LINEAR_WEIGHT_PREPACKED 1
 
 size_t int8k_linear_workspace_bytes(int T, int K, int N, int flags);
+size_t int8k_linear_call_workspace_bytes(int T, int K, int N, int flags);
 
 int int8k_linear(const int8_t* x, const int8_t* W, void* out, int dtype, const float* scale_x,
                  int n_scale_x, const float* scale_W, int n_scale_W, const float* bias, int T,

@@ -833,7 +833,7 @@ torch::Tensor int8_linear_torch(torch::Tensor x, torch::Tensor W, torch::Tensor 
                                      .device(x.device()));
     const int code = dtype_code(y), flags = prepacked ? INT8K_LINEAR_WEIGHT_PREPACKED : 0;
     const int t = as_int(T, "rows of x"), k = as_int(K, "K"), n = as_int(N, "N");
-    const size_t ws_bytes = int8k_linear_workspace_bytes(t, k, n, flags);
+    const size_t ws_bytes = int8k_linear_call_workspace_bytes(t, k, n, flags);
     auto ws = workspace(ws_bytes, x.device());
     check_status(int8k_linear(xc.data_ptr<int8_t>(), wc.data_ptr<int8_t>(), y.data_ptr(), code,
                               sx.data_ptr<float>(), (int)sx.numel(), sw.data_ptr<float>(),

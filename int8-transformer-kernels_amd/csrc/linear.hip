@@ -599,7 +599,9 @@ struct LinearPlan {
 //  - skinny (packed weights): per 1024 of K and round of 256 blocks, less for few rows, whose lanes
 //    load the same lines (T = 1, 4096 -> 6144 8.6, 4096 -> 128256 92).
 // Chosen / fastest over those sizes: 1.01 in the mean, 1.23 at worst.
-constexpr double kReadRate = 5.9;  // TB/s
+constexpr double kReadRate = 5.9;    // TB/s
+constexpr int kMidSplitTiles = 512;  // 128 x 128 tiles split over K, at most
+constexpr int kStreamRows = 512;     // rows streamed, at most
 
 LinearPlan linear_plan(int M, int K, int N, bool packed) {
     LinearPlan pl{};
@@ -628,7 +630,7 @@ LinearPlan linear_plan(int M, int K, int N, bool packed) {
     }
     const long long mid_tiles = ceil_div(M, kMidB) * ceil_div(N, kMidB);
     // split where the blocks of whole K leave CUs without their two
-    const long long most = mid_tiles <= 512 ? std::min(16LL, (long long)steps) : 1;
+    const long long most = mid_tiles <= kMidSplitTiles ? std::min(16LL, (long long)steps) : 1;
     for (long long sp = 1; sp <= most; ++sp) {
         const long long st = ceil_div((long long)steps, sp), n = ceil_div((long long)steps, st);
         if (n != sp) continue;  // the same plan as fewer splits
@@ -656,7 +658,7 @@ LinearPlan linear_plan(int M, int K, int N, bool packed) {
             better((packed ? 3.8 : 4.05) + std::max(two, mb / kReadRate) + 0.5 * out, LinearRoute::kSmallTwo);
         }
     }
-    if (M <= 512) {
+    if (M <= kStreamRows) {
         const StreamPlan sp = stream_plan(M, N, K);
         const double rate = packed || (!ragged && N % 4096 != 0) ? kReadRate : ragged ? 3.6 : 4.9;
         const double start = sp.mt == 1 ? (packed ? 5.7 : 6.4) : (packed ? 8.1 : 8.9);
@@ -780,9 +782,25 @@ static bool linear_shape_ok(int T, int K, int N) {
            (long long)T * N < (1LL << 36);
 }
 
-extern "C" size_t int8k_linear_workspace_bytes(int T, int K, int N, int flags) {
+extern "C" size_t int8k_linear_call_workspace_bytes(int T, int K, int N, int flags) {
     if (!linear_shape_ok(T, K, N)) return 0;
     return linear_plan(T, K, N, (flags & INT8K_LINEAR_WEIGHT_PREPACKED) != 0).bytes(T, N);
+}
+
+extern "C" size_t int8k_linear_workspace_bytes(int T, int K, int N, int flags) {
+    if (!linear_shape_ok(T, K, N)) return 0;
+    const bool packed = (flags & INT8K_LINEAR_WEIGHT_PREPACKED) != 0;
+    size_t need = 0;
+    auto cover = [&](int first, int last) {
+        need = std::max(need, linear_plan(first, K, N, packed).bytes(last, N));
+    };
+    const int few = std::min(T, kStreamRows);
+    for (int t = 1; t <= few; ++t) cover(t, t);
+    // Past the streamed rows the estimates of 32 rows differ in their terms per row alone, and the
+    // steepest are those of the K splits, steeper the more there are: none has more than the first.
+    for (int t = few + 1; t <= T && ceil_div(t, kMidB) * ceil_div(N, kMidB) <= kMidSplitTiles; t += 32)
+        cover(t, std::min(t + 31, T));
+    return need;
 }
 
 extern "C" int int8k_linear(const int8_t* x, const int8_t* W, void* out, int dtype,

@@ -345,11 +345,10 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * kAhead, 0);
     };
     // The weights of a lane's four keys of chunk ch, 32 (ch / 4) + 8 (ch % 4) + 4 h + 0..3, their
-    // scores being registers 4 (ch % 4) .. + 3 of its half's: p = 2^(x - m), P = p sV as
-    // P + R in fp16.  Returns the sum of e.  sQ sK comes from an MFMA over 4 x 4 blocks (lanes 4b .. 4b + 3, the
+    // scores being registers 4 (ch % 4) .. + 3 of s: e = 2^(x - m), p = fp16(e sV), r = fp16(e sV - p).
+    // Returns the sum of e.  sQ sK comes from an MFMA over 4 x 4 blocks (lanes 4b .. 4b + 3, the
     // outer product of a lane's own key scale with the lanes' query scales), which leaves one
-    // multiplication less per score than sK read as it is (2% at 8192 tokens, 32 heads
-    // of 128).
+    // multiplication less per score than sK read as it is (2% at 8192 tokens, 32 heads of 128).
     typedef float v4f __attribute__((ext_vector_type(4)));
     auto scale_qk = [&](int ch, const float* sc) {
         return __builtin_amdgcn_mfma_f32_4x4x1f32(sc[32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + (lane & 3)], qscale,

@@ -67,6 +67,7 @@ _SIGNATURES = {
     "int8k_mlp_sync_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint)]),
     "int8k_decode_paged_bad_page_ids": (_I, [ctypes.POINTER(ctypes.c_uint)]),
     "int8k_linear_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "int8k_linear_call_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "int8k_linear": (_I, [_P, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _SZ, _P]),
     "int8k_qk_norm_rope": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P, _F, _P, _P, _P] + [_I] * 6 + [_P]),
     "int8k_qk_norm_rope_quantize": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P, _F] + [_P] * 6 +
@@ -545,7 +546,13 @@ ATTN_ZERO_REST = 4           # INT8K_ATTN_ZERO_REST
 
 
 def linear_workspace_bytes(T, K, N, flags=0):
+    """Serves every call of up to T rows."""
     return load().int8k_linear_workspace_bytes(T, K, N, flags)
+
+
+def linear_call_workspace_bytes(T, K, N, flags=0):
+    """What a call of exactly T rows needs."""
+    return load().int8k_linear_call_workspace_bytes(T, K, N, flags)
 
 
 def linear(x, W, scale_x, scale_W, bias=None, flags=0, dtype=None, out=None, workspace=None):
@@ -558,8 +565,8 @@ def linear(x, W, scale_x, scale_W, bias=None, flags=0, dtype=None, out=None, wor
     if out is None:
         out = torch.empty((T, N), dtype=dtype or torch.float16, device=x.device)
     if workspace is None:
-        workspace = torch.empty(max(linear_workspace_bytes(T, K, N, flags), 1), dtype=torch.uint8,
-                                device=x.device)
+        n = linear_call_workspace_bytes(T, K, N, flags)
+        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=x.device)
     check("int8k_linear", load().int8k_linear(
         _ptr(x), _ptr(W), _ptr(out), _dtype_code(out), _ptr(scale_x), scale_x.numel(),
         _ptr(scale_W), scale_W.numel(), _ptr(bias), T, K, N, flags, _ptr(workspace),

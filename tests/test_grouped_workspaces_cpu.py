@@ -9,3 +9,25 @@ def test_linear_reads_wide_stored_weights_on_a_route_that_streams_them(capi, K, 
     # One token against weights as stored: the tiles of 64 columns read 64 bytes a row and are
     # slower than the routes that stream whole lines or split K, which leave partials.
     assert capi.linear_workspace_bytes(1, K, N) >= N * 4
+
+
+@pytest.mark.parametrize("flags", [0, PACKED])
+@pytest.mark.parametrize("K,N", [(4096, 4096), (4096, 6144), (2048, 2560), (14336, 4096), (16384, 16), (131056, 512),
+                                 (1024, 1024), (4096, 28672)])
+def test_linear_workspace_covers_shorter_calls(capi, K, N, flags):
+    # allocated once for the largest batch, used for every one below it
+    need, longest = 0, 0
+    for T in list(range(1, 700)) + [1000, 1023, 1024, 1025, 1500, 2048, 3000, 4096]:
+        need = max(need, capi.linear_call_workspace_bytes(T, K, N, flags))
+        if T in (1, 2, 31, 32, 33, 64, 65, 100, 333, 512, 513, 600, 699) or T >= 1000:
+            whole = capi.linear_workspace_bytes(T, K, N, flags)
+            assert whole >= max(need, longest), T
+            longest = whole
+
+
+def test_linear_workspace_between_the_ranges(capi):
+    # past the streamed rows the query steps by 32 rows: every call inside is covered
+    for K, N in ((14336, 4096), (131056, 512), (16384, 8192)):
+        for T in (545, 800, 1500):
+            whole = capi.linear_workspace_bytes(T, K, N)
+            assert all(capi.linear_call_workspace_bytes(t, K, N) <= whole for t in range(513, T + 1))
