@@ -530,8 +530,9 @@ int int8k_kv4_cache_read(const uint8_t* pages, const float* scales, const int32_
  *   out = sum_j softmax_j(q . k_j sQ sK_j / sqrt(D)) v_j sV_j, q . k exact int32.
  * A page id outside [0, num_pages) reads page num_pages-1 and is counted
  * (int8k_kv4_bad_ids).  Entries past a sequence's length are never read.  The workspace
- * (16-byte aligned) holds partial states of sequences that are split over blocks; the query's
- * answer does not depend on max_context.  0: no workspace is needed. */
+ * (16-byte aligned) holds partial states of sequences that are split over blocks; one of the
+ * queried size serves every call of up to B sequences with the same heads, whatever its
+ * max_context.  0: no workspace is needed. */
 size_t int8k_decode_attention_kv4_paged_workspace_bytes(int B, int heads, int kv_heads,
                                                         int max_context, int head_dim);
 

@@ -586,7 +586,6 @@ __global__ __launch_bounds__(D) void kv4_combine_kernel(const float* __restrict_
 
 struct Kv4Plan {
     int groups, rows, waves, nsplit;
-    int max_split;  // most splits of any context: sizes the workspace
     size_t lds(int D) const { return (size_t)waves * (2 * kMaxRows + rows * (D + 4)) * 4; }
 };
 
@@ -608,11 +607,11 @@ Kv4Plan kv4_plan(int B, int Hq, int Hkv, int max_context) {
     const long long units = (long long)B * Hkv * pl.groups;
     const long long tiles = ceil_div(max_context, kTile);
     constexpr int kCus = 256, kResident = 16;  // waves per CU
-    pl.max_split = (int)std::min<long long>(64, std::max<long long>(1, 1024 / units));
+    const int max_split = (int)std::min<long long>(64, std::max<long long>(1, 1024 / units));
     pl.nsplit = 1, pl.waves = 4;
     long long best = -1;
     for (int s : {1, 2, 3, 4, 5, 6, 8, 11, 16, 24, 32, 48, 64}) {
-        if (s > pl.max_split || s > tiles) break;
+        if (s > max_split || s > tiles) break;
         for (int w : {4, 8}) {
             const long long blocks = units * s;
             const long long waves = ceil_div(blocks, kCus) * w;  // per CU
@@ -645,9 +644,8 @@ void with_head_dim(int D, F&& f) {
 struct Kv4Partials {
     size_t ml_bytes, bytes;
 };
-Kv4Partials kv4_partials(int B, int Hq, int nsplit, int D) {
-    if (nsplit == 1) return {0, 0};
-    const size_t parts = (size_t)B * Hq * nsplit;
+Kv4Partials kv4_partials(size_t parts, int D) {
+    if (parts == 0) return {0, 0};
     const size_t ml = round_up(parts * 2 * sizeof(float), kWorkspaceAlign);
     return {ml, ml + round_up(parts * D * sizeof(float), kWorkspaceAlign)};
 }
@@ -739,7 +737,12 @@ extern "C" size_t int8k_decode_attention_kv4_paged_workspace_bytes(int B, int he
     if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 ||
         (head_dim != 64 && head_dim != 128))
         return 0;
-    return kv4_partials(B, heads, kv4_plan(B, heads, kv_heads, max_context).max_split, head_dim).bytes;
+    // b sequences are split into at most min(64, 1024 / (b units)) each, and b of them into no
+    // more than min(64 b, 1024 / units) together: that grows with b, where the plan's own need does not
+    const Kv4Plan pl = kv4_plan(1, heads, kv_heads, max_context);
+    const long long splits = 1024 / ((long long)kv_heads * pl.groups);
+    if (splits < 2) return 0;
+    return kv4_partials((size_t)heads * std::min(64LL * B, splits), head_dim).bytes;
 }
 
 extern "C" int int8k_decode_attention_forward_kv4_paged(
@@ -763,7 +766,8 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
         return INT8K_ERR_MISALIGNED;
     if ((long long)B * heads >= (1LL << 22)) return INT8K_ERR_UNSUPPORTED;
     const Kv4Plan pl = kv4_plan(B, heads, kv_heads, max_context);
-    const Kv4Partials part = kv4_partials(B, heads, pl.nsplit, head_dim);
+    const Kv4Partials part =
+        kv4_partials(pl.nsplit > 1 ? (size_t)B * heads * pl.nsplit : 0, head_dim);
     if (part.bytes > 0) {
         if (!workspace || workspace_bytes < part.bytes) return INT8K_ERR_WORKSPACE;
         if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;

@@ -4,9 +4,10 @@ import pytest
 import torch
 
 import int8k_capi as capi
-from grouped_helpers import quantize_rows, rows
+from grouped_helpers import kv4_case, quantize_rows, rows
 from test_heads_gpu import _case as heads_case
 from test_heads_gpu import _to
+from test_kv4_gpu import _decode
 
 pytestmark = pytest.mark.gpu
 
@@ -37,6 +38,22 @@ def test_linear_in_one_workspace(ext, gpu, K, N, packed):
             assert torch.equal(y, want), T
         assert torch.equal(capi.linear(x[:T], w, sx[:T].contiguous(), sw, bias=b, flags=packed), want)
         assert own_ok() and whole_ok(), T
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(8, 2, 128), (12, 12, 64), (32, 1, 64)])
+def test_decode_in_one_workspace(ext, gpu, H, Hkv, D):
+    B = 150
+    lens = [1 + 37 * b % 3000 for b in range(B)]
+    c = kv4_case(H + D, B, H, Hkv, D, 64, lens, gpu)
+    size = capi.decode_kv4_paged_workspace_bytes(B, H, Hkv, c["max_context"], D)
+    ws, ok = _workspace(size, gpu)
+    for n in (1, 2, 3, 5, 17, 40, 85, 86, 127, 128, 150):
+        part = dict(c, **{k: c[k][:n].contiguous() for k in ("Q", "sQ", "tables", "lens")})
+        want = _decode(ext, part)
+        args = (part["Q"], c["K"], c["V"], part["sQ"], c["sK"], c["sV"], part["tables"], part["lens"], c["max_context"])
+        assert torch.equal(capi.decode_attention_kv4_paged(*args, workspace=ws), want), n
+        assert torch.equal(capi.decode_attention_kv4_paged(*args), want), n
+        assert ok(), n
 
 
 @pytest.mark.parametrize("quantize", [False, True])

@@ -31,3 +31,10 @@ def test_linear_workspace_between_the_ranges(capi):
         for T in (545, 800, 1500):
             whole = capi.linear_workspace_bytes(T, K, N)
             assert all(capi.linear_call_workspace_bytes(t, K, N) <= whole for t in range(513, T + 1))
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 8, 128), (12, 12, 64), (8, 1, 128), (48, 2, 64), (32, 1, 64), (1, 1, 64)])
+def test_decode_workspace_covers_smaller_batches(capi, H, Hkv, D):
+    sizes = [capi.decode_kv4_paged_workspace_bytes(B, H, Hkv, 16384, D) for B in range(1, 1300)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    assert {capi.decode_kv4_paged_workspace_bytes(7, H, Hkv, n, D) for n in (1, 100, 4096, 1 << 20)} == {sizes[6]}
