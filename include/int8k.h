@@ -532,7 +532,9 @@ int int8k_kv4_cache_read(const uint8_t* pages, const float* scales, const int32_
  * (int8k_kv4_bad_ids).  Entries past a sequence's length are never read.  The workspace
  * (16-byte aligned) holds partial states of sequences that are split over blocks; one of the
  * queried size serves every call of up to B sequences with the same heads, whatever its
- * max_context.  0: no workspace is needed. */
+ * max_context.  0: no workspace is needed.  How a sequence is split, and so the order of its fp32
+ * sums, follows B and max_context: under others a result agrees within the rounding of those
+ * sums, not bit for bit. */
 size_t int8k_decode_attention_kv4_paged_workspace_bytes(int B, int heads, int kv_heads,
                                                         int max_context, int head_dim);
 

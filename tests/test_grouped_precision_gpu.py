@@ -56,3 +56,21 @@ def test_decode_precision(ext, gpu, B, H, Hkv, L, D):
     k = torch.from_numpy(G.kv4_unpack(c["K"].cpu().numpy()))
     smax = _smax(c["Q"], c["sQ"], k.to(gpu), c["sK"], D)
     assert_within(np64(out), ref, _bound(ref, mag, L, vmax, smax), f"B{B} D{D}")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_under_other_plans(ext, gpu, D):
+    # the plan, and with it the order of the sums, follows max_context and the batch; the result
+    # stays within the bound of the one value
+    c = kv4_case(21 + D, 3, 8, 2, D, 64, [5, 300, 411], gpu)
+    ref, mag = G.kv4_decode(*(c[k].cpu().numpy() for k in ("Q", "K", "V", "sQ", "sK", "sV", "tables", "lens")))
+    k = torch.from_numpy(G.kv4_unpack(c["K"].cpu().numpy()))
+    bound = _bound(ref, mag, 411, float(7 * c["sV"].max()), _smax(c["Q"], c["sQ"], k.to(gpu), c["sK"], D))
+    wide = torch.full((3, 1000), -1, dtype=torch.int32, device=gpu)
+    wide[:, :c["tables"].shape[1]] = c["tables"]
+    for top in (411, 1000, 4096, 64000):
+        assert_within(np64(_decode(ext, dict(c, tables=wide, max_context=top))), ref, bound, f"max_context {top}")
+    many = {n: c[n].repeat(*([100] + [1] * (c[n].dim() - 1))) for n in ("Q", "sQ", "tables", "lens")}
+    out = np64(_decode(ext, dict(c, **many))).reshape(100, 3, 8, D)
+    for i in range(100):
+        assert_within(out[i], ref, bound, f"batch {i}")
