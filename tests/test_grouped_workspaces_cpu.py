@@ -1,7 +1,11 @@
 """Workspace sizes of the grouped-query serving entry points, without a GPU."""
+import ctypes
+
 import pytest
+import torch
 
 PACKED = 1
+WORKSPACE, MISALIGNED = 3, 4
 
 
 @pytest.mark.parametrize("K,N", [(4096, 28672), (4096, 128256), (8192, 28672)])
@@ -38,3 +42,34 @@ def test_decode_workspace_covers_smaller_batches(capi, H, Hkv, D):
     sizes = [capi.decode_kv4_paged_workspace_bytes(B, H, Hkv, 16384, D) for B in range(1, 1300)]
     assert sizes == sorted(sizes) and sizes[0] > 0
     assert {capi.decode_kv4_paged_workspace_bytes(7, H, Hkv, n, D) for n in (1, 100, 4096, 1 << 20)} == {sizes[6]}
+
+
+# The refusals are reached before any launch only where a call does need a workspace: not on a
+# machine whose GPU would run the made-up pointers if it did not.
+no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers")
+
+
+@no_gpu
+@pytest.mark.parametrize("T,K,N,flags", [(1, 4096, 4096, 0), (300, 14336, 4096, 0), (16, 8192, 1024, PACKED)])
+def test_linear_refuses_workspaces_it_cannot_use(capi, T, K, N, flags):
+    need = capi.linear_call_workspace_bytes(T, K, N, flags)
+    assert need > 0
+    P = [ctypes.c_void_p(0x10000 * (i + 1)) for i in range(6)]
+    call = lambda ws, n: capi.load().int8k_linear(  # noqa: E731
+        P[0], P[1], P[2], 0, P[3], 1, P[4], 1, None, T, K, N, flags, ws, n, None)
+    assert call(None, 1 << 40) == WORKSPACE
+    assert call(P[5], 0) == WORKSPACE
+    assert call(P[5], need - 1) == WORKSPACE
+    assert call(ctypes.c_void_p(0x60008), need) == MISALIGNED
+
+
+@no_gpu
+@pytest.mark.parametrize("B,H,Hkv,D,top", [(1, 32, 8, 128, 16384), (2, 12, 12, 64, 4096)])
+def test_decode_refuses_workspaces_it_cannot_use(capi, B, H, Hkv, D, top):
+    P = [ctypes.c_void_p(0x10000 * (i + 1)) for i in range(10)]
+    call = lambda ws, n: capi.load().int8k_decode_attention_forward_kv4_paged(  # noqa: E731
+        *P[:9], B, H, Hkv, D, 1000, 64, 256, top, ws, n, None)
+    assert call(None, 1 << 40) == WORKSPACE
+    assert call(P[9], 0) == WORKSPACE
+    assert call(P[9], 1024) == WORKSPACE  # less than any split's states
+    assert call(ctypes.c_void_p(0x90008), 1 << 40) == MISALIGNED

@@ -28,3 +28,19 @@ def test_linear_wide(ext, gpu, T, K, N, packed, dt):
     ref += b.double()
     over = (y.double() - ref).abs() - (f32 + HALF[dt] * (ref.abs() + f32) + TINY[dt])
     assert torch.isfinite(y).all() and over.max().item() <= 0
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("K,N", [(4096, 2048), (1040, 6000), (512, 16400)])
+def test_rows_do_not_depend_on_the_route(ext, gpu, K, N, packed):
+    # the sum is exact and its value one expression: a row's bits are those of a call of its own
+    g = torch.Generator(device=gpu).manual_seed(K)
+    T = 2500
+    x = torch.randint(-128, 128, (T, K), dtype=torch.int8, device=gpu, generator=g)
+    w = torch.randint(-128, 128, (N, K) if packed else (K, N), dtype=torch.int8, device=gpu, generator=g)
+    sx, sw = (torch.rand(n, device=gpu, generator=g) * 0.01 for n in (T, N))
+    b = torch.randn(N, device=gpu, generator=g)
+    want = ext.int8_linear(x, w, sx, sw, bias=b, prepacked=packed, dtype=torch.float32)
+    for n in (1, 20, 64, 130, 333, 512, 700, 1500):
+        y = ext.int8_linear(x[-n:], w, sx[-n:], sw, bias=b, prepacked=packed, dtype=torch.float32)
+        assert torch.equal(y, want[-n:]), n
