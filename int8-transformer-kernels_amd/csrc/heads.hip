@@ -63,20 +63,6 @@ __device__ __forceinline__ float load_one(const void* x, size_t i) {
     return __uint_as_float((uint32_t)u << 16);
 }
 
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-
-// Two values rounded to numbers of a 16-bit dtype (to nearest even), packed.
-template <int DT>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-    if constexpr (DT == INT8K_DTYPE_F16) {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
-    } else {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
-    }
-}
-
 // Values as numbers of the dtype.
 template <int DT>
 __device__ __forceinline__ void round_all(float (&v)[8]) {

@@ -135,16 +135,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const uint8_t* __restrict
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == INT8K_DTYPE_F16) {
-                w[i] = __half_as_ushort(f16_of_f32(y[2 * i])) |
-                       ((uint32_t)__half_as_ushort(f16_of_f32(y[2 * i + 1])) << 16);
-            } else {
-                auto rn = [](float v) {
-                    const uint32_t u = __float_as_uint(v);
-                    return v != v ? (u >> 16) | 0x40u : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
-                };
-                w[i] = rn(y[2 * i]) | (rn(y[2 * i + 1]) << 16);
-            }
+            float lo = y[2 * i], hi = y[2 * i + 1];
+            asm("" : "+v"(lo), "+v"(hi));
+            w[i] = pack_pair<DT>(lo, hi);
         }
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + o) = make_uint4(w[0], w[1], w[2], w[3]);
     }

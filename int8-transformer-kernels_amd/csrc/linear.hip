@@ -36,20 +36,6 @@ __device__ __forceinline__ float linear_value(int acc, float sx, float sw, float
     return static_cast<float>(acc) * sx * sw + b;
 }
 
-// Two values as numbers of a 16-bit dtype.
-template <int DT>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-    if constexpr (DT == INT8K_DTYPE_F16) {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
-    } else {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
-    }
-}
-
 // 4 consecutive values to dst (8 or 16 bytes).
 template <int DT>
 __device__ __forceinline__ void store_four(void* dst, const float (&v)[4]) {

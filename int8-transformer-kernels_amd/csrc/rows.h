@@ -115,6 +115,20 @@ __device__ __forceinline__ void unpack_chunk(const uint4& w, float (&v)[Vec<DT>:
     }
 }
 
+// Two values as numbers of a 16-bit dtype (to nearest even), packed.  A product handed over here
+// must be pinned as the fp32 number it is (f16_of_f32): clang may round it to fp16 in one step.
+template <int DT>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    if constexpr (DT == INT8K_DTYPE_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
+    }
+}
+
 // Reduction over the aligned group of 1 << lg lanes that holds one row; every
 // lane of the group gets it.  On the VALU: DPP inside a 16-lane row (after the
 // xor 1 and xor 2 steps a quad's lanes agree, so the mirrors pair whole quads and
