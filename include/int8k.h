@@ -481,8 +481,8 @@ int int8k_rope_bad_positions(unsigned int* count);
  * Each query attends to the keys of its sequence, with INT8K_ATTN_CAUSAL to those up to
  * itself; the math is int8k_attention_forward's.  Rows of tokens that no sequence holds
  * (padding behind the last one) are left as they were, or written as zeros with
- * INT8K_ATTN_ZERO_REST.  head_dim a multiple of 16 up to 256.  Q, K, V 16-byte, out
- * 8-byte aligned. */
+ * INT8K_ATTN_ZERO_REST.  head_dim a multiple of 16 up to 256, num_seqs at most 65536 (else
+ * INT8K_ERR_UNSUPPORTED).  Q, K, V 16-byte, out 8-byte aligned. */
 #define INT8K_ATTN_OUT_THD 2
 #define INT8K_ATTN_ZERO_REST 4
 

@@ -64,6 +64,8 @@ __device__ __forceinline__ int wave_sum(int v) {
 }
 
 constexpr int kLongTiles = 8;
+// Every block reads the bounds of all sequences, so the time grows with their square.
+constexpr int kMaxSeqs = 1 << 16;
 
 // The query tile that rank `i` of the packed order is: sequence tokens [start, start + len),
 // tile qt of them.  False past the last tile; `i` is then the rank behind it.
@@ -582,7 +584,8 @@ struct PackedArgs {
 template <int D>
 int launch_packed(const PackedArgs& a, hipStream_t stream) {
     constexpr int kQ = 32 * kPackedWaves, kThreads = 64 * kPackedWaves;
-    const long long ranks = (long long)a.T / kQ + a.n + 1;
+    // (a tile that is not whole is the last of a sequence that holds a token)
+    const long long ranks = (long long)a.T / kQ + std::min(a.n, a.T) + 1;
     const float qk = (1.0f / std::sqrt((float)a.dm)) * kLog2e;
     constexpr int kLds = PackedLds<D>::kBytes;
     if (ranks * a.heads * kThreads >= (1LL << 32)) return INT8K_ERR_UNSUPPORTED;
@@ -624,7 +627,7 @@ extern "C" int int8k_attention_forward_packed(
     if (num_seqs <= 0 || total_tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
         heads % kv_heads != 0)
         return INT8K_ERR_INVALID_ARGUMENT;
-    if (!on_mfma(head_dim)) return INT8K_ERR_UNSUPPORTED;
+    if (!on_mfma(head_dim) || num_seqs > kMaxSeqs) return INT8K_ERR_UNSUPPORTED;
     if ((long long)total_tokens * head_dim >= (1LL << 32)) return INT8K_ERR_UNSUPPORTED;  // buffer range
     if (!aligned_to(Q, 16) || !aligned_to(K, 16) || !aligned_to(V, 16) || !aligned_to(out, 8) ||
         !aligned_to(scale_Q, 4) || !aligned_to(scale_K, 4) || !aligned_to(scale_V, 4) ||
