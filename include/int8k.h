@@ -529,7 +529,8 @@ int int8k_kv4_cache_read(const uint8_t* pages, const float* scales, const int32_
  *   out fp16 [B, heads, D]
  *   out = sum_j softmax_j(q . k_j sQ sK_j / sqrt(D)) v_j sV_j, q . k exact int32.
  * A page id outside [0, num_pages) reads page num_pages-1 and is counted
- * (int8k_kv4_bad_ids).  Entries past a sequence's length are never read.  The workspace
+ * (int8k_kv4_bad_ids).  Entries past a sequence's length are never read.  max_context is at
+ * most 2^30 (else INT8K_ERR_UNSUPPORTED).  The workspace
  * (16-byte aligned) holds partial states of sequences that are split over blocks; one of the
  * queried size serves every call of up to B sequences with the same heads, whatever its
  * max_context.  0: no workspace is needed.  How a sequence is split, and so the order of its fp32

@@ -757,7 +757,8 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
         !aligned_to(scale_Q, 4) || !aligned_to(sK_pages, 4) || !aligned_to(sV_pages, 4) ||
         !aligned_to(block_tables, 4) || !aligned_to(context_lens, 4) || !aligned_to(out, 8))
         return INT8K_ERR_MISALIGNED;
-    if ((long long)B * heads >= (1LL << 22)) return INT8K_ERR_UNSUPPORTED;
+    // (positions, a few tiles past the last among them, are int)
+    if ((long long)B * heads >= (1LL << 22) || max_context > (1 << 30)) return INT8K_ERR_UNSUPPORTED;
     const Kv4Plan pl = kv4_plan(B, heads, kv_heads, max_context);
     const Kv4Partials part =
         kv4_partials(pl.nsplit > 1 ? (size_t)B * heads * pl.nsplit : 0, head_dim);
