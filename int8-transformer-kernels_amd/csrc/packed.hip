@@ -14,21 +14,25 @@
 //  - V enters as exact fp16 and its scale goes into the weights p sV, each carried in two fp16, its
 //    rounding and what that leaves (22 bits); l sums p in fp32.  The error against 64 bits is that
 //    of the formula in fp32 with the output rounded once (1.1-1.3 times it with one fp16 a
-//    weight, 1.8 with V sV rounded beside it).  The second product with V costs 36-40% more time
-//    at D = 128, 13% at 64 and 26% at 256: 325 us against 231 for the prompts below.
+//    weight, 1.8 with V sV rounded beside it).  The second product with V costs 22-30% more
+//    time at D = 128, 13% at 64 and 17% at 256: 304 us against 238 for the prompts below.
 //  - Only a wave's first tile takes the exact step that finds a maximum; diagonal and ragged
 //    tiles run the ordinary step with a mask.  Prompts of 300 to 2000 tokens gain 6-20%.
 //
 // What bounds it: each wave's own chain of scores, softmax and product.  At D = 128 a tile is 40
-// large MFMAs (1340 cycles with the small ones) and 311 vector instructions, 32 of them
-// exponentials of two slots (1380 cycles); by the counters a wave takes 5500 cycles for it, 22% of
-// them waiting on LDS and the barrier and 40% to issue, two waves share a SIMD, and the clock
-// falls to 1.84 GHz under the load (2.4 at most).  Measured: 325 us for prompts of 333, 4096, 17,
-// 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8 key heads of 128 (49.6 G multiply-adds under
-// the mask in each product); 802-827 us for one prompt of 8192; 9.3 us for five requests of at most
-// 70.  Tried:
-//  - the product of one half of a tile among the softmax of the other: 850 us for the long prompt;
-//  - wave priorities around the products or the softmax: 827-834 us;
+// large MFMAs (1340 cycles with the small ones) and 330 vector instructions, 32 of them
+// exponentials of two slots (1450 cycles).  Two waves share a SIMD, but the matrix and the vector
+// units overlap by half at best (32 MFMAs and 256 vector instructions, interleaved or from two
+// waves: 710-740 ns, 530 and 320 by themselves); by the counters a wave waits 22% of its time on
+// LDS and the barrier, and the clock falls to 1.84 GHz under the load (2.4 at most).  Measured:
+// 304-322 us for prompts of 333, 4096, 17, 1000, 2500, 1, 200 and 45 tokens, 32 heads on 8 key heads
+// of 128 (49.6 G multiply-adds under the mask in each product); 780 us for one prompt of 8192; 9
+// us for five requests of at most 70.  Tried:
+//  - the product of one half of a tile among the softmax of the other: 3% slower;
+//  - wave priorities around the products or the softmax: no gain;
+//  - the sum of p times the tile's largest |sV| as the bound on its weights, one instruction a
+//    tile in place of 16: it overestimates so much that tiles leave the ordinary step often (325
+//    us); that step's maximum spares the exact one two passes (307 without);
 //  and with one fp16 a weight (231 us, 590-600 and 9):
 //  - the softmax of a tile next to the MFMAs of its neighbours in one block of instructions (the
 //    next scores and the last product with V): no gain, with three K buffers and all 256 registers;
@@ -161,7 +165,7 @@ struct PackedLds {
     static constexpr int kVBytes = kKV * kVRow * 2;
     static constexpr int kV = 2 * kKBytes;
     static constexpr int kS = kV + 2 * kVBytes;
-    static constexpr int kSFloats = 2 * kKV + 4;  // sK, sV, the largest |sV|
+    static constexpr int kSFloats = 2 * kKV;  // sK, sV
     static constexpr int kBytes = kS + 2 * kSFloats * 4;
 };
 
@@ -290,8 +294,6 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         float* s = reinterpret_cast<float*>(smem + L::kS) + (i & 1) * L::kSFloats;
         s[lane] = l.k;
         s[kKV + lane] = l.v;
-        const float top = row_reduce(fabsf(l.v), 6, [](float a, float b) { return fmaxf(a, b); });
-        if (lane == 0) s[2 * kKV] = top;
     };
 
     // ---- compute
@@ -348,9 +350,10 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     };
     // The weights of a lane's four keys of chunk ch, 32 (ch / 4) + 8 (ch % 4) + 4 h + 0..3, their
     // scores being registers 4 (ch % 4) .. + 3 of s: e = 2^(x - m), p = fp16(e sV), r = fp16(e sV - p).
-    // Returns the sum of e.  sQ sK comes from an MFMA over 4 x 4 blocks (lanes 4b .. 4b + 3, the
-    // outer product of a lane's own key scale with the lanes' query scales), which leaves one
-    // multiplication less per score than sK read as it is (2% at 8192 tokens, 32 heads of 128).
+    // Returns the sum of e; wide takes in the largest |e sV|.  sQ sK comes from an MFMA over 4 x 4
+    // blocks (lanes 4b .. 4b + 3, the outer product of a lane's own key scale with the lanes'
+    // query scales), which leaves one multiplication less per score than sK read as it is (2% at
+    // 8192 tokens, 32 heads of 128).
     typedef float v4f __attribute__((ext_vector_type(4)));
     auto scale_qk = [&](int ch, const float* sc) {
         return __builtin_amdgcn_mfma_f32_4x4x1f32(sc[32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + (lane & 3)], qscale,
@@ -359,7 +362,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
     auto scale_v = [&](int ch, const float* sc) {
         return *reinterpret_cast<const v4f*>(sc + kKV + 32 * (ch >> 2) + 8 * (ch & 3) + 4 * h);
     };
-    auto weights = [&](int ch, const v16i& s, const float* sc, v8h (&p)[4], v8h (&r)[4], auto mask, auto seen) {
+    auto weights = [&](int ch, const v16i& s, const float* sc, v8h (&p)[4], v8h (&r)[4], float& wide, auto mask, auto seen) {
         const int T = ch >> 2, g = ch & 3;
         const v4f sqk = scale_qk(ch, sc), sv = scale_v(ch, sc);
         float e[4], w[4];
@@ -374,6 +377,8 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
                 w[c] = ok ? w[c] : 0.f;
             }
         }
+        wide = fmaxf(fmaxf(wide, fabsf(w[0])), fabsf(w[1]));
+        wide = fmaxf(fmaxf(wide, fabsf(w[2])), fabsf(w[3]));
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {
             typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -387,46 +392,54 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         return (e[0] + e[1]) + (e[2] + e[3]);
     };
     auto k_buf = [&](int i) { return smem + (i & 1) * L::kKBytes; };
-    float over = 1.f;  // not 0: the query's weights leave the range of m
-    // The exact path: sets m so that the largest weight p sV of the tile is 1 and rescales O and l.
+    // 0 where the query's weights fit m; else the largest of them, or infinity
+    float over = INFINITY;
+    // The exact path: sets m by the tile's largest weight and rescales O and l.
     auto slow = [&](int i, const float* sc, v8h (&p)[4], v8h (&r)[4]) {
         const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
         auto seen = [&](int key) { return key <= last; };
         const v16i sacc[2] = {scores(k_buf(i), 0), scores(k_buf(i), 1)};
-        float top = -INFINITY;
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-            const v4f sqk = scale_qk(ch, sc);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float x = static_cast<float>(sacc[ch >> 2][4 * (ch & 3) + c]) * sqk[c];
-                top = fmaxf(top, seen(32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + c) ? x : -INFINITY);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        top = max_xor32(top);
-        const float base = top == -INFINITY ? 0.f : top;
-        float pm = 0.f;
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-            const v4f sqk = scale_qk(ch, sc), sv = scale_v(ch, sc);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float x = sv[c] * fast_exp2(fmaf(static_cast<float>(sacc[ch >> 2][4 * (ch & 3) + c]),
-                                                       sqk[c], -base));
-                pm = fmaxf(pm, seen(32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + c) ? fabsf(x) : 0.f);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        pm = max_xor32(pm);
         // The largest weight becomes 2^kPackedTopExp, which fp16 holds exactly.  Below 2^-14 fp16
         // steps by 2^-24, so a weight is off by at most 2^-33 of the largest, and long flat
         // tails add up; the factor of 234 up to kPackedMaxWeight is the room before a tile
-        // (the sum of its weights) takes this path again.
-        const float shift = pm > 0.f && pm < INFINITY ? __builtin_amdgcn_logf(pm) : 0.f;
+        // takes this path again.  The step that was left has found the largest under m, unless
+        // it left fp32's range or there is no m yet.
+        const float left = max_xor32(over);
+        float raised = m + __builtin_amdgcn_logf(left) - kPackedTopExp;
+        if (__ballot(left == INFINITY) != 0) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch) {
+                const v4f sqk = scale_qk(ch, sc);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float x = static_cast<float>(sacc[ch >> 2][4 * (ch & 3) + c]) * sqk[c];
+                    top = fmaxf(top, seen(32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + c) ? x : -INFINITY);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            top = max_xor32(top);
+            const float base = top == -INFINITY ? 0.f : top;
+            float pm = 0.f;
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch) {
+                const v4f sqk = scale_qk(ch, sc), sv = scale_v(ch, sc);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float x = sv[c] * fast_exp2(fmaf(static_cast<float>(sacc[ch >> 2][4 * (ch & 3) + c]),
+                                                           sqk[c], -base));
+                    pm = fmaxf(pm, seen(32 * (ch >> 2) + 8 * (ch & 3) + 4 * h + c) ? fabsf(x) : 0.f);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            pm = max_xor32(pm);
+            const float shift = pm > 0.f && pm < INFINITY ? __builtin_amdgcn_logf(pm) : 0.f;
+            const float set =
+                fmaxf(m, top + fminf(fmaxf(shift - kPackedTopExp, -kPackedMaxShift), kPackedMaxShift));
+            raised = left == INFINITY ? set : raised;
+        }
         // (a query whose weights fit keeps its m, whatever its neighbours in the wave hold)
-        const float raised = fmaxf(m, top + fminf(fmaxf(shift - kPackedTopExp, -kPackedMaxShift), kPackedMaxShift));
-        const float m_new = max_xor32(over) != 0.f ? raised : m;
+        const float m_new = left != 0.f ? raised : m;
         const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));
         m = m_new;
         l *= alpha;
@@ -434,10 +447,10 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         for (int j = 0; j < NS; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[j][r] *= alpha;
-        float psum = 0.f;  // (summed as in a step that keeps m)
+        float psum = 0.f, wide = 0.f;  // (summed as in a step that keeps m)
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            psum += weights(c, sacc[c >> 2], sc, p, r, std::true_type{}, seen);
+            psum += weights(c, sacc[c >> 2], sc, p, r, wide, std::true_type{}, seen);
             __builtin_amdgcn_sched_barrier(0);
         }
         l += psum;
@@ -479,16 +492,15 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
             const float* sc = scales_of(i);
             const int last = (CAUSAL ? min(q, S - 1) : S - 1) - tile_of(i) * kKV;  // last key seen
             v8h p[4], r[4];
-            float psum = 0.f;
+            float psum = 0.f, wide = 0.f;
             const v16i sacc[2] = {scores(k_buf(i), 0), scores(k_buf(i), 1)};
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                psum += weights(c, sacc[c >> 2], sc, p, r, mask, [&](int key) { return key <= last; });
+                psum += weights(c, sacc[c >> 2], sc, p, r, wide, mask, [&](int key) { return key <= last; });
                 // (keeps the scales of all chunks from being read first: 2-9% at D = 256)
                 if (c & 1) __builtin_amdgcn_sched_barrier(0);
             }
-            // every weight is at most the sum of p times the tile's largest |sV|
-            over = psum * sc[2 * kKV] <= kPackedMaxWeight && psum <= 0x1p60f ? 0.f : 1.f;
+            over = psum <= 0x1p60f ? (wide <= kPackedMaxWeight ? 0.f : wide) : INFINITY;
             if (__ballot(over != 0.f) != 0) return false;
             l += psum;
             product(v_buf(i), p, r);
