@@ -437,6 +437,10 @@ __global__ __launch_bounds__(512) void kv4_decode_kernel(Kv4Decode p) {
             pw[j] = (_Float16)w[j];
             pr[j] = (_Float16)(w[j] - (float)pw[j]);
         }
+        if (slow) {  // (a weight past fp16's range, by an infinite value scale, leaves no rest)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pr[j] = fabsf(w[j]) < 65520.f ? pr[j] : (_Float16)0.f;
+        }
         // codes of a byte of two keys: 0x6400 | n is 1024 + n in fp16 and 0x6400 | 16 n is
         // 1024 + 16 n, both exact, as are the sums below
         uint32_t magic = 0x64006400u;
