@@ -186,6 +186,8 @@ constexpr float kPackedMaxWeight = 60000.f;  // fp16 weights stay below it
 constexpr float kPackedMaxShift = 60.f;      // |m - running maximum| where m is set
 constexpr float kPackedTopExp = 8.f;         // the largest weight there is 2^kPackedTopExp
 
+struct ExactStep : std::true_type {};  // the step that sets m; masked, as some of the others are
+
 template <int D, bool CAUSAL, bool PAD, typename OutRow>
 __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restrict__ Qh,
                                              const int8_t* __restrict__ Kh,
@@ -384,7 +386,13 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
             typedef _Float16 h2 __attribute__((ext_vector_type(2)));
             typedef float f2 __attribute__((ext_vector_type(2)));
             const h2 top = __builtin_convertvector((f2){w[c], w[c + 1]}, h2);
-            const h2 rest = __builtin_convertvector((f2){minus_half<0>(w[c], top), minus_half<1>(w[c + 1], top)}, h2);
+            float rest0 = minus_half<0>(w[c], top), rest1 = minus_half<1>(w[c + 1], top);
+            if constexpr (std::is_same_v<decltype(mask), ExactStep>) {
+                // (a weight past fp16's range, by an infinite value scale, leaves no rest)
+                rest0 = fabsf(w[c]) < 65520.f ? rest0 : 0.f;
+                rest1 = fabsf(w[c + 1]) < 65520.f ? rest1 : 0.f;
+            }
+            const h2 rest = __builtin_convertvector((f2){rest0, rest1}, h2);
             const int at = 4 * (g & 1) + c;
             p[2 * T + (g >> 1)][at] = top.x, p[2 * T + (g >> 1)][at + 1] = top.y;
             r[2 * T + (g >> 1)][at] = rest.x, r[2 * T + (g >> 1)][at + 1] = rest.y;
@@ -450,7 +458,7 @@ __device__ __forceinline__ void packed_block(char* smem, const int8_t* __restric
         float psum = 0.f, wide = 0.f;  // (summed as in a step that keeps m)
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            psum += weights(c, sacc[c >> 2], sc, p, r, wide, std::true_type{}, seen);
+            psum += weights(c, sacc[c >> 2], sc, p, r, wide, ExactStep{}, seen);
             __builtin_amdgcn_sched_barrier(0);
         }
         l += psum;

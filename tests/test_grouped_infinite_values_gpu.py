@@ -6,12 +6,32 @@ import torch
 from grouped_helpers import kv4_case
 from oracle import grouped_oracle as G
 from test_kv4_gpu import _decode
+from test_packed_gpu import _args, _case
 
 pytestmark = pytest.mark.gpu
 
 
 def _clamp(t):
     return t.double().nan_to_num(nan=0.0, posinf=1.0, neginf=-1.0)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("at,causal", [(0, True), (70, True), (299, True), (70, False), (299, False)])
+def test_packed(ext, gpu, at, causal, D, sign):
+    c = _case([300, 40], 4, 2, D, gpu, seed=4)
+    c["V"][:, at, ::5] = 0
+    want = ext.int8_attention_forward_packed(*_args(c), is_causal=causal)
+    c["sV"][:, at] = sign * float("inf")
+    out = ext.int8_attention_forward_packed(*_args(c), is_causal=causal)
+    first = at if causal else 0
+    assert torch.equal(out[:, :first], want[:, :first]) and torch.equal(out[:, 300:], want[:, 300:])
+    for h in range(4):
+        v = c["V"][h // 2, at]
+        rows = out[h, first:300]
+        nan, inf = v == 0, sign * torch.sign(v.double())
+        assert rows[:, nan].isnan().all()
+        assert (_clamp(rows[:, ~nan]) == inf[~nan]).all()
 
 
 @pytest.mark.parametrize("D", [64, 128])
