@@ -5,7 +5,7 @@
 // x int8 [T, K]; w int8 [K, N] as stored, or [N, K] packed; y fp16, bf16 or fp32, rounded once
 // from the fp32 value.  The products run on the loops of the MLP's GEMMs (gemm_i8.h,
 // gemm_i8_paths.h); the routes differ in how the result leaves:
-//   skinny   32 x 32 tiles, K over the waves of a block (few tokens, small packed weights)
+//   skinny   32 x 32 tiles, K over the waves of a block (few tokens, packed weights)
 //   stream   the weights streamed once over all CUs, exact int32 partials, then rows
 //   small    64 x 64 tiles, four blocks per CU, or one of two wave groups that halve K
 //   mid      128 x 128 tiles, two blocks per CU; K split into partials where CUs would idle
