@@ -569,9 +569,9 @@ struct LinearPlan {
 // The route with the least estimated time (us).  Fitted to every route timed at 318 sizes: T = 1 to
 // 4096, K = 16 to 131056, N = 16 to 128256, weights that come from memory wherever they do not fit
 // its cache.  No estimate is below the time to read the weights: 5.9 TB/s is the most that any
-// route reached (525 MB in 89 us), and the routes that reach less have their own rate.  `steps`
-// are 128 deep; `cold` is 1 for weights of 16 MiB and more, whose loads take longer than those of
-// small ones.
+// route reached (525 MB in 89 us; a stream that only reads 7.0), and the routes that reach less
+// have their own rate.  `steps` are 128 deep; `cold` is 1 for weights of 16 MiB and more, whose
+// loads take longer than those of small ones.
 //  - small: a step of a block takes a load's latency, or from 256 blocks on its share of the
 //    CU (T = 512, 4096 -> 4096: 21 packed, 26 as stored).  As stored it reads 64 bytes a row:
 //    5.0 TB/s, 3.7 where rows lie a multiple of 4096 bytes apart (28672 columns 35.5 us, 28736 28.8);
