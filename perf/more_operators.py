@@ -276,7 +276,7 @@ def _own_append(c, d, ext):
 def _own_tree(c, d, ext):
     return ext.int8_tree_attention_forward_paged(
         d["q"], d["K"], d["V"], d["sq"], d["sK"], d["sV"], d["tables"], d["lens"], d["words"],
-        c["max_len"] + c["N"], node_counts=d["counts"], out_bshd=c["rows"])
+        min(c["max_len"] + c["N"], d["tables"].shape[1] * c["page"]), node_counts=d["counts"], out_bshd=c["rows"])
 
 
 def _own_move(c, d, ext):
