@@ -546,6 +546,122 @@ int int8k_decode_attention_forward_kv4_paged(
     int head_dim, int num_pages, int page_size, int max_pages_per_seq, int max_context,
     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Operators over the paged INT8 cache with grouped heads (no counterparts in */
+/* the reference): its writer, its readers for drafted trees and for selected */
+/* blocks, and its upkeep.                                                    */
+/*   K_pages / V_pages int8 [num_pages, kv_heads, page_size, head_dim]         */
+/*   sK_pages / sV_pages fp32 [num_pages, kv_heads, page_size]                 */
+/* the layout of int8k_decode_attention_forward_paged, which reads it too     */
+/* where kv_heads is the query's.  head_dim 64 or 128, page_size a power of    */
+/* two in [16, 1024], num_pages * page_size below 2^31; pages 16-byte aligned. */
+/* A slot is page id * page_size + offset.                                    */
+/* ------------------------------------------------------------------------ */
+
+/* int8k_qk_norm_rope_quantize whose keys and values go into the cache: row slots[b*S + t]
+ * (int32, device) of every key head takes that token's, byte for byte what the other call
+ * returns.  q int8 [B, heads, S, head_dim] and scale_q [B, heads, S] as there.  A negative
+ * slot stores no key and no value (its query is computed all the same); slots past the cache
+ * are left out and counted (int8k_paged_bad_ids).  The slots of one call must be distinct: of
+ * two tokens on one slot either may win, piece by piece. */
+int int8k_qk_norm_rope_append(const void* x, int dtype, const float* cos, const float* sin,
+                              int max_positions, int rot_dim, const int32_t* positions,
+                              const float* q_weight, const float* k_weight, float eps, int8_t* q,
+                              float* scale_q, int8_t* K_pages, int8_t* V_pages, float* sK_pages,
+                              float* sV_pages, const int32_t* slots, int B, int S, int heads,
+                              int kv_heads, int head_dim, int num_pages, int page_size, int flags,
+                              void* stream);
+
+/* Attention of a tree of drafted tokens per sequence:
+ *   Q int8 [B, heads, nodes, D], scale_Q fp32 [B*heads*nodes]; heads a multiple of kv_heads
+ *   block_tables int32 [B, max_pages_per_seq] as the paged decode's
+ *   context_lens int32 [B]: positions of sequence b before the tree; its nodes' keys and values
+ *     are in the cache behind them, node i at position context_lens[b] + i
+ *   node_counts int32 [B] or NULL: nodes of each sequence (at most `nodes`; NULL: `nodes`)
+ *   tree_mask int64 [nodes, mask_words], mask_words = ceil(nodes / 64), one for all sequences
+ *     (mask_batch_stride 0) or one per sequence, mask_batch_stride elements apart: bit j % 64 of
+ *     word j / 64 of row i is set where node i sees node j (itself among them).  NULL: j <= i
+ *   out fp16 [B, heads, nodes, D], or [B, nodes, heads, D] with INT8K_ATTN_OUT_BSHD
+ * Node i attends to all positions before the tree and to the nodes it sees:
+ *   out = sum_j softmax_j(q . k_j sQ sK_j / sqrt(D)) v_j sV_j, q . k exact int32.
+ * Rows that see nothing, and rows of nodes past a sequence's, are zeros.  Negative lengths and
+ * counts are 0; positions from max_context on are not attended to (context_lens are cut to it,
+ * then the nodes).  A page id outside [0, num_pages) reads page num_pages-1 and is counted
+ * (int8k_paged_bad_ids); entries past a sequence's last position are never read.  nodes at most
+ * 256, max_context at most 2^30, B*heads*nodes below 2^24 (else INT8K_ERR_UNSUPPORTED).  Q
+ * 16-byte, out 8-byte aligned.  The workspace (16-byte aligned) holds partial states; one of the
+ * queried size serves every call of up to B*nodes tokens with the same heads, whatever its
+ * max_context.  How a sequence is split, and so the order of its fp32 sums, follows B, nodes and
+ * max_context: under others a result agrees within the rounding of those sums, not bit for bit. */
+size_t int8k_tree_attention_paged_workspace_bytes(int B, int heads, int kv_heads, int nodes,
+                                                  int max_context, int head_dim);
+
+int int8k_tree_attention_forward_paged(
+    const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
+    const float* scale_Q, const float* sK_pages, const float* sV_pages,
+    const int32_t* block_tables, const int32_t* context_lens, const int64_t* tree_mask,
+    int mask_words, long long mask_batch_stride, const int32_t* node_counts, int B, int heads,
+    int kv_heads, int nodes, int head_dim, int num_pages, int page_size, int max_pages_per_seq,
+    int max_context, int flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies rows (codes and scales of K and V, every key head) from slots src_slots[l][i] to
+ * dst_slots[l][i] (int32 [lists, pairs], device): all rows of a list are read before any of them
+ * is written, so a destination may be a source of another pair of the list (the accepted path of
+ * a drafted tree moves together).  A slot that one list writes must be in no other list, and the
+ * destinations of a list distinct.  A pair with a negative slot is left out; one with a slot past
+ * the cache too, and is counted (int8k_paged_bad_ids).  pairs at most 256 (else
+ * INT8K_ERR_UNSUPPORTED). */
+int int8k_kv_cache_move_paged(int8_t* K_pages, int8_t* V_pages, float* sK_pages, float* sV_pages,
+                              const int32_t* src_slots, const int32_t* dst_slots, int lists,
+                              int pairs, int kv_heads, int head_dim, int num_pages, int page_size,
+                              void* stream);
+
+/* The mean key of whole pages page_ids (int32 [count], device), for the sparse decode:
+ *   K_means int8 [num_pages, kv_heads, D], sK_means fp32 [num_pages, kv_heads]:
+ *   m = f32(sum over the page's rows of code * scale / page_size), summed in 64 bits, then
+ *   quantized as int8k_quantize_per_token does (a NaN in m makes the scale NaN).
+ * All page_size rows enter, so a page is due once it is full.  Negative ids are skipped, ids past
+ * the cache too, and counted (int8k_paged_bad_ids).  Other pages' means are left as they were.
+ * K_means 16-byte aligned. */
+int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages, const int32_t* page_ids,
+                        int8_t* K_means, float* sK_means, int count, int kv_heads, int head_dim,
+                        int num_pages, int page_size, void* stream);
+
+/* Decode attention (one token per sequence) over selected blocks of the cache; block i of
+ * sequence b is the positions i * page_size .. of its context, on page block_tables[b][i]:
+ *   Q int8 [B, heads, D], scale_Q fp32 [B*heads]; heads a multiple of kv_heads
+ *   score(b, key head, i) = max over the key head's query heads of ((q . m_i) sM_i) sQ, q . m
+ *     exact, the products in 64 bits; m_i, sM_i the page's K_means and sK_means
+ *   taken: the last block, and the top_pages - 1 others with the highest scores (of equal ones
+ *     the lowest i; a block whose scores are all NaN comes last); all of them where there are
+ *     no more than top_pages
+ *   selected int32 [B, kv_heads, top_pages]: the blocks taken, ascending, -1 behind them
+ *   out fp16 [B, heads, D]: the paged decode's over the positions of the blocks taken.
+ * A length of 0 gives a zero row; lengths past max_context are cut to it.  The means of a
+ * sequence's last block are not read.  Page ids outside [0, num_pages) read page num_pages-1 and
+ * are counted (int8k_paged_bad_ids); entries past a sequence's last block are never read.
+ * max_context at most 2^30, B*kv_heads at most 65535 (else INT8K_ERR_UNSUPPORTED).  The workspace
+ * (16-byte aligned) holds scores, the selection and partial states; one of the queried size serves
+ * every call of up to B sequences, max_context positions and top_pages blocks with the same heads
+ * and page size.  Splits as for the tree. */
+size_t int8k_decode_attention_paged_sparse_workspace_bytes(int B, int heads, int kv_heads,
+                                                           int max_context, int page_size,
+                                                           int top_pages, int head_dim);
+
+int int8k_decode_attention_forward_paged_sparse(
+    const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
+    int32_t* selected, const float* scale_Q, const float* sK_pages, const float* sV_pages,
+    const int8_t* K_means, const float* sK_means, const int32_t* block_tables,
+    const int32_t* context_lens, int B, int heads, int kv_heads, int head_dim, int num_pages,
+    int page_size, int max_pages_per_seq, int max_context, int top_pages, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/* Diagnostics of these operators: *count receives, for the current device since the library was
+ * loaded, the tokens appended to slots past the cache, the pairs moved to or from such slots, the
+ * page ids past the cache given to int8k_kv_page_means, and the page ids outside [0, num_pages)
+ * met by the two attentions (at least once per work unit).  Synchronises with the device. */
+int int8k_paged_bad_ids(unsigned int* count);
+
 /* Diagnostics of the 4-bit cache: *count receives, for the current device since the
  * library was loaded, the tokens appended to slots past the cache plus the work units of
  * decodes that met a page id outside [0, num_pages) among the entries their positions

@@ -32,7 +32,8 @@ CALIB_LIB_NAME = "libint8k_calib.so"
 EXT_NAME = "int8_ext"
 
 HIP_SOURCES = ["status.hip", "decode.hip", "mlp.hip", "prefill.hip", "quant.hip", "producer.hip",
-               "noalloc.hip", "linear.hip", "heads.hip", "packed.hip", "kv4.hip"]
+               "noalloc.hip", "linear.hip", "heads.hip", "packed.hip", "kv4.hip",
+               "paged.hip", "pages.hip"]
 
 # -packed-fp32-ops: keep v_pk_{add,mul,fma}_f32 out of the generated code.
 HIP_FLAGS = [

@@ -7,7 +7,8 @@
 //   (y_t, y_{t + rot_dim/2}), or (y_2t, y_2t+1) interleaved, by cos[pos][t], sin[pos][t];
 // dims from rot_dim on and the value heads pass through.  The result is rounded to x's dtype
 // once and stored as heads [B, H, S, D], or quantized per row as int8k_quantize_per_token
-// quantizes those rounded rows.
+// quantizes those rounded rows.  Quantized keys and values can go straight to the rows `slots`
+// of a paged cache [num_pages, kv_heads, page, D] instead: only where a row is stored differs.
 //
 // Memory-bound: x is read once and the heads are written once.  A lane holds both elements of
 // its 8 pairs, 16 elements of a row (D / 16 lanes per row), so the rotation needs no exchange
@@ -19,12 +20,14 @@
 #include <algorithm>
 #include <cmath>
 
+#include "pages.h"
 #include "rows.h"
 
 namespace int8k {
 namespace {
 
 __device__ unsigned int g_rope_bad_positions;
+__device__ unsigned int g_append_bad_slots;
 
 struct HeadsArgs {
     const void* x;
@@ -40,6 +43,8 @@ struct HeadsArgs {
     int lg;           // 1 << lg lanes per row
     int heads_per_wave;
     float inv_dim;    // 1 / D
+    const int32_t* slots;  // PAGED: row page * page_size + offset of each token's key and value
+    int num_pages, log2_page;
 };
 
 // How the 8 pairs of lane item c lie in a row.
@@ -171,8 +176,8 @@ __device__ __forceinline__ void split_pairs(const float (&lo)[8], const float (&
 // The heads [h0, h1) of one part (0 queries, 1 keys, 2 values) for this lane's token.
 template <int DT, bool QUANT, int LAYOUT>
 __device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0, int h1, size_t in,
-                                           size_t row, int cc, bool has, bool ok, int ia, int ib,
-                                           const float* cs, const float* sn) {
+                                           size_t row, size_t row_step, int cc, bool has, bool ok,
+                                           int ia, int ib, const float* cs, const float* sn) {
     // element indices of the pairs of this item
     auto pair = [&](int i, int& ka, int& kb) {
         if constexpr (LAYOUT == kSplitAny) pair_at(8 * cc + i, p.half, ka, kb);
@@ -221,7 +226,6 @@ __device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0,
             cb[i] = wb[i] * c, sa[i] = wa[i] * s;
         }
     }
-    const size_t row_step = (size_t)p.S;
     auto heads = [&](Raw8<DT> lo, Raw8<DT> hi, float (&ga)[8], float (&gv)[8], size_t r) {
         float a[8], v[8];
         if constexpr (LAYOUT == kSplitAny) {
@@ -329,7 +333,7 @@ __device__ __forceinline__ void part_heads(const HeadsArgs& p, int part, int h0,
     }
 }
 
-template <int DT, bool QUANT, int LAYOUT>
+template <int DT, bool QUANT, int LAYOUT, bool PAGED>
 __global__ __launch_bounds__(256, LAYOUT == kSplitAny ? 3 : 4) void qk_norm_rope_kernel(HeadsArgs p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -358,19 +362,35 @@ __global__ __launch_bounds__(256, LAYOUT == kSplitAny ? 3 : 4) void qk_norm_rope
     const long long b = t / p.S;
     const long long s = t - b * p.S;
     const size_t in = (size_t)t * total * p.D;
+    bool stored = ok;  // a negative slot stores no key and no value; one past the cache is counted
+    size_t cache_row = 0;
+    if constexpr (PAGED) {
+        const int slot = p.slots[t];
+        const bool past = slot >= ((long long)p.num_pages << p.log2_page);
+        if (blockIdx.y == 0) {
+            const uint64_t bad = __ballot(past && c == 0 && t_raw < p.tokens);
+            if (bad != 0 && lane == 0) atomicAdd(&g_append_bad_slots, (unsigned)__popcll(bad));
+        }
+        stored = ok && slot >= 0 && !past;
+        const int at = stored ? slot : 0, page = at >> p.log2_page;
+        cache_row = (((size_t)page * p.kv_heads) << p.log2_page) + (at - (page << p.log2_page));
+    }
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
         const int first = part == 0 ? 0 : part == 1 ? p.heads : p.heads + p.kv_heads;
         const int count = part == 0 ? p.heads : p.kv_heads;
         const int a = max(h0, first), e = min(h1, first + count);
-        if (a < e)
-            part_heads<DT, QUANT, LAYOUT>(p, part, a, e, in + (size_t)a * p.D,
-                                          ((size_t)b * count + (a - first)) * p.S + s, cc, has, ok,
-                                          ia, ib, cs, sn);
+        if (a >= e) continue;
+        const bool paged = PAGED && part > 0;
+        const size_t row = paged ? cache_row + ((size_t)(a - first) << p.log2_page)
+                                 : ((size_t)b * count + (a - first)) * p.S + s;
+        const size_t step = paged ? (size_t)1 << p.log2_page : (size_t)p.S;
+        part_heads<DT, QUANT, LAYOUT>(p, part, a, e, in + (size_t)a * p.D, row, step, cc, has,
+                                      paged ? stored : ok, ia, ib, cs, sn);
     }
 }
 
-template <bool QUANT>
+template <bool QUANT, bool PAGED>
 int launch_heads(HeadsArgs p, int dtype, bool interleaved, hipStream_t stream) {
     const int items = p.D / 16;
     while ((1 << p.lg) < items) ++p.lg;
@@ -386,20 +406,27 @@ int launch_heads(HeadsArgs p, int dtype, bool interleaved, hipStream_t stream) {
     const int layout = interleaved ? kInterleaved : p.half % 8 == 0 ? kSplit : kSplitAny;
     with_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (layout == kSplit) qk_norm_rope_kernel<DT, QUANT, kSplit><<<grid, 256, 0, stream>>>(p);
+        if (layout == kSplit)
+            qk_norm_rope_kernel<DT, QUANT, kSplit, PAGED><<<grid, 256, 0, stream>>>(p);
         else if (layout == kInterleaved)
-            qk_norm_rope_kernel<DT, QUANT, kInterleaved><<<grid, 256, 0, stream>>>(p);
-        else qk_norm_rope_kernel<DT, QUANT, kSplitAny><<<grid, 256, 0, stream>>>(p);
+            qk_norm_rope_kernel<DT, QUANT, kInterleaved, PAGED><<<grid, 256, 0, stream>>>(p);
+        else qk_norm_rope_kernel<DT, QUANT, kSplitAny, PAGED><<<grid, 256, 0, stream>>>(p);
     });
     return check_launch("qk_norm_rope_kernel");
 }
 
-template <bool QUANT>
+// Where keys and values go to a paged cache (slots not null).
+struct HeadsCache {
+    const int32_t* slots = nullptr;
+    int num_pages = 0, page_size = 0;
+};
+
+template <bool QUANT, bool PAGED = false>
 int heads_entry(const void* x, int dtype, const float* cos, const float* sin, int max_positions,
                 int rot_dim, const int32_t* positions, const float* q_weight,
                 const float* k_weight, float eps, void* const (&y)[3], int8_t* const (&q)[3],
                 float* const (&s)[3], int B, int S, int heads, int kv_heads, int head_dim,
-                int flags, void* stream) {
+                int flags, void* stream, const HeadsCache& cache = {}) {
     clear_last_error();
     if (!x || !cos || !sin || !positions) return INT8K_ERR_INVALID_ARGUMENT;
     for (int i = 0; i < 3; ++i)
@@ -410,6 +437,12 @@ int heads_entry(const void* x, int dtype, const float* cos, const float* sin, in
         rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim || heads > 65535 || kv_heads > 65535)
         return INT8K_ERR_INVALID_ARGUMENT;
     if (head_dim % 16 || head_dim > 256) return INT8K_ERR_UNSUPPORTED;
+    if constexpr (PAGED) {
+        if (!cache.slots) return INT8K_ERR_INVALID_ARGUMENT;
+        if (const int st = check_pages(cache.num_pages, cache.page_size, kv_heads, head_dim)) return st;
+        if (!aligned_to(cache.slots, 4) || !aligned_to(q[1], 16) || !aligned_to(q[2], 16))
+            return INT8K_ERR_MISALIGNED;
+    }
     if (!aligned_to(x, 16) || !aligned_to(cos, 4) || !aligned_to(sin, 4) ||
         !aligned_to(positions, 4) || !aligned_to(q_weight, 4) || !aligned_to(k_weight, 4))
         return INT8K_ERR_MISALIGNED;
@@ -423,7 +456,10 @@ int heads_entry(const void* x, int dtype, const float* cos, const float* sin, in
     p.tokens = (long long)B * S;
     p.S = S, p.heads = heads, p.kv_heads = kv_heads, p.D = head_dim;
     p.max_pos = max_positions, p.half = rot_dim / 2, p.inv_dim = 1.f / (float)head_dim;
-    return launch_heads<QUANT>(p, dtype, (flags & INT8K_ROPE_INTERLEAVED) != 0, as_stream(stream));
+    if constexpr (PAGED)
+        p.slots = cache.slots, p.num_pages = cache.num_pages, p.log2_page = log2_of(cache.page_size);
+    return launch_heads<QUANT, PAGED>(p, dtype, (flags & INT8K_ROPE_INTERLEAVED) != 0,
+                                      as_stream(stream));
 }
 
 }  // namespace
@@ -452,6 +488,25 @@ extern "C" int int8k_qk_norm_rope_quantize(
                              {scale_q, scale_k, scale_v}, B, S, heads, kv_heads, head_dim, flags,
                              stream);
 }
+
+extern "C" int int8k_qk_norm_rope_append(
+    const void* x, int dtype, const float* cos, const float* sin, int max_positions, int rot_dim,
+    const int32_t* positions, const float* q_weight, const float* k_weight, float eps, int8_t* q,
+    float* scale_q, int8_t* K_pages, int8_t* V_pages, float* sK_pages, float* sV_pages,
+    const int32_t* slots, int B, int S, int heads, int kv_heads, int head_dim, int num_pages,
+    int page_size, int flags, void* stream) {
+    return heads_entry<true, true>(x, dtype, cos, sin, max_positions, rot_dim, positions, q_weight,
+                                   k_weight, eps, {nullptr, nullptr, nullptr},
+                                   {q, K_pages, V_pages}, {scale_q, sK_pages, sV_pages}, B, S,
+                                   heads, kv_heads, head_dim, flags, stream,
+                                   {slots, num_pages, page_size});
+}
+
+namespace int8k {
+int append_bad_slots(unsigned int* count) {
+    return read_counter(&g_append_bad_slots, "hipMemcpyFromSymbol(g_append_bad_slots)", count);
+}
+}  // namespace int8k
 
 extern "C" int int8k_rope_bad_positions(unsigned int* count) {
     clear_last_error();

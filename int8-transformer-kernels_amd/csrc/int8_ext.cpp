@@ -843,13 +843,25 @@ torch::Tensor int8_linear_torch(torch::Tensor x, torch::Tensor W, torch::Tensor 
     return y;
 }
 
-// x (B, S, (heads + 2 kv_heads) * D) or (T, ...) -> heads (B, H, S, D) or (H, T, D) of q, k, v:
-// norms of queries and keys where weights are given, rotation by cos/sin (P, rot_dim / 2) at
-// `positions` int32 (one per token); in x's dtype, or as per-token int8 with fp32 scales.
-static std::vector<torch::Tensor> qk_norm_rope_impl(
-    torch::Tensor x, int64_t heads, int64_t kv_heads, torch::Tensor cos, torch::Tensor sin,
-    torch::Tensor positions, c10::optional<torch::Tensor> q_weight,
-    c10::optional<torch::Tensor> k_weight, double eps, bool interleaved, bool quant) {
+namespace {
+
+// The checked inputs of the calls that norm and rotate the heads of a fused QKV projection.
+struct HeadsCall {
+    int64_t B, S, D;
+    torch::Tensor x, cos, sin, positions, w[2];
+    int code, rot, top, flags;
+    float eps;
+    const float* weight(int i) const { return w[i].defined() ? w[i].data_ptr<float>() : nullptr; }
+    // rows of n heads per token: (B, n, S), or (n, S) for a 2-D x
+    std::vector<int64_t> rows(int64_t n) const {
+        return x.dim() == 2 ? std::vector<int64_t>{n, S} : std::vector<int64_t>{B, n, S};
+    }
+};
+
+HeadsCall check_heads(const torch::Tensor& x, int64_t heads, int64_t kv_heads,
+                      const torch::Tensor& cos, const torch::Tensor& sin,
+                      const torch::Tensor& positions, const c10::optional<torch::Tensor>& q_weight,
+                      const c10::optional<torch::Tensor>& k_weight, double eps, bool interleaved) {
     TORCH_CHECK(x.device().is_cuda(), "x must be a CUDA tensor");
     TORCH_CHECK((x.dim() == 2 || x.dim() == 3) && x.numel() > 0,
                 "x must be a non-empty (batch, seq, width) or (tokens, width) tensor");
@@ -857,61 +869,73 @@ static std::vector<torch::Tensor> qk_norm_rope_impl(
                 "heads and kv_heads must be positive");
     const int64_t parts = heads + 2 * kv_heads;
     TORCH_CHECK(x.size(-1) % parts == 0, "last dim must be (heads + 2 * kv_heads) * head_dim");
-    const int64_t D = x.size(-1) / parts;
-    const int64_t B = x.dim() == 3 ? x.size(0) : 1, S = x.size(-2);
-    TORCH_CHECK(D % 16 == 0 && D <= 256, "head_dim must be a multiple of 16 up to 256");
+    HeadsCall h;
+    h.D = x.size(-1) / parts;
+    h.B = x.dim() == 3 ? x.size(0) : 1, h.S = x.size(-2);
+    TORCH_CHECK(h.D % 16 == 0 && h.D <= 256, "head_dim must be a multiple of 16 up to 256");
     check_float32(cos, "cos");
     check_float32(sin, "sin");
     check_int32(positions, "positions");
     TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(0) >= 1,
                 "cos and sin must be (positions, rot_dim / 2) of one shape");
-    TORCH_CHECK(cos.size(1) >= 1 && 2 * cos.size(1) <= D, "rot_dim must be in [2, head_dim]");
-    TORCH_CHECK(positions.numel() == B * S, "positions must have one element per token");
+    TORCH_CHECK(cos.size(1) >= 1 && 2 * cos.size(1) <= h.D, "rot_dim must be in [2, head_dim]");
+    TORCH_CHECK(positions.numel() == h.B * h.S, "positions must have one element per token");
     for (const auto* t : {&cos, &sin, &positions}) check_on(*t, x, "cos, sin and positions");
-    torch::Tensor w[2];
     const c10::optional<torch::Tensor>* given[2] = {&q_weight, &k_weight};
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
     for (int i = 0; i < 2; ++i) {
         if (!given[i]->has_value() || !(*given[i])->defined()) continue;
-        TORCH_CHECK((*given[i])->numel() == D, "norm weights must have head_dim elements");
-        w[i] = (*given[i])->to(x.device(), torch::kFloat32).contiguous();
+        TORCH_CHECK((*given[i])->numel() == h.D, "norm weights must have head_dim elements");
+        h.w[i] = (*given[i])->to(x.device(), torch::kFloat32).contiguous();
     }
-    const int code = dtype_code(x);
-    auto xc = dense16(x);
-    auto cc = cos.contiguous(), sc = sin.contiguous(), pc = positions.contiguous();
+    h.code = dtype_code(x);
+    h.x = dense16(x), h.cos = cos.contiguous(), h.sin = sin.contiguous();
+    h.positions = positions.contiguous();
+    h.rot = 2 * (int)cos.size(1), h.top = as_int(cos.size(0), "rows of cos");
+    h.flags = interleaved ? INT8K_ROPE_INTERLEAVED : 0, h.eps = (float)eps;
+    as_int(h.B, "batch"), as_int(h.S, "seq");
+    return h;
+}
+
+torch::Tensor empty_on(std::vector<int64_t> shape, at::ScalarType t, const torch::Tensor& with) {
+    return torch::empty(shape, torch::TensorOptions().dtype(t).device(with.device()));
+}
+
+}  // namespace
+
+// x (B, S, (heads + 2 kv_heads) * D) or (T, ...) -> heads (B, H, S, D) or (H, T, D) of q, k, v:
+// norms of queries and keys where weights are given, rotation by cos/sin (P, rot_dim / 2) at
+// `positions` int32 (one per token); in x's dtype, or as per-token int8 with fp32 scales.
+static std::vector<torch::Tensor> qk_norm_rope_impl(
+    torch::Tensor x, int64_t heads, int64_t kv_heads, torch::Tensor cos, torch::Tensor sin,
+    torch::Tensor positions, c10::optional<torch::Tensor> q_weight,
+    c10::optional<torch::Tensor> k_weight, double eps, bool interleaved, bool quant) {
+    const HeadsCall c =
+        check_heads(x, heads, kv_heads, cos, sin, positions, q_weight, k_weight, eps, interleaved);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
     std::vector<torch::Tensor> outs;
     for (const int64_t n : {heads, kv_heads, kv_heads}) {
-        std::vector<int64_t> rows = {B, n, S};
-        if (x.dim() == 2) rows.erase(rows.begin());
-        auto shape = rows;
-        shape.push_back(D);
-        outs.push_back(torch::empty(shape, torch::TensorOptions()
-                                               .dtype(quant ? torch::kInt8 : x.scalar_type())
-                                               .device(x.device())));
-        if (quant)
-            outs.push_back(torch::empty(
-                rows, torch::TensorOptions().dtype(torch::kFloat32).device(x.device())));
+        auto shape = c.rows(n);
+        shape.push_back(c.D);
+        outs.push_back(empty_on(shape, quant ? torch::kInt8 : x.scalar_type(), x));
+        if (quant) outs.push_back(empty_on(c.rows(n), torch::kFloat32, x));
     }
-    const int flags = interleaved ? INT8K_ROPE_INTERLEAVED : 0;
-    const int rot = 2 * (int)cos.size(1), top = as_int(cos.size(0), "rows of cos");
-    const float *wq = w[0].defined() ? w[0].data_ptr<float>() : nullptr,
-                *wk = w[1].defined() ? w[1].data_ptr<float>() : nullptr;
-    const int b = as_int(B, "batch"), s = as_int(S, "seq");
     if (quant) {
         auto q = [&](int i) { return outs[2 * i].data_ptr<int8_t>(); };
         auto sp = [&](int i) { return outs[2 * i + 1].data_ptr<float>(); };
         check_status(int8k_qk_norm_rope_quantize(
-                         xc.data_ptr(), code, cc.data_ptr<float>(), sc.data_ptr<float>(), top, rot,
-                         pc.data_ptr<int32_t>(), wq, wk, (float)eps, q(0), sp(0), q(1), sp(1),
-                         q(2), sp(2), b, s, (int)heads, (int)kv_heads, (int)D, flags,
-                         current_stream(x)),
+                         c.x.data_ptr(), c.code, c.cos.data_ptr<float>(), c.sin.data_ptr<float>(),
+                         c.top, c.rot, c.positions.data_ptr<int32_t>(), c.weight(0), c.weight(1),
+                         c.eps, q(0), sp(0), q(1), sp(1), q(2), sp(2), (int)c.B, (int)c.S,
+                         (int)heads, (int)kv_heads, (int)c.D, c.flags, current_stream(x)),
                      "qk_norm_rope_quantize");
     } else {
-        check_status(int8k_qk_norm_rope(xc.data_ptr(), code, cc.data_ptr<float>(),
-                                        sc.data_ptr<float>(), top, rot, pc.data_ptr<int32_t>(),
-                                        wq, wk, (float)eps, outs[0].data_ptr(),
-                                        outs[1].data_ptr(), outs[2].data_ptr(), b, s, (int)heads,
-                                        (int)kv_heads, (int)D, flags, current_stream(x)),
+        check_status(int8k_qk_norm_rope(c.x.data_ptr(), c.code, c.cos.data_ptr<float>(),
+                                        c.sin.data_ptr<float>(), c.top, c.rot,
+                                        c.positions.data_ptr<int32_t>(), c.weight(0), c.weight(1),
+                                        c.eps, outs[0].data_ptr(), outs[1].data_ptr(),
+                                        outs[2].data_ptr(), (int)c.B, (int)c.S, (int)heads,
+                                        (int)kv_heads, (int)c.D, c.flags, current_stream(x)),
                      "qk_norm_rope");
     }
     return outs;
@@ -1118,6 +1142,251 @@ torch::Tensor int8_decode_attention_forward_kv4_paged_torch(
     return out;
 }
 
+namespace {
+
+struct PageDims {
+    int num_pages, kv_heads, page, head_dim;
+};
+
+// One side of a paged INT8 cache: pages int8 (num_pages, kv_heads, page, head_dim), scales fp32
+// (num_pages, kv_heads, page).
+PageDims check_pages(const torch::Tensor& pages, const torch::Tensor& scales, const char* name) {
+    TORCH_CHECK(pages.device().is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(pages.dtype() == torch::kInt8, name, " must be int8");
+    TORCH_CHECK(pages.dim() == 4 && pages.numel() > 0, name,
+                " must be (num_pages, kv_heads, page, head_dim)");
+    TORCH_CHECK(pages.is_contiguous() && scales.is_contiguous(), name,
+                " and its scales must be contiguous");
+    TORCH_CHECK(aligned16(pages), name, " must be 16-byte aligned");
+    check_float32(scales, "cache scales");
+    check_on(scales, pages, "cache scales");
+    TORCH_CHECK(scales.numel() == pages.size(0) * pages.size(1) * pages.size(2),
+                "cache scales must have num_pages * kv_heads * page elements");
+    const int64_t D = pages.size(3), P = pages.size(2);
+    TORCH_CHECK(D == 64 || D == 128, "the paged cache supports head_dim 64 or 128");
+    TORCH_CHECK(P >= 16 && P <= 1024 && (P & (P - 1)) == 0,
+                "page must be a power of two in [16, 1024]");
+    return {as_int(pages.size(0), "num_pages"), as_int(pages.size(1), "kv_heads"), (int)P, (int)D};
+}
+
+PageDims check_cache(const torch::Tensor& K_pages, const torch::Tensor& V_pages,
+                     const torch::Tensor& sK_pages, const torch::Tensor& sV_pages) {
+    const PageDims d = check_pages(K_pages, sK_pages, "K_pages");
+    check_pages(V_pages, sV_pages, "V_pages");
+    TORCH_CHECK(K_pages.sizes() == V_pages.sizes(), "K_pages/V_pages shape mismatch");
+    check_on(V_pages, K_pages, "every input");
+    return d;
+}
+
+// The mean keys of its pages: int8 (num_pages, kv_heads, head_dim), fp32 (num_pages, kv_heads).
+void check_means(const torch::Tensor& means, const torch::Tensor& scales, const torch::Tensor& pages) {
+    TORCH_CHECK(means.dtype() == torch::kInt8, "K_means must be int8");
+    check_float32(scales, "sK_means");
+    TORCH_CHECK(means.dim() == 3 && means.size(0) == pages.size(0) &&
+                    means.size(1) == pages.size(1) && means.size(2) == pages.size(3),
+                "K_means must be (num_pages, kv_heads, head_dim)");
+    TORCH_CHECK(scales.numel() == pages.size(0) * pages.size(1),
+                "sK_means must have num_pages * kv_heads elements");
+    TORCH_CHECK(means.is_contiguous() && scales.is_contiguous(), "K_means and sK_means must be contiguous");
+    TORCH_CHECK(aligned16(means), "K_means must be 16-byte aligned");
+    check_on(means, pages, "every input");
+    check_on(scales, pages, "every input");
+}
+
+// Query, tables and lengths of an attention over the cache; head_dim is Q's last dim.
+void check_queries(const torch::Tensor& Q, const torch::Tensor& scale_Q,
+                   const torch::Tensor& block_tables, const torch::Tensor& context_lens,
+                   int64_t max_context, const PageDims& d, const torch::Tensor& K_pages) {
+    TORCH_CHECK(Q.dtype() == torch::kInt8, "Q must be int8");
+    TORCH_CHECK(Q.numel() > 0, "Q must not be empty");
+    TORCH_CHECK(Q.size(-1) == d.head_dim, "Q/K head_dim mismatch");
+    TORCH_CHECK(Q.size(1) % d.kv_heads == 0, "heads must be a multiple of kv_heads");
+    check_float32(scale_Q, "scale_Q");
+    check_int32(block_tables, "block_tables");
+    check_int32(context_lens, "context_lens");
+    TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == Q.size(0) &&
+                    context_lens.numel() == Q.size(0),
+                "block_tables (batch, max_pages) / context_lens (batch,) shape mismatch");
+    for (const auto* t : {&Q, &scale_Q, &block_tables, &context_lens})
+        check_on(*t, K_pages, "every input");
+    TORCH_CHECK(max_context >= 1 && max_context <= block_tables.size(1) * d.page,
+                "max_context must be in [1, max_pages * page]");
+}
+
+}  // namespace
+
+// qk_norm_rope_quantize whose keys and values go into rows `slots` int32 (one per token) of the
+// paged cache, in place.  Returns [q, s_q].
+std::vector<torch::Tensor> qk_norm_rope_append_torch(
+    torch::Tensor x, int64_t heads, int64_t kv_heads, torch::Tensor cos, torch::Tensor sin,
+    torch::Tensor positions, torch::Tensor K_pages, torch::Tensor V_pages, torch::Tensor sK_pages,
+    torch::Tensor sV_pages, torch::Tensor slots, c10::optional<torch::Tensor> q_weight,
+    c10::optional<torch::Tensor> k_weight, double eps, bool interleaved) {
+    const PageDims d = check_cache(K_pages, V_pages, sK_pages, sV_pages);
+    const HeadsCall c =
+        check_heads(x, heads, kv_heads, cos, sin, positions, q_weight, k_weight, eps, interleaved);
+    TORCH_CHECK(kv_heads == d.kv_heads && c.D == d.head_dim, "cache/new-token shape mismatch");
+    check_int32(slots, "slots");
+    TORCH_CHECK(slots.numel() == c.B * c.S, "slots must have one element per token");
+    check_on(slots, x, "slots");
+    check_on(K_pages, x, "the cache");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    auto sl = slots.contiguous();
+    auto shape = c.rows(heads);
+    shape.push_back(c.D);
+    auto q = empty_on(shape, torch::kInt8, x), sq = empty_on(c.rows(heads), torch::kFloat32, x);
+    check_status(int8k_qk_norm_rope_append(
+                     c.x.data_ptr(), c.code, c.cos.data_ptr<float>(), c.sin.data_ptr<float>(),
+                     c.top, c.rot, c.positions.data_ptr<int32_t>(), c.weight(0), c.weight(1), c.eps,
+                     q.data_ptr<int8_t>(), sq.data_ptr<float>(), K_pages.data_ptr<int8_t>(),
+                     V_pages.data_ptr<int8_t>(), sK_pages.data_ptr<float>(),
+                     sV_pages.data_ptr<float>(), sl.data_ptr<int32_t>(), (int)c.B, (int)c.S,
+                     (int)heads, (int)kv_heads, (int)c.D, d.num_pages, d.page, c.flags,
+                     current_stream(x)),
+                 "qk_norm_rope_append");
+    return {q, sq};
+}
+
+// Attention of N drafted tokens per sequence over the paged cache that holds them behind
+// context_lens: Q int8 (B, H, N, D); tree_mask int64 (N, words) or (B, N, words), bit j of row i
+// set where token i sees token j (none: the tokens up to itself); node_counts int32 (B,).
+// Returns fp16 (B, H, N, D), or (B, N, H, D) with out_bshd.
+torch::Tensor int8_tree_attention_forward_paged_torch(
+    torch::Tensor Q, torch::Tensor K_pages, torch::Tensor V_pages, torch::Tensor scale_Q,
+    torch::Tensor sK_pages, torch::Tensor sV_pages, torch::Tensor block_tables,
+    torch::Tensor context_lens, c10::optional<torch::Tensor> tree_mask, int64_t max_context,
+    c10::optional<torch::Tensor> node_counts, bool out_bshd) {
+    const PageDims d = check_cache(K_pages, V_pages, sK_pages, sV_pages);
+    TORCH_CHECK(Q.dim() == 4, "expected Q (batch, heads, nodes, head_dim)");
+    check_queries(Q, scale_Q, block_tables, context_lens, max_context, d, K_pages);
+    const int64_t B = Q.size(0), H = Q.size(1), N = Q.size(2), D = Q.size(3), W = (N + 63) / 64;
+    TORCH_CHECK(N <= 256, "a tree has at most 256 nodes");
+    torch::Tensor mask, counts;
+    int64_t each = 0;
+    if (tree_mask.has_value() && tree_mask->defined()) {
+        const torch::Tensor& t = *tree_mask;
+        TORCH_CHECK(t.dtype() == torch::kInt64, "tree_mask must be int64");
+        check_on(t, Q, "tree_mask");
+        TORCH_CHECK((t.dim() == 2 || (t.dim() == 3 && t.size(0) == B)) && t.size(-2) == N &&
+                        t.size(-1) == W,
+                    "tree_mask must be (nodes, ceil(nodes / 64)), or that for each sequence");
+        if (t.dim() == 3) each = N * W;
+    }
+    if (node_counts.has_value() && node_counts->defined()) {
+        check_int32(*node_counts, "node_counts");
+        check_on(*node_counts, Q, "node_counts");
+        TORCH_CHECK(node_counts->numel() == B, "node_counts must be (batch,)");
+    }
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(Q.device());
+    if (tree_mask.has_value() && tree_mask->defined()) mask = tree_mask->contiguous();
+    if (node_counts.has_value() && node_counts->defined()) counts = node_counts->contiguous();
+    auto q = dense16(Q);
+    auto sQ = flat_scale(scale_Q, B * H * N, "scale_Q");
+    auto bt = block_tables.contiguous(), cl = context_lens.contiguous();
+    auto out = empty_on(out_bshd ? std::vector<int64_t>{B, N, H, D} : std::vector<int64_t>{B, H, N, D},
+                        torch::kFloat16, Q);
+    const int b = as_int(B, "batch"), h = as_int(H, "heads"), top = as_int(max_context, "max_context");
+    const size_t ws_bytes =
+        int8k_tree_attention_paged_workspace_bytes(b, h, d.kv_heads, (int)N, top, d.head_dim);
+    auto ws = workspace(ws_bytes, Q.device());
+    check_status(int8k_tree_attention_forward_paged(
+                     q.data_ptr<int8_t>(), K_pages.data_ptr<int8_t>(), V_pages.data_ptr<int8_t>(),
+                     reinterpret_cast<uint16_t*>(out.data_ptr<at::Half>()), sQ.data_ptr<float>(),
+                     sK_pages.data_ptr<float>(), sV_pages.data_ptr<float>(),
+                     bt.data_ptr<int32_t>(), cl.data_ptr<int32_t>(),
+                     mask.defined() ? mask.data_ptr<int64_t>() : nullptr,
+                     mask.defined() ? (int)W : 0, each,
+                     counts.defined() ? counts.data_ptr<int32_t>() : nullptr, b, h, d.kv_heads,
+                     (int)N, d.head_dim, d.num_pages, d.page,
+                     as_int(block_tables.size(1), "max_pages"), top,
+                     out_bshd ? INT8K_ATTN_OUT_BSHD : 0, ws.data(), ws_bytes, current_stream(Q)),
+                 "int8_tree_attention_forward_paged");
+    return out;
+}
+
+// Rows src_slots -> dst_slots, int32 (lists, pairs) or (pairs,), of the paged cache, in place; the
+// rows of a list are all read before any is written.
+void kv_cache_move_paged_torch(torch::Tensor K_pages, torch::Tensor V_pages,
+                               torch::Tensor sK_pages, torch::Tensor sV_pages,
+                               torch::Tensor src_slots, torch::Tensor dst_slots) {
+    const PageDims d = check_cache(K_pages, V_pages, sK_pages, sV_pages);
+    for (const auto* t : {&src_slots, &dst_slots}) {
+        check_int32(*t, "slots");
+        check_on(*t, K_pages, "slots");
+    }
+    TORCH_CHECK((src_slots.dim() == 1 || src_slots.dim() == 2) && src_slots.numel() > 0 &&
+                    src_slots.sizes() == dst_slots.sizes(),
+                "src_slots and dst_slots must be non-empty (lists, pairs) or (pairs,) of one shape");
+    const int64_t pairs = src_slots.size(-1);
+    TORCH_CHECK(pairs <= 256, "a list moves at most 256 rows");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(K_pages.device());
+    auto src = src_slots.contiguous(), dst = dst_slots.contiguous();
+    check_status(int8k_kv_cache_move_paged(
+                     K_pages.data_ptr<int8_t>(), V_pages.data_ptr<int8_t>(),
+                     sK_pages.data_ptr<float>(), sV_pages.data_ptr<float>(),
+                     src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(),
+                     as_int(src.numel() / pairs, "lists"), (int)pairs, d.kv_heads, d.head_dim,
+                     d.num_pages, d.page, current_stream(K_pages)),
+                 "kv_cache_move_paged");
+}
+
+// The mean keys of whole pages `page_ids` int32 (n,) into K_means int8 (num_pages, kv_heads, D)
+// and sK_means fp32, in place.
+void kv_page_means_torch(torch::Tensor K_pages, torch::Tensor sK_pages, torch::Tensor page_ids,
+                         torch::Tensor K_means, torch::Tensor sK_means) {
+    const PageDims d = check_pages(K_pages, sK_pages, "K_pages");
+    check_means(K_means, sK_means, K_pages);
+    check_int32(page_ids, "page_ids");
+    check_on(page_ids, K_pages, "page_ids");
+    TORCH_CHECK(page_ids.dim() == 1 && page_ids.numel() > 0, "page_ids must be a non-empty (n,)");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(K_pages.device());
+    auto ids = page_ids.contiguous();
+    check_status(int8k_kv_page_means(K_pages.data_ptr<int8_t>(), sK_pages.data_ptr<float>(),
+                                     ids.data_ptr<int32_t>(), K_means.data_ptr<int8_t>(),
+                                     sK_means.data_ptr<float>(), as_int(ids.numel(), "page_ids"),
+                                     d.kv_heads, d.head_dim, d.num_pages, d.page,
+                                     current_stream(K_pages)),
+                 "kv_page_means");
+}
+
+// Decode over the top_pages blocks of each sequence and key head whose page means score highest
+// (the last block always): Q int8 (B, H, D).  Returns fp16 (B, H, D) and the blocks int32
+// (B, kv_heads, top_pages), ascending, -1 behind the last.
+std::tuple<torch::Tensor, torch::Tensor> int8_decode_attention_forward_paged_sparse_torch(
+    torch::Tensor Q, torch::Tensor K_pages, torch::Tensor V_pages, torch::Tensor scale_Q,
+    torch::Tensor sK_pages, torch::Tensor sV_pages, torch::Tensor K_means, torch::Tensor sK_means,
+    torch::Tensor block_tables, torch::Tensor context_lens, int64_t max_context,
+    int64_t top_pages) {
+    const PageDims d = check_cache(K_pages, V_pages, sK_pages, sV_pages);
+    check_means(K_means, sK_means, K_pages);
+    TORCH_CHECK(Q.dim() == 3, "expected Q (batch, heads, head_dim)");
+    check_queries(Q, scale_Q, block_tables, context_lens, max_context, d, K_pages);
+    TORCH_CHECK(top_pages >= 1, "top_pages must be positive");
+    const int64_t B = Q.size(0), H = Q.size(1), D = Q.size(2);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(Q.device());
+    auto q = dense16(Q);
+    auto sQ = flat_scale(scale_Q, B * H, "scale_Q");
+    auto bt = block_tables.contiguous(), cl = context_lens.contiguous();
+    auto out = empty_on({B, H, D}, torch::kFloat16, Q);
+    const int b = as_int(B, "batch"), h = as_int(H, "heads"),
+              top = as_int(max_context, "max_context"), n = as_int(top_pages, "top_pages");
+    auto which = empty_on({B, d.kv_heads, top_pages}, torch::kInt32, Q);
+    const size_t ws_bytes = int8k_decode_attention_paged_sparse_workspace_bytes(
+        b, h, d.kv_heads, top, d.page, n, d.head_dim);
+    auto ws = workspace(ws_bytes, Q.device());
+    check_status(int8k_decode_attention_forward_paged_sparse(
+                     q.data_ptr<int8_t>(), K_pages.data_ptr<int8_t>(), V_pages.data_ptr<int8_t>(),
+                     reinterpret_cast<uint16_t*>(out.data_ptr<at::Half>()),
+                     which.data_ptr<int32_t>(), sQ.data_ptr<float>(), sK_pages.data_ptr<float>(),
+                     sV_pages.data_ptr<float>(), K_means.data_ptr<int8_t>(),
+                     sK_means.data_ptr<float>(), bt.data_ptr<int32_t>(), cl.data_ptr<int32_t>(), b,
+                     h, d.kv_heads, d.head_dim, d.num_pages, d.page,
+                     as_int(block_tables.size(1), "max_pages"), top, n, ws.data(), ws_bytes,
+                     current_stream(Q)),
+                 "int8_decode_attention_forward_paged_sparse");
+    return {out, which};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("int8_attention_forward", &int8_attention_forward_torch,
           "INT8 attention with per-token quantization — returns FP16 (optional is_causal; "
@@ -1218,5 +1487,37 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           &int8_decode_attention_forward_kv4_paged_torch,
           "INT8 query decode attention over a paged 4-bit KV cache with grouped heads — returns "
           "FP16");
+    // The paged INT8 cache with grouped heads.
+    m.def("qk_norm_rope_append", &qk_norm_rope_append_torch,
+          "qk_norm_rope_quantize with keys and values stored in rows `slots` of a paged INT8 KV "
+          "cache (in place) — returns [q, s_q]",
+          py::arg("x"), py::arg("heads"), py::arg("kv_heads"), py::arg("cos"), py::arg("sin"),
+          py::arg("positions"), py::arg("K_pages"), py::arg("V_pages"), py::arg("sK_pages"),
+          py::arg("sV_pages"), py::arg("slots"), py::arg("q_weight") = py::none(),
+          py::arg("k_weight") = py::none(), py::arg("eps") = 1e-6,
+          py::arg("interleaved") = false);
+    m.def("int8_tree_attention_forward_paged", &int8_tree_attention_forward_paged_torch,
+          "INT8 attention of a tree of drafted tokens per sequence over a paged KV cache with "
+          "grouped heads — returns FP16 (B, H, N, D), or (B, N, H, D) with out_bshd",
+          py::arg("Q"), py::arg("K_pages"), py::arg("V_pages"), py::arg("scale_Q"),
+          py::arg("sK_pages"), py::arg("sV_pages"), py::arg("block_tables"),
+          py::arg("context_lens"), py::arg("tree_mask"), py::arg("max_context"),
+          py::arg("node_counts") = py::none(), py::arg("out_bshd") = false);
+    m.def("kv_cache_move_paged", &kv_cache_move_paged_torch,
+          "Move rows src_slots to dst_slots of a paged INT8 KV cache (in place)", py::arg("K_pages"),
+          py::arg("V_pages"), py::arg("sK_pages"), py::arg("sV_pages"), py::arg("src_slots"),
+          py::arg("dst_slots"));
+    m.def("kv_page_means", &kv_page_means_torch,
+          "The mean keys of pages of a paged INT8 KV cache as int8 and scales (in place)",
+          py::arg("K_pages"), py::arg("sK_pages"), py::arg("page_ids"), py::arg("K_means"),
+          py::arg("sK_means"));
+    m.def("int8_decode_attention_forward_paged_sparse",
+          &int8_decode_attention_forward_paged_sparse_torch,
+          "INT8 decode attention over the blocks of a paged KV cache whose means score highest — "
+          "returns (FP16, the blocks)",
+          py::arg("Q"), py::arg("K_pages"), py::arg("V_pages"), py::arg("scale_Q"),
+          py::arg("sK_pages"), py::arg("sV_pages"), py::arg("K_means"), py::arg("sK_means"),
+          py::arg("block_tables"), py::arg("context_lens"), py::arg("max_context"),
+          py::arg("top_pages"));
     m.attr("abi_version") = int8k_abi_version();
 }

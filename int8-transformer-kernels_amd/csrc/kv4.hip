@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "pages.h"
 #include "rows.h"
 
 namespace int8k {
@@ -624,14 +625,6 @@ Kv4Plan kv4_plan(int B, int Hq, int Hkv, int max_context) {
     return pl;
 }
 
-int log2_of(int page) {
-    int l = 0;
-    while ((1 << l) < page) ++l;
-    return l;
-}
-
-bool page_ok(int page) { return page >= 16 && page <= 1024 && (page & (page - 1)) == 0; }
-
 template <typename F>
 void with_head_dim(int D, F&& f) {
     if (D == 64) f(std::integral_constant<int, 64>{});
@@ -645,18 +638,6 @@ Kv4Partials kv4_partials(size_t parts, int D) {
     if (parts == 0) return {0, 0};
     const size_t ml = round_up(parts * 2 * sizeof(float), kWorkspaceAlign);
     return {ml, ml + round_up(parts * D * sizeof(float), kWorkspaceAlign)};
-}
-
-// Shared checks of the cache's shape: INT8K_OK or the status to return.
-int check_cache(int num_pages, int page_size, int kv_heads, int head_dim) {
-    if (num_pages <= 0 || kv_heads <= 0) return INT8K_ERR_INVALID_ARGUMENT;
-    if (head_dim != 64 && head_dim != 128) return INT8K_ERR_UNSUPPORTED;
-    if (!page_ok(page_size)) return INT8K_ERR_UNSUPPORTED;
-    // slots are int32
-    if ((long long)num_pages * page_size > 0x7fffffffLL) return INT8K_ERR_UNSUPPORTED;
-    if ((long long)num_pages * page_size >= (1LL << 40) / ((long long)kv_heads * head_dim))
-        return INT8K_ERR_UNSUPPORTED;
-    return INT8K_OK;
 }
 
 }  // namespace
@@ -675,7 +656,7 @@ extern "C" int int8k_kv4_cache_append(const void* k_new, const void* v_new, int 
         return INT8K_ERR_INVALID_ARGUMENT;
     if (T <= 0 || dtype < INT8K_DTYPE_F16 || dtype > INT8K_DTYPE_F32)
         return INT8K_ERR_INVALID_ARGUMENT;
-    if (const int st = check_cache(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
     const int w = dtype == INT8K_DTYPE_F32 ? 4 : 8;  // elements per 16 bytes
     for (long long s : {k_token_stride, k_head_stride, v_token_stride, v_head_stride})
         if (s % w) return INT8K_ERR_MISALIGNED;
@@ -713,7 +694,7 @@ extern "C" int int8k_kv4_cache_read(const uint8_t* pages, const float* scales,
     if (!pages || !scales || !slots || !out) return INT8K_ERR_INVALID_ARGUMENT;
     if (T <= 0 || dtype < INT8K_DTYPE_F16 || dtype > INT8K_DTYPE_F32)
         return INT8K_ERR_INVALID_ARGUMENT;
-    if (const int st = check_cache(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
     if (!aligned_to(pages, 16) || !aligned_to(scales, 4) || !aligned_to(slots, 4) ||
         !aligned_to(out, 16))
         return INT8K_ERR_MISALIGNED;
@@ -754,7 +735,7 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
         return INT8K_ERR_INVALID_ARGUMENT;
     if (B <= 0 || heads <= 0 || max_pages_per_seq <= 0 || max_context <= 0)
         return INT8K_ERR_INVALID_ARGUMENT;
-    if (const int st = check_cache(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
     if (heads % kv_heads || (long long)max_context > (long long)max_pages_per_seq * page_size)
         return INT8K_ERR_INVALID_ARGUMENT;
     if (!aligned_to(Q, 16) || !aligned_to(K_pages, 16) || !aligned_to(V_pages, 16) ||

@@ -1,0 +1,688 @@
+// paged.hip — attention over the paged INT8 cache with grouped heads: a tree of drafted tokens per
+// sequence, and one token per sequence over selected blocks; gfx950.
+//
+//   Q int8 [B, Hq, N, D], scales [B * Hq * N]; the N tokens of sequence b lie in the cache at
+//   positions len_b .. len_b + count_b - 1 (count_b <= N).  Token i sees every position below
+//   len_b and those len_b + j whose bit j is set in its mask (without masks: j <= i).
+//   out = sum_j softmax_j(q . k_j sQ sK_j / sqrt(D)) v_j sV_j, q . k exact int32
+//
+// The query rows of a key head (its Hq / Hkv heads times N tokens, which lie side by side in Q)
+// share its keys: F fragments of 16 of them are the columns of MFMA tiles over 32 positions,
+//   S^T[32 keys x 16 q] = K . Q^T    v_mfma_i32_16x16x64_i8
+//   O^T[D x 16 q]      += V^T . P^T  v_mfma_f32_16x16x32_f16, V as exact fp16
+// In the accumulator layout lane l holds query l % 16 and rows 4 (l / 16) + r.  Rows are keys in
+// the order 4 (m % 4) + m / 4, so lane group g = l / 16 ends up with the scores of keys 4 j + g,
+// j = 0..7, as the B operand of the second product wants them: P never changes lanes.  The A
+// operand of that product is 8 keys of one dim per lane: lane l reads D / 16 bytes of those 8
+// rows and picks a byte of two keys at a time (v_perm), which an XOR and a packed addition turn
+// into two fp16.  Every cache row is read and V converted once for all F fragments; no LDS in
+// the loop.
+//
+// p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
+// that the largest weight p sV of the tile that set it lies in [2^9, 2^10), and a tile whose
+// weights stay in fp16's range under the current m needs no exchange between lanes and no
+// rescaling.  l sums p and O the weighted codes, both in fp32.  A weight is carried as two fp16,
+// its rounding and what that leaves (22 bits): in one, the rounding of a row's largest weights
+// outweighs that of the output.  Below 2^-14 fp16 steps by 2^-24, so a weight is off by at most
+// 2^-25 beside a largest one of 2^9 or more, and long flat tails add up.
+#include <algorithm>
+#include <cmath>
+
+#include "pages.h"
+#include "rows.h"
+
+namespace int8k {
+namespace {
+
+__device__ unsigned int g_attend_bad_ids;
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+constexpr int kTile = 32;               // positions per tile
+constexpr float kMaxWeight = 60000.f;   // fp16 weights stay below it
+constexpr float kMaxSum = 0x1p60f;      // and the sum of a lane's 8 p below this
+constexpr int kMaxShift = 60;           // |m - running maximum| where m is set
+constexpr int kTopExp = 10;             // the largest weight there: below 2^kTopExp
+
+struct Attend {
+    const int8_t *Q, *K, *V;
+    const float *sQ, *sK, *sV;
+    const int32_t* tables;               // page ids of sequence b and key head h:
+    long long table_batch, table_head;   //   from b table_batch + h table_head
+    const int32_t* lens;                 // its positions before the tree: b len_batch + h len_head
+    int len_batch, len_head;
+    bool tree;                           // the N tokens are in the cache behind those positions
+    const int32_t* counts;               // tokens of each sequence, or null (N)
+    const int64_t* mask;                 // [B or 1][N][words], or null
+    long long mask_batch;
+    int words;
+    uint16_t* out;                       // [B, Hq, N, D], or [B, N, Hq, D] with bshd
+    bool bshd;
+    float *part_ml, *part_acc;           // [rows][nsplit][2] and [..][D] (nsplit > 1)
+    int B, Hq, Hkv, N, num_pages, log2_page, max_context;
+    int groups, nsplit;                  // blocks of query rows per key head, splits of a sequence
+    float qk;
+};
+
+// What a sequence holds: `prefix` positions that every token sees, `total` with the tokens'.
+struct Extent {
+    int prefix, total, count;
+};
+__device__ __forceinline__ Extent extent_of(const Attend& p, int b, int kvh) {
+    Extent e;
+    e.prefix = min(max(p.lens[b * p.len_batch + kvh * p.len_head], 0), p.max_context);
+    e.count = !p.tree ? 0 : p.counts == nullptr ? p.N : min(max(p.counts[b], 0), p.N);
+    e.total = min(e.prefix + e.count, p.max_context);
+    return e;
+}
+
+// Whether token `node` sees the token `j` of its sequence's tree.
+__device__ __forceinline__ bool sees(const Attend& p, const int64_t* masks, int node, int j) {
+    return masks == nullptr ? j <= node : (masks[(size_t)node * p.words + (j >> 6)] >> (j & 63)) & 1;
+}
+
+// Whether row `node` attends to any position (tokens past the sequence's do not).
+__device__ bool attends(const Attend& p, int b, int node, const Extent& e) {
+    if (!p.tree) return e.prefix > 0;
+    if (node >= e.count) return false;
+    if (e.prefix > 0) return true;
+    const int64_t* masks = p.mask == nullptr ? nullptr : p.mask + b * p.mask_batch;
+    for (int j = 0; j < e.total; ++j)
+        if (sees(p, masks, node, j)) return true;
+    return false;
+}
+
+// Value of lane N of each row of 16 lanes (DPP row_newbcast).
+template <int N>
+__device__ __forceinline__ float bcast16(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xF, 0xF, true));
+}
+
+// max or sum over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float max_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return max_xor32(fmaxf(__int_as_float(a[0]), __int_as_float(a[1])));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return sum_xor32(__int_as_float(a[0]) + __int_as_float(a[1]));
+}
+
+template <int D>
+struct AttendTile {
+    static constexpr int kK = D / 64;   // 16-byte pieces of a K row per lane
+    static constexpr int kV = D / 64;   // 4-byte words of a V row per lane
+    v4i k[2][kK];                       // row 4 (m % 4) + m / 4 (+ 16): bytes 64 i + 16 g ..
+    uint32_t v[8][kV];                  // key 4 j + g: bytes D / 16 m ..
+    float sk, sv;                       // lane n of a row of lanes: key 4 (n % 8) + g
+};
+
+template <int D, int F>
+__global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
+    using Tile = AttendTile<D>;
+    constexpr int NF = D / 16;          // fragments of O^T
+    constexpr int MR = 16 * F;          // query rows per block
+    constexpr int kORow = D + 4;        // floats per row of O in LDS
+    extern __shared__ __align__(16) float s_merge[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nw = blockDim.x >> 6;
+    const int g = lane >> 4, m16 = lane & 15;
+
+    // Block -> (sequence, split), key head and rows of it.  Blocks go to the 8 XCDs in turn; the
+    // blocks of one piece of a sequence, which share pages, run one after the other on one XCD.
+    const int heads_here = p.Hkv * p.groups;
+    const int local = (int)blockIdx.x / 8;
+    const int piece = local / heads_here * 8 + (int)blockIdx.x % 8;
+    if (piece >= p.B * p.nsplit) return;
+    const int b = piece / p.nsplit, split = piece % p.nsplit;
+    const int kvh = local % heads_here / p.groups, grp = local % p.groups;
+    const int all_rows = p.Hq / p.Hkv * p.N;
+    const int row0_q = grp * MR, rows = min(MR, all_rows - row0_q);
+    const size_t first_row = ((size_t)b * p.Hq + (size_t)kvh * (p.Hq / p.Hkv)) * p.N + row0_q;
+    Extent e = extent_of(p, b, kvh);
+    e.prefix = __builtin_amdgcn_readfirstlane(e.prefix);
+    e.total = __builtin_amdgcn_readfirstlane(e.total);
+    const int tiles = (e.total + kTile - 1) / kTile;
+    const int per_split = (tiles + p.nsplit - 1) / p.nsplit;
+    const int t_begin = min(split * per_split, tiles), t_end = min(t_begin + per_split, tiles);
+    const int32_t* __restrict__ table = p.tables + b * p.table_batch + kvh * p.table_head;
+    const int pmask = (1 << p.log2_page) - 1;
+    const int64_t* masks = p.mask == nullptr ? nullptr : p.mask + b * p.mask_batch;
+
+    // this lane's query row of each fragment (rows past the last hold zeros)
+    v4i qf[F][Tile::kK];
+    float qs[F];
+    int node[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        const int r = min(16 * f + m16, rows - 1);
+        const bool ok = 16 * f + m16 < rows;
+        node[f] = (row0_q + r) % p.N;
+        qs[f] = ok ? p.sQ[first_row + r] * p.qk : 0.f;
+#pragma unroll
+        for (int i = 0; i < Tile::kK; ++i)
+            qf[f][i] = ok ? *reinterpret_cast<const v4i*>(p.Q + (first_row + r) * D + 64 * i + 16 * g)
+                          : v4i{0, 0, 0, 0};
+    }
+
+    // lane offsets inside 16 rows
+    const uint32_t k_off = (uint32_t)(4 * (m16 & 3) + (m16 >> 2)) * D + 16 * g;
+    const uint32_t v_off = (uint32_t)g * D + D / 16 * m16;
+    const int s_off = 4 * (m16 & 3) + g;        // row of this lane's scales inside its 16
+    const bool s_upper = (m16 & 4) != 0;        // they lie in the second 16 keys
+    bool bad = false;
+
+    // The two runs of 16 rows of tile t: their page ids (a page holds whole runs; entries past
+    // the last position are not read), and from those the first row of each.  The ids are read a
+    // tile before the rows are needed, which is a tile before the data is.
+    const bool two_pages = p.log2_page == 4;
+    int id0 = 0, id1 = 0;
+    auto fetch_ids = [&](int t) {
+        if (t >= t_end) return;
+        id0 = table[(t * kTile) >> p.log2_page];
+        if (two_pages) id1 = table[min(t * kTile + 16, e.total - 1) >> p.log2_page];
+    };
+    size_t row0 = 0, row1 = 0;
+    auto rows_of_ids = [&](int t) {
+        if (t >= t_end) return;
+        auto first = [&](int raw, int key) {
+            const int page = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
+            bad = bad || page != raw;
+            return (((size_t)page * p.Hkv + kvh) << p.log2_page) + (size_t)(key & pmask);
+        };
+        const int raw0 = __builtin_amdgcn_readfirstlane(id0);
+        row0 = first(raw0, t * kTile);
+        row1 = row0 + 16;
+        if (two_pages) row1 = first(__builtin_amdgcn_readfirstlane(id1), t * kTile + 16);
+    };
+    auto load = [&](Tile& r) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const size_t row = h == 0 ? row0 : row1;
+            const int8_t* kb = p.K + row * D + k_off;
+#pragma unroll
+            for (int i = 0; i < Tile::kK; ++i) r.k[h][i] = *reinterpret_cast<const v4i*>(kb + 64 * i);
+            const int8_t* vb = p.V + row * D + v_off;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (D == 128) {
+                    const v2u w = *reinterpret_cast<const v2u*>(vb + 4 * j * D);
+                    r.v[4 * h + j][0] = w.x, r.v[4 * h + j][1] = w.y;
+                } else {
+                    r.v[4 * h + j][0] = *reinterpret_cast<const uint32_t*>(vb + 4 * j * D);
+                }
+            }
+        }
+        const size_t srow = (s_upper ? row1 : row0) + s_off;
+        r.sk = p.sK[srow];
+        r.sv = p.sV[srow];
+    };
+
+    v4f o[F][NF];
+    float m[F], l[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        m[f] = -INFINITY, l[f] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NF; ++i) o[f][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto compute = [&](const Tile& r, int t) {
+        const float skj[8] = {bcast16<0>(r.sk), bcast16<1>(r.sk), bcast16<2>(r.sk), bcast16<3>(r.sk),
+                              bcast16<4>(r.sk), bcast16<5>(r.sk), bcast16<6>(r.sk), bcast16<7>(r.sk)};
+        const float svj[8] = {bcast16<0>(r.sv), bcast16<1>(r.sv), bcast16<2>(r.sv), bcast16<3>(r.sv),
+                              bcast16<4>(r.sv), bcast16<5>(r.sv), bcast16<6>(r.sv), bcast16<7>(r.sv)};
+        const bool partial = t * kTile + kTile > e.prefix;  // wave-uniform
+        v8h pw[F], pr[F];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            v4i sa[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sa[h] = v4i{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < Tile::kK; ++i)
+                    sa[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[h][i], qf[f][i], sa[h], 0, 0, 0);
+            }
+            // u_j = q . k_j sK_j of key 4 j + g
+            float u[8], w[8], pj[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = static_cast<float>(sa[j >> 2][j & 3]) * skj[j];
+            auto weights = [&]() {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    pj[j] = fast_exp2(fmaf(u[j], qs[f], -m[f]));
+                    w[j] = pj[j] * svj[j];
+                }
+            };
+            auto sum8 = [&]() {
+                return ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+            };
+            float psum = 0.f;
+            bool slow = partial;
+            if (!partial) {
+                weights();
+                psum = sum8();
+                float wide = fmaxf(fabsf(w[0]), fabsf(w[1]));
+#pragma unroll
+                for (int j = 2; j < 8; j += 2) wide = fmaxf(wide, fmaxf(fabsf(w[j]), fabsf(w[j + 1])));
+                // (the first tile, whose m is -inf, has an infinite sum)
+                slow = __ballot(fmaxf(wide, psum * (kMaxWeight / kMaxSum)) > kMaxWeight) != 0;
+            }
+            if (slow) {
+                // the exact maximum, then the largest weight under it
+                float top = -INFINITY, pm = 0.f;
+                bool seen[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int pos = t * kTile + 4 * j + g;
+                    seen[j] = pos < e.prefix ||
+                              (pos < e.total && sees(p, masks, node[f], pos - e.prefix));
+                    if (seen[j]) top = fmaxf(top, u[j] * qs[f]);
+                }
+                top = max_groups(top);
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (seen[j]) pm = fmaxf(pm, fabsf(fast_exp2(fmaf(u[j], qs[f], -base)) * svj[j]));
+                pm = max_groups(pm);
+                int ex = 0;
+                if (pm > 0.f && pm < INFINITY) frexpf(pm, &ex);
+                const float m_new =
+                    fmaxf(m[f], top + (float)min(max(ex - kTopExp, -kMaxShift), kMaxShift));
+                const float alpha = fast_exp2(m[f] - (m_new == -INFINITY ? 0.f : m_new));
+                m[f] = m_new;
+                l[f] *= alpha;
+#pragma unroll
+                for (int i = 0; i < NF; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[f][i][c] *= alpha;
+                weights();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)  // unseen rows may hold anything
+                    if (!seen[j]) pj[j] = w[j] = 0.f;
+                psum = sum8();
+            }
+            l[f] += psum;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                pw[f][j] = (_Float16)w[j];
+                pr[f][j] = (_Float16)(w[j] - (float)pw[f][j]);
+            }
+            if (slow) {  // (a weight past fp16's range, by an infinite value scale, leaves no rest)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pr[f][j] = fabsf(w[j]) < 65520.f ? pr[f][j] : (_Float16)0.f;
+            }
+        }
+        // byte c of two keys, c + 128 as an unsigned number u: 0x6400 | u is 1024 + u in fp16, and
+        // the sum below exact
+        const h2 bias = {(_Float16)-1152.f, (_Float16)-1152.f};
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            v8h v;
+            const uint32_t byte = i & 3;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t c = __builtin_amdgcn_perm(r.v[2 * j + 1][i >> 2], r.v[2 * j][i >> 2],
+                                                         byte | 0x0c000c00u | ((4u + byte) << 16));
+                const h2 a = __builtin_bit_cast(h2, c ^ 0x64806480u) + bias;
+                v[2 * j] = a.x, v[2 * j + 1] = a.y;
+            }
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                o[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[f], o[f][i], 0, 0, 0);
+                o[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pr[f], o[f][i], 0, 0, 0);
+            }
+        }
+    };
+
+    {
+        int t = t_begin + wave;
+        Tile ra, rb;
+        // Data of tile t in ra, rows of tile t + nw, ids of tile t + 2 nw.  The loads are not
+        // conditional: past the last tile they repeat its rows.
+        fetch_ids(t);
+        rows_of_ids(t);
+        fetch_ids(t + nw);
+        if (t < t_end) load(ra);
+        rows_of_ids(t + nw);
+        fetch_ids(t + 2 * nw);
+        while (t < t_end) {
+            load(rb);
+            rows_of_ids(t + 2 * nw);
+            fetch_ids(t + 3 * nw);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(ra, t);
+            t += nw;
+            if (t >= t_end) break;
+            load(ra);
+            rows_of_ids(t + 2 * nw);
+            fetch_ids(t + 3 * nw);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(rb, t);
+            t += nw;
+        }
+    }
+    if (bad && lane == 0) atomicAdd(&g_attend_bad_ids, 1u);
+
+    // Join the waves: m, l and O of each row go to LDS, then element by element.
+    // Layout: [wave][m of MR rows][l of MR rows][MR rows][kORow].
+    constexpr int kWaveWords = 2 * MR + MR * kORow;
+    float* mine = s_merge + wave * kWaveWords;
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        const float lf = sum_groups(l[f]);
+        const int r = 16 * f + m16;
+        if (g == 0) mine[r] = m[f], mine[MR + r] = lf;
+        float* orow = mine + 2 * MR + r * kORow;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)  // rows 4 g + c of the fragments: dims NF (4 g + c) ..
+#pragma unroll
+            for (int i = 0; i < NF; i += 4)
+                *reinterpret_cast<float4*>(orow + NF * (4 * g + c) + i) =
+                    make_float4(o[f][i][c], o[f][i + 1][c], o[f][i + 2][c], o[f][i + 3][c]);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < rows * D; x += blockDim.x) {
+        const int row = x / D, d = x % D;
+        float top = -INFINITY, sum = 0.f, acc = 0.f;
+        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_merge[w * kWaveWords + row]);
+        const float use = top == -INFINITY ? 0.f : top;
+        for (int w = 0; w < nw; ++w) {
+            const float* q = s_merge + w * kWaveWords;
+            const float a = fast_exp2(q[row] - use);
+            sum += q[MR + row] * a;
+            acc += q[2 * MR + row * kORow + d] * a;
+        }
+        if (p.nsplit == 1) {
+            const int r = row0_q + row, n = r % p.N, h = kvh * (p.Hq / p.Hkv) + r / p.N;
+            const size_t at = p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : first_row + row;
+            p.out[at * D + d] =
+                attends(p, b, n, e) ? __half_as_ushort(f16_of_f32(acc / sum)) : (uint16_t)0;
+        } else {
+            const size_t part = (first_row + row) * p.nsplit + split;
+            if (d == 0) p.part_ml[2 * part] = top, p.part_ml[2 * part + 1] = sum;
+            p.part_acc[part * D + d] = acc;
+        }
+    }
+}
+
+// Joins the splits of each row, one thread per dim: eight partials in flight at a time (slots
+// past the last repeat it with weight zero).
+template <int D>
+__global__ __launch_bounds__(D) void paged_combine_kernel(Attend p) {
+    const size_t row = blockIdx.x;
+    const int d = threadIdx.x, nsplit = p.nsplit;
+    const int n = (int)(row % p.N), h = (int)(row / p.N % p.Hq), b = (int)(row / p.N / p.Hq);
+    const float2* r = reinterpret_cast<const float2*>(p.part_ml) + row * nsplit;
+    const float* x = p.part_acc + row * nsplit * D + d;
+    const bool any = attends(p, b, n, extent_of(p, b, h / (p.Hq / p.Hkv)));
+    float m = -INFINITY, sum = 0.f, a = 0.f;
+    for (int i0 = 0; i0 < nsplit; i0 += 8) {
+        float2 s[8];
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = min(i0 + k, nsplit - 1);
+            s[k] = r[i];
+            v[k] = x[(size_t)i * D];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
+        const float use = top == -INFINITY ? 0.f : top;
+        const float keep = fast_exp2(m - use);
+        sum *= keep;
+        a *= keep;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = i0 + k < nsplit ? fast_exp2(s[k].x - use) : 0.f;
+            // (a repeated slot must not turn an infinite partial into NaN)
+            sum += i0 + k < nsplit ? s[k].y * f : 0.f;
+            a += i0 + k < nsplit ? v[k] * f : 0.f;
+        }
+        m = top;
+    }
+    const size_t at = p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : row;
+    p.out[at * D + d] = any ? __half_as_ushort(f16_of_f32(a / sum)) : (uint16_t)0;
+}
+
+// ------------------------------------------------------------------ host side
+
+struct AttendPlan {
+    int frags, groups, waves, nsplit;
+};
+
+constexpr int kMaxSplit = 64, kMaxBlocks = 1024;
+
+// rows: query rows per key head
+AttendPlan attend_plan(int B, int rows, int Hkv, int context) {
+    AttendPlan pl{};
+    pl.frags = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    pl.groups = (rows + 16 * pl.frags - 1) / (16 * pl.frags);
+    pl.waves = 4;
+    const long long units = (long long)B * Hkv * pl.groups;
+    const long long tiles = ceil_div(context, kTile);
+    long long s = std::min<long long>(kMaxSplit, std::max<long long>(1, kMaxBlocks / units));
+    s = std::min(s, ceil_div(tiles, 2 * pl.waves));
+    pl.nsplit = (int)std::max<long long>(1, s);
+    return pl;
+}
+
+struct Partials {
+    size_t ml_bytes, bytes;
+};
+Partials partials_of(size_t parts, int D) {
+    if (parts == 0) return {0, 0};
+    const size_t ml = round_up(parts * 2 * sizeof(float), kWorkspaceAlign);
+    return {ml, ml + round_up(parts * D * sizeof(float), kWorkspaceAlign)};
+}
+Partials plan_partials(const AttendPlan& pl, size_t rows, int D) {
+    return partials_of(pl.nsplit > 1 ? rows * pl.nsplit : 0, D);
+}
+
+// Room for every plan of at most `rows` query rows in all: a plan has at most kMaxSplit splits, and
+// kMaxBlocks blocks of at most 64 rows where it has more than one split.
+Partials most_partials(size_t rows, int D) {
+    return partials_of(std::min<size_t>(kMaxSplit * rows, 64 * kMaxBlocks), D);
+}
+
+template <int D, int F>
+int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipStream_t stream) {
+    constexpr int kWave = (2 * 16 * F + 16 * F * (D + 4)) * 4;  // bytes of LDS per wave
+    static PerDeviceOnce once;
+    const int st = once.run([] {
+        const hipError_t e = hipFuncSetAttribute(
+            reinterpret_cast<const void*>(&paged_attend_kernel<D, F>),
+            hipFuncAttributeMaxDynamicSharedMemorySize, (F == 4 ? 4 : 8) * kWave);
+        if (e == hipSuccess) return (int)INT8K_OK;
+        set_last_error("hipFuncSetAttribute", e);
+        return (int)INT8K_ERR_HIP;
+    });
+    if (st != INT8K_OK) return st;
+    paged_attend_kernel<D, F><<<blocks, 64 * pl.waves, pl.waves * kWave, stream>>>(p);
+    return check_launch("paged_attend_kernel");
+}
+
+template <int D>
+int launch_attend(Attend p, const AttendPlan& pl, void* workspace, hipStream_t stream) {
+    const size_t rows = (size_t)p.B * p.Hq * p.N;
+    p.groups = pl.groups, p.nsplit = pl.nsplit;
+    p.part_ml = static_cast<float*>(workspace);
+    p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                          plan_partials(pl, rows, D).ml_bytes);
+    const unsigned blocks =
+        (unsigned)(ceil_div((long long)p.B * pl.nsplit, 8) * 8 * p.Hkv * pl.groups);
+    const int st = pl.frags == 1   ? launch_instance<D, 1>(p, pl, blocks, stream)
+                   : pl.frags == 2 ? launch_instance<D, 2>(p, pl, blocks, stream)
+                                   : launch_instance<D, 4>(p, pl, blocks, stream);
+    if (st != INT8K_OK || pl.nsplit == 1) return st;
+    paged_combine_kernel<D><<<(unsigned)rows, D, 0, stream>>>(p);
+    return check_launch("paged_combine_kernel");
+}
+
+int run_attend(const Attend& p, const AttendPlan& pl, int D, void* workspace, hipStream_t stream) {
+    return D == 64 ? launch_attend<64>(p, pl, workspace, stream)
+                   : launch_attend<128>(p, pl, workspace, stream);
+}
+
+// Sizes that the grid and the row indexes hold.
+bool attend_fits(long long B, long long heads, long long kv_heads, long long nodes, int max_context,
+                 const AttendPlan& pl) {
+    return B * heads * nodes < (1LL << 24) && max_context <= (1 << 30) &&
+           (ceil_div(B * pl.nsplit, 8) * 8 * kv_heads * pl.groups) * pl.waves < (1LL << 25);
+}
+
+constexpr int kMaxNodes = 256;
+
+}  // namespace
+
+int attend_bad_ids(unsigned int* count) {
+    return read_counter(&g_attend_bad_ids, "hipMemcpyFromSymbol(g_attend_bad_ids)", count);
+}
+}  // namespace int8k
+
+using namespace int8k;
+
+extern "C" size_t int8k_tree_attention_paged_workspace_bytes(int B, int heads, int kv_heads,
+                                                             int nodes, int max_context,
+                                                             int head_dim) {
+    if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || nodes <= 0 ||
+        nodes > kMaxNodes || max_context <= 0 || (head_dim != 64 && head_dim != 128) ||
+        (long long)B * heads * nodes >= (1LL << 24))
+        return 0;
+    return most_partials((size_t)B * heads * nodes, head_dim).bytes;
+}
+
+extern "C" int int8k_tree_attention_forward_paged(
+    const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
+    const float* scale_Q, const float* sK_pages, const float* sV_pages,
+    const int32_t* block_tables, const int32_t* context_lens, const int64_t* tree_mask,
+    int mask_words, long long mask_batch_stride, const int32_t* node_counts, int B, int heads,
+    int kv_heads, int nodes, int head_dim, int num_pages, int page_size, int max_pages_per_seq,
+    int max_context, int flags, void* workspace, size_t workspace_bytes, void* stream) {
+    clear_last_error();
+    if (!Q || !K_pages || !V_pages || !out || !scale_Q || !sK_pages || !sV_pages ||
+        !block_tables || !context_lens)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (B <= 0 || heads <= 0 || nodes <= 0 || max_pages_per_seq <= 0 || max_context <= 0 ||
+        (flags & ~INT8K_ATTN_OUT_BSHD))
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (tree_mask && (mask_words != (nodes + 63) / 64 ||
+                      (mask_batch_stride != 0 && mask_batch_stride < (long long)nodes * mask_words)))
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (heads % kv_heads || (long long)max_context > (long long)max_pages_per_seq * page_size)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (!aligned_to(Q, 16) || !aligned_to(K_pages, 16) || !aligned_to(V_pages, 16) ||
+        !aligned_to(scale_Q, 4) || !aligned_to(sK_pages, 4) || !aligned_to(sV_pages, 4) ||
+        !aligned_to(block_tables, 4) || !aligned_to(context_lens, 4) || !aligned_to(out, 8) ||
+        !aligned_to(tree_mask, 8) || !aligned_to(node_counts, 4))
+        return INT8K_ERR_MISALIGNED;
+    if (nodes > kMaxNodes || (long long)B * heads * nodes >= (1LL << 24))
+        return INT8K_ERR_UNSUPPORTED;
+    const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context);
+    if (!attend_fits(B, heads, kv_heads, nodes, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
+    const size_t need = plan_partials(pl, (size_t)B * heads * nodes, head_dim).bytes;
+    if (need > 0) {
+        if (!workspace || workspace_bytes < need) return INT8K_ERR_WORKSPACE;
+        if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
+    }
+    Attend p{};
+    p.Q = Q, p.K = K_pages, p.V = V_pages, p.sQ = scale_Q, p.sK = sK_pages, p.sV = sV_pages;
+    p.tables = block_tables, p.table_batch = max_pages_per_seq, p.table_head = 0;
+    p.lens = context_lens, p.len_batch = 1, p.len_head = 0;
+    p.tree = true, p.counts = node_counts, p.mask = tree_mask, p.mask_batch = mask_batch_stride;
+    p.words = mask_words, p.out = out, p.bshd = (flags & INT8K_ATTN_OUT_BSHD) != 0;
+    p.B = B, p.Hq = heads, p.Hkv = kv_heads, p.N = nodes, p.num_pages = num_pages;
+    p.log2_page = log2_of(page_size), p.max_context = max_context;
+    p.qk = (1.0f / std::sqrt((float)head_dim)) * kLog2e;
+    return run_attend(p, pl, head_dim, workspace, as_stream(stream));
+}
+
+extern "C" size_t int8k_decode_attention_paged_sparse_workspace_bytes(int B, int heads,
+                                                                      int kv_heads,
+                                                                      int max_context,
+                                                                      int page_size, int top_pages,
+                                                                      int head_dim) {
+    if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 ||
+        page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) || top_pages <= 0 ||
+        (head_dim != 64 && head_dim != 128) || (long long)B * heads >= (1LL << 24) ||
+        max_context > (1 << 30))
+        return 0;
+    const SelectSpace sel = select_space(B, kv_heads, max_context, page_size, top_pages);
+    return sel.bytes + most_partials((size_t)B * heads, head_dim).bytes;
+}
+
+extern "C" int int8k_decode_attention_forward_paged_sparse(
+    const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
+    int32_t* selected, const float* scale_Q, const float* sK_pages, const float* sV_pages,
+    const int8_t* K_means, const float* sK_means, const int32_t* block_tables,
+    const int32_t* context_lens, int B, int heads, int kv_heads, int head_dim, int num_pages,
+    int page_size, int max_pages_per_seq, int max_context, int top_pages, void* workspace,
+    size_t workspace_bytes, void* stream) {
+    clear_last_error();
+    if (!Q || !K_pages || !V_pages || !out || !selected || !scale_Q || !sK_pages || !sV_pages ||
+        !K_means || !sK_means || !block_tables || !context_lens)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (B <= 0 || heads <= 0 || max_pages_per_seq <= 0 || max_context <= 0 || top_pages <= 0)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (heads % kv_heads || (long long)max_context > (long long)max_pages_per_seq * page_size)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (!aligned_to(Q, 16) || !aligned_to(K_pages, 16) || !aligned_to(V_pages, 16) ||
+        !aligned_to(K_means, 16) || !aligned_to(scale_Q, 4) || !aligned_to(sK_pages, 4) ||
+        !aligned_to(sV_pages, 4) || !aligned_to(sK_means, 4) || !aligned_to(block_tables, 4) ||
+        !aligned_to(context_lens, 4) || !aligned_to(out, 8) || !aligned_to(selected, 4))
+        return INT8K_ERR_MISALIGNED;
+    const int context = (int)std::min<long long>(max_context, (long long)top_pages * page_size);
+    if ((long long)B * heads >= (1LL << 24) || max_context > (1 << 30) ||
+        (long long)B * kv_heads > 65535 || (long long)B * kv_heads * top_pages >= (1LL << 31))
+        return INT8K_ERR_UNSUPPORTED;
+    const AttendPlan pl = attend_plan(B, heads / kv_heads, kv_heads, context);
+    if (!attend_fits(B, heads, kv_heads, 1, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
+    const SelectSpace sel = select_space(B, kv_heads, max_context, page_size, top_pages);
+    if (!workspace ||
+        workspace_bytes < sel.bytes + plan_partials(pl, (size_t)B * heads, head_dim).bytes)
+        return INT8K_ERR_WORKSPACE;
+    if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
+
+    char* ws = static_cast<char*>(workspace);
+    Select s{};
+    s.Q = Q, s.sQ = scale_Q, s.means = K_means, s.s_means = sK_means, s.tables = block_tables;
+    s.lens = context_lens, s.keys = reinterpret_cast<uint64_t*>(ws + sel.keys);
+    s.pages = reinterpret_cast<int32_t*>(ws + sel.pages);
+    s.positions = reinterpret_cast<int32_t*>(ws + sel.positions), s.selected = selected;
+    s.B = B, s.Hq = heads, s.Hkv = kv_heads, s.D = head_dim, s.num_pages = num_pages;
+    s.log2_page = log2_of(page_size), s.max_pages = max_pages_per_seq, s.max_context = max_context;
+    s.max_blocks = (int)ceil_div(max_context, page_size), s.top = top_pages;
+    if (const int st = launch_select(s, as_stream(stream))) return st;
+
+    Attend p{};
+    p.Q = Q, p.K = K_pages, p.V = V_pages, p.sQ = scale_Q, p.sK = sK_pages, p.sV = sV_pages;
+    p.tables = s.pages, p.table_batch = (long long)kv_heads * top_pages, p.table_head = top_pages;
+    p.lens = s.positions, p.len_batch = kv_heads, p.len_head = 1;
+    p.tree = false, p.out = out;
+    p.B = B, p.Hq = heads, p.Hkv = kv_heads, p.N = 1, p.num_pages = num_pages;
+    p.log2_page = s.log2_page, p.max_context = context;
+    p.qk = (1.0f / std::sqrt((float)head_dim)) * kLog2e;
+    return run_attend(p, pl, head_dim, ws + sel.bytes, as_stream(stream));
+}
+
+extern "C" int int8k_paged_bad_ids(unsigned int* count) {
+    clear_last_error();
+    if (!count) return INT8K_ERR_INVALID_ARGUMENT;
+    unsigned int n[3] = {0, 0, 0};
+    for (int i = 0; i < 3; ++i) {
+        const int st = i == 0 ? append_bad_slots(n) : i == 1 ? attend_bad_ids(n + 1) : pages_bad_ids(n + 2);
+        if (st != INT8K_OK) return st;
+    }
+    *count = n[0] + n[1] + n[2];
+    return INT8K_OK;
+}

@@ -1,0 +1,388 @@
+// pages.hip — upkeep of the paged INT8 cache: moving rows, the mean key of each page, and the
+// selection of blocks by those means; gfx950.
+#include <algorithm>
+#include <cmath>
+
+#include "pages.h"
+#include "rows.h"
+
+namespace int8k {
+namespace {
+
+__device__ unsigned int g_pages_bad_ids;
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------ move
+// Rows src -> dst of every key head, list by list: a block takes one list of one head of one side,
+// reads all its rows into registers and writes them after a barrier, so a destination may be
+// another pair's source.  Latency-bound: one dependent load after the slots.
+
+struct Move {
+    int8_t* pages[2];
+    float* scales[2];
+    const int32_t *src, *dst;
+    int pairs, Hkv, num_pages, log2_page;
+};
+
+constexpr int kMaxPairs = 256;
+
+template <int D, int ITEMS>
+__global__ __launch_bounds__(256) void move_rows_kernel(Move p) {
+    constexpr int C = D / 16;  // 16-byte pieces of a row
+    const int h = (int)(blockIdx.x % (unsigned)p.Hkv), list = (int)(blockIdx.x / (unsigned)p.Hkv);
+    const int side = blockIdx.y, T = blockDim.x;
+    const int32_t *src = p.src + (size_t)list * p.pairs, *dst = p.dst + (size_t)list * p.pairs;
+    const long long cap = (long long)p.num_pages << p.log2_page;
+    auto row_of = [&](int slot) {
+        const int page = slot >> p.log2_page;
+        return (((size_t)page * p.Hkv + h) << p.log2_page) + (slot - (page << p.log2_page));
+    };
+    // the pair's rows, or false where it is left out
+    auto rows = [&](int i, size_t& from, size_t& to) {
+        const int s = src[i], d = dst[i];
+        if (s < 0 || d < 0 || s >= cap || d >= cap) return false;
+        from = row_of(s), to = row_of(d);
+        return true;
+    };
+    uint4 v[ITEMS];
+    size_t at[ITEMS];
+    bool have[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int x = threadIdx.x + k * T;
+        size_t from = 0;
+        have[k] = x < p.pairs * C && rows(x / C, from, at[k]);
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (have[k]) v[k] = *reinterpret_cast<const uint4*>(p.pages[side] + from * D + 16 * (x % C));
+    }
+    // the scales, one or more per thread
+    constexpr int kScales = (ITEMS + C - 1) / C;
+    float sc[kScales];
+    size_t sat[kScales];
+    bool shave[kScales];
+#pragma unroll
+    for (int k = 0; k < kScales; ++k) {
+        const int x = threadIdx.x + k * T;
+        size_t from = 0;
+        shave[k] = x < p.pairs && rows(x, from, sat[k]);
+        sc[k] = shave[k] ? p.scales[side][from] : 0.f;
+        if (h == 0 && side == 0 && x < p.pairs && (src[x] >= cap || dst[x] >= cap))
+            atomicAdd(&g_pages_bad_ids, 1u);
+    }
+    // the data has arrived, not only been asked for, before any thread writes
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) reload_barrier(v[k]);
+#pragma unroll
+    for (int k = 0; k < kScales; ++k) asm volatile("" : "+v"(sc[k]));
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int x = threadIdx.x + k * T;
+        if (have[k]) *reinterpret_cast<uint4*>(p.pages[side] + at[k] * D + 16 * (x % C)) = v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kScales; ++k)
+        if (shave[k]) p.scales[side][sat[k]] = sc[k];
+}
+
+// ------------------------------------------------------------------ means
+// m_d = sum over a page's rows of code * scale / page, summed in 64 bits (so that a code beside a
+// rounding border does not depend on the order of the sum), rounded to fp32 and quantized as
+// int8k_quantize_per_token does; a NaN in a mean makes the scale NaN.
+
+template <int D>
+__global__ __launch_bounds__(256) void page_means_kernel(const int8_t* __restrict__ pages,
+                                                         const float* __restrict__ scales,
+                                                         const int32_t* __restrict__ ids,
+                                                         int8_t* __restrict__ means,
+                                                         float* __restrict__ s_means, int Hkv,
+                                                         int num_pages, int log2_page) {
+    constexpr int L = D / 16, R = 64 / L;  // lanes per row, rows per wave load
+    __shared__ double s_sum[4][D];
+    const int h = (int)(blockIdx.x % (unsigned)Hkv), id = ids[blockIdx.x / (unsigned)Hkv];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    if (id < 0 || id >= num_pages) {  // the whole block leaves
+        if (id >= 0 && h == 0 && threadIdx.x == 0) atomicAdd(&g_pages_bad_ids, 1u);
+        return;
+    }
+    const size_t unit = (size_t)id * Hkv + h, row0 = unit << log2_page;
+    const int page = 1 << log2_page;
+    double acc[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.0;
+    for (int r = wave * R + lane / L; r < page; r += nw * R) {
+        const uint4 w = *reinterpret_cast<const uint4*>(pages + (row0 + r) * D + 16 * (lane % L));
+        const double s = (double)scales[row0 + r];
+        const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            acc[i] = fma((double)(int)(int8_t)((d[i >> 2] >> (8 * (i & 3))) & 0xff), s, acc[i]);
+    }
+    // over the wave's rows, then over the waves
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int x = L; x < 64; x <<= 1) acc[i] += __shfl_xor(acc[i], x);
+    if (lane < L)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s_sum[wave][16 * lane + i] = acc[i];
+    __syncthreads();
+    if (wave != 0) return;
+    constexpr int W = D / 64;
+    float m[W];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        double sum = 0.0;
+        for (int w = 0; w < nw; ++w) sum += s_sum[w][W * lane + i];
+        m[i] = (float)(sum / page);
+        top = max(top, __float_as_uint(m[i]) & 0x7fffffffu);
+    }
+    top = __float_as_uint(row_reduce(__uint_as_float(top), 6, [](float a, float b) {
+        return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+    }));
+    const float amax = __uint_as_float(top);
+    const float s = (amax < 1e-8f ? 1e-8f : amax) / 127.f;
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) c |= ((uint32_t)quant_code(m[i], s) & 0xffu) << (8 * i);
+    int8_t* out = means + unit * D + W * lane;
+    if constexpr (W == 2) *reinterpret_cast<uint16_t*>(out) = (uint16_t)c;
+    else *out = (int8_t)c;
+    if (lane == 0) s_means[unit] = s;
+}
+
+// ------------------------------------------------------------------ selection
+// score of a block = max over the heads of the group of (q . mean) sMean sQ, q . mean exact, the
+// products in 64 bits in that order, so the order of two scores is that of the formula.  The
+// last block is taken always and has no score.
+
+__device__ __forceinline__ int blocks_of(const Select& p, int b, int& len) {
+    len = min(max(p.lens[b], 0), p.max_context);
+    return (len + (1 << p.log2_page) - 1) >> p.log2_page;
+}
+
+// Larger scores have larger keys; NaN, which no score is above, has 0.
+__device__ __forceinline__ uint64_t score_key(double s) {
+    if (s != s) return 0;
+    const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);  // (one zero)
+    return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
+    constexpr int L = D / 16, kRows = 256 / L, kEach = 2;  // lanes per mean, means per block, per lane
+    const int row = blockIdx.y, b = row / p.Hkv, h = row % p.Hkv, G = p.Hq / p.Hkv;
+    int len;
+    const int n = blocks_of(p, b, len);
+    if (n <= p.top) return;  // all are taken
+    const int first = blockIdx.x * (kRows * kEach) + threadIdx.x / L, c = threadIdx.x % L;
+    if ((int)(blockIdx.x * (kRows * kEach)) >= n - 1) return;
+    v4i mean[kEach];
+    double sm[kEach], best[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int i = min(first + k * kRows, n - 2);
+        const int raw = p.tables[(size_t)b * p.max_pages + i];
+        const int id = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
+        if (id != raw && h == 0 && c == 0 && first + k * kRows < n - 1) atomicAdd(&g_pages_bad_ids, 1u);
+        const size_t unit = (size_t)id * p.Hkv + h;
+        mean[k] = *reinterpret_cast<const v4i*>(p.means + unit * D + 16 * c);
+        sm[k] = (double)p.s_means[unit];
+        best[k] = -INFINITY;
+    }
+    bool any[kEach] = {};
+    for (int g = 0; g < G; ++g) {
+        const size_t qrow = (size_t)b * p.Hq + h * G + g;
+        const v4i q = *reinterpret_cast<const v4i*>(p.Q + qrow * D + 16 * c);
+        const double sq = (double)p.sQ[qrow];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            int dot = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = __builtin_amdgcn_sdot4(q[i], mean[k][i], dot, false);
+            dot = L == 8 ? group8_sum(dot) : group4_sum(dot);
+            const double s = ((double)dot * sm[k]) * sq;
+            any[k] = any[k] || s == s;
+            best[k] = s > best[k] ? s : best[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int i = first + k * kRows;
+        if (c == 0 && i < n - 1)
+            p.keys[(size_t)row * p.max_blocks + i] = any[k] ? score_key(best[k]) : 0;
+    }
+}
+
+constexpr int kSelectThreads = 1024;
+
+// Sum of v over the threads before this one, and over all.
+__device__ __forceinline__ int block_prefix(int v, int* s_wave, int& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int below = __shfl_up(x, d);
+        x += lane >= d ? below : 0;
+    }
+    __syncthreads();
+    if (lane == 63) s_wave[wave] = x;
+    __syncthreads();
+    int before = 0;
+    all = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+        before += w < wave ? s_wave[w] : 0;
+        all += s_wave[w];
+    }
+    return before + x - v;
+}
+
+// The top - 1 largest keys (ties: the lowest blocks) and the last block, by digits of 8 bits from
+// the highest: the digit that the last taken key has, until all keys that share its digits so far
+// are taken.
+__global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p) {
+    __shared__ int s_count[256], s_wave[kSelectThreads / 64], s_digit, s_above;
+    const int row = blockIdx.x, b = row / p.Hkv, t = threadIdx.x;
+    int len;
+    const int n = blocks_of(p, b, len), page = 1 << p.log2_page;
+    const uint64_t* keys = p.keys + (size_t)row * p.max_blocks;
+    const int32_t* table = p.tables + (size_t)b * p.max_pages;
+    int32_t* selected = p.selected + (size_t)row * p.top;
+    int32_t* pages = p.pages + (size_t)row * p.top;
+    const int taken = min(n, p.top);
+    if (t == 0) p.positions[row] = taken == 0 ? 0 : (taken - 1) * page + len - (n - 1) * page;
+    for (int i = taken + t; i < p.top; i += blockDim.x) selected[i] = -1;
+    if (n <= p.top) {
+        for (int i = t; i < n; i += blockDim.x) selected[i] = i, pages[i] = table[i];
+        return;
+    }
+    int need = p.top - 1;  // of the keys that share the digits so far
+    uint64_t prefix = 0;   // those digits
+    int shift = 64;        // keys >> shift == prefix share them (64: all)
+    bool exact = need == 0;  // all that share them are taken (top 1: none)
+    auto shares = [&](uint64_t k) { return shift == 64 || (k >> shift) == prefix; };
+    while (!exact && shift > 0) {
+        for (int i = t; i < 256; i += blockDim.x) s_count[i] = 0;
+        __syncthreads();
+        for (int i = t; i < n - 1; i += blockDim.x) {
+            const uint64_t k = keys[i];
+            if (shares(k)) atomicAdd(&s_count[(k >> (shift - 8)) & 255], 1);
+        }
+        __syncthreads();
+        if (t < 64) {
+            // lane t: digits 255 - 4 t down to 252 - 4 t
+            int c[4], mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = s_count[255 - 4 * t - i], mine += c[i];
+            int x = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int below = __shfl_up(x, d);
+                x += t >= d ? below : 0;
+            }
+            int above = x - mine;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (above < need && need <= above + c[i]) s_digit = 255 - 4 * t - i, s_above = above;
+                above += c[i];
+            }
+        }
+        __syncthreads();
+        shift -= 8;
+        prefix = prefix << 8 | (uint64_t)s_digit;
+        need -= s_above;
+        exact = need == s_count[s_digit];
+        __syncthreads();
+    }
+    int base = 0, ties = 0;
+    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+        const int i = i0 + t;
+        const uint64_t k = i < n - 1 ? keys[i] : 0;
+        const uint64_t high = shift == 64 ? 0 : k >> shift;
+        const bool same = i < n - 1 && shift < 64 && high == prefix;
+        int total;
+        const int rank = block_prefix(same ? 1 : 0, s_wave, total) + ties;
+        ties += total;
+        const bool take = i == n - 1 || (i < n - 1 && shift < 64 && (high > prefix || (same && rank < need)));
+        const int at = block_prefix(take ? 1 : 0, s_wave, total) + base;
+        base += total;
+        if (take && at < p.top) selected[at] = i, pages[at] = table[i];
+    }
+}
+
+}  // namespace
+
+int launch_select(const Select& s, hipStream_t stream) {
+    const int rows = s.B * s.Hkv;
+    const int per = 256 / (s.D / 16) * 2;
+    if (s.max_blocks > s.top) {
+        const dim3 grid((unsigned)ceil_div(s.max_blocks, per), (unsigned)rows);
+        if (s.D == 64) block_scores_kernel<64><<<grid, 256, 0, stream>>>(s);
+        else block_scores_kernel<128><<<grid, 256, 0, stream>>>(s);
+        if (const int st = check_launch("block_scores_kernel")) return st;
+    }
+    select_blocks_kernel<<<(unsigned)rows, kSelectThreads, 0, stream>>>(s);
+    return check_launch("select_blocks_kernel");
+}
+
+int pages_bad_ids(unsigned int* count) {
+    return read_counter(&g_pages_bad_ids, "hipMemcpyFromSymbol(g_pages_bad_ids)", count);
+}
+}  // namespace int8k
+
+using namespace int8k;
+
+extern "C" int int8k_kv_cache_move_paged(int8_t* K_pages, int8_t* V_pages, float* sK_pages,
+                                         float* sV_pages, const int32_t* src_slots,
+                                         const int32_t* dst_slots, int lists, int pairs,
+                                         int kv_heads, int head_dim, int num_pages, int page_size,
+                                         void* stream) {
+    clear_last_error();
+    if (!K_pages || !V_pages || !sK_pages || !sV_pages || !src_slots || !dst_slots)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (lists <= 0 || pairs <= 0) return INT8K_ERR_INVALID_ARGUMENT;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (!aligned_to(K_pages, 16) || !aligned_to(V_pages, 16) || !aligned_to(sK_pages, 4) ||
+        !aligned_to(sV_pages, 4) || !aligned_to(src_slots, 4) || !aligned_to(dst_slots, 4))
+        return INT8K_ERR_MISALIGNED;
+    if (pairs > kMaxPairs || (long long)lists * kv_heads >= (1LL << 23)) return INT8K_ERR_UNSUPPORTED;
+    Move p{{K_pages, V_pages}, {sK_pages, sV_pages}, src_slots, dst_slots, pairs, kv_heads,
+           num_pages, log2_of(page_size)};
+    const int items = pairs * (head_dim / 16);
+    const dim3 grid((unsigned)(lists * kv_heads), 2);
+    const unsigned threads = (unsigned)std::min<long long>(256, ceil_div(items, 64) * 64);
+    const hipStream_t s = as_stream(stream);
+    if (head_dim == 64) {
+        if (items <= 256) move_rows_kernel<64, 1><<<grid, threads, 0, s>>>(p);
+        else move_rows_kernel<64, 4><<<grid, threads, 0, s>>>(p);
+    } else {
+        if (items <= 256) move_rows_kernel<128, 1><<<grid, threads, 0, s>>>(p);
+        else move_rows_kernel<128, 8><<<grid, threads, 0, s>>>(p);
+    }
+    return check_launch("move_rows_kernel");
+}
+
+extern "C" int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages,
+                                   const int32_t* page_ids, int8_t* K_means, float* sK_means,
+                                   int count, int kv_heads, int head_dim, int num_pages,
+                                   int page_size, void* stream) {
+    clear_last_error();
+    if (!K_pages || !sK_pages || !page_ids || !K_means || !sK_means || count <= 0)
+        return INT8K_ERR_INVALID_ARGUMENT;
+    if (const int st = check_pages(num_pages, page_size, kv_heads, head_dim)) return st;
+    if (!aligned_to(K_pages, 16) || !aligned_to(sK_pages, 4) || !aligned_to(page_ids, 4) ||
+        !aligned_to(K_means, 16) || !aligned_to(sK_means, 4))
+        return INT8K_ERR_MISALIGNED;
+    if ((long long)count * kv_heads >= (1LL << 23)) return INT8K_ERR_UNSUPPORTED;
+    const unsigned blocks = (unsigned)(count * kv_heads), threads = 256;
+    const hipStream_t s = as_stream(stream);
+    if (head_dim == 64)
+        page_means_kernel<64><<<blocks, threads, 0, s>>>(K_pages, sK_pages, page_ids, K_means,
+                                                         sK_means, kv_heads, num_pages, log2_of(page_size));
+    else
+        page_means_kernel<128><<<blocks, threads, 0, s>>>(K_pages, sK_pages, page_ids, K_means,
+                                                          sK_means, kv_heads, num_pages, log2_of(page_size));
+    return check_launch("page_means_kernel");
+}

@@ -79,6 +79,16 @@ _SIGNATURES = {
     "int8k_decode_attention_kv4_paged_workspace_bytes": (_SZ, [_I] * 5),
     "int8k_decode_attention_forward_kv4_paged": (_I, [_P] * 9 + [_I] * 8 + [_P, _SZ, _P]),
     "int8k_kv4_bad_ids": (_I, [ctypes.POINTER(ctypes.c_uint)]),
+    "int8k_qk_norm_rope_append": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P, _F] + [_P] * 7 +
+                                  [_I] * 8 + [_P]),
+    "int8k_tree_attention_paged_workspace_bytes": (_SZ, [_I] * 6),
+    "int8k_tree_attention_forward_paged": (_I, [_P] * 10 + [_I, _LL, _P] + [_I] * 10 +
+                                           [_P, _SZ, _P]),
+    "int8k_kv_cache_move_paged": (_I, [_P] * 6 + [_I] * 6 + [_P]),
+    "int8k_kv_page_means": (_I, [_P] * 5 + [_I] * 5 + [_P]),
+    "int8k_decode_attention_paged_sparse_workspace_bytes": (_SZ, [_I] * 7),
+    "int8k_decode_attention_forward_paged_sparse": (_I, [_P] * 12 + [_I] * 9 + [_P, _SZ, _P]),
+    "int8k_paged_bad_ids": (_I, [ctypes.POINTER(ctypes.c_uint)]),
 }
 
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
@@ -675,4 +685,111 @@ def kv4_bad_ids() -> int:
     since load."""
     n = ctypes.c_uint(0)
     check("int8k_kv4_bad_ids", load().int8k_kv4_bad_ids(ctypes.byref(n)))
+    return int(n.value)
+
+
+# --------------------------------------------------------------------------
+# the paged INT8 cache with grouped heads
+# --------------------------------------------------------------------------
+
+
+def qk_norm_rope_append(x, heads, kv_heads, cos, sin, positions, K_pages, V_pages, sK_pages,
+                        sV_pages, slots, q_weight=None, k_weight=None, eps=1e-6, flags=0):
+    """x [B, S, (heads + 2 kv_heads) * D]: queries as (int8 [B, heads, S, D], fp32 scales), keys
+    and values into rows `slots` int32 [B*S] of the pages [num_pages, kv_heads, page, D]."""
+    import torch
+
+    B, S, width = x.shape
+    D = width // (heads + 2 * kv_heads)
+    q = torch.empty((B, heads, S, D), dtype=torch.int8, device=x.device)
+    sq = torch.empty((B, heads, S), dtype=torch.float32, device=x.device)
+    check("int8k_qk_norm_rope_append", load().int8k_qk_norm_rope_append(
+        _ptr(x), _dtype_code(x), _ptr(cos), _ptr(sin), cos.shape[0], 2 * cos.shape[1],
+        _ptr(positions), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(q), _ptr(sq),
+        _ptr(K_pages), _ptr(V_pages), _ptr(sK_pages), _ptr(sV_pages), _ptr(slots), B, S, heads,
+        kv_heads, D, K_pages.shape[0], K_pages.shape[2], flags, _stream(x)))
+    return q, sq
+
+
+def tree_attention_paged_workspace_bytes(B, heads, kv_heads, nodes, max_context, D):
+    return load().int8k_tree_attention_paged_workspace_bytes(B, heads, kv_heads, nodes,
+                                                             max_context, D)
+
+
+def tree_attention_paged(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, block_tables, context_lens,
+                         tree_mask, max_context, node_counts=None, out_bshd=False, out=None,
+                         workspace=None):
+    """Qi int8 [B, H, N, D] against int8 pages [num_pages, Hkv, page, D]; tree_mask int64
+    [N, words], [B, N, words] or None -> fp16 [B, H, N, D] ([B, N, H, D] with out_bshd)."""
+    import torch
+
+    B, H, N, D = Qi.shape
+    NP, Hkv, P, _ = K_pages.shape
+    if out is None:
+        out = torch.empty((B, N, H, D) if out_bshd else (B, H, N, D), dtype=torch.float16,
+                          device=Qi.device)
+    if workspace is None:
+        n = tree_attention_paged_workspace_bytes(B, H, Hkv, N, max_context, D)
+        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=Qi.device)
+    words = tree_mask.shape[-1] if tree_mask is not None else 0
+    each = N * words if tree_mask is not None and tree_mask.dim() == 3 else 0
+    check("int8k_tree_attention_forward_paged", load().int8k_tree_attention_forward_paged(
+        _ptr(Qi), _ptr(K_pages), _ptr(V_pages), _ptr(out), _ptr(sQ), _ptr(sK_pages),
+        _ptr(sV_pages), _ptr(block_tables), _ptr(context_lens), _ptr(tree_mask), words, each,
+        _ptr(node_counts), B, H, Hkv, N, D, NP, P, block_tables.shape[1], max_context,
+        ATTN_OUT_BSHD if out_bshd else 0, _ptr(workspace), workspace.numel(), _stream(Qi)))
+    return out
+
+
+def kv_cache_move_paged(K_pages, V_pages, sK_pages, sV_pages, src_slots, dst_slots):
+    """Rows src_slots -> dst_slots, int32 [lists, pairs], of every key head."""
+    NP, H, P, D = K_pages.shape
+    lists, pairs = src_slots.shape
+    check("int8k_kv_cache_move_paged", load().int8k_kv_cache_move_paged(
+        _ptr(K_pages), _ptr(V_pages), _ptr(sK_pages), _ptr(sV_pages), _ptr(src_slots),
+        _ptr(dst_slots), lists, pairs, H, D, NP, P, _stream(K_pages)))
+
+
+def kv_page_means(K_pages, sK_pages, page_ids, K_means, sK_means):
+    """The mean keys of pages `page_ids` int32 [n] into K_means int8 [num_pages, Hkv, D]."""
+    NP, H, P, D = K_pages.shape
+    check("int8k_kv_page_means", load().int8k_kv_page_means(
+        _ptr(K_pages), _ptr(sK_pages), _ptr(page_ids), _ptr(K_means), _ptr(sK_means),
+        page_ids.numel(), H, D, NP, P, _stream(K_pages)))
+
+
+def decode_paged_sparse_workspace_bytes(B, heads, kv_heads, max_context, page, top_pages, D):
+    return load().int8k_decode_attention_paged_sparse_workspace_bytes(
+        B, heads, kv_heads, max_context, page, top_pages, D)
+
+
+def decode_attention_paged_sparse(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, K_means, sK_means,
+                                  block_tables, context_lens, max_context, top_pages, out=None,
+                                  workspace=None):
+    """Qi int8 [B, H, D] over the `top_pages` blocks of each sequence and key head with the
+    highest scores -> (fp16 [B, H, D], the blocks int32 [B, Hkv, top_pages])."""
+    import torch
+
+    B, H, D = Qi.shape
+    NP, Hkv, P, _ = K_pages.shape
+    if out is None:
+        out = torch.empty((B, H, D), dtype=torch.float16, device=Qi.device)
+    which = torch.empty((B, Hkv, top_pages), dtype=torch.int32, device=Qi.device)
+    if workspace is None:
+        n = decode_paged_sparse_workspace_bytes(B, H, Hkv, max_context, P, top_pages, D)
+        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=Qi.device)
+    check("int8k_decode_attention_forward_paged_sparse",
+          load().int8k_decode_attention_forward_paged_sparse(
+              _ptr(Qi), _ptr(K_pages), _ptr(V_pages), _ptr(out), _ptr(which), _ptr(sQ),
+              _ptr(sK_pages), _ptr(sV_pages), _ptr(K_means), _ptr(sK_means), _ptr(block_tables),
+              _ptr(context_lens), B, H, Hkv, D, NP, P, block_tables.shape[1], max_context,
+              top_pages, _ptr(workspace), workspace.numel(), _stream(Qi)))
+    return out, which
+
+
+def paged_bad_ids() -> int:
+    """Slots and page ids outside the paged INT8 cache that its operators met, on the current
+    device since load."""
+    n = ctypes.c_uint(0)
+    check("int8k_paged_bad_ids", load().int8k_paged_bad_ids(ctypes.byref(n)))
     return int(n.value)
