@@ -169,18 +169,6 @@ struct PackedLds {
     static constexpr int kBytes = kS + 2 * kSFloats * 4;
 };
 
-// w less half I of t, exactly where t is w rounded to fp16 (one instruction: the compiler widens
-// the half first).
-template <int I, typename H2>
-__device__ __forceinline__ float minus_half(float w, H2 t) {
-    float d;
-    if constexpr (I == 0)
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(t), "v"(w));
-    else
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(t), "v"(w));
-    return d;
-}
-
 constexpr int kPackedWaves = 4;              // per block, 32 queries each
 constexpr float kPackedMaxWeight = 60000.f;  // fp16 weights stay below it
 constexpr float kPackedMaxShift = 60.f;      // |m - running maximum| where m is set

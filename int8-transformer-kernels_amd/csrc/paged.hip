@@ -53,8 +53,7 @@ struct Attend {
     const float *sQ, *sK, *sV;
     const int32_t* tables;               // page ids of sequence b and key head h:
     long long table_batch, table_head;   //   from b table_batch + h table_head
-    const int32_t* lens;                 // its positions before the tree: b len_batch + h len_head
-    int len_batch, len_head;
+    const int32_t* lens;                 // [B]: positions before the tree
     bool tree;                           // the N tokens are in the cache behind those positions
     const int32_t* counts;               // tokens of each sequence, or null (N)
     const int64_t* mask;                 // [B or 1][N][words], or null
@@ -62,9 +61,10 @@ struct Attend {
     int words;
     uint16_t* out;                       // [B, Hq, N, D], or [B, N, Hq, D] with bshd
     bool bshd;
-    float *part_ml, *part_acc;           // [rows][nsplit][2] and [..][D] (nsplit > 1)
+    float *part_ml, *part_acc;           // [piece][Hq * N][2] and [..][D]
     int B, Hq, Hkv, N, num_pages, log2_page, max_context;
-    int groups, nsplit;                  // blocks of query rows per key head, splits of a sequence
+    int groups;                          // blocks of query rows per key head
+    int pieces, min_tiles;               // see Piece; 0: a sequence is one piece
     float qk;
 };
 
@@ -72,27 +72,108 @@ struct Attend {
 struct Extent {
     int prefix, total, count;
 };
-__device__ __forceinline__ Extent extent_of(const Attend& p, int b, int kvh) {
+__device__ __forceinline__ Extent extent_of(const Attend& p, int b) {
     Extent e;
-    e.prefix = min(max(p.lens[b * p.len_batch + kvh * p.len_head], 0), p.max_context);
+    e.prefix = min(max(p.lens[b], 0), p.max_context);
     e.count = !p.tree ? 0 : p.counts == nullptr ? p.N : min(max(p.counts[b], 0), p.N);
     e.total = min(e.prefix + e.count, p.max_context);
     return e;
 }
 
-// Whether token `node` sees the token `j` of its sequence's tree.
-__device__ __forceinline__ bool sees(const Attend& p, const int64_t* masks, int node, int j) {
-    return masks == nullptr ? j <= node : (masks[(size_t)node * p.words + (j >> 6)] >> (j & 63)) & 1;
+// The lowest n bits (none below 0, all from 32).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+// Which of the nodes first .. first + 31 token `node` sees, bit by bit (`first` may be negative).
+__device__ __forceinline__ uint32_t seen_nodes(const uint32_t* masks, int words, int node, int first) {
+    if (masks == nullptr) return low_bits(node + 1 - first);
+    const int w = first >> 5, shift = first & 31;
+    const uint32_t* row = masks + (size_t)node * (2 * words);
+    const uint32_t lo = w >= 0 && w < 2 * words ? row[w] : 0u;
+    const uint32_t hi = w + 1 >= 0 && w + 1 < 2 * words ? row[w + 1] : 0u;
+    return shift == 0 ? lo : lo >> shift | hi << (32 - shift);
+}
+
+// The mask words of sequence b, in halves, or null.
+__device__ __forceinline__ const uint32_t* masks_of(const Attend& p, int b) {
+    return p.mask == nullptr ? nullptr
+                             : reinterpret_cast<const uint32_t*>(p.mask + b * p.mask_batch);
 }
 
 // Whether row `node` attends to any position (tokens past the sequence's do not).
-__device__ bool attends(const Attend& p, int b, int node, const Extent& e) {
+__device__ __forceinline__ bool attends(const Attend& p, int b, int node, const Extent& e) {
     if (!p.tree) return e.prefix > 0;
     if (node >= e.count) return false;
     if (e.prefix > 0) return true;
-    const int64_t* masks = p.mask == nullptr ? nullptr : p.mask + b * p.mask_batch;
-    for (int j = 0; j < e.total; ++j)
-        if (sees(p, masks, node, j)) return true;
+    const uint32_t* masks = masks_of(p, b);
+    uint32_t any = 0;
+    for (int j = 0; j < e.total; j += 32)
+        any |= seen_nodes(masks, p.words, node, j) & low_bits(e.total - j);
+    return any != 0;
+}
+
+// How the sequences are cut.  Their lengths are on the device, so every wave works the cut out from
+// them: into p.pieces pieces over all sequences, at least one each, whose largest is about as small
+// as can be, but p.min_tiles.  The host takes as many pieces as the GPU holds at a time, so all
+// blocks run at once and end together however unequal the lengths are.
+struct Piece {
+    int b, index, count, first;  // sequence, which of its pieces, how many, number of its first
+    int tiles;                   // of a piece
+};
+
+__device__ __forceinline__ int wave_sum(int v) {
+    v = group8_sum(v);
+    v += dpp_row_mirror(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = (int)(a[0] + a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane((int)(b[0] + b[1]));
+}
+
+// The piece that `found(first, count, b)` picks among the sequences (for one of them at most).
+template <typename Found>
+__device__ __forceinline__ bool find_piece(const Attend& p, Piece& piece, Found&& found) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int b) {
+        return b < p.B ? (extent_of(p, b).total + kTile - 1) / kTile : 0;
+    };
+    int mine = tiles_of(lane), all = mine;
+    for (int b = lane + 64; b < p.B; b += 64) all += tiles_of(b);
+    const unsigned total = (unsigned)wave_sum(all), P = (unsigned)p.pieces;
+    auto count_of = [&](unsigned tiles, unsigned each) { return max((tiles + each - 1) / each, 1u); };
+    // pieces of total / (P - B) are few enough, of less than total / P too many
+    unsigned lo = max((total + P - 1) / P, 1u), hi = max((total + P - p.B - 1) / (P - p.B), 1u);
+    for (int step = 0; step < 6 && lo < hi; ++step) {
+        const unsigned mid = (lo + hi) / 2;
+        int count = lane < p.B ? (int)count_of(mine, mid) : 0;
+        for (int b = lane + 64; b < p.B; b += 64) count += (int)count_of(tiles_of(b), mid);
+        if ((unsigned)wave_sum(count) <= P) hi = mid;
+        else lo = mid + 1;
+    }
+    const unsigned each = max(hi, (unsigned)p.min_tiles);
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        if (b0 > 0) mine = tiles_of(b0 + lane);
+        const int count = b0 + lane < p.B ? (int)count_of(mine, each) : 0;
+        int upto = count;  // inclusive sum over the lanes
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int below = __shfl_up(upto, d);
+            upto += lane >= d ? below : 0;
+        }
+        const int first = before + upto - count;
+        const uint64_t at = __ballot(count > 0 && found(first, count, b0 + lane));
+        if (at != 0) {
+            const int src = __builtin_ctzll(at);
+            piece.b = b0 + src;
+            piece.count = __builtin_amdgcn_readlane(count, src);
+            piece.tiles = __builtin_amdgcn_readlane((mine + count - 1) / max(count, 1), src);
+            piece.first = __builtin_amdgcn_readlane(first, src);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
     return false;
 }
 
@@ -113,6 +194,17 @@ __device__ __forceinline__ float sum_groups(float v) {
     return sum_xor32(__int_as_float(a[0]) + __int_as_float(a[1]));
 }
 
+// Four dims of an output row, acc / sum; a row that attends to nothing is zero.
+__device__ __forceinline__ void store_row(const Attend& p, size_t at, const float4& acc, float sum,
+                                          bool any) {
+    float v[4] = {acc.x / sum, acc.y / sum, acc.z / sum, acc.w / sum};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("" : "+v"(v[i]));  // (see f16_of_f32)
+    *reinterpret_cast<uint2*>(p.out + at) =
+        any ? make_uint2(pack_pair<INT8K_DTYPE_F16>(v[0], v[1]), pack_pair<INT8K_DTYPE_F16>(v[2], v[3]))
+            : make_uint2(0, 0);
+}
+
 template <int D>
 struct AttendTile {
     static constexpr int kK = D / 64;   // 16-byte pieces of a K row per lane
@@ -123,7 +215,7 @@ struct AttendTile {
 };
 
 template <int D, int F>
-__global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
+__global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend p) {
     using Tile = AttendTile<D>;
     constexpr int NF = D / 16;          // fragments of O^T
     constexpr int MR = 16 * F;          // query rows per block
@@ -134,26 +226,35 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     const int nw = blockDim.x >> 6;
     const int g = lane >> 4, m16 = lane & 15;
 
-    // Block -> (sequence, split), key head and rows of it.  Blocks go to the 8 XCDs in turn; the
-    // blocks of one piece of a sequence, which share pages, run one after the other on one XCD.
+    // Block -> piece of a sequence, key head and rows of it.  Blocks go to the 8 XCDs in turn; the
+    // blocks of one piece, which share pages, run one after the other on one XCD.
     const int heads_here = p.Hkv * p.groups;
     const int local = (int)blockIdx.x / 8;
-    const int piece = local / heads_here * 8 + (int)blockIdx.x % 8;
-    if (piece >= p.B * p.nsplit) return;
-    const int b = piece / p.nsplit, split = piece % p.nsplit;
+    const int number = local / heads_here * 8 + (int)blockIdx.x % 8;
+    Piece piece{number, 0, 1, number, 0};
+    if (p.pieces == 0) {
+        if (number >= p.B) return;
+    } else {
+        if (!find_piece(p, piece, [&](int first, int count, int) {
+                return number >= first && number < first + count;
+            }))
+            return;
+        piece.index = number - piece.first;
+    }
+    const int b = piece.b;
     const int kvh = local % heads_here / p.groups, grp = local % p.groups;
     const int all_rows = p.Hq / p.Hkv * p.N;
     const int row0_q = grp * MR, rows = min(MR, all_rows - row0_q);
     const size_t first_row = ((size_t)b * p.Hq + (size_t)kvh * (p.Hq / p.Hkv)) * p.N + row0_q;
-    Extent e = extent_of(p, b, kvh);
+    Extent e = extent_of(p, b);
     e.prefix = __builtin_amdgcn_readfirstlane(e.prefix);
     e.total = __builtin_amdgcn_readfirstlane(e.total);
     const int tiles = (e.total + kTile - 1) / kTile;
-    const int per_split = (tiles + p.nsplit - 1) / p.nsplit;
-    const int t_begin = min(split * per_split, tiles), t_end = min(t_begin + per_split, tiles);
+    const int t_begin = piece.index * piece.tiles;
+    const int t_end = piece.count == 1 ? tiles : min(t_begin + piece.tiles, tiles);
     const int32_t* __restrict__ table = p.tables + b * p.table_batch + kvh * p.table_head;
     const int pmask = (1 << p.log2_page) - 1;
-    const int64_t* masks = p.mask == nullptr ? nullptr : p.mask + b * p.mask_batch;
+    const uint32_t* masks = masks_of(p, b);
 
     // this lane's query row of each fragment (rows past the last hold zeros)
     v4i qf[F][Tile::kK];
@@ -205,21 +306,23 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const size_t row = h == 0 ? row0 : row1;
-            const int8_t* kb = p.K + row * D + k_off;
+            const __amdgpu_buffer_rsrc_t kb = make_buffer(p.K + row * D, 16 * D);
+            const __amdgpu_buffer_rsrc_t vb = make_buffer(p.V + row * D, 16 * D);
 #pragma unroll
-            for (int i = 0; i < Tile::kK; ++i) r.k[h][i] = *reinterpret_cast<const v4i*>(kb + 64 * i);
-            const int8_t* vb = p.V + row * D + v_off;
+            for (int i = 0; i < Tile::kK; ++i)
+                r.k[h][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, k_off, 64 * i, 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (D == 128) {
-                    const v2u w = *reinterpret_cast<const v2u*>(vb + 4 * j * D);
+                    const v2u w = __builtin_amdgcn_raw_buffer_load_b64(vb, v_off, 4 * j * D, 0);
                     r.v[4 * h + j][0] = w.x, r.v[4 * h + j][1] = w.y;
                 } else {
-                    r.v[4 * h + j][0] = *reinterpret_cast<const uint32_t*>(vb + 4 * j * D);
+                    r.v[4 * h + j][0] = __builtin_amdgcn_raw_buffer_load_b32(vb, v_off, 4 * j * D, 0);
                 }
             }
         }
-        const size_t srow = (s_upper ? row1 : row0) + s_off;
+        const size_t first = row0, second = row1;
+        const size_t srow = (s_upper ? second : first) + s_off;
         r.sk = p.sK[srow];
         r.sv = p.sV[srow];
     };
@@ -264,26 +367,52 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
             auto sum8 = [&]() {
                 return ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
             };
-            float psum = 0.f;
+            // the weights as two fp16; one past fp16's range (checked where it may be: an infinite
+            // value scale) leaves no rest
+            auto split = [&](auto checked) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    typedef float f2 __attribute__((ext_vector_type(2)));
+                    const h2 top = __builtin_convertvector((f2){w[j], w[j + 1]}, h2);
+                    float rest0 = minus_half<0>(w[j], top), rest1 = minus_half<1>(w[j + 1], top);
+                    if constexpr (decltype(checked)::value) {
+                        rest0 = fabsf(w[j]) < 65520.f ? rest0 : 0.f;
+                        rest1 = fabsf(w[j + 1]) < 65520.f ? rest1 : 0.f;
+                    }
+                    const h2 rest = __builtin_convertvector((f2){rest0, rest1}, h2);
+                    pw[f][j] = top.x, pw[f][j + 1] = top.y;
+                    pr[f][j] = rest.x, pr[f][j + 1] = rest.y;
+                }
+            };
             bool slow = partial;
             if (!partial) {
                 weights();
-                psum = sum8();
+                const float psum = sum8();
                 float wide = fmaxf(fabsf(w[0]), fabsf(w[1]));
 #pragma unroll
                 for (int j = 2; j < 8; j += 2) wide = fmaxf(wide, fmaxf(fabsf(w[j]), fabsf(w[j + 1])));
                 // (the first tile, whose m is -inf, has an infinite sum)
                 slow = __ballot(fmaxf(wide, psum * (kMaxWeight / kMaxSum)) > kMaxWeight) != 0;
+                if (!slow) {
+                    l[f] += psum;
+                    split(std::false_type{});
+                }
             }
             if (slow) {
                 // the exact maximum, then the largest weight under it
                 float top = -INFINITY, pm = 0.f;
+                uint32_t visible = ~0u;  // keys of the tile
+                if (partial) {
+                    const int first = t * kTile - e.prefix;  // node of the tile's first key
+                    visible = low_bits(-first);
+                    if (p.tree) visible |= seen_nodes(masks, p.words, node[f], first);
+                    visible &= low_bits(e.total - t * kTile);
+                }
+                visible >>= g;
                 bool seen[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int pos = t * kTile + 4 * j + g;
-                    seen[j] = pos < e.prefix ||
-                              (pos < e.total && sees(p, masks, node[f], pos - e.prefix));
+                    seen[j] = (visible >> (4 * j)) & 1;
                     if (seen[j]) top = fmaxf(top, u[j] * qs[f]);
                 }
                 top = max_groups(top);
@@ -307,17 +436,8 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)  // unseen rows may hold anything
                     if (!seen[j]) pj[j] = w[j] = 0.f;
-                psum = sum8();
-            }
-            l[f] += psum;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                pw[f][j] = (_Float16)w[j];
-                pr[f][j] = (_Float16)(w[j] - (float)pw[f][j]);
-            }
-            if (slow) {  // (a weight past fp16's range, by an infinite value scale, leaves no rest)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) pr[f][j] = fabsf(w[j]) < 65520.f ? pr[f][j] : (_Float16)0.f;
+                l[f] += sum8();
+                split(std::true_type{});
             }
         }
         // byte c of two keys, c + 128 as an unsigned number u: 0x6400 | u is 1024 + u in fp16, and
@@ -335,10 +455,11 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
                 v[2 * j] = a.x, v[2 * j + 1] = a.y;
             }
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
+            for (int f = 0; f < F; ++f)
                 o[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[f], o[f][i], 0, 0, 0);
+#pragma unroll
+            for (int f = 0; f < F; ++f)
                 o[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pr[f], o[f][i], 0, 0, 0);
-            }
         }
     };
 
@@ -371,107 +492,134 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     }
     if (bad && lane == 0) atomicAdd(&g_attend_bad_ids, 1u);
 
-    // Join the waves: m, l and O of each row go to LDS, then element by element.
-    // Layout: [wave][m of MR rows][l of MR rows][MR rows][kORow].
-    constexpr int kWaveWords = 2 * MR + MR * kORow;
-    float* mine = s_merge + wave * kWaveWords;
+    // Join the waves: m and l of each row go to LDS, and O scaled to the rows' common maximum, which
+    // are then added four dims at a time (element by element, with the factors worked out by each
+    // thread, the join took 11 us of the 78 of 16 sequences with trees of 16).
+    // Layout: [wave][m, l of MR rows], then [wave][MR rows][kORow].
+    float* s_ml = s_merge;
+    float* s_o = s_merge + nw * 2 * MR;
 #pragma unroll
     for (int f = 0; f < F; ++f) {
         const float lf = sum_groups(l[f]);
+        if (g == 0)
+            s_ml[wave * 2 * MR + 16 * f + m16] = m[f], s_ml[wave * 2 * MR + MR + 16 * f + m16] = lf;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
         const int r = 16 * f + m16;
-        if (g == 0) mine[r] = m[f], mine[MR + r] = lf;
-        float* orow = mine + 2 * MR + r * kORow;
+        float top = -INFINITY;
+        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_ml[w * 2 * MR + r]);
+        const float scale = top == -INFINITY ? 0.f : fast_exp2(m[f] - top);
+        float* orow = s_o + (wave * MR + r) * kORow;
 #pragma unroll
         for (int c = 0; c < 4; ++c)  // rows 4 g + c of the fragments: dims NF (4 g + c) ..
 #pragma unroll
             for (int i = 0; i < NF; i += 4)
                 *reinterpret_cast<float4*>(orow + NF * (4 * g + c) + i) =
-                    make_float4(o[f][i][c], o[f][i + 1][c], o[f][i + 2][c], o[f][i + 3][c]);
+                    make_float4(o[f][i][c] * scale, o[f][i + 1][c] * scale, o[f][i + 2][c] * scale,
+                                o[f][i + 3][c] * scale);
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < rows * D; x += blockDim.x) {
-        const int row = x / D, d = x % D;
-        float top = -INFINITY, sum = 0.f, acc = 0.f;
-        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_merge[w * kWaveWords + row]);
+    constexpr int L = D / 4;  // threads per row
+    for (int x = threadIdx.x; x < rows * L; x += blockDim.x) {
+        const int row = x / L, d = x % L * 4;
+        float top = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_ml[w * 2 * MR + row]);
         const float use = top == -INFINITY ? 0.f : top;
         for (int w = 0; w < nw; ++w) {
-            const float* q = s_merge + w * kWaveWords;
-            const float a = fast_exp2(q[row] - use);
-            sum += q[MR + row] * a;
-            acc += q[2 * MR + row * kORow + d] * a;
+            sum = fmaf(s_ml[w * 2 * MR + MR + row], fast_exp2(s_ml[w * 2 * MR + row] - use), sum);
+            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * MR + row) * kORow + d);
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
         }
-        if (p.nsplit == 1) {
+        if (piece.count == 1) {
             const int r = row0_q + row, n = r % p.N, h = kvh * (p.Hq / p.Hkv) + r / p.N;
             const size_t at = p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : first_row + row;
-            p.out[at * D + d] =
-                attends(p, b, n, e) ? __half_as_ushort(f16_of_f32(acc / sum)) : (uint16_t)0;
+            store_row(p, at * D + d, acc, sum, attends(p, b, n, e));
         } else {
-            const size_t part = (first_row + row) * p.nsplit + split;
-            if (d == 0) p.part_ml[2 * part] = top, p.part_ml[2 * part + 1] = sum;
-            p.part_acc[part * D + d] = acc;
+            const size_t part = ((size_t)number * p.Hkv + kvh) * all_rows + row0_q + row;
+            if (d == 0) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(top, sum);
+            *reinterpret_cast<float4*>(p.part_acc + part * D + d) = acc;
         }
     }
 }
 
-// Joins the splits of each row, one thread per dim: eight partials in flight at a time (slots
-// past the last repeat it with weight zero).
+// Joins the pieces of each row of a sequence that has several, four dims per thread: four partials
+// in flight at a time (slots past the last repeat it with weight zero).
 template <int D>
-__global__ __launch_bounds__(D) void paged_combine_kernel(Attend p) {
-    const size_t row = blockIdx.x;
-    const int d = threadIdx.x, nsplit = p.nsplit;
-    const int n = (int)(row % p.N), h = (int)(row / p.N % p.Hq), b = (int)(row / p.N / p.Hq);
-    const float2* r = reinterpret_cast<const float2*>(p.part_ml) + row * nsplit;
-    const float* x = p.part_acc + row * nsplit * D + d;
-    const bool any = attends(p, b, n, extent_of(p, b, h / (p.Hq / p.Hkv)));
-    float m = -INFINITY, sum = 0.f, a = 0.f;
-    for (int i0 = 0; i0 < nsplit; i0 += 8) {
-        float2 s[8];
-        float v[8];
+constexpr int kCombineRows = 256 / (D / 4);  // rows per block, all of one sequence
+
+template <int D>
+__global__ __launch_bounds__(256) void paged_combine_kernel(Attend p, int blocks_each) {
+    constexpr int L = D / 4;
+    const int b = (int)blockIdx.x / blocks_each, all_rows = p.Hq * p.N;
+    const int row = (int)blockIdx.x % blocks_each * kCombineRows<D> + (int)threadIdx.x / L;
+    const int c = threadIdx.x % L;
+    Piece piece;
+    find_piece(p, piece, [&](int, int, int seq) { return seq == b; });
+    if (piece.count == 1 || row >= all_rows) return;  // one piece: written already
+    const size_t part = (size_t)piece.first * all_rows + row;
+    const float2* r = reinterpret_cast<const float2*>(p.part_ml) + part;
+    const float4* x = reinterpret_cast<const float4*>(p.part_acc) + part * L + c;
+    float m = -INFINITY, sum = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < piece.count; i0 += 4) {
+        float2 s[4];
+        float4 v[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int i = min(i0 + k, nsplit - 1);
+        for (int k = 0; k < 4; ++k) {
+            const size_t i = (size_t)min(i0 + k, piece.count - 1) * all_rows;
             s[k] = r[i];
-            v[k] = x[(size_t)i * D];
+            v[k] = x[i * L];
         }
         float top = m;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, s[k].x);
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, s[k].x);
         const float use = top == -INFINITY ? 0.f : top;
         const float keep = fast_exp2(m - use);
         sum *= keep;
-        a *= keep;
+        a.x *= keep, a.y *= keep, a.z *= keep, a.w *= keep;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float f = i0 + k < nsplit ? fast_exp2(s[k].x - use) : 0.f;
-            // (a repeated slot must not turn an infinite partial into NaN)
-            sum += i0 + k < nsplit ? s[k].y * f : 0.f;
-            a += i0 + k < nsplit ? v[k] * f : 0.f;
+        for (int k = 0; k < 4; ++k) {
+            if (i0 + k >= piece.count) continue;  // (it must not turn an infinite partial into NaN)
+            const float f = fast_exp2(s[k].x - use);
+            sum = fmaf(s[k].y, f, sum);
+            a.x = fmaf(v[k].x, f, a.x), a.y = fmaf(v[k].y, f, a.y);
+            a.z = fmaf(v[k].z, f, a.z), a.w = fmaf(v[k].w, f, a.w);
         }
         m = top;
     }
-    const size_t at = p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : row;
-    p.out[at * D + d] = any ? __half_as_ushort(f16_of_f32(a / sum)) : (uint16_t)0;
+    const int h = row / p.N, n = row - h * p.N;
+    const size_t at = p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : (size_t)b * all_rows + row;
+    store_row(p, at * D + 4 * c, a, sum, attends(p, b, n, extent_of(p, b)));
 }
 
 // ------------------------------------------------------------------ host side
 
 struct AttendPlan {
-    int frags, groups, waves, nsplit;
+    int frags, groups, waves;
+    int pieces, min_tiles;  // 0: one piece per sequence
+    int slots(int B) const { return pieces > 0 ? pieces : B; }
 };
 
-constexpr int kMaxSplit = 64, kMaxBlocks = 1024;
+constexpr int kMaxSplit = 64;      // pieces per sequence, on average
+constexpr int kMaxBlocks = 1024;   // of a cut
 
 // rows: query rows per key head
 AttendPlan attend_plan(int B, int rows, int Hkv, int context) {
     AttendPlan pl{};
-    pl.frags = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    pl.frags = rows <= 16 ? 1 : 2;
     pl.groups = (rows + 16 * pl.frags - 1) / (16 * pl.frags);
     pl.waves = 4;
-    const long long units = (long long)B * Hkv * pl.groups;
+    const long long heads = (long long)Hkv * pl.groups;  // blocks per piece
     const long long tiles = ceil_div(context, kTile);
-    long long s = std::min<long long>(kMaxSplit, std::max<long long>(1, kMaxBlocks / units));
-    s = std::min(s, ceil_div(tiles, 2 * pl.waves));
-    pl.nsplit = (int)std::max<long long>(1, s);
+    const long long resident = pl.frags == 1 ? 768 : 512;
+    pl.min_tiles = pl.waves;
+    // (the sum of all tiles is an int)
+    pl.pieces = (int)std::min<long long>({(long long)kMaxSplit * B, resident / heads,
+                                          B * ceil_div(tiles, pl.min_tiles)});
+    if (pl.pieces <= B || B * tiles >= (1LL << 31)) pl.pieces = 0;
     return pl;
 }
 
@@ -483,12 +631,12 @@ Partials partials_of(size_t parts, int D) {
     const size_t ml = round_up(parts * 2 * sizeof(float), kWorkspaceAlign);
     return {ml, ml + round_up(parts * D * sizeof(float), kWorkspaceAlign)};
 }
-Partials plan_partials(const AttendPlan& pl, size_t rows, int D) {
-    return partials_of(pl.nsplit > 1 ? rows * pl.nsplit : 0, D);
+// rows: of one sequence, all heads
+Partials plan_partials(const AttendPlan& pl, int B, size_t rows, int D) {
+    return partials_of(pl.pieces > 0 ? pl.slots(B) * rows : 0, D);
 }
-
-// Room for every plan of at most `rows` query rows in all: a plan has at most kMaxSplit splits, and
-// kMaxBlocks blocks of at most 64 rows where it has more than one split.
+// Room for every plan of at most `rows` query rows in all: a cut has at most kMaxSplit pieces per
+// sequence, and at most kMaxBlocks blocks of 64 rows.
 Partials most_partials(size_t rows, int D) {
     return partials_of(std::min<size_t>(kMaxSplit * rows, 64 * kMaxBlocks), D);
 }
@@ -512,18 +660,17 @@ int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipS
 
 template <int D>
 int launch_attend(Attend p, const AttendPlan& pl, void* workspace, hipStream_t stream) {
-    const size_t rows = (size_t)p.B * p.Hq * p.N;
-    p.groups = pl.groups, p.nsplit = pl.nsplit;
+    p.groups = pl.groups, p.pieces = pl.pieces, p.min_tiles = pl.min_tiles;
     p.part_ml = static_cast<float*>(workspace);
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                          plan_partials(pl, rows, D).ml_bytes);
-    const unsigned blocks =
-        (unsigned)(ceil_div((long long)p.B * pl.nsplit, 8) * 8 * p.Hkv * pl.groups);
+                                          plan_partials(pl, p.B, (size_t)p.Hq * p.N, D).ml_bytes);
+    const unsigned blocks = (unsigned)(ceil_div(pl.slots(p.B), 8) * 8 * p.Hkv * pl.groups);
     const int st = pl.frags == 1   ? launch_instance<D, 1>(p, pl, blocks, stream)
                    : pl.frags == 2 ? launch_instance<D, 2>(p, pl, blocks, stream)
                                    : launch_instance<D, 4>(p, pl, blocks, stream);
-    if (st != INT8K_OK || pl.nsplit == 1) return st;
-    paged_combine_kernel<D><<<(unsigned)rows, D, 0, stream>>>(p);
+    if (st != INT8K_OK || pl.pieces == 0) return st;
+    const int blocks_each = (int)ceil_div((long long)p.Hq * p.N, kCombineRows<D>);
+    paged_combine_kernel<D><<<(unsigned)(p.B * blocks_each), 256, 0, stream>>>(p, blocks_each);
     return check_launch("paged_combine_kernel");
 }
 
@@ -536,7 +683,7 @@ int run_attend(const Attend& p, const AttendPlan& pl, int D, void* workspace, hi
 bool attend_fits(long long B, long long heads, long long kv_heads, long long nodes, int max_context,
                  const AttendPlan& pl) {
     return B * heads * nodes < (1LL << 24) && max_context <= (1 << 30) &&
-           (ceil_div(B * pl.nsplit, 8) * 8 * kv_heads * pl.groups) * pl.waves < (1LL << 25);
+           ceil_div(pl.slots((int)B), 8) * 8 * kv_heads * pl.groups * pl.waves < (1LL << 25);
 }
 
 constexpr int kMaxNodes = 256;
@@ -589,7 +736,7 @@ extern "C" int int8k_tree_attention_forward_paged(
         return INT8K_ERR_UNSUPPORTED;
     const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context);
     if (!attend_fits(B, heads, kv_heads, nodes, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
-    const size_t need = plan_partials(pl, (size_t)B * heads * nodes, head_dim).bytes;
+    const size_t need = plan_partials(pl, B, (size_t)heads * nodes, head_dim).bytes;
     if (need > 0) {
         if (!workspace || workspace_bytes < need) return INT8K_ERR_WORKSPACE;
         if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
@@ -597,7 +744,7 @@ extern "C" int int8k_tree_attention_forward_paged(
     Attend p{};
     p.Q = Q, p.K = K_pages, p.V = V_pages, p.sQ = scale_Q, p.sK = sK_pages, p.sV = sV_pages;
     p.tables = block_tables, p.table_batch = max_pages_per_seq, p.table_head = 0;
-    p.lens = context_lens, p.len_batch = 1, p.len_head = 0;
+    p.lens = context_lens;
     p.tree = true, p.counts = node_counts, p.mask = tree_mask, p.mask_batch = mask_batch_stride;
     p.words = mask_words, p.out = out, p.bshd = (flags & INT8K_ATTN_OUT_BSHD) != 0;
     p.B = B, p.Hq = heads, p.Hkv = kv_heads, p.N = nodes, p.num_pages = num_pages;
@@ -649,7 +796,7 @@ extern "C" int int8k_decode_attention_forward_paged_sparse(
     if (!attend_fits(B, heads, kv_heads, 1, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
     const SelectSpace sel = select_space(B, kv_heads, max_context, page_size, top_pages);
     if (!workspace ||
-        workspace_bytes < sel.bytes + plan_partials(pl, (size_t)B * heads, head_dim).bytes)
+        workspace_bytes < sel.bytes + plan_partials(pl, B, (size_t)heads, head_dim).bytes)
         return INT8K_ERR_WORKSPACE;
     if (!aligned_to(workspace, 16)) return INT8K_ERR_MISALIGNED;
 
@@ -667,7 +814,7 @@ extern "C" int int8k_decode_attention_forward_paged_sparse(
     Attend p{};
     p.Q = Q, p.K = K_pages, p.V = V_pages, p.sQ = scale_Q, p.sK = sK_pages, p.sV = sV_pages;
     p.tables = s.pages, p.table_batch = (long long)kv_heads * top_pages, p.table_head = top_pages;
-    p.lens = s.positions, p.len_batch = kv_heads, p.len_head = 1;
+    p.lens = s.positions;
     p.tree = false, p.out = out;
     p.B = B, p.Hq = heads, p.Hkv = kv_heads, p.N = 1, p.num_pages = num_pages;
     p.log2_page = s.log2_page, p.max_context = context;

@@ -45,7 +45,7 @@ int pages_bad_ids(unsigned int* count);      // pages.hip
 // head, from the scores of its blocks by their pages' mean keys,
 //   selected [B, Hkv, top]   the blocks taken, ascending, -1 behind the last
 //   pages [B, Hkv, top]      their page ids as the table has them
-//   positions [B, Hkv]       how many positions they hold
+//   positions [B]            how many positions they hold, for every key head
 struct Select {
     const int8_t *Q, *means;
     const float *sQ, *s_means;
@@ -65,7 +65,7 @@ inline SelectSpace select_space(int B, int kv_heads, int max_context, int page_s
     SelectSpace s{};
     s.pages = round_up(rows * (size_t)ceil_div(max_context, page_size) * sizeof(uint64_t), kWorkspaceAlign);
     s.positions = s.pages + round_up(rows * top * sizeof(int32_t), kWorkspaceAlign);
-    s.bytes = s.positions + round_up(rows * sizeof(int32_t), kWorkspaceAlign);
+    s.bytes = s.positions + round_up((size_t)B * sizeof(int32_t), kWorkspaceAlign);
     return s;
 }
 

@@ -252,7 +252,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
     int32_t* selected = p.selected + (size_t)row * p.top;
     int32_t* pages = p.pages + (size_t)row * p.top;
     const int taken = min(n, p.top);
-    if (t == 0) p.positions[row] = taken == 0 ? 0 : (taken - 1) * page + len - (n - 1) * page;
+    if (t == 0 && row % p.Hkv == 0)
+        p.positions[b] = taken == 0 ? 0 : (taken - 1) * page + len - (n - 1) * page;
     for (int i = taken + t; i < p.top; i += blockDim.x) selected[i] = -1;
     if (n <= p.top) {
         for (int i = t; i < n; i += blockDim.x) selected[i] = i, pages[i] = table[i];
