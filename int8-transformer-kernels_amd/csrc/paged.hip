@@ -65,6 +65,7 @@ struct Attend {
     int B, Hq, Hkv, N, num_pages, log2_page, max_context;
     int groups;                          // blocks of query rows per key head
     int pieces, min_tiles;               // see Piece; 0: a sequence is one piece
+    int slots;                           // pieces that the grid has room for
     float qk;
 };
 
@@ -207,17 +208,25 @@ __device__ __forceinline__ void store_row(const Attend& p, size_t at, const floa
 
 template <int D>
 struct AttendTile {
-    static constexpr int kK = D / 64;   // 16-byte pieces of a K row per lane
     static constexpr int kV = D / 64;   // 4-byte words of a V row per lane
-    v4i k[2][kK];                       // row 4 (m % 4) + m / 4 (+ 16): bytes 64 i + 16 g ..
     uint32_t v[8][kV];                  // key 4 j + g: bytes D / 16 m ..
-    float sk, sv;                       // lane n of a row of lanes: key 4 (n % 8) + g
+    float sk[2], sv[2];                 // lane n of a row of lanes: key 4 (n % 4) + g (+ 16)
 };
 
+// Where piece c (16 bytes) of K row r of 16 lies in LDS: pieces are exchanged inside runs of 256
+// bytes, so that both the 16 lanes that write a run and those that read one piece of all 16 rows
+// meet every bank once.
+template <int D>
+__device__ __forceinline__ uint32_t k_slot(int r, int c) {
+    constexpr int C = D / 16, RP = 256 / D;
+    return (r / RP) * 256 + ((r % RP) * C + (c ^ (r / RP % C))) * 16;
+}
+
 template <int D, int F>
-__global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend p) {
+__global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     using Tile = AttendTile<D>;
     constexpr int NF = D / 16;          // fragments of O^T
+    constexpr int KI = D / 64;          // loads of 1 KiB per 16 rows
     constexpr int MR = 16 * F;          // query rows per block
     constexpr int kORow = D + 4;        // floats per row of O in LDS
     extern __shared__ __align__(16) float s_merge[];
@@ -226,15 +235,16 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
     const int nw = blockDim.x >> 6;
     const int g = lane >> 4, m16 = lane & 15;
 
-    // Block -> piece of a sequence, key head and rows of it.  Blocks go to the 8 XCDs in turn; the
-    // blocks of one piece, which share pages, run one after the other on one XCD.
-    const int heads_here = p.Hkv * p.groups;
-    const int local = (int)blockIdx.x / 8;
-    const int number = local / heads_here * 8 + (int)blockIdx.x % 8;
+    // Block -> piece of a sequence, key head and rows of it.  Blocks go to the 8 XCDs in turn; each
+    // XCD takes a run of the (piece, key head) pairs, and the blocks of one pair, which read the same
+    // rows, one after the other.
+    const int units = p.slots * p.Hkv, each_xcd = (units + 7) / 8;
+    const int local = (int)blockIdx.x / 8 / p.groups;
+    const int unit = (int)blockIdx.x % 8 * each_xcd + local;
+    if (local >= each_xcd || unit >= units) return;
+    const int number = unit / p.Hkv, kvh = unit % p.Hkv, grp = (int)blockIdx.x / 8 % p.groups;
     Piece piece{number, 0, 1, number, 0};
-    if (p.pieces == 0) {
-        if (number >= p.B) return;
-    } else {
+    if (p.pieces > 0) {
         if (!find_piece(p, piece, [&](int first, int count, int) {
                 return number >= first && number < first + count;
             }))
@@ -242,7 +252,6 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
         piece.index = number - piece.first;
     }
     const int b = piece.b;
-    const int kvh = local % heads_here / p.groups, grp = local % p.groups;
     const int all_rows = p.Hq / p.Hkv * p.N;
     const int row0_q = grp * MR, rows = min(MR, all_rows - row0_q);
     const size_t first_row = ((size_t)b * p.Hq + (size_t)kvh * (p.Hq / p.Hkv)) * p.N + row0_q;
@@ -257,7 +266,7 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
     const uint32_t* masks = masks_of(p, b);
 
     // this lane's query row of each fragment (rows past the last hold zeros)
-    v4i qf[F][Tile::kK];
+    v4i qf[F][KI];
     float qs[F];
     int node[F];
 #pragma unroll
@@ -267,50 +276,82 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
         node[f] = (row0_q + r) % p.N;
         qs[f] = ok ? p.sQ[first_row + r] * p.qk : 0.f;
 #pragma unroll
-        for (int i = 0; i < Tile::kK; ++i)
+        for (int i = 0; i < KI; ++i)
             qf[f][i] = ok ? *reinterpret_cast<const v4i*>(p.Q + (first_row + r) * D + 64 * i + 16 * g)
                           : v4i{0, 0, 0, 0};
     }
 
+    // K goes through LDS, a tile of this wave's own: the MFMA wants piece g of 16 rows from 16 lanes
+    // side by side, and loads in that order take four times as long as whole lines (46 against 11
+    // cycles of a CU per KiB: the loads of a wave's tile 365 cycles, 225 so).
+    char* s_k = reinterpret_cast<char*>(s_merge) + wave * (kTile * D);
+    uint32_t k_write[KI], k_read[KI];
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+        const int at = 64 * i + lane;  // piece of the 16 rows
+        k_write[i] = k_slot<D>(at / NF, at % NF);
+        k_read[i] = k_slot<D>(4 * (m16 & 3) + (m16 >> 2), 4 * i + g);
+    }
     // lane offsets inside 16 rows
-    const uint32_t k_off = (uint32_t)(4 * (m16 & 3) + (m16 >> 2)) * D + 16 * g;
     const uint32_t v_off = (uint32_t)g * D + D / 16 * m16;
-    const int s_off = 4 * (m16 & 3) + g;        // row of this lane's scales inside its 16
-    const bool s_upper = (m16 & 4) != 0;        // they lie in the second 16 keys
+    const uint32_t s_off = 4 * (4 * (m16 & 3) + g);  // bytes of this lane's scales
     bool bad = false;
 
     // The two runs of 16 rows of tile t: their page ids (a page holds whole runs; entries past
-    // the last position are not read), and from those the first row of each.  The ids are read a
-    // tile before the rows are needed, which is a tile before the data is.
+    // the last position are not read), and from those the first row of each.  Past the last tile
+    // ids and rows stay as they are.
     const bool two_pages = p.log2_page == 4;
-    int id0 = 0, id1 = 0;
+    int id[2] = {0, 0};
     auto fetch_ids = [&](int t) {
         if (t >= t_end) return;
-        id0 = table[(t * kTile) >> p.log2_page];
-        if (two_pages) id1 = table[min(t * kTile + 16, e.total - 1) >> p.log2_page];
+        id[0] = table[(t * kTile) >> p.log2_page];
+        if (two_pages) id[1] = table[min(t * kTile + 16, e.total - 1) >> p.log2_page];
     };
-    size_t row0 = 0, row1 = 0;
-    auto rows_of_ids = [&](int t) {
+    struct Rows {
+        size_t first[2];
+    };
+    auto rows_of_ids = [&](int t, Rows& rows) {
         if (t >= t_end) return;
         auto first = [&](int raw, int key) {
             const int page = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
             bad = bad || page != raw;
             return (((size_t)page * p.Hkv + kvh) << p.log2_page) + (size_t)(key & pmask);
         };
-        const int raw0 = __builtin_amdgcn_readfirstlane(id0);
-        row0 = first(raw0, t * kTile);
-        row1 = row0 + 16;
-        if (two_pages) row1 = first(__builtin_amdgcn_readfirstlane(id1), t * kTile + 16);
+        rows.first[0] = first(__builtin_amdgcn_readfirstlane(id[0]), t * kTile);
+        rows.first[1] = rows.first[0] + 16;
+        if (two_pages) rows.first[1] = first(__builtin_amdgcn_readfirstlane(id[1]), t * kTile + 16);
     };
-    auto load = [&](Tile& r) {
+    v4i k_raw[2][KI], k[2][KI];  // a tile's rows as loaded, and as the MFMA takes them
+    auto load_k = [&](const Rows& rows) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const size_t row = h == 0 ? row0 : row1;
-            const __amdgpu_buffer_rsrc_t kb = make_buffer(p.K + row * D, 16 * D);
-            const __amdgpu_buffer_rsrc_t vb = make_buffer(p.V + row * D, 16 * D);
+            const __amdgpu_buffer_rsrc_t kb = make_buffer(p.K + rows.first[h] * D, 16 * D);
 #pragma unroll
-            for (int i = 0; i < Tile::kK; ++i)
-                r.k[h][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, k_off, 64 * i, 0));
+            for (int i = 0; i < KI; ++i)
+                k_raw[h][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, lane * 16, 1024 * i, 0));
+        }
+    };
+    auto write_k = [&]() {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < KI; ++i)
+                *reinterpret_cast<v4i*>(s_k + h * 16 * D + k_write[i]) = k_raw[h][i];
+    };
+    auto read_k = [&]() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's LDS accesses are in order
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < KI; ++i)
+                k[h][i] = *reinterpret_cast<const v4i*>(s_k + h * 16 * D + k_read[i]);
+    };
+    auto load_v = [&](Tile& r, const Rows& rows) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const size_t row = rows.first[h];
+            const __amdgpu_buffer_rsrc_t vb = make_buffer(p.V + row * D, 16 * D);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (D == 128) {
@@ -320,11 +361,11 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
                     r.v[4 * h + j][0] = __builtin_amdgcn_raw_buffer_load_b32(vb, v_off, 4 * j * D, 0);
                 }
             }
+            r.sk[h] = __builtin_bit_cast(
+                float, __builtin_amdgcn_raw_buffer_load_b32(make_buffer(p.sK + row, 64), s_off, 0, 0));
+            r.sv[h] = __builtin_bit_cast(
+                float, __builtin_amdgcn_raw_buffer_load_b32(make_buffer(p.sV + row, 64), s_off, 0, 0));
         }
-        const size_t first = row0, second = row1;
-        const size_t srow = (s_upper ? second : first) + s_off;
-        r.sk = p.sK[srow];
-        r.sv = p.sV[srow];
     };
 
     v4f o[F][NF];
@@ -336,71 +377,71 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
         for (int i = 0; i < NF; ++i) o[f][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto compute = [&](const Tile& r, int t) {
-        const float skj[8] = {bcast16<0>(r.sk), bcast16<1>(r.sk), bcast16<2>(r.sk), bcast16<3>(r.sk),
-                              bcast16<4>(r.sk), bcast16<5>(r.sk), bcast16<6>(r.sk), bcast16<7>(r.sk)};
-        const float svj[8] = {bcast16<0>(r.sv), bcast16<1>(r.sv), bcast16<2>(r.sv), bcast16<3>(r.sv),
-                              bcast16<4>(r.sv), bcast16<5>(r.sv), bcast16<6>(r.sv), bcast16<7>(r.sv)};
+    auto compute = [&](const Tile& r, int t, auto next_k) {
+        const float svj[8] = {bcast16<0>(r.sv[0]), bcast16<1>(r.sv[0]), bcast16<2>(r.sv[0]), bcast16<3>(r.sv[0]),
+                              bcast16<0>(r.sv[1]), bcast16<1>(r.sv[1]), bcast16<2>(r.sv[1]), bcast16<3>(r.sv[1])};
         const bool partial = t * kTile + kTile > e.prefix;  // wave-uniform
-        v8h pw[F], pr[F];
+        // the dot products of key 4 j + g, and sK sQ / sqrt(D) of it and this lane's query: an MFMA
+        // over 4 x 4 blocks, the outer product of the lanes' key scales with their query scales
+        float dot[F][8], scale[F][8];
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            v4i sa[2];
+        for (int f = 0; f < F; ++f)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                sa[h] = v4i{0, 0, 0, 0};
+                v4i a = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < Tile::kK; ++i)
-                    sa[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[h][i], qf[f][i], sa[h], 0, 0, 0);
+                for (int i = 0; i < KI; ++i)
+                    a = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[h][i], qf[f][i], a, 0, 0, 0);
+                const v4f c = __builtin_amdgcn_mfma_f32_4x4x1f32(r.sk[h], qs[f], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    dot[f][4 * h + j] = static_cast<float>(a[j]), scale[f][4 * h + j] = c[j];
             }
-            // u_j = q . k_j sK_j of key 4 j + g
-            float u[8], w[8], pj[8];
+        v8h pw[F], pr[F];
+        float w[F][8], psum[F];
+        auto weights = [&](int f) {
+            float pj[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = static_cast<float>(sa[j >> 2][j & 3]) * skj[j];
-            auto weights = [&]() {
+            for (int j = 0; j < 8; ++j) {
+                pj[j] = fast_exp2(fmaf(dot[f][j], scale[f][j], -m[f]));
+                w[f][j] = pj[j] * svj[j];
+            }
+            psum[f] = ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+        };
+        // the weights as two fp16; one past fp16's range (checked where it may be: an infinite
+        // value scale) leaves no rest
+        auto split = [&](int f, auto checked) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    pj[j] = fast_exp2(fmaf(u[j], qs[f], -m[f]));
-                    w[j] = pj[j] * svj[j];
+            for (int j = 0; j < 8; j += 2) {
+                typedef float f2 __attribute__((ext_vector_type(2)));
+                const h2 top = __builtin_convertvector((f2){w[f][j], w[f][j + 1]}, h2);
+                float rest0 = minus_half<0>(w[f][j], top), rest1 = minus_half<1>(w[f][j + 1], top);
+                if constexpr (decltype(checked)::value) {
+                    rest0 = fabsf(w[f][j]) < 65520.f ? rest0 : 0.f;
+                    rest1 = fabsf(w[f][j + 1]) < 65520.f ? rest1 : 0.f;
                 }
-            };
-            auto sum8 = [&]() {
-                return ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
-            };
-            // the weights as two fp16; one past fp16's range (checked where it may be: an infinite
-            // value scale) leaves no rest
-            auto split = [&](auto checked) {
+                const h2 rest = __builtin_convertvector((f2){rest0, rest1}, h2);
+                pw[f][j] = top.x, pw[f][j + 1] = top.y;
+                pr[f][j] = rest.x, pr[f][j + 1] = rest.y;
+            }
+        };
+        bool slow = partial;
+        if (!partial) {
+            float wide = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    typedef float f2 __attribute__((ext_vector_type(2)));
-                    const h2 top = __builtin_convertvector((f2){w[j], w[j + 1]}, h2);
-                    float rest0 = minus_half<0>(w[j], top), rest1 = minus_half<1>(w[j + 1], top);
-                    if constexpr (decltype(checked)::value) {
-                        rest0 = fabsf(w[j]) < 65520.f ? rest0 : 0.f;
-                        rest1 = fabsf(w[j + 1]) < 65520.f ? rest1 : 0.f;
-                    }
-                    const h2 rest = __builtin_convertvector((f2){rest0, rest1}, h2);
-                    pw[f][j] = top.x, pw[f][j + 1] = top.y;
-                    pr[f][j] = rest.x, pr[f][j + 1] = rest.y;
-                }
-            };
-            bool slow = partial;
-            if (!partial) {
-                weights();
-                const float psum = sum8();
-                float wide = fmaxf(fabsf(w[0]), fabsf(w[1]));
+            for (int f = 0; f < F; ++f) {
+                weights(f);
 #pragma unroll
-                for (int j = 2; j < 8; j += 2) wide = fmaxf(wide, fmaxf(fabsf(w[j]), fabsf(w[j + 1])));
+                for (int j = 0; j < 8; j += 2) wide = fmaxf(wide, fmaxf(fabsf(w[f][j]), fabsf(w[f][j + 1])));
                 // (the first tile, whose m is -inf, has an infinite sum)
-                slow = __ballot(fmaxf(wide, psum * (kMaxWeight / kMaxSum)) > kMaxWeight) != 0;
-                if (!slow) {
-                    l[f] += psum;
-                    split(std::false_type{});
-                }
+                wide = fmaxf(wide, psum[f] * (kMaxWeight / kMaxSum));
             }
-            if (slow) {
-                // the exact maximum, then the largest weight under it
-                float top = -INFINITY, pm = 0.f;
+            slow = __ballot(wide > kMaxWeight) != 0;
+        }
+        if (slow) {
+            // the exact maximum, then the largest weight under it
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
                 uint32_t visible = ~0u;  // keys of the tile
                 if (partial) {
                     const int first = t * kTile - e.prefix;  // node of the tile's first key
@@ -409,37 +450,50 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
                     visible &= low_bits(e.total - t * kTile);
                 }
                 visible >>= g;
-                bool seen[8];
+                float top = -INFINITY, pm = 0.f, pj[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    seen[j] = (visible >> (4 * j)) & 1;
-                    if (seen[j]) top = fmaxf(top, u[j] * qs[f]);
+                for (int j = 0; j < 8; ++j) {  // unseen rows may hold anything
+                    dot[f][j] = (visible >> (4 * j)) & 1 ? dot[f][j] * scale[f][j] : -INFINITY;
+                    top = fmaxf(top, dot[f][j]);
                 }
                 top = max_groups(top);
                 const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (seen[j]) pm = fmaxf(pm, fabsf(fast_exp2(fmaf(u[j], qs[f], -base)) * svj[j]));
+                for (int j = 0; j < 8; ++j) {
+                    pj[j] = fast_exp2(dot[f][j] - base);
+                    w[f][j] = (visible >> (4 * j)) & 1 ? pj[j] * svj[j] : 0.f;
+                    pm = fmaxf(pm, fabsf(w[f][j]));
+                }
                 pm = max_groups(pm);
                 int ex = 0;
                 if (pm > 0.f && pm < INFINITY) frexpf(pm, &ex);
                 const float m_new =
                     fmaxf(m[f], top + (float)min(max(ex - kTopExp, -kMaxShift), kMaxShift));
-                const float alpha = fast_exp2(m[f] - (m_new == -INFINITY ? 0.f : m_new));
+                const float use = m_new == -INFINITY ? 0.f : m_new;
+                if (__ballot(m[f] != -INFINITY) != 0) {  // (not the wave's first tile)
+                    const float alpha = fast_exp2(m[f] - use);
+                    l[f] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < NF; ++i)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[f][i][c] *= alpha;
+                }
                 m[f] = m_new;
-                l[f] *= alpha;
+                const float shift = fast_exp2(base - use);  // 2^(s - base) to 2^(s - m)
+                float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < NF; ++i)
+                for (int j = 0; j < 8; ++j) w[f][j] *= shift, sum += pj[j];
+                l[f] = fmaf(sum, shift, l[f]);
+                split(f, std::true_type{});
+            }
+        } else {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) o[f][i][c] *= alpha;
-                weights();
-#pragma unroll
-                for (int j = 0; j < 8; ++j)  // unseen rows may hold anything
-                    if (!seen[j]) pj[j] = w[j] = 0.f;
-                l[f] += sum8();
-                split(std::true_type{});
+            for (int f = 0; f < F; ++f) {
+                l[f] += psum[f];
+                split(f, std::false_type{});
             }
         }
+        next_k();
         // byte c of two keys, c + 128 as an unsigned number u: 0x6400 | u is 1024 + u in fp16, and
         // the sum below exact
         const h2 bias = {(_Float16)-1152.f, (_Float16)-1152.f};
@@ -464,32 +518,50 @@ __global__ __launch_bounds__(F == 4 ? 256 : 512) void paged_attend_kernel(Attend
     };
 
     {
+        // While tile t is computed: V of tile t + nw is on its way from the start, K of it is taken
+        // through LDS between the softmax and the product with V, and K of tile t + 2 nw is asked
+        // for then.  Loads past the last tile repeat its rows: in a branch, the wait for this
+        // tile's data would have to cover the next one's as well.
         int t = t_begin + wave;
         Tile ra, rb;
-        // Data of tile t in ra, rows of tile t + nw, ids of tile t + 2 nw.  The loads are not
-        // conditional: past the last tile they repeat its rows.
+        Rows r1{}, r2{};
         fetch_ids(t);
-        rows_of_ids(t);
+        rows_of_ids(t, r1);
         fetch_ids(t + nw);
-        if (t < t_end) load(ra);
-        rows_of_ids(t + nw);
+        if (t < t_end) {
+            load_k(r1);
+            load_v(ra, r1);
+        }
+        rows_of_ids(t + nw, r1);
+        r2 = r1;
         fetch_ids(t + 2 * nw);
+        if (t < t_end) {
+            write_k();
+            load_k(r1);
+            read_k();
+        }
+        rows_of_ids(t + 2 * nw, r2);
+        fetch_ids(t + 3 * nw);
+        auto step = [&](Tile& now, Tile& next) {
+            load_v(next, r1);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(now, t, [&]() {
+                write_k();
+                load_k(r2);
+                read_k();
+            });
+            r1 = r2;
+            rows_of_ids(t + 3 * nw, r2);
+            fetch_ids(t + 4 * nw);
+            t += nw;
+        };
         while (t < t_end) {
-            load(rb);
-            rows_of_ids(t + 2 * nw);
-            fetch_ids(t + 3 * nw);
-            __builtin_amdgcn_sched_barrier(0);
-            compute(ra, t);
-            t += nw;
+            step(ra, rb);
             if (t >= t_end) break;
-            load(ra);
-            rows_of_ids(t + 2 * nw);
-            fetch_ids(t + 3 * nw);
-            __builtin_amdgcn_sched_barrier(0);
-            compute(rb, t);
-            t += nw;
+            step(rb, ra);
         }
     }
+    __syncthreads();  // the tiles of K give way to the join
     if (bad && lane == 0) atomicAdd(&g_attend_bad_ids, 1u);
 
     // Join the waves: m and l of each row go to LDS, and O scaled to the rows' common maximum, which
@@ -604,22 +676,39 @@ struct AttendPlan {
 };
 
 constexpr int kMaxSplit = 64;      // pieces per sequence, on average
-constexpr int kMaxBlocks = 1024;   // of a cut
+constexpr int kMaxBlocks = 1024;   // of a cut: four rounds of 256 CUs
 
-// rows: query rows per key head
-AttendPlan attend_plan(int B, int rows, int Hkv, int context) {
+// rows: query rows per key head.
+// Two fragments share a tile's loads and conversions where one alone would leave a block to half of
+// the CUs anyhow (us with one / two: 16 sequences of 8192 x 32 rows x 8 heads 59 / 53; 2 of 4096 x
+// 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).
+// A CU runs one block of 8 waves at a time.  The number of pieces is the one with the least estimated time
+// (0.01 us): a round of blocks costs 4 us and 1.1 us per tile of a wave with one fragment, 1.9 with
+// two (0.8 and 1.3 at head dim 64); the join of pieces 6 us; lengths are taken to be 3/4 of
+// max_context in the mean, which a sequence in one piece does not profit from.  Estimated /
+// measured, us: 16 sequences of 8192, 64 rows, one piece each 65 / 68, two 74 / 80; 13 of 3001, 12
+// heads of 64 13 / 17, cut 15 / 20; 8 of 8192, 16 heads of 64 in one piece 30 / 36, in two 23 / 29;
+// 1 of 1000, 20 rows 8 / 12, cut 14 / 12; 4 of 4096, 32 rows 22 / 27, cut 15 / 19.
+AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
+    constexpr int kCus = 256;
     AttendPlan pl{};
-    pl.frags = rows <= 16 ? 1 : 2;
+    pl.waves = 8;
+    pl.min_tiles = pl.waves;
+    pl.frags = rows > 16 && (long long)B * Hkv * ceil_div(rows, 16) >= kCus / 2 ? 2 : 1;
     pl.groups = (rows + 16 * pl.frags - 1) / (16 * pl.frags);
-    pl.waves = 4;
     const long long heads = (long long)Hkv * pl.groups;  // blocks per piece
     const long long tiles = ceil_div(context, kTile);
-    const long long resident = pl.frags == 1 ? 768 : 512;
-    pl.min_tiles = pl.waves;
-    // (the sum of all tiles is an int)
-    pl.pieces = (int)std::min<long long>({(long long)kMaxSplit * B, resident / heads,
-                                          B * ceil_div(tiles, pl.min_tiles)});
-    if (pl.pieces <= B || B * tiles >= (1LL << 31)) pl.pieces = 0;
+    const long long tile_time = pl.frags == 1 ? (D == 64 ? 80 : 110) : (D == 64 ? 130 : 190);
+    auto round = [&](long long t) { return 400 + ceil_div(t, pl.waves) * tile_time; };
+    long long best = ceil_div(B * heads, kCus) * round(tiles);
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+        const long long pieces = std::min<long long>({(long long)kMaxSplit * B, rounds * kCus / heads,
+                                                      B * ceil_div(tiles, pl.min_tiles)});
+        // (the sum of all tiles is an int)
+        if (pieces <= B || B * tiles >= (1LL << 31)) continue;
+        const long long time = ceil_div(pieces * heads, kCus) * round(ceil_div(3 * B * tiles, 4 * pieces)) + 600;
+        if (time < best) best = time, pl.pieces = (int)pieces;
+    }
     return pl;
 }
 
@@ -636,9 +725,9 @@ Partials plan_partials(const AttendPlan& pl, int B, size_t rows, int D) {
     return partials_of(pl.pieces > 0 ? pl.slots(B) * rows : 0, D);
 }
 // Room for every plan of at most `rows` query rows in all: a cut has at most kMaxSplit pieces per
-// sequence, and at most kMaxBlocks blocks of 64 rows.
+// sequence, and at most kMaxBlocks blocks of 32 rows.
 Partials most_partials(size_t rows, int D) {
-    return partials_of(std::min<size_t>(kMaxSplit * rows, 64 * kMaxBlocks), D);
+    return partials_of(std::min<size_t>(kMaxSplit * rows, 32 * kMaxBlocks), D);
 }
 
 template <int D, int F>
@@ -648,7 +737,7 @@ int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipS
     const int st = once.run([] {
         const hipError_t e = hipFuncSetAttribute(
             reinterpret_cast<const void*>(&paged_attend_kernel<D, F>),
-            hipFuncAttributeMaxDynamicSharedMemorySize, (F == 4 ? 4 : 8) * kWave);
+            hipFuncAttributeMaxDynamicSharedMemorySize, 8 * kWave);
         if (e == hipSuccess) return (int)INT8K_OK;
         set_last_error("hipFuncSetAttribute", e);
         return (int)INT8K_ERR_HIP;
@@ -660,14 +749,13 @@ int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipS
 
 template <int D>
 int launch_attend(Attend p, const AttendPlan& pl, void* workspace, hipStream_t stream) {
-    p.groups = pl.groups, p.pieces = pl.pieces, p.min_tiles = pl.min_tiles;
+    p.groups = pl.groups, p.pieces = pl.pieces, p.min_tiles = pl.min_tiles, p.slots = pl.slots(p.B);
     p.part_ml = static_cast<float*>(workspace);
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           plan_partials(pl, p.B, (size_t)p.Hq * p.N, D).ml_bytes);
-    const unsigned blocks = (unsigned)(ceil_div(pl.slots(p.B), 8) * 8 * p.Hkv * pl.groups);
-    const int st = pl.frags == 1   ? launch_instance<D, 1>(p, pl, blocks, stream)
-                   : pl.frags == 2 ? launch_instance<D, 2>(p, pl, blocks, stream)
-                                   : launch_instance<D, 4>(p, pl, blocks, stream);
+    const unsigned blocks = (unsigned)(ceil_div((long long)p.slots * p.Hkv, 8) * 8 * pl.groups);
+    const int st = pl.frags == 1 ? launch_instance<D, 1>(p, pl, blocks, stream)
+                                 : launch_instance<D, 2>(p, pl, blocks, stream);
     if (st != INT8K_OK || pl.pieces == 0) return st;
     const int blocks_each = (int)ceil_div((long long)p.Hq * p.N, kCombineRows<D>);
     paged_combine_kernel<D><<<(unsigned)(p.B * blocks_each), 256, 0, stream>>>(p, blocks_each);
@@ -683,7 +771,7 @@ int run_attend(const Attend& p, const AttendPlan& pl, int D, void* workspace, hi
 bool attend_fits(long long B, long long heads, long long kv_heads, long long nodes, int max_context,
                  const AttendPlan& pl) {
     return B * heads * nodes < (1LL << 24) && max_context <= (1 << 30) &&
-           ceil_div(pl.slots((int)B), 8) * 8 * kv_heads * pl.groups * pl.waves < (1LL << 25);
+           ceil_div(pl.slots((int)B) * kv_heads, 8) * 8 * pl.groups * pl.waves < (1LL << 25);
 }
 
 constexpr int kMaxNodes = 256;
@@ -734,7 +822,7 @@ extern "C" int int8k_tree_attention_forward_paged(
         return INT8K_ERR_MISALIGNED;
     if (nodes > kMaxNodes || (long long)B * heads * nodes >= (1LL << 24))
         return INT8K_ERR_UNSUPPORTED;
-    const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context);
+    const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context, head_dim);
     if (!attend_fits(B, heads, kv_heads, nodes, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
     const size_t need = plan_partials(pl, B, (size_t)heads * nodes, head_dim).bytes;
     if (need > 0) {
@@ -792,7 +880,7 @@ extern "C" int int8k_decode_attention_forward_paged_sparse(
     if ((long long)B * heads >= (1LL << 24) || max_context > (1 << 30) ||
         (long long)B * kv_heads > 65535 || (long long)B * kv_heads * top_pages >= (1LL << 31))
         return INT8K_ERR_UNSUPPORTED;
-    const AttendPlan pl = attend_plan(B, heads / kv_heads, kv_heads, context);
+    const AttendPlan pl = attend_plan(B, heads / kv_heads, kv_heads, context, head_dim);
     if (!attend_fits(B, heads, kv_heads, 1, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
     const SelectSpace sel = select_space(B, kv_heads, max_context, page_size, top_pages);
     if (!workspace ||

@@ -91,52 +91,101 @@ __global__ __launch_bounds__(256) void move_rows_kernel(Move p) {
 // rounding border does not depend on the order of the sum), rounded to fp32 and quantized as
 // int8k_quantize_per_token does; a NaN in a mean makes the scale NaN.
 
+// One wave per page and key head up to 64 rows (four waves of a few rows each spend more on joining
+// their sums than on the rows: 2048 pages of 64 rows, 8 heads of 128, 84 us, MEANS so), two or four
+// for longer pages.  A lane owns 16 dims of every 64 / L-th row and loads four rows ahead.
+
+// a of this lane plus a of the lane 32 (16) away where the lane is in the lower half of 64 (32), the
+// same of b where it is in the upper: two values of two lanes become one of each.
+template <int HALF>
+__device__ __forceinline__ double fold(double a, double b) {
+    auto swapped = [](uint32_t x, uint32_t y) {
+        if constexpr (HALF == 32) return __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        else return __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    };
+    const uint64_t u = (uint64_t)__double_as_longlong(a), v = (uint64_t)__double_as_longlong(b);
+    const auto lo = swapped((uint32_t)u, (uint32_t)v), hi = swapped((uint32_t)(u >> 32), (uint32_t)(v >> 32));
+    return __longlong_as_double((long long)((uint64_t)hi[0] << 32 | lo[0])) +
+           __longlong_as_double((long long)((uint64_t)hi[1] << 32 | lo[1]));
+}
+
 template <int D>
 __global__ __launch_bounds__(256) void page_means_kernel(const int8_t* __restrict__ pages,
                                                          const float* __restrict__ scales,
                                                          const int32_t* __restrict__ ids,
                                                          int8_t* __restrict__ means,
-                                                         float* __restrict__ s_means, int Hkv,
-                                                         int num_pages, int log2_page) {
+                                                         float* __restrict__ s_means, int units,
+                                                         int Hkv, int num_pages, int log2_page,
+                                                         int waves) {
     constexpr int L = D / 16, R = 64 / L;  // lanes per row, rows per wave load
+    constexpr int kAhead = 4;
     __shared__ double s_sum[4][D];
-    const int h = (int)(blockIdx.x % (unsigned)Hkv), id = ids[blockIdx.x / (unsigned)Hkv];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    if (id < 0 || id >= num_pages) {  // the whole block leaves
-        if (id >= 0 && h == 0 && threadIdx.x == 0) atomicAdd(&g_pages_bad_ids, 1u);
-        return;
-    }
-    const size_t unit = (size_t)id * Hkv + h, row0 = unit << log2_page;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = wave & (waves - 1);  // of the unit's rows
+    const int u = (int)blockIdx.x * (4 / waves) + wave / waves;
+    const int h = u % Hkv, id = u < units ? __builtin_amdgcn_readfirstlane(ids[u / Hkv]) : -1;
+    const bool ok = id >= 0 && id < num_pages;
+    if (id >= num_pages && h == 0 && part == 0 && lane == 0) atomicAdd(&g_pages_bad_ids, 1u);
+    const size_t unit = ok ? (size_t)id * Hkv + h : 0, row0 = unit << log2_page;
     const int page = 1 << log2_page;
     double acc[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.0;
-    for (int r = wave * R + lane / L; r < page; r += nw * R) {
-        const uint4 w = *reinterpret_cast<const uint4*>(pages + (row0 + r) * D + 16 * (lane % L));
-        const double s = (double)scales[row0 + r];
-        const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+    if (ok) {
+        const uint4* rows = reinterpret_cast<const uint4*>(pages + row0 * D) + lane % L;
+        uint4 w[kAhead];
+        float s[kAhead];
+        auto load = [&](int k, int r) {  // past the last row: a zero scale
+            const int at = min(r, page - 1);
+            w[k] = rows[at * L];
+            s[k] = r < page ? scales[row0 + at] : 0.f;
+        };
+        const int step = waves * R;
+        int r = part * R + lane / L;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            acc[i] = fma((double)(int)(int8_t)((d[i >> 2] >> (8 * (i & 3))) & 0xff), s, acc[i]);
+        for (int k = 0; k < kAhead; ++k) load(k, r + k * step);
+        for (int r0 = part * R; r0 < page; r0 += kAhead * step, r += kAhead * step) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (r0 + k * step >= page) break;
+                const uint32_t d[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                const double sd = (double)s[k];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    acc[i] = fma((double)(int)(int8_t)((d[i >> 2] >> (8 * (i & 3))) & 0xff), sd, acc[i]);
+                load(k, r + (kAhead + k) * step);
+            }
+        }
     }
-    // over the wave's rows, then over the waves
+    // Over the wave's rows: lanes 32 and 16 apart exchange halves of the dims, so that each ends
+    // with 4, 4 (lane / 16) .. of its 16; the rest of the lanes are L .. 8 apart.
+    double half[8], sum[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 8; ++i) half[i] = fold<32>(acc[i], acc[i + 8]);
 #pragma unroll
-        for (int x = L; x < 64; x <<= 1) acc[i] += __shfl_xor(acc[i], x);
-    if (lane < L)
+    for (int i = 0; i < 4; ++i) sum[i] = fold<16>(half[i], half[i + 4]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_sum[wave][16 * lane + i] = acc[i];
-    __syncthreads();
-    if (wave != 0) return;
-    constexpr int W = D / 64;
-    float m[W];
+    for (int x = L; x < 16; x <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor(sum[i], x);
+    const int dim = 16 * (lane % L) + 8 * (lane / 32) + 4 * (lane / 16 % 2);
+    if (waves > 1) {
+        if (lane % 16 < L)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_sum[wave][dim + i] = sum[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i] = 0.0;
+            for (int k = 0; k < waves; ++k) sum[i] += s_sum[(wave & ~(waves - 1)) + k][dim + i];
+        }
+    }
+    if (!ok || part != 0) return;
+    float m[4];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-        double sum = 0.0;
-        for (int w = 0; w < nw; ++w) sum += s_sum[w][W * lane + i];
-        m[i] = (float)(sum / page);
+    for (int i = 0; i < 4; ++i) {
+        m[i] = (float)(sum[i] / page);
         top = max(top, __float_as_uint(m[i]) & 0x7fffffffu);
     }
     top = __float_as_uint(row_reduce(__uint_as_float(top), 6, [](float a, float b) {
@@ -146,10 +195,8 @@ __global__ __launch_bounds__(256) void page_means_kernel(const int8_t* __restric
     const float s = (amax < 1e-8f ? 1e-8f : amax) / 127.f;
     uint32_t c = 0;
 #pragma unroll
-    for (int i = 0; i < W; ++i) c |= ((uint32_t)quant_code(m[i], s) & 0xffu) << (8 * i);
-    int8_t* out = means + unit * D + W * lane;
-    if constexpr (W == 2) *reinterpret_cast<uint16_t*>(out) = (uint16_t)c;
-    else *out = (int8_t)c;
+    for (int i = 0; i < 4; ++i) c |= ((uint32_t)quant_code(m[i], s) & 0xffu) << (8 * i);
+    if (lane % 16 < L) *reinterpret_cast<uint32_t*>(means + unit * D + dim) = c;
     if (lane == 0) s_means[unit] = s;
 }
 
@@ -170,35 +217,35 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
-    constexpr int L = D / 16, kRows = 256 / L, kEach = 2;  // lanes per mean, means per block, per lane
-    const int row = blockIdx.y, b = row / p.Hkv, h = row % p.Hkv, G = p.Hq / p.Hkv;
-    int len;
-    const int n = blocks_of(p, b, len);
-    if (n <= p.top) return;  // all are taken
-    const int first = blockIdx.x * (kRows * kEach) + threadIdx.x / L, c = threadIdx.x % L;
-    if ((int)(blockIdx.x * (kRows * kEach)) >= n - 1) return;
-    v4i mean[kEach];
-    double sm[kEach], best[kEach];
+// The keys of the scored blocks first, first + each, .. (EACH of them, those below n - 1) for one
+// sequence and key head by a group of D / 16 lanes, which hold 16 dims each: put(k, block, key) on
+// every lane of the group.
+template <int D, int EACH, typename Put>
+__device__ __forceinline__ void score_blocks(const Select& p, int b, int h, int n, int first, int each,
+                                             Put&& put) {
+    constexpr int L = D / 16;
+    const int c = threadIdx.x % L, G = p.Hq / p.Hkv;
+    v4i mean[EACH];
+    double sm[EACH], best[EACH];
+    bool any[EACH];
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        const int i = min(first + k * kRows, n - 2);
+    for (int k = 0; k < EACH; ++k) {
+        const int i = min(first + k * each, n - 2);  // blocks past the last repeat it
         const int raw = p.tables[(size_t)b * p.max_pages + i];
         const int id = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
-        if (id != raw && h == 0 && c == 0 && first + k * kRows < n - 1) atomicAdd(&g_pages_bad_ids, 1u);
+        if (id != raw && h == 0 && c == 0 && first + k * each < n - 1) atomicAdd(&g_pages_bad_ids, 1u);
         const size_t unit = (size_t)id * p.Hkv + h;
         mean[k] = *reinterpret_cast<const v4i*>(p.means + unit * D + 16 * c);
         sm[k] = (double)p.s_means[unit];
         best[k] = -INFINITY;
+        any[k] = false;
     }
-    bool any[kEach] = {};
     for (int g = 0; g < G; ++g) {
-        const size_t qrow = (size_t)b * p.Hq + h * G + g;
-        const v4i q = *reinterpret_cast<const v4i*>(p.Q + qrow * D + 16 * c);
-        const double sq = (double)p.sQ[qrow];
+        const size_t row = (size_t)b * p.Hq + h * G + g;
+        const v4i q = *reinterpret_cast<const v4i*>(p.Q + row * D + 16 * c);
+        const double sq = (double)p.sQ[row];
 #pragma unroll
-        for (int k = 0; k < kEach; ++k) {
+        for (int k = 0; k < EACH; ++k) {
             int dot = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) dot = __builtin_amdgcn_sdot4(q[i], mean[k][i], dot, false);
@@ -209,11 +256,21 @@ __global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
         }
     }
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        const int i = first + k * kRows;
-        if (c == 0 && i < n - 1)
-            p.keys[(size_t)row * p.max_blocks + i] = any[k] ? score_key(best[k]) : 0;
-    }
+    for (int k = 0; k < EACH; ++k)
+        if (first + k * each < n - 1) put(first + k * each, any[k] ? score_key(best[k]) : 0);
+}
+
+// Scores by blocks of their own, for long contexts of few sequences.
+template <int D>
+__global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
+    constexpr int L = D / 16, kRows = 256 / L, kEach = 2;
+    const int row = blockIdx.y, b = row / p.Hkv, h = row % p.Hkv;
+    int len;
+    const int n = blocks_of(p, b, len), base = blockIdx.x * (kRows * kEach);
+    if (n <= p.top || base >= n - 1) return;  // all are taken, or none is here
+    score_blocks<D, kEach>(p, b, h, n, base + threadIdx.x / L, kRows, [&](int i, uint64_t key) {
+        if (threadIdx.x % L == 0) p.keys[(size_t)row * p.max_blocks + i] = key;
+    });
 }
 
 constexpr int kSelectThreads = 1024;
@@ -241,13 +298,15 @@ __device__ __forceinline__ int block_prefix(int v, int* s_wave, int& all) {
 
 // The top - 1 largest keys (ties: the lowest blocks) and the last block, by digits of 8 bits from
 // the highest: the digit that the last taken key has, until all keys that share its digits so far
-// are taken.
+// are taken.  Where the keys fit LDS and the scores are soon worked out, the block does that itself
+// (SCORE: us of both kernels / of one: FUSED).
+template <int D, bool SCORE>
 __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p) {
+    extern __shared__ uint64_t s_keys[];
     __shared__ int s_count[256], s_wave[kSelectThreads / 64], s_digit, s_above;
     const int row = blockIdx.x, b = row / p.Hkv, t = threadIdx.x;
     int len;
     const int n = blocks_of(p, b, len), page = 1 << p.log2_page;
-    const uint64_t* keys = p.keys + (size_t)row * p.max_blocks;
     const int32_t* table = p.tables + (size_t)b * p.max_pages;
     int32_t* selected = p.selected + (size_t)row * p.top;
     int32_t* pages = p.pages + (size_t)row * p.top;
@@ -258,6 +317,16 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
     if (n <= p.top) {
         for (int i = t; i < n; i += blockDim.x) selected[i] = i, pages[i] = table[i];
         return;
+    }
+    const uint64_t* keys = p.keys + (size_t)row * p.max_blocks;
+    if constexpr (SCORE) {
+        constexpr int L = D / 16, kRows = kSelectThreads / L, kEach = 4;
+        for (int i = t / L; i < n - 1; i += kRows * kEach)
+            score_blocks<D, kEach>(p, b, row % p.Hkv, n, i, kRows, [&](int at, uint64_t key) {
+                if (t % L == 0) s_keys[at] = key;
+            });
+        keys = s_keys;
+        __syncthreads();
     }
     int need = p.top - 1;  // of the keys that share the digits so far
     uint64_t prefix = 0;   // those digits
@@ -315,16 +384,25 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
 
 }  // namespace
 
+constexpr int kFusedBlocks = 1024;
+
 int launch_select(const Select& s, hipStream_t stream) {
     const int rows = s.B * s.Hkv;
-    const int per = 256 / (s.D / 16) * 2;
-    if (s.max_blocks > s.top) {
+    // one kernel up to a few rounds of scores per block, more where the rows fill the GPU anyhow
+    const bool fused = s.max_blocks <= s.top || s.max_blocks <= kFusedBlocks ||
+                       (rows >= 128 && s.max_blocks <= 4 * kFusedBlocks);
+    if (!fused) {
+        const int per = 256 / (s.D / 16) * 2;
         const dim3 grid((unsigned)ceil_div(s.max_blocks, per), (unsigned)rows);
         if (s.D == 64) block_scores_kernel<64><<<grid, 256, 0, stream>>>(s);
         else block_scores_kernel<128><<<grid, 256, 0, stream>>>(s);
         if (const int st = check_launch("block_scores_kernel")) return st;
+        select_blocks_kernel<64, false><<<(unsigned)rows, kSelectThreads, 0, stream>>>(s);
+    } else {
+        const size_t lds = s.max_blocks > s.top ? (size_t)s.max_blocks * sizeof(uint64_t) : 0;
+        if (s.D == 64) select_blocks_kernel<64, true><<<(unsigned)rows, kSelectThreads, lds, stream>>>(s);
+        else select_blocks_kernel<128, true><<<(unsigned)rows, kSelectThreads, lds, stream>>>(s);
     }
-    select_blocks_kernel<<<(unsigned)rows, kSelectThreads, 0, stream>>>(s);
     return check_launch("select_blocks_kernel");
 }
 
@@ -377,13 +455,14 @@ extern "C" int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages,
         !aligned_to(K_means, 16) || !aligned_to(sK_means, 4))
         return INT8K_ERR_MISALIGNED;
     if ((long long)count * kv_heads >= (1LL << 23)) return INT8K_ERR_UNSUPPORTED;
-    const unsigned blocks = (unsigned)(count * kv_heads), threads = 256;
+    const int units = count * kv_heads, waves = page_size <= 64 ? 1 : page_size <= 256 ? 2 : 4;
+    const unsigned blocks = (unsigned)ceil_div(units, 4 / waves);
     const hipStream_t s = as_stream(stream);
     if (head_dim == 64)
-        page_means_kernel<64><<<blocks, threads, 0, s>>>(K_pages, sK_pages, page_ids, K_means,
-                                                         sK_means, kv_heads, num_pages, log2_of(page_size));
+        page_means_kernel<64><<<blocks, 256, 0, s>>>(K_pages, sK_pages, page_ids, K_means, sK_means, units,
+                                                     kv_heads, num_pages, log2_of(page_size), waves);
     else
-        page_means_kernel<128><<<blocks, threads, 0, s>>>(K_pages, sK_pages, page_ids, K_means,
-                                                          sK_means, kv_heads, num_pages, log2_of(page_size));
+        page_means_kernel<128><<<blocks, 256, 0, s>>>(K_pages, sK_pages, page_ids, K_means, sK_means, units,
+                                                      kv_heads, num_pages, log2_of(page_size), waves);
     return check_launch("page_means_kernel");
 }
