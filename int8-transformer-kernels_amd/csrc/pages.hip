@@ -225,9 +225,19 @@ __device__ __forceinline__ void score_blocks(const Select& p, int b, int h, int 
                                              Put&& put) {
     constexpr int L = D / 16;
     const int c = threadIdx.x % L, G = p.Hq / p.Hkv;
-    v4i mean[EACH];
-    double sm[EACH], best[EACH];
+    constexpr int kHeads = 4;  // whose queries are loaded at a time, the first with the means
+    v4i mean[EACH], q[kHeads];
+    double sm[EACH], best[EACH], sq[kHeads];
     bool any[EACH];
+    auto load_heads = [&](int g0) {
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g) {
+            const size_t row = (size_t)b * p.Hq + h * G + min(g0 + g, G - 1);
+            q[g] = *reinterpret_cast<const v4i*>(p.Q + row * D + 16 * c);
+            sq[g] = (double)p.sQ[row];
+        }
+    };
+    load_heads(0);
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
         const int i = min(first + k * each, n - 2);  // blocks past the last repeat it
@@ -240,19 +250,20 @@ __device__ __forceinline__ void score_blocks(const Select& p, int b, int h, int 
         best[k] = -INFINITY;
         any[k] = false;
     }
-    for (int g = 0; g < G; ++g) {
-        const size_t row = (size_t)b * p.Hq + h * G + g;
-        const v4i q = *reinterpret_cast<const v4i*>(p.Q + row * D + 16 * c);
-        const double sq = (double)p.sQ[row];
+    for (int g0 = 0; g0 < G; g0 += kHeads) {
+        if (g0 > 0) load_heads(g0);
 #pragma unroll
-        for (int k = 0; k < EACH; ++k) {
-            int dot = 0;
+        for (int g = 0; g < kHeads; ++g) {  // (heads past the last repeat it)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dot = __builtin_amdgcn_sdot4(q[i], mean[k][i], dot, false);
-            dot = L == 8 ? group8_sum(dot) : group4_sum(dot);
-            const double s = ((double)dot * sm[k]) * sq;
-            any[k] = any[k] || s == s;
-            best[k] = s > best[k] ? s : best[k];
+            for (int k = 0; k < EACH; ++k) {
+                int dot = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dot = __builtin_amdgcn_sdot4(q[g][i], mean[k][i], dot, false);
+                dot = L == 8 ? group8_sum(dot) : group4_sum(dot);
+                const double s = ((double)dot * sm[k]) * sq[g];
+                any[k] = any[k] || s == s;
+                best[k] = s > best[k] ? s : best[k];
+            }
         }
     }
 #pragma unroll
@@ -275,35 +286,64 @@ __global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
 
 constexpr int kSelectThreads = 1024;
 
-// Sum of v over the threads before this one, and over all.
-__device__ __forceinline__ int block_prefix(int v, int* s_wave, int& all) {
+__device__ __forceinline__ double score_of(uint64_t key) {
+    return __longlong_as_double((long long)(key >> 63 ? key & ~(1ull << 63) : ~key));
+}
+
+// How many threads before this one hold true, and how many of all.
+__device__ __forceinline__ int count_before(bool v, int* s_wave, int& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int below = __shfl_up(x, d);
-        x += lane >= d ? below : 0;
-    }
+    const uint64_t set = __ballot(v);
     __syncthreads();
-    if (lane == 63) s_wave[wave] = x;
+    if (lane == 0) s_wave[wave] = __popcll(set);
     __syncthreads();
     int before = 0;
     all = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
-        before += w < wave ? s_wave[w] : 0;
-        all += s_wave[w];
+#pragma unroll
+    for (int w = 0; w < kSelectThreads / 64; ++w) {
+        const int count = s_wave[w];
+        before += w < wave ? count : 0;
+        all += count;
     }
-    return before + x - v;
+    return before + __builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
 }
 
-// The top - 1 largest keys (ties: the lowest blocks) and the last block, by digits of 8 bits from
-// the highest: the digit that the last taken key has, until all keys that share its digits so far
-// are taken.  Where the keys fit LDS and the scores are soon worked out, the block does that itself
-// (SCORE: us of both kernels / of one: FUSED).
+// The bin of s_count[256] that holds the need-th largest, and how many lie in the bins above it.
+__device__ __forceinline__ void find_bin(const int* s_count, int need, int& s_bin, int& s_above) {
+    const int t = threadIdx.x;
+    if (t >= 64) return;
+    int c[4], mine = 0;  // lane t: bins 255 - 4 t down to 252 - 4 t
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = s_count[255 - 4 * t - i], mine += c[i];
+    int x = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int below = __shfl_up(x, d);
+        x += t >= d ? below : 0;
+    }
+    int above = x - mine;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (above < need && need <= above + c[i]) s_bin = 255 - 4 * t - i, s_above = above;
+        above += c[i];
+    }
+}
+
+// The top - 1 largest keys (ties: the lowest blocks) and the last block.  The scores are counted in
+// 256 equal bins between their smallest and largest; the few in the bin that the last taken one
+// lies in are ranked among each other.  Where that does not do (an infinite or NaN score, all equal,
+// a bin of more than kList), by digits of 8 bits of the keys from the highest, until all keys that
+// share the digits of the last taken one so far are taken.
+// Where the keys fit LDS and the scores are soon worked out, the block does that itself (SCORE).
+constexpr int kList = 256;
+
 template <int D, bool SCORE>
 __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p) {
     extern __shared__ uint64_t s_keys[];
-    __shared__ int s_count[256], s_wave[kSelectThreads / 64], s_digit, s_above;
+    __shared__ int s_count[256], s_wave[kSelectThreads / 64], s_bin, s_above, s_listed;
+    __shared__ float s_low[kSelectThreads / 64], s_high[kSelectThreads / 64];
+    __shared__ uint64_t s_key[kList];
+    __shared__ int s_at[kList];
     const int row = blockIdx.x, b = row / p.Hkv, t = threadIdx.x;
     int len;
     const int n = blocks_of(p, b, len), page = 1 << p.log2_page;
@@ -328,55 +368,96 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
         keys = s_keys;
         __syncthreads();
     }
-    int need = p.top - 1;  // of the keys that share the digits so far
-    uint64_t prefix = 0;   // those digits
-    int shift = 64;        // keys >> shift == prefix share them (64: all)
-    bool exact = need == 0;  // all that share them are taken (top 1: none)
-    auto shares = [&](uint64_t k) { return shift == 64 || (k >> shift) == prefix; };
+    int need = p.top - 1;
+    auto emit = [&](auto takes) {  // the taken blocks in order
+        int base = 0;
+        for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+            const int i = i0 + t;
+            const bool take = i == n - 1 || (i < n - 1 && takes(i));
+            int total;
+            const int at = count_before(take, s_wave, total) + base;
+            base += total;
+            if (take && at < p.top) selected[at] = i, pages[at] = table[i];
+        }
+    };
+    if (need == 0) return emit([](int) { return false; });
+
+    float low = INFINITY, high = -INFINITY;
+    bool odd = false;
+    for (int i = t; i < n - 1; i += blockDim.x) {
+        const uint64_t k = keys[i];
+        const float s = (float)score_of(k);
+        odd = odd || k == 0 || !(fabsf(s) < INFINITY);
+        low = fminf(low, s), high = fmaxf(high, s);
+    }
+    low = row_reduce(low, 6, [](float x, float y) { return fminf(x, y); });
+    high = row_reduce(high, 6, [](float x, float y) { return fmaxf(x, y); });
+    if (t % 64 == 0) s_low[t / 64] = low, s_high[t / 64] = high;
+    if (t < 256) s_count[t] = 0;
+    if (t == 0) s_listed = 0;
+    odd = __syncthreads_or(odd);
+#pragma unroll
+    for (int w = 0; w < kSelectThreads / 64; ++w) low = fminf(low, s_low[w]), high = fmaxf(high, s_high[w]);
+    const double scale = 256.0 / ((double)high - (double)low);
+    if (!odd && high > low && scale < 1e300) {
+        // (rounded bounds: the cut to 0 .. 255 keeps the order)
+        auto bin_of = [&](uint64_t k) { return (int)fmin(fmax((score_of(k) - (double)low) * scale, 0.0), 255.0); };
+        for (int i = t; i < n - 1; i += blockDim.x) atomicAdd(&s_count[bin_of(keys[i])], 1);
+        __syncthreads();
+        find_bin(s_count, need, s_bin, s_above);
+        __syncthreads();
+        const int bin = s_bin, listed = s_count[bin];
+        need -= s_above;
+        if (listed <= kList) {
+            for (int i = t; i < n - 1; i += blockDim.x) {
+                const uint64_t k = keys[i];
+                if (bin_of(k) != bin) continue;
+                const int at = atomicAdd(&s_listed, 1);
+                s_key[at] = k, s_at[at] = i;
+            }
+            __syncthreads();
+            return emit([&](int i) {
+                const uint64_t k = keys[i];
+                const int mine = bin_of(k);
+                if (mine != bin) return mine > bin;
+                int before = 0;
+                for (int j = 0; j < listed; ++j)
+                    before += s_key[j] > k || (s_key[j] == k && s_at[j] < i) ? 1 : 0;
+                return before < need;
+            });
+        }
+        need += s_above;
+    }
+
+    uint64_t prefix = 0;  // the digits so far; need: of the keys that share them
+    int shift = 64;       // keys >> shift == prefix share them (64: all)
+    bool exact = false;   // all that share them are taken
     while (!exact && shift > 0) {
-        for (int i = t; i < 256; i += blockDim.x) s_count[i] = 0;
+        __syncthreads();
+        if (t < 256) s_count[t] = 0;
         __syncthreads();
         for (int i = t; i < n - 1; i += blockDim.x) {
             const uint64_t k = keys[i];
-            if (shares(k)) atomicAdd(&s_count[(k >> (shift - 8)) & 255], 1);
+            if (shift == 64 || (k >> shift) == prefix) atomicAdd(&s_count[(k >> (shift - 8)) & 255], 1);
         }
         __syncthreads();
-        if (t < 64) {
-            // lane t: digits 255 - 4 t down to 252 - 4 t
-            int c[4], mine = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = s_count[255 - 4 * t - i], mine += c[i];
-            int x = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int below = __shfl_up(x, d);
-                x += t >= d ? below : 0;
-            }
-            int above = x - mine;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (above < need && need <= above + c[i]) s_digit = 255 - 4 * t - i, s_above = above;
-                above += c[i];
-            }
-        }
+        find_bin(s_count, need, s_bin, s_above);
         __syncthreads();
         shift -= 8;
-        prefix = prefix << 8 | (uint64_t)s_digit;
+        prefix = prefix << 8 | (uint64_t)s_bin;
         need -= s_above;
-        exact = need == s_count[s_digit];
-        __syncthreads();
+        exact = need == s_count[s_bin];
     }
     int base = 0, ties = 0;
     for (int i0 = 0; i0 < n; i0 += blockDim.x) {
         const int i = i0 + t;
-        const uint64_t k = i < n - 1 ? keys[i] : 0;
-        const uint64_t high = shift == 64 ? 0 : k >> shift;
-        const bool same = i < n - 1 && shift < 64 && high == prefix;
+        const uint64_t high_digits = i < n - 1 ? keys[i] >> shift : 0;
+        const bool same = i < n - 1 && high_digits == prefix;
         int total;
-        const int rank = block_prefix(same ? 1 : 0, s_wave, total) + ties;
+        const int rank = count_before(same, s_wave, total) + ties;
         ties += total;
-        const bool take = i == n - 1 || (i < n - 1 && shift < 64 && (high > prefix || (same && rank < need)));
-        const int at = block_prefix(take ? 1 : 0, s_wave, total) + base;
+        const bool take = i == n - 1 || (i < n - 1 && (high_digits > prefix || (same && rank < need)));
+        const int at = count_before(take, s_wave, total) + base;
         base += total;
         if (take && at < p.top) selected[at] = i, pages[at] = table[i];
     }
