@@ -589,12 +589,16 @@ int int8k_qk_norm_rope_append(const void* x, int dtype, const float* cos, const 
  * then the nodes).  A page id outside [0, num_pages) reads page num_pages-1 and is counted
  * (int8k_paged_bad_ids); entries past a sequence's last position are never read.  nodes at most
  * 256, max_context at most 2^30, B*heads*nodes below 2^24 (else INT8K_ERR_UNSUPPORTED).  Q
- * 16-byte, out 8-byte aligned.  The workspace (16-byte aligned) holds partial states; one of the
- * queried size serves every call of up to B*nodes tokens with the same heads, whatever its
- * max_context.  How a sequence is split, and so the order of its fp32 sums, follows B, nodes and
- * max_context: under others a result agrees within the rounding of those sums, not bit for bit. */
+ * 16-byte, out 8-byte aligned.  The workspace (16-byte aligned) holds partial states: one of
+ * int8k_tree_attention_paged_workspace_bytes serves every call of up to B*nodes tokens with the
+ * same heads, whatever its max_context; _call_workspace_bytes is what a call of exactly these
+ * sizes needs (0: none), for callers that allocate per call.  How a sequence is split, and so the
+ * order of its fp32 sums, follows B, nodes, max_context and the lengths of the batch: under others
+ * a result agrees within the rounding of those sums, not bit for bit. */
 size_t int8k_tree_attention_paged_workspace_bytes(int B, int heads, int kv_heads, int nodes,
                                                   int max_context, int head_dim);
+size_t int8k_tree_attention_paged_call_workspace_bytes(int B, int heads, int kv_heads, int nodes,
+                                                       int max_context, int head_dim);
 
 int int8k_tree_attention_forward_paged(
     const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
@@ -641,12 +645,16 @@ int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages, const int3
  * sequence's last block are not read.  Page ids outside [0, num_pages) read page num_pages-1 and
  * are counted (int8k_paged_bad_ids); entries past a sequence's last block are never read.
  * max_context at most 2^30, B*kv_heads at most 65535 (else INT8K_ERR_UNSUPPORTED).  The workspace
- * (16-byte aligned) holds scores, the selection and partial states; one of the queried size serves
- * every call of up to B sequences, max_context positions and top_pages blocks with the same heads
- * and page size.  Splits as for the tree. */
+ * (16-byte aligned) holds scores, the selection and partial states: one of
+ * int8k_decode_attention_paged_sparse_workspace_bytes serves every call of up to B sequences,
+ * max_context positions and top_pages blocks with the same heads and page size;
+ * _call_workspace_bytes is what a call of exactly these sizes needs.  Splits as for the tree. */
 size_t int8k_decode_attention_paged_sparse_workspace_bytes(int B, int heads, int kv_heads,
                                                            int max_context, int page_size,
                                                            int top_pages, int head_dim);
+size_t int8k_decode_attention_paged_sparse_call_workspace_bytes(int B, int heads, int kv_heads,
+                                                                int max_context, int page_size,
+                                                                int top_pages, int head_dim);
 
 int int8k_decode_attention_forward_paged_sparse(
     const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,

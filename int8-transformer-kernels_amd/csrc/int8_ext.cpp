@@ -1287,7 +1287,7 @@ torch::Tensor int8_tree_attention_forward_paged_torch(
                         torch::kFloat16, Q);
     const int b = as_int(B, "batch"), h = as_int(H, "heads"), top = as_int(max_context, "max_context");
     const size_t ws_bytes =
-        int8k_tree_attention_paged_workspace_bytes(b, h, d.kv_heads, (int)N, top, d.head_dim);
+        int8k_tree_attention_paged_call_workspace_bytes(b, h, d.kv_heads, (int)N, top, d.head_dim);
     auto ws = workspace(ws_bytes, Q.device());
     check_status(int8k_tree_attention_forward_paged(
                      q.data_ptr<int8_t>(), K_pages.data_ptr<int8_t>(), V_pages.data_ptr<int8_t>(),
@@ -1371,7 +1371,7 @@ std::tuple<torch::Tensor, torch::Tensor> int8_decode_attention_forward_paged_spa
     const int b = as_int(B, "batch"), h = as_int(H, "heads"),
               top = as_int(max_context, "max_context"), n = as_int(top_pages, "top_pages");
     auto which = empty_on({B, d.kv_heads, top_pages}, torch::kInt32, Q);
-    const size_t ws_bytes = int8k_decode_attention_paged_sparse_workspace_bytes(
+    const size_t ws_bytes = int8k_decode_attention_paged_sparse_call_workspace_bytes(
         b, h, d.kv_heads, top, d.page, n, d.head_dim);
     auto ws = workspace(ws_bytes, Q.device());
     check_status(int8k_decode_attention_forward_paged_sparse(

@@ -676,37 +676,39 @@ struct AttendPlan {
 };
 
 constexpr int kMaxSplit = 64;      // pieces per sequence, on average
-constexpr int kMaxBlocks = 1024;   // of a cut: four rounds of 256 CUs
+constexpr int kMaxBlocks = 2048;   // of a cut: four rounds
 
 // rows: query rows per key head.
 // Two fragments share a tile's loads and conversions where one alone would leave a block to half of
 // the CUs anyhow (us with one / two: 16 sequences of 8192 x 32 rows x 8 heads 59 / 53; 2 of 4096 x
 // 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).
-// A CU runs one block of 8 waves at a time.  The number of pieces is the one with the least estimated time
-// (0.01 us): a round of blocks costs 4 us and 1.1 us per tile of a wave with one fragment, 1.9 with
-// two (0.8 and 1.3 at head dim 64); the join of pieces 6 us; lengths are taken to be 3/4 of
-// max_context in the mean, which a sequence in one piece does not profit from.  Estimated /
-// measured, us: 16 sequences of 8192, 64 rows, one piece each 65 / 68, two 74 / 80; 13 of 3001, 12
-// heads of 64 13 / 17, cut 15 / 20; 8 of 8192, 16 heads of 64 in one piece 30 / 36, in two 23 / 29;
-// 1 of 1000, 20 rows 8 / 12, cut 14 / 12; 4 of 4096, 32 rows 22 / 27, cut 15 / 19.
+// A CU runs one block of 8 waves at a time, two where a wave takes at most 128 registers (one
+// fragment at head dim 64).  The number of pieces is the one with the least estimated
+// time (0.01 us) for sequences of max_context: a round of blocks costs 8 us and 1.1 us per tile of
+// a wave with one fragment, 1.9 with two (0.8 and 1.3 at head dim 64), the join of pieces 8 us.
+// Sequences that are much shorter gain little by more pieces: the long ones then share memory with
+// fewer.  Measured, us, one piece each / cut, the chosen one first: 16 of up to 8192, 64 rows 68 / 74; 4
+// of up to 16384, 256 rows 115 / 125; 13 of 3001, 12 heads of 64 17 / 20; 1 of 1000, 20 rows 12 / 12;
+// cut / one piece each: 8 of up to 8192, 16 heads of 64 29 / 36; 16 of 8192, 32 rows 53 / 68; 4 of
+// 4096, 32 rows 19 / 27; 8 of 16384, 4 rows 47 / 105.
 AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
-    constexpr int kCus = 256;
     AttendPlan pl{};
     pl.waves = 8;
     pl.min_tiles = pl.waves;
-    pl.frags = rows > 16 && (long long)B * Hkv * ceil_div(rows, 16) >= kCus / 2 ? 2 : 1;
+    pl.frags = rows > 16 && (long long)B * Hkv * ceil_div(rows, 16) >= 128 ? 2 : 1;
     pl.groups = (rows + 16 * pl.frags - 1) / (16 * pl.frags);
     const long long heads = (long long)Hkv * pl.groups;  // blocks per piece
     const long long tiles = ceil_div(context, kTile);
+    const int at_once = D == 64 && pl.frags == 1 ? 512 : 256;
     const long long tile_time = pl.frags == 1 ? (D == 64 ? 80 : 110) : (D == 64 ? 130 : 190);
-    auto round = [&](long long t) { return 400 + ceil_div(t, pl.waves) * tile_time; };
-    long long best = ceil_div(B * heads, kCus) * round(tiles);
+    auto round = [&](long long t) { return 800 + ceil_div(t, pl.waves) * tile_time; };
+    long long best = ceil_div(B * heads, at_once) * round(tiles);
     for (int rounds = 1; rounds <= 4; ++rounds) {
-        const long long pieces = std::min<long long>({(long long)kMaxSplit * B, rounds * kCus / heads,
+        const long long pieces = std::min<long long>({(long long)kMaxSplit * B, rounds * at_once / heads,
                                                       B * ceil_div(tiles, pl.min_tiles)});
         // (the sum of all tiles is an int)
         if (pieces <= B || B * tiles >= (1LL << 31)) continue;
-        const long long time = ceil_div(pieces * heads, kCus) * round(ceil_div(3 * B * tiles, 4 * pieces)) + 600;
+        const long long time = ceil_div(pieces * heads, at_once) * round(ceil_div(B * tiles, pieces)) + 800;
         if (time < best) best = time, pl.pieces = (int)pieces;
     }
     return pl;
@@ -785,14 +787,34 @@ int attend_bad_ids(unsigned int* count) {
 
 using namespace int8k;
 
+namespace {
+bool tree_query_ok(int B, int heads, int kv_heads, int nodes, int max_context, int head_dim) {
+    return B > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && nodes > 0 &&
+           nodes <= kMaxNodes && max_context > 0 && (head_dim == 64 || head_dim == 128) &&
+           (long long)B * heads * nodes < (1LL << 24);
+}
+bool sparse_query_ok(int B, int heads, int kv_heads, int max_context, int page_size, int top_pages,
+                     int head_dim) {
+    return B > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && max_context > 0 &&
+           max_context <= (1 << 30) && page_size >= 16 && page_size <= 1024 &&
+           (page_size & (page_size - 1)) == 0 && top_pages > 0 &&
+           (head_dim == 64 || head_dim == 128) && (long long)B * heads < (1LL << 24);
+}
+}  // namespace
+
 extern "C" size_t int8k_tree_attention_paged_workspace_bytes(int B, int heads, int kv_heads,
                                                              int nodes, int max_context,
                                                              int head_dim) {
-    if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || nodes <= 0 ||
-        nodes > kMaxNodes || max_context <= 0 || (head_dim != 64 && head_dim != 128) ||
-        (long long)B * heads * nodes >= (1LL << 24))
-        return 0;
+    if (!tree_query_ok(B, heads, kv_heads, nodes, max_context, head_dim)) return 0;
     return most_partials((size_t)B * heads * nodes, head_dim).bytes;
+}
+
+extern "C" size_t int8k_tree_attention_paged_call_workspace_bytes(int B, int heads, int kv_heads,
+                                                                  int nodes, int max_context,
+                                                                  int head_dim) {
+    if (!tree_query_ok(B, heads, kv_heads, nodes, max_context, head_dim)) return 0;
+    const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context, head_dim);
+    return plan_partials(pl, B, (size_t)heads * nodes, head_dim).bytes;
 }
 
 extern "C" int int8k_tree_attention_forward_paged(
@@ -841,18 +863,20 @@ extern "C" int int8k_tree_attention_forward_paged(
     return run_attend(p, pl, head_dim, workspace, as_stream(stream));
 }
 
-extern "C" size_t int8k_decode_attention_paged_sparse_workspace_bytes(int B, int heads,
-                                                                      int kv_heads,
-                                                                      int max_context,
-                                                                      int page_size, int top_pages,
-                                                                      int head_dim) {
-    if (B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_context <= 0 ||
-        page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) || top_pages <= 0 ||
-        (head_dim != 64 && head_dim != 128) || (long long)B * heads >= (1LL << 24) ||
-        max_context > (1 << 30))
-        return 0;
-    const SelectSpace sel = select_space(B, kv_heads, max_context, page_size, top_pages);
-    return sel.bytes + most_partials((size_t)B * heads, head_dim).bytes;
+extern "C" size_t int8k_decode_attention_paged_sparse_workspace_bytes(
+    int B, int heads, int kv_heads, int max_context, int page_size, int top_pages, int head_dim) {
+    if (!sparse_query_ok(B, heads, kv_heads, max_context, page_size, top_pages, head_dim)) return 0;
+    return select_space(B, kv_heads, max_context, page_size, top_pages).bytes +
+           most_partials((size_t)B * heads, head_dim).bytes;
+}
+
+extern "C" size_t int8k_decode_attention_paged_sparse_call_workspace_bytes(
+    int B, int heads, int kv_heads, int max_context, int page_size, int top_pages, int head_dim) {
+    if (!sparse_query_ok(B, heads, kv_heads, max_context, page_size, top_pages, head_dim)) return 0;
+    const int context = (int)std::min<long long>(max_context, (long long)top_pages * page_size);
+    const AttendPlan pl = attend_plan(B, heads / kv_heads, kv_heads, context, head_dim);
+    return select_space(B, kv_heads, max_context, page_size, top_pages).bytes +
+           plan_partials(pl, B, (size_t)heads, head_dim).bytes;
 }
 
 extern "C" int int8k_decode_attention_forward_paged_sparse(

@@ -82,11 +82,13 @@ _SIGNATURES = {
     "int8k_qk_norm_rope_append": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P, _F] + [_P] * 7 +
                                   [_I] * 8 + [_P]),
     "int8k_tree_attention_paged_workspace_bytes": (_SZ, [_I] * 6),
+    "int8k_tree_attention_paged_call_workspace_bytes": (_SZ, [_I] * 6),
     "int8k_tree_attention_forward_paged": (_I, [_P] * 10 + [_I, _LL, _P] + [_I] * 10 +
                                            [_P, _SZ, _P]),
     "int8k_kv_cache_move_paged": (_I, [_P] * 6 + [_I] * 6 + [_P]),
     "int8k_kv_page_means": (_I, [_P] * 5 + [_I] * 5 + [_P]),
     "int8k_decode_attention_paged_sparse_workspace_bytes": (_SZ, [_I] * 7),
+    "int8k_decode_attention_paged_sparse_call_workspace_bytes": (_SZ, [_I] * 7),
     "int8k_decode_attention_forward_paged_sparse": (_I, [_P] * 12 + [_I] * 9 + [_P, _SZ, _P]),
     "int8k_paged_bad_ids": (_I, [ctypes.POINTER(ctypes.c_uint)]),
 }
@@ -712,8 +714,15 @@ def qk_norm_rope_append(x, heads, kv_heads, cos, sin, positions, K_pages, V_page
 
 
 def tree_attention_paged_workspace_bytes(B, heads, kv_heads, nodes, max_context, D):
+    """Serves every call of up to B * nodes tokens with the same heads."""
     return load().int8k_tree_attention_paged_workspace_bytes(B, heads, kv_heads, nodes,
                                                              max_context, D)
+
+
+def tree_attention_paged_call_workspace_bytes(B, heads, kv_heads, nodes, max_context, D):
+    """What a call of exactly these sizes needs."""
+    return load().int8k_tree_attention_paged_call_workspace_bytes(B, heads, kv_heads, nodes,
+                                                                  max_context, D)
 
 
 def tree_attention_paged(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, block_tables, context_lens,
@@ -729,7 +738,7 @@ def tree_attention_paged(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, block_tab
         out = torch.empty((B, N, H, D) if out_bshd else (B, H, N, D), dtype=torch.float16,
                           device=Qi.device)
     if workspace is None:
-        n = tree_attention_paged_workspace_bytes(B, H, Hkv, N, max_context, D)
+        n = tree_attention_paged_call_workspace_bytes(B, H, Hkv, N, max_context, D)
         workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=Qi.device)
     words = tree_mask.shape[-1] if tree_mask is not None else 0
     each = N * words if tree_mask is not None and tree_mask.dim() == 3 else 0
@@ -759,7 +768,14 @@ def kv_page_means(K_pages, sK_pages, page_ids, K_means, sK_means):
 
 
 def decode_paged_sparse_workspace_bytes(B, heads, kv_heads, max_context, page, top_pages, D):
+    """Serves every call of up to B sequences, max_context positions and top_pages blocks."""
     return load().int8k_decode_attention_paged_sparse_workspace_bytes(
+        B, heads, kv_heads, max_context, page, top_pages, D)
+
+
+def decode_paged_sparse_call_workspace_bytes(B, heads, kv_heads, max_context, page, top_pages, D):
+    """What a call of exactly these sizes needs."""
+    return load().int8k_decode_attention_paged_sparse_call_workspace_bytes(
         B, heads, kv_heads, max_context, page, top_pages, D)
 
 
@@ -776,7 +792,7 @@ def decode_attention_paged_sparse(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, 
         out = torch.empty((B, H, D), dtype=torch.float16, device=Qi.device)
     which = torch.empty((B, Hkv, top_pages), dtype=torch.int32, device=Qi.device)
     if workspace is None:
-        n = decode_paged_sparse_workspace_bytes(B, H, Hkv, max_context, P, top_pages, D)
+        n = decode_paged_sparse_call_workspace_bytes(B, H, Hkv, max_context, P, top_pages, D)
         workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=Qi.device)
     check("int8k_decode_attention_forward_paged_sparse",
           load().int8k_decode_attention_forward_paged_sparse(

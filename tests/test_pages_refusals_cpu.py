@@ -96,6 +96,7 @@ def test_counter_refuses_null(capi):
 @pytest.mark.parametrize("D", [64, 128])
 def test_a_workspace_serves_smaller_calls(capi, H, Hkv, D):
     tree, sparse = capi.tree_attention_paged_workspace_bytes, capi.decode_paged_sparse_workspace_bytes
+    tree_call, sparse_call = capi.tree_attention_paged_call_workspace_bytes, capi.decode_paged_sparse_call_workspace_bytes
     for B, N, L in ((8, 16, 4000), (64, 64, 100000), (1, 256, 20)):
         big = tree(B, H, Hkv, N, L, D)
         for b in {1, 2, 3, 5, B // 2, B} - {0}:
@@ -103,22 +104,24 @@ def test_a_workspace_serves_smaller_calls(capi, H, Hkv, D):
                 for l in (1, 333, 5000, 200000):
                     if b <= B:
                         assert tree(b, H, Hkv, n, l, D) <= big
+                        assert tree_call(b, H, Hkv, n, l, D) <= big
     for B, L, top in ((8, 4000, 10), (64, 100000, 64)):
         big = sparse(B, H, Hkv, L, 64, top, D)
         for b in (1, 3, B):
             for l in (1, 333, L):
                 for k in (1, 7, top):
                     assert sparse(b, H, Hkv, l, 64, k, D) <= big
+                    assert 0 < sparse_call(b, H, Hkv, l, 64, k, D) <= big
 
 
 def test_workspace_queries_of_bad_arguments_are_0(capi):
     tree, sparse = capi.tree_attention_paged_workspace_bytes, capi.decode_paged_sparse_workspace_bytes
     for a in ((0, 8, 2, 4, 100, 64), (1, 8, 3, 4, 100, 64), (1, 8, 2, 0, 100, 64), (1, 8, 2, 257, 100, 64), (1, 8, 2, 4, 0, 64),
               (1, 8, 2, 4, 100, 96), (1 << 20, 8, 2, 4, 100, 64)):
-        assert tree(*a) == 0
+        assert tree(*a) == 0 and capi.tree_attention_paged_call_workspace_bytes(*a) == 0
     for a in ((0, 8, 2, 100, 16, 4, 64), (1, 8, 3, 100, 16, 4, 64), (1, 8, 2, 0, 16, 4, 64), (1, 8, 2, 100, 24, 4, 64),
               (1, 8, 2, 100, 16, 0, 64), (1, 8, 2, 100, 16, 4, 80)):
-        assert sparse(*a) == 0
+        assert sparse(*a) == 0 and capi.decode_paged_sparse_call_workspace_bytes(*a) == 0
 
 
 def test_torch_ops_refuse_cpu_tensors(ext):

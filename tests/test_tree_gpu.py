@@ -79,7 +79,7 @@ def test_any_mask_bits(ext, gpu):
 
 
 @pytest.mark.parametrize("B,N,H,Hkv,D,L", [(1, 5, 8, 8, 128, 20001), (2, 16, 4, 1, 64, 9000), (1, 1, 2, 1, 64, 70000),
-                                           (40, 4, 4, 2, 128, 300), (3, 32, 12, 2, 128, 5000), (1, 256, 16, 2, 64, 3000)])
+                                           (40, 4, 4, 2, 128, 300), (130, 1, 2, 1, 64, 5000), (70, 2, 3, 3, 128, 2600), (3, 32, 12, 2, 128, 5000), (1, 256, 16, 2, 64, 3000)])
 def test_long_and_wide(ext, gpu, B, N, H, Hkv, D, L):
     c = tree_case(L + B, [max(1, L - 37 * b) for b in range(B)], N, H, Hkv, D, 32, gpu)
     _check(c, _run(ext, c))
