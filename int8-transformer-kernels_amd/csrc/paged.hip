@@ -298,8 +298,8 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     bool bad = false;
 
     // The two runs of 16 rows of tile t: their page ids (a page holds whole runs; entries past
-    // the last position are not read), and from those the first row of each.  Past the last tile
-    // ids and rows stay as they are.
+    // the last position are not read), and from those their numbers in the cache (below 2^32 by
+    // check_pages).  Past the last tile both stay as they are.
     const bool two_pages = p.log2_page == 4;
     int id[2] = {0, 0};
     auto fetch_ids = [&](int t) {
@@ -308,24 +308,24 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
         if (two_pages) id[1] = table[min(t * kTile + 16, e.total - 1) >> p.log2_page];
     };
     struct Rows {
-        size_t first[2];
+        uint32_t run[2];
     };
     auto rows_of_ids = [&](int t, Rows& rows) {
         if (t >= t_end) return;
-        auto first = [&](int raw, int key) {
-            const int page = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
-            bad = bad || page != raw;
-            return (((size_t)page * p.Hkv + kvh) << p.log2_page) + (size_t)(key & pmask);
+        auto run = [&](int raw, int key) {
+            const uint32_t page = min((uint32_t)raw, (uint32_t)(p.num_pages - 1));
+            bad = bad || page != (uint32_t)raw;
+            return ((page * (uint32_t)p.Hkv + (uint32_t)kvh) << (p.log2_page - 4)) + ((uint32_t)(key & pmask) >> 4);
         };
-        rows.first[0] = first(__builtin_amdgcn_readfirstlane(id[0]), t * kTile);
-        rows.first[1] = rows.first[0] + 16;
-        if (two_pages) rows.first[1] = first(__builtin_amdgcn_readfirstlane(id[1]), t * kTile + 16);
+        rows.run[0] = run(__builtin_amdgcn_readfirstlane(id[0]), t * kTile);
+        rows.run[1] = rows.run[0] + 1;
+        if (two_pages) rows.run[1] = run(__builtin_amdgcn_readfirstlane(id[1]), t * kTile + 16);
     };
     v4i k_raw[2][KI], k[2][KI];  // a tile's rows as loaded, and as the MFMA takes them
     auto load_k = [&](const Rows& rows) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const __amdgpu_buffer_rsrc_t kb = make_buffer(p.K + rows.first[h] * D, 16 * D);
+            const __amdgpu_buffer_rsrc_t kb = make_buffer(p.K + (size_t)rows.run[h] * (16 * D), 16 * D);
 #pragma unroll
             for (int i = 0; i < KI; ++i)
                 k_raw[h][i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kb, lane * 16, 1024 * i, 0));
@@ -350,8 +350,8 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     auto load_v = [&](Tile& r, const Rows& rows) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const size_t row = rows.first[h];
-            const __amdgpu_buffer_rsrc_t vb = make_buffer(p.V + row * D, 16 * D);
+            const size_t run = rows.run[h];
+            const __amdgpu_buffer_rsrc_t vb = make_buffer(p.V + run * (16 * D), 16 * D);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (D == 128) {
@@ -362,9 +362,9 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
                 }
             }
             r.sk[h] = __builtin_bit_cast(
-                float, __builtin_amdgcn_raw_buffer_load_b32(make_buffer(p.sK + row, 64), s_off, 0, 0));
+                float, __builtin_amdgcn_raw_buffer_load_b32(make_buffer(p.sK + run * 16, 64), s_off, 0, 0));
             r.sv[h] = __builtin_bit_cast(
-                float, __builtin_amdgcn_raw_buffer_load_b32(make_buffer(p.sV + row, 64), s_off, 0, 0));
+                float, __builtin_amdgcn_raw_buffer_load_b32(make_buffer(p.sV + run * 16, 64), s_off, 0, 0));
         }
     };
 
@@ -683,14 +683,15 @@ constexpr int kMaxBlocks = 2048;   // of a cut: four rounds
 // the CUs anyhow (us with one / two: 16 sequences of 8192 x 32 rows x 8 heads 59 / 53; 2 of 4096 x
 // 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).
 // A CU runs one block of 8 waves at a time, two where a wave takes at most 128 registers (one
-// fragment at head dim 64).  The number of pieces is the one with the least estimated
-// time (0.01 us) for sequences of max_context: a round of blocks costs 8 us and 1.1 us per tile of
-// a wave with one fragment, 1.9 with two (0.8 and 1.3 at head dim 64), the join of pieces 8 us.
-// Sequences that are much shorter gain little by more pieces: the long ones then share memory with
-// fewer.  Measured, us, one piece each / cut, the chosen one first: 16 of up to 8192, 64 rows 68 / 74; 4
-// of up to 16384, 256 rows 115 / 125; 13 of 3001, 12 heads of 64 17 / 20; 1 of 1000, 20 rows 12 / 12;
-// cut / one piece each: 8 of up to 8192, 16 heads of 64 29 / 36; 16 of 8192, 32 rows 53 / 68; 4 of
-// 4096, 32 rows 19 / 27; 8 of 16384, 4 rows 47 / 105.
+// fragment at head dim 64).  The number of pieces is the one with the least estimated time (0.01 us)
+// for sequences of max_context: a round of blocks costs 7 us and 1.1 us per tile of a wave with one
+// fragment, 1.9 with two (at head dim 64 0.8, 1.3 where two blocks share a CU, and 1.3), the join of
+// pieces 5 us.  Sequences that are much shorter gain little by more pieces: the long ones then share
+// memory with fewer.  Measured, us, the chosen one first: in one piece each / cut 16 of up to 8192,
+// 64 rows 68 / 74; 4 of up to 16384, 256 rows 115 / 125; 13 of up to 3001, 12 heads of 64 17 / 20; 1 of
+// 1000, 20 rows 12 / 12; cut / in one piece 8 of up to 8192, 16 heads of 64 29 / 36; 16 of up to 8192,
+// 32 rows 53 / 68; 4 of up to 4096, 32 rows 19 / 27; 8 of up to 16384, 4 rows 47 / 105; 1 of 2048, 4
+// rows 13 / 15.
 AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
     AttendPlan pl{};
     pl.waves = 8;
@@ -699,16 +700,18 @@ AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
     pl.groups = (rows + 16 * pl.frags - 1) / (16 * pl.frags);
     const long long heads = (long long)Hkv * pl.groups;  // blocks per piece
     const long long tiles = ceil_div(context, kTile);
-    const int at_once = D == 64 && pl.frags == 1 ? 512 : 256;
-    const long long tile_time = pl.frags == 1 ? (D == 64 ? 80 : 110) : (D == 64 ? 130 : 190);
-    auto round = [&](long long t) { return 800 + ceil_div(t, pl.waves) * tile_time; };
-    long long best = ceil_div(B * heads, at_once) * round(tiles);
+    const bool two = D == 64 && pl.frags == 1;  // blocks per CU
+    auto time_of = [&](long long blocks, long long t) {
+        const long long tile = two ? (blocks > 256 ? 130 : 80) : pl.frags == 1 ? 110 : D == 64 ? 130 : 190;
+        return ceil_div(blocks, two ? 512 : 256) * (700 + ceil_div(t, pl.waves) * tile);
+    };
+    long long best = time_of(B * heads, tiles);
     for (int rounds = 1; rounds <= 4; ++rounds) {
-        const long long pieces = std::min<long long>({(long long)kMaxSplit * B, rounds * at_once / heads,
+        const long long pieces = std::min<long long>({(long long)kMaxSplit * B, rounds * (two ? 512 : 256) / heads,
                                                       B * ceil_div(tiles, pl.min_tiles)});
         // (the sum of all tiles is an int)
         if (pieces <= B || B * tiles >= (1LL << 31)) continue;
-        const long long time = ceil_div(pieces * heads, at_once) * round(ceil_div(B * tiles, pieces)) + 800;
+        const long long time = time_of(pieces * heads, ceil_div(B * tiles, pieces)) + 500;
         if (time < best) best = time, pl.pieces = (int)pieces;
     }
     return pl;

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void move_rows_kernel(Move p) {
 // int8k_quantize_per_token does; a NaN in a mean makes the scale NaN.
 
 // One wave per page and key head up to 64 rows (four waves of a few rows each spend more on joining
-// their sums than on the rows: 2048 pages of 64 rows, 8 heads of 128, 84 us, MEANS so), two or four
+// their sums than on the rows: 2048 pages of 64 rows, 8 heads of 128, 84 us, 33 so), two or four
 // for longer pages.  A lane owns 16 dims of every 64 / L-th row and loads four rows ahead.
 
 // a of this lane plus a of the lane 32 (16) away where the lane is in the lower half of 64 (32), the
@@ -217,33 +217,38 @@ __device__ __forceinline__ uint64_t score_key(double s) {
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// The keys of the scored blocks first, first + each, .. (EACH of them, those below n - 1) for one
-// sequence and key head by a group of D / 16 lanes, which hold 16 dims each: put(k, block, key) on
-// every lane of the group.
-template <int D, int EACH, typename Put>
-__device__ __forceinline__ void score_blocks(const Select& p, int b, int h, int n, int first, int each,
-                                             Put&& put) {
-    constexpr int L = D / 16;
-    const int c = threadIdx.x % L, G = p.Hq / p.Hkv;
+// A group of D / 16 lanes, which hold 16 dims each, scores kEach blocks.  (In the selection's block,
+// which spares a launch: 40.2 against 41.4 us for 32 sequences of 512 blocks, 27.5 against 23.9 for one
+// of 1024, 42 against 22 for one of 4096.)
+template <int D>
+__global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
+    constexpr int L = D / 16, kRows = 256 / L, kEach = 2;
     constexpr int kHeads = 4;  // whose queries are loaded at a time, the first with the means
-    v4i mean[EACH], q[kHeads];
-    double sm[EACH], best[EACH], sq[kHeads];
-    bool any[EACH];
+    const int row = blockIdx.y, b = row / p.Hkv, h = row % p.Hkv, G = p.Hq / p.Hkv;
+    const int base = blockIdx.x * (kRows * kEach), first = base + threadIdx.x / L, c = threadIdx.x % L;
+    v4i q[kHeads];
+    double sq[kHeads];
     auto load_heads = [&](int g0) {
 #pragma unroll
         for (int g = 0; g < kHeads; ++g) {
-            const size_t row = (size_t)b * p.Hq + h * G + min(g0 + g, G - 1);
-            q[g] = *reinterpret_cast<const v4i*>(p.Q + row * D + 16 * c);
-            sq[g] = (double)p.sQ[row];
+            const size_t at = (size_t)b * p.Hq + h * G + min(g0 + g, G - 1);
+            q[g] = *reinterpret_cast<const v4i*>(p.Q + at * D + 16 * c);
+            sq[g] = (double)p.sQ[at];
         }
     };
     load_heads(0);
+    int len;
+    const int n = blocks_of(p, b, len);
+    if (n <= p.top || base >= n - 1) return;  // all are taken, or none is here
+    v4i mean[kEach];
+    double sm[kEach], best[kEach];
+    bool any[kEach];
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-        const int i = min(first + k * each, n - 2);  // blocks past the last repeat it
+    for (int k = 0; k < kEach; ++k) {
+        const int i = min(first + k * kRows, n - 2);  // blocks past the last repeat it
         const int raw = p.tables[(size_t)b * p.max_pages + i];
         const int id = (int)min((unsigned)raw, (unsigned)(p.num_pages - 1));
-        if (id != raw && h == 0 && c == 0 && first + k * each < n - 1) atomicAdd(&g_pages_bad_ids, 1u);
+        if (id != raw && h == 0 && c == 0 && first + k * kRows < n - 1) atomicAdd(&g_pages_bad_ids, 1u);
         const size_t unit = (size_t)id * p.Hkv + h;
         mean[k] = *reinterpret_cast<const v4i*>(p.means + unit * D + 16 * c);
         sm[k] = (double)p.s_means[unit];
@@ -255,7 +260,7 @@ __device__ __forceinline__ void score_blocks(const Select& p, int b, int h, int 
 #pragma unroll
         for (int g = 0; g < kHeads; ++g) {  // (heads past the last repeat it)
 #pragma unroll
-            for (int k = 0; k < EACH; ++k) {
+            for (int k = 0; k < kEach; ++k) {
                 int dot = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) dot = __builtin_amdgcn_sdot4(q[g][i], mean[k][i], dot, false);
@@ -267,21 +272,10 @@ __device__ __forceinline__ void score_blocks(const Select& p, int b, int h, int 
         }
     }
 #pragma unroll
-    for (int k = 0; k < EACH; ++k)
-        if (first + k * each < n - 1) put(first + k * each, any[k] ? score_key(best[k]) : 0);
-}
-
-// Scores by blocks of their own, for long contexts of few sequences.
-template <int D>
-__global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
-    constexpr int L = D / 16, kRows = 256 / L, kEach = 2;
-    const int row = blockIdx.y, b = row / p.Hkv, h = row % p.Hkv;
-    int len;
-    const int n = blocks_of(p, b, len), base = blockIdx.x * (kRows * kEach);
-    if (n <= p.top || base >= n - 1) return;  // all are taken, or none is here
-    score_blocks<D, kEach>(p, b, h, n, base + threadIdx.x / L, kRows, [&](int i, uint64_t key) {
-        if (threadIdx.x % L == 0) p.keys[(size_t)row * p.max_blocks + i] = key;
-    });
+    for (int k = 0; k < kEach; ++k) {
+        const int i = first + k * kRows;
+        if (c == 0 && i < n - 1) p.keys[(size_t)row * p.max_blocks + i] = any[k] ? score_key(best[k]) : 0;
+    }
 }
 
 constexpr int kSelectThreads = 1024;
@@ -334,12 +328,9 @@ __device__ __forceinline__ void find_bin(const int* s_count, int need, int& s_bi
 // lies in are ranked among each other.  Where that does not do (an infinite or NaN score, all equal,
 // a bin of more than kList), by digits of 8 bits of the keys from the highest, until all keys that
 // share the digits of the last taken one so far are taken.
-// Where the keys fit LDS and the scores are soon worked out, the block does that itself (SCORE).
 constexpr int kList = 256;
 
-template <int D, bool SCORE>
 __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p) {
-    extern __shared__ uint64_t s_keys[];
     __shared__ int s_count[256], s_wave[kSelectThreads / 64], s_bin, s_above, s_listed;
     __shared__ float s_low[kSelectThreads / 64], s_high[kSelectThreads / 64];
     __shared__ uint64_t s_key[kList];
@@ -359,15 +350,6 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
         return;
     }
     const uint64_t* keys = p.keys + (size_t)row * p.max_blocks;
-    if constexpr (SCORE) {
-        constexpr int L = D / 16, kRows = kSelectThreads / L, kEach = 4;
-        for (int i = t / L; i < n - 1; i += kRows * kEach)
-            score_blocks<D, kEach>(p, b, row % p.Hkv, n, i, kRows, [&](int at, uint64_t key) {
-                if (t % L == 0) s_keys[at] = key;
-            });
-        keys = s_keys;
-        __syncthreads();
-    }
     int need = p.top - 1;
     auto emit = [&](auto takes) {  // the taken blocks in order
         int base = 0;
@@ -465,25 +447,16 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
 
 }  // namespace
 
-constexpr int kFusedBlocks = 1024;
-
 int launch_select(const Select& s, hipStream_t stream) {
     const int rows = s.B * s.Hkv;
-    // one kernel up to a few rounds of scores per block, more where the rows fill the GPU anyhow
-    const bool fused = s.max_blocks <= s.top || s.max_blocks <= kFusedBlocks ||
-                       (rows >= 128 && s.max_blocks <= 4 * kFusedBlocks);
-    if (!fused) {
+    if (s.max_blocks > s.top) {
         const int per = 256 / (s.D / 16) * 2;
         const dim3 grid((unsigned)ceil_div(s.max_blocks, per), (unsigned)rows);
         if (s.D == 64) block_scores_kernel<64><<<grid, 256, 0, stream>>>(s);
         else block_scores_kernel<128><<<grid, 256, 0, stream>>>(s);
         if (const int st = check_launch("block_scores_kernel")) return st;
-        select_blocks_kernel<64, false><<<(unsigned)rows, kSelectThreads, 0, stream>>>(s);
-    } else {
-        const size_t lds = s.max_blocks > s.top ? (size_t)s.max_blocks * sizeof(uint64_t) : 0;
-        if (s.D == 64) select_blocks_kernel<64, true><<<(unsigned)rows, kSelectThreads, lds, stream>>>(s);
-        else select_blocks_kernel<128, true><<<(unsigned)rows, kSelectThreads, lds, stream>>>(s);
     }
+    select_blocks_kernel<<<(unsigned)rows, kSelectThreads, 0, stream>>>(s);
     return check_launch("select_blocks_kernel");
 }
 
