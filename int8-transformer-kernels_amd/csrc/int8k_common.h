@@ -176,39 +176,6 @@ __device__ __forceinline__ uint32_t biased_bytes_to_f16x2(uint32_t w0x, uint32_t
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// A buffer descriptor whose loads convert: data format 8_8_8_8 with numeric
-// format SSCALED turns each byte into the float of its signed value, and the
-// d16 variant of the format load packs the four as fp16.  So V arrives as exact
-// fp16 with no VALU work.  Offsets at or past `bytes` read as zero.
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ i32x4 make_v_descriptor(const void* base, uint32_t bytes) {
-    constexpr uint32_t kDstSelXYZW = 4 | (5 << 3) | (6 << 6) | (7 << 9);
-    constexpr uint32_t kNumFormatSscaled = 3, kDataFormat8888 = 10;
-    const uint64_t b = reinterpret_cast<uint64_t>(base);
-    i32x4 d;
-    d.x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b));
-    d.y = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(b >> 32) & 0xffffu);  // stride 0
-    d.z = __builtin_amdgcn_readfirstlane(bytes);
-    d.w = kDstSelXYZW | (kNumFormatSscaled << 12) | (kDataFormat8888 << 15);
-    return d;
-}
-
-// The LLVM intrinsic behind the typed ("format") raw buffer load, which clang
-// exposes no builtin for; declared by name so the compiler schedules it and
-// tracks its wait counts like any other load.
-typedef _Float16 v4h_t __attribute__((ext_vector_type(4)));
-extern "C" __device__ v4h_t int8k_raw_buffer_load_format_v4f16(i32x4 rsrc, int voffset, int soffset,
-                                                              int aux)
-    __asm("llvm.amdgcn.raw.buffer.load.format.v4f16");
-
-// Four int8 at voff + soff as four fp16, packed {b0, b1} {b2, b3}.
-__device__ __forceinline__ uint2 load_v_f16x4(const i32x4& desc, uint32_t voff, uint32_t soff) {
-    const v4h_t h = int8k_raw_buffer_load_format_v4f16(desc, (int)voff, (int)soff, 0);
-    typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-    const v2u r = __builtin_bit_cast(v2u, h);
-    return make_uint2(r.x, r.y);
-}
-
 // w less half I of t, exactly where t is w rounded to fp16 (one instruction: the compiler widens
 // the half first).
 template <int I, typename H2>

@@ -428,15 +428,16 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
         bool slow = partial;
         if (!partial) {
             float wide = 0.f;
+            bool past = false;
 #pragma unroll
             for (int f = 0; f < F; ++f) {
                 weights(f);
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) wide = fmaxf(wide, fmaxf(fabsf(w[f][j]), fabsf(w[f][j + 1])));
-                // (the first tile, whose m is -inf, has an infinite sum)
-                wide = fmaxf(wide, psum[f] * (kMaxWeight / kMaxSum));
+                // (while m is -inf the sum is infinite, or NaN where a score is -inf too)
+                past = past || !(psum[f] <= kMaxSum);
             }
-            slow = __ballot(wide > kMaxWeight) != 0;
+            slow = __ballot(past || wide > kMaxWeight) != 0;
         }
         if (slow) {
             // the exact maximum, then the largest weight under it

@@ -156,6 +156,19 @@ def test_a_node_reaches_only_the_rows_that_see_it(ext, gpu):
     assert torch.isfinite(out[0, :2]).all() and torch.isfinite(out[0, 2:, [0, 1, 4, 5]]).all()
 
 
+def test_scores_of_minus_infinity_weigh_nothing(ext, gpu):
+    # the first tiles of a wave hold no other
+    c = tree_case(12, [300, 20], 5, 8, 2, 128, 32, gpu)
+    c["Q"] = -c["Q"].abs().clamp(min=1)
+    for pos in list(range(40)) + list(range(256, 288)):
+        p = int(c["tables"][0, pos // 32])
+        c["K"][p, :, pos % 32], c["sK"][p, :, pos % 32] = 1, float("inf")
+    out = _run(ext, c)
+    assert torch.isfinite(out).all()
+    with np.errstate(invalid="ignore"):
+        _check(c, out)
+
+
 @pytest.mark.parametrize("spread", [1e-6, 1e4])
 def test_value_scales_of_very_different_sizes(ext, gpu, spread):
     c = tree_case(10, [500, 900], 12, 8, 2, 128, 32, gpu)
