@@ -15,8 +15,18 @@
 // j = 0..7, as the B operand of the second product wants them: P never changes lanes.  The A
 // operand of that product is 8 keys of one dim per lane: lane l reads D / 16 bytes of those 8
 // rows and picks a byte of two keys at a time (v_perm), which an XOR and a packed addition turn
-// into two fp16.  Every cache row is read and V converted once for all F fragments; no LDS in
-// the loop.
+// into two fp16.  K passes through LDS, where a wave's loads of whole lines become that layout.
+// A wave takes one or two fragments of every 8th tile of a piece of a sequence, and the 8 waves of
+// a block are joined in LDS; or, where a key head has many rows, R = 4 or 8 waves take two
+// fragments each of the same tiles, which they load and convert in turn and share through LDS.
+// Pieces are joined by a second kernel.
+//
+// Bound by memory with one fragment (8 sequences of 16384, one token of 4 heads on 8: 5.2 TB/s) and
+// by the issue of instructions with two: 32 rows x 32 keys take 300 vector instructions (190 with
+// R = 8: V's conversion is shared) beside 44 MFMAs, each of which keeps the SIMD from vector ones
+// for about 10 of its 16 cycles.  16 sequences of up to 8192 with trees of 16, 32 heads on 8 of
+// 128: 67 us (2.6 TB/s, 0.32 PFLOP/s); 4 of 16320 with trees of 64: 104 us (0.41 PFLOP/s; 115 without
+// R = 8).
 //
 // p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
 // that the largest weight p sV of the tile that set it lies in [2^9, 2^10), and a tile whose
@@ -43,6 +53,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 32;               // positions per tile
+constexpr int kWaves = 8;               // per block
 constexpr float kMaxWeight = 60000.f;   // fp16 weights stay below it
 constexpr float kMaxSum = 0x1p60f;      // and the sum of a lane's 8 p below this
 constexpr int kMaxShift = 60;           // |m - running maximum| where m is set
@@ -63,7 +74,7 @@ struct Attend {
     bool bshd;
     float *part_ml, *part_acc;           // [piece][Hq * N][2] and [..][D]
     int B, Hq, Hkv, N, num_pages, log2_page, max_context;
-    int groups;                          // blocks of query rows per key head
+    int groups;                          // blocks per piece and key head
     int pieces, min_tiles;               // see Piece; 0: a sequence is one piece
     int slots;                           // pieces that the grid has room for
     float qk;
@@ -222,17 +233,19 @@ __device__ __forceinline__ uint32_t k_slot(int r, int c) {
     return (r / RP) * 256 + ((r % RP) * C + (c ^ (r / RP % C))) * 16;
 }
 
-template <int D, int F>
+template <int D, int F, int R>
 __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     using Tile = AttendTile<D>;
     constexpr int NF = D / 16;          // fragments of O^T
     constexpr int KI = D / 64;          // loads of 1 KiB per 16 rows
-    constexpr int MR = 16 * F;          // query rows per block
+    constexpr int MR = 16 * F;          // query rows per wave
+    constexpr int BR = MR * R;          // and per block
     constexpr int kORow = D + 4;        // floats per row of O in LDS
     extern __shared__ __align__(16) float s_merge[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nw = blockDim.x >> 6;
+    constexpr int nw = kWaves;
+    const int mine = wave & (R - 1), slice = wave / R;  // which rows of the block's, which of its waves on them
     const int g = lane >> 4, m16 = lane & 15;
 
     // Block -> piece of a sequence, key head and rows of it.  Blocks go to the 8 XCDs in turn; each
@@ -253,7 +266,7 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     }
     const int b = piece.b;
     const int all_rows = p.Hq / p.Hkv * p.N;
-    const int row0_q = grp * MR, rows = min(MR, all_rows - row0_q);
+    const int row0_q = grp * BR, rows = min(BR, all_rows - row0_q);
     const size_t first_row = ((size_t)b * p.Hq + (size_t)kvh * (p.Hq / p.Hkv)) * p.N + row0_q;
     Extent e = extent_of(p, b);
     e.prefix = __builtin_amdgcn_readfirstlane(e.prefix);
@@ -271,8 +284,8 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     int node[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-        const int r = min(16 * f + m16, rows - 1);
-        const bool ok = 16 * f + m16 < rows;
+        const int r = min(MR * mine + 16 * f + m16, rows - 1);
+        const bool ok = MR * mine + 16 * f + m16 < rows;
         node[f] = (row0_q + r) % p.N;
         qs[f] = ok ? p.sQ[first_row + r] * p.qk : 0.f;
 #pragma unroll
@@ -377,9 +390,23 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
         for (int i = 0; i < NF; ++i) o[f][i] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto compute = [&](const Tile& r, int t, auto next_k) {
-        const float svj[8] = {bcast16<0>(r.sv[0]), bcast16<1>(r.sv[0]), bcast16<2>(r.sv[0]), bcast16<3>(r.sv[0]),
-                              bcast16<0>(r.sv[1]), bcast16<1>(r.sv[1]), bcast16<2>(r.sv[1]), bcast16<3>(r.sv[1])};
+    // byte c of two keys, c + 128 as an unsigned number u: 0x6400 | u is 1024 + u in fp16, and the
+    // sum below exact
+    auto v_of = [&](const Tile& r, int i) {
+        const h2 bias = {(_Float16)-1152.f, (_Float16)-1152.f};
+        const uint32_t byte = i & 3;
+        v8h v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t c = __builtin_amdgcn_perm(r.v[2 * j + 1][i >> 2], r.v[2 * j][i >> 2],
+                                                     byte | 0x0c000c00u | ((4u + byte) << 16));
+            const h2 a = __builtin_bit_cast(h2, c ^ 0x64806480u) + bias;
+            v[2 * j] = a.x, v[2 * j + 1] = a.y;
+        }
+        return v;
+    };
+    // a tile with scales sk[h] of this lane and svj[j] of key 4 j + g, and fragment i of V by v_at
+    auto compute = [&](const float (&sk)[2], const float (&svj)[8], int t, auto next_k, auto v_at) {
         const bool partial = t * kTile + kTile > e.prefix;  // wave-uniform
         // the dot products of key 4 j + g, and sK sQ / sqrt(D) of it and this lane's query: an MFMA
         // over 4 x 4 blocks, the outer product of the lanes' key scales with their query scales
@@ -392,7 +419,7 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
 #pragma unroll
                 for (int i = 0; i < KI; ++i)
                     a = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[h][i], qf[f][i], a, 0, 0, 0);
-                const v4f c = __builtin_amdgcn_mfma_f32_4x4x1f32(r.sk[h], qs[f], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                const v4f c = __builtin_amdgcn_mfma_f32_4x4x1f32(sk[h], qs[f], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     dot[f][4 * h + j] = static_cast<float>(a[j]), scale[f][4 * h + j] = c[j];
@@ -495,30 +522,102 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
             }
         }
         next_k();
-        // byte c of two keys, c + 128 as an unsigned number u: 0x6400 | u is 1024 + u in fp16, and
-        // the sum below exact
-        const h2 bias = {(_Float16)-1152.f, (_Float16)-1152.f};
 #pragma unroll
-        for (int i = 0; i < NF; ++i) {
-            v8h v;
-            const uint32_t byte = i & 3;
+        for (int i = 0; i < NF; i += 2) {
+            const v8h v[2] = {v_at(i), v_at(i + 1)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t c = __builtin_amdgcn_perm(r.v[2 * j + 1][i >> 2], r.v[2 * j][i >> 2],
-                                                         byte | 0x0c000c00u | ((4u + byte) << 16));
-                const h2 a = __builtin_bit_cast(h2, c ^ 0x64806480u) + bias;
-                v[2 * j] = a.x, v[2 * j + 1] = a.y;
-            }
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int f = 0; f < F; ++f)
-                o[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[f], o[f][i], 0, 0, 0);
+                for (int f = 0; f < F; ++f)
+                    o[f][i + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[x], pw[f], o[f][i + x], 0, 0, 0);
 #pragma unroll
-            for (int f = 0; f < F; ++f)
-                o[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pr[f], o[f][i], 0, 0, 0);
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int f = 0; f < F; ++f)
+                    o[f][i + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[x], pr[f], o[f][i + x], 0, 0, 0);
         }
     };
 
-    {
+    if constexpr (R > 1) {
+        // 8 tiles at a time: every wave loads and converts one of them, and the R waves of a slice
+        // read the slice's R from LDS, V as the A operands of the MFMA.  The next 8 are on their
+        // way meanwhile.
+        char* s_v = reinterpret_cast<char*>(s_merge) + kWaves * kTile * D;
+        float* s_s = reinterpret_cast<float*>(s_v + kWaves * kTile * D * 2);  // [tile][sK, sV][g][j]
+        const bool any_rows = MR * mine < rows;
+        // the queries have arrived: a wait for them inside the loop would be one for the next tiles'
+        // loads too
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            asm volatile("" : "+v"(qs[f]));
+#pragma unroll
+            for (int i = 0; i < KI; ++i) asm volatile("" : "+v"(qf[f][i]));
+        }
+        Tile raw;
+        Rows at{};
+        int t = t_begin + wave;
+        fetch_ids(t);
+        rows_of_ids(t, at);
+        fetch_ids(t + nw);
+        if (t < t_end) {
+            load_k(at);
+            load_v(raw, at);
+        }
+        for (int t0 = t_begin; t0 < t_end; t0 += nw, t += nw) {
+            if (t < t_end) {
+                write_k();
+#pragma unroll
+                for (int i = 0; i < NF; ++i)
+                    *reinterpret_cast<v8h*>(s_v + (wave * NF + i) * 1024 + lane * 16) = v_of(raw, i);
+                if (m16 < 4)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        s_s[wave * 64 + 8 * g + 4 * h + m16] = raw.sk[h];
+                        s_s[wave * 64 + 32 + 8 * g + 4 * h + m16] = raw.sv[h];
+                    }
+            }
+            __syncthreads();
+            rows_of_ids(t + nw, at);
+            if (t + nw < t_end) {
+                load_k(at);
+                load_v(raw, at);
+            }
+            fetch_ids(t + 2 * nw);
+            if (any_rows && t0 + slice * R < t_end) {
+                float sk[2], svj[8];
+                auto take_k = [&](int slot) {
+                    const char* tk = reinterpret_cast<const char*>(s_merge) + slot * (kTile * D);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < KI; ++i)
+                            k[h][i] = *reinterpret_cast<const v4i*>(tk + h * 16 * D + k_read[i]);
+                    const float* ts = s_s + slot * 64 + 8 * g;
+                    sk[0] = ts[m16 & 3], sk[1] = ts[4 + (m16 & 3)];
+                };
+                take_k(slice * R);
+                for (int u = 0; u < R; ++u) {
+                    const int slot = slice * R + u;
+                    if (t0 + slot >= t_end) break;
+                    const char* tv = s_v + slot * (kTile * D * 2) + lane * 16;
+                    auto v_at = [&](int i) { return *reinterpret_cast<const v8h*>(tv + i * 1024); };
+                    v8h v[NF];
+#pragma unroll
+                    for (int i = 0; i < NF / 2; ++i) v[i] = v_at(i);
+#pragma unroll
+                    for (int j = 0; j < 8; j += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(s_s + slot * 64 + 32 + 8 * g + j);
+                        svj[j] = x.x, svj[j + 1] = x.y, svj[j + 2] = x.z, svj[j + 3] = x.w;
+                    }
+                    compute(sk, svj, t0 + slot, [&]() { take_k(min(slot + 1, kWaves - 1)); }, [&](int i) {
+                        if (i < NF / 2) v[i + NF / 2] = v_at(i + NF / 2);
+                        return v[i];
+                    });
+                }
+            }
+            __syncthreads();
+        }
+    } else {
         // While tile t is computed: V of tile t + nw is on its way from the start, K of it is taken
         // through LDS between the softmax and the product with V, and K of tile t + 2 nw is asked
         // for then.  Loads past the last tile repeat its rows: in a branch, the wait for this
@@ -546,11 +645,16 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
         auto step = [&](Tile& now, Tile& next) {
             load_v(next, r1);
             __builtin_amdgcn_sched_barrier(0);
-            compute(now, t, [&]() {
-                write_k();
-                load_k(r2);
-                read_k();
-            });
+            const float svj[8] = {bcast16<0>(now.sv[0]), bcast16<1>(now.sv[0]), bcast16<2>(now.sv[0]),
+                                  bcast16<3>(now.sv[0]), bcast16<0>(now.sv[1]), bcast16<1>(now.sv[1]),
+                                  bcast16<2>(now.sv[1]), bcast16<3>(now.sv[1])};
+            compute(now.sk, svj, t,
+                    [&]() {
+                        write_k();
+                        load_k(r2);
+                        read_k();
+                    },
+                    [&](int i) { return v_of(now, i); });
             r1 = r2;
             rows_of_ids(t + 3 * nw, r2);
             fetch_ids(t + 4 * nw);
@@ -582,7 +686,7 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     for (int f = 0; f < F; ++f) {
         const int r = 16 * f + m16;
         float top = -INFINITY;
-        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_ml[w * 2 * MR + r]);
+        for (int w = mine; w < nw; w += R) top = fmaxf(top, s_ml[w * 2 * MR + r]);
         const float scale = top == -INFINITY ? 0.f : fast_exp2(m[f] - top);
         float* orow = s_o + (wave * MR + r) * kORow;
 #pragma unroll
@@ -599,11 +703,12 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
         const int row = x / L, d = x % L * 4;
         float top = -INFINITY, sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < nw; ++w) top = fmaxf(top, s_ml[w * 2 * MR + row]);
+        const int at = row % MR;
+        for (int w = row / MR; w < nw; w += R) top = fmaxf(top, s_ml[w * 2 * MR + at]);
         const float use = top == -INFINITY ? 0.f : top;
-        for (int w = 0; w < nw; ++w) {
-            sum = fmaf(s_ml[w * 2 * MR + MR + row], fast_exp2(s_ml[w * 2 * MR + row] - use), sum);
-            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * MR + row) * kORow + d);
+        for (int w = row / MR; w < nw; w += R) {
+            sum = fmaf(s_ml[w * 2 * MR + MR + at], fast_exp2(s_ml[w * 2 * MR + at] - use), sum);
+            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * MR + at) * kORow + d);
             acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
         }
         if (piece.count == 1) {
@@ -671,49 +776,69 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(Attend p, int blocks
 // ------------------------------------------------------------------ host side
 
 struct AttendPlan {
-    int frags, groups, waves;
+    int frags, share, groups;
     int pieces, min_tiles;  // 0: one piece per sequence
     int slots(int B) const { return pieces > 0 ? pieces : B; }
 };
 
-constexpr int kMaxSplit = 64;      // pieces per sequence, on average
-constexpr int kMaxBlocks = 2048;   // of a cut: four rounds
+constexpr int kMaxSplit = 64;            // pieces per sequence, on average
+constexpr int kMaxPartRows = 1 << 16;    // rows of all pieces of a cut
 
 // rows: query rows per key head.
 // Two fragments share a tile's loads and conversions where one alone would leave a block to half of
 // the CUs anyhow (us with one / two: 16 sequences of 8192 x 32 rows x 8 heads 59 / 53; 2 of 4096 x
-// 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).
-// A CU runs one block of 8 waves at a time, two where a wave takes at most 128 registers (one
-// fragment at head dim 64).  The number of pieces is the one with the least estimated time (0.01 us)
-// for sequences of max_context: a round of blocks costs 7 us and 1.1 us per tile of a wave with one
-// fragment, 1.9 with two (at head dim 64 0.8, 1.3 where two blocks share a CU, and 1.3), the join of
-// pieces 5 us.  Sequences that are much shorter gain little by more pieces: the long ones then share
-// memory with fewer.  Measured, us, the chosen one first: in one piece each / cut 16 of up to 8192,
-// 64 rows 68 / 74; 4 of up to 16384, 256 rows 115 / 125; 13 of up to 3001, 12 heads of 64 17 / 20; 1 of
-// 1000, 20 rows 12 / 12; cut / in one piece 8 of up to 8192, 16 heads of 64 29 / 36; 16 of up to 8192,
-// 32 rows 53 / 68; 4 of up to 4096, 32 rows 19 / 27; 8 of up to 16384, 4 rows 47 / 105; 1 of 2048, 4
-// rows 13 / 15.
+// 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).  With two,
+// the waves of a block take 32 rows each of the same keys, one, four or eight of them, and a
+// sequence is cut into k pieces (on average: into B k pieces of equal tiles); both are those of
+// the least estimated time.
+// The estimate (0.01 us), for sequences of max_context: a CU runs one block of 8 waves at a time,
+// two where a wave takes at most 128 registers (one fragment at head dim 64), and the (piece, key
+// head) pairs go to the 8 XCDs of 32 CUs in equal runs.  A round of blocks costs 7 us (12 where
+// waves share tiles) and a time per tile of a wave; the join of pieces 5 us and its bytes.
+// Measured, us, one / four / eight waves on the same keys, the best k of each: 4 sequences of 16384,
+// 256 rows, 8 heads 124 / 107 / 95; 16 of 2064, 256 rows 83 / 66 / 75; 32 of 732, 128 rows 50 / 34 / -;
+// 19 of 692, 380 rows 96 / 60 / 82; 8 of 732, 128 rows 16 / 28 / -; 4 of 3100, 800 rows, 2 heads
+// 30 / 41 / 37.  (Two lost to one or to four: 136, 80, 43, 81, 24 and 42.)  The chosen cut and the
+// other, one wave each: in one piece / cut 16 of up to 8192, 64 rows 68 / 74; 13 of up to 3001, 12
+// heads of 64 17 / 20; 1 of 1000, 20 rows 12 / 12; cut / in one piece 8 of up to 8192, 16 heads of 64
+// 29 / 36; 16 of up to 8192, 32 rows 53 / 68; 4 of up to 4096, 32 rows 19 / 27; 8 of up to 16384, 4 rows
+// 47 / 105; 1 of 2048, 4 rows 13 / 15.
 AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
     AttendPlan pl{};
-    pl.waves = 8;
-    pl.min_tiles = pl.waves;
+    pl.min_tiles = kWaves;
     pl.frags = rows > 16 && (long long)B * Hkv * ceil_div(rows, 16) >= 128 ? 2 : 1;
-    pl.groups = (rows + 16 * pl.frags - 1) / (16 * pl.frags);
-    const long long heads = (long long)Hkv * pl.groups;  // blocks per piece
     const long long tiles = ceil_div(context, kTile);
     const bool two = D == 64 && pl.frags == 1;  // blocks per CU
-    auto time_of = [&](long long blocks, long long t) {
-        const long long tile = two ? (blocks > 256 ? 130 : 80) : pl.frags == 1 ? 110 : D == 64 ? 130 : 190;
-        return ceil_div(blocks, two ? 512 : 256) * (700 + ceil_div(t, pl.waves) * tile);
-    };
-    long long best = time_of(B * heads, tiles);
-    for (int rounds = 1; rounds <= 4; ++rounds) {
-        const long long pieces = std::min<long long>({(long long)kMaxSplit * B, rounds * (two ? 512 : 256) / heads,
-                                                      B * ceil_div(tiles, pl.min_tiles)});
-        // (the sum of all tiles is an int)
-        if (pieces <= B || B * tiles >= (1LL << 31)) continue;
-        const long long time = time_of(pieces * heads, ceil_div(B * tiles, pieces)) + 500;
-        if (time < best) best = time, pl.pieces = (int)pieces;
+    const long long cus = two ? 64 : 32;        // blocks per XCD and round
+    long long best = -1;
+    for (int share = 1; share <= 8; share *= share == 1 ? 4 : 2) {
+        if (share > 1 && (pl.frags == 1 || rows <= 16 * share)) break;
+        const long long groups = ceil_div(rows, 16 * pl.frags * share);
+        auto time_of = [&](long long k) {
+            const long long blocks = ceil_div(k * B * Hkv, 8) * groups;  // of an XCD
+            const long long t = ceil_div(tiles, k);                      // tiles of a block
+            const long long each = share == 1 ? ceil_div(t, kWaves)      // and of a wave
+                                              : t / kWaves * share + std::min<long long>(t % kWaves, share);
+            const long long tile = two ? (blocks > 32 ? 130 : 80)
+                                   : pl.frags == 1 ? 110
+                                   : share == 1 ? (D == 64 ? 130 : 190)
+                                                : (share == 4 ? 150 : 125) * (D == 64 ? 2 : 3) / 3;
+            const long long join = k == 1 ? 0 : 500 + k * B * Hkv * rows * D / 5000;
+            return ceil_div(blocks, cus) * ((share == 1 ? 700 : 1200) + each * tile) + join;
+        };
+        auto consider = [&](long long k) {
+            const long long time = time_of(k);
+            if (best >= 0 && time >= best) return;
+            best = time;
+            pl.share = share, pl.groups = (int)groups, pl.pieces = k == 1 ? 0 : (int)(k * B);
+        };
+        consider(1);
+        for (int rounds = 1; rounds <= 4; ++rounds) {
+            const long long k = std::min<long long>({kMaxSplit, rounds * cus * 8 / (B * Hkv * groups),
+                                                     ceil_div(tiles, pl.min_tiles)});
+            // (the sum of all tiles is an int)
+            if (k > 1 && k * B * Hkv * rows <= kMaxPartRows && B * tiles < (1LL << 31)) consider(k);
+        }
     }
     return pl;
 }
@@ -731,25 +856,26 @@ Partials plan_partials(const AttendPlan& pl, int B, size_t rows, int D) {
     return partials_of(pl.pieces > 0 ? pl.slots(B) * rows : 0, D);
 }
 // Room for every plan of at most `rows` query rows in all: a cut has at most kMaxSplit pieces per
-// sequence, and at most kMaxBlocks blocks of 32 rows.
+// sequence, and at most kMaxPartRows rows of them.
 Partials most_partials(size_t rows, int D) {
-    return partials_of(std::min<size_t>(kMaxSplit * rows, 32 * kMaxBlocks), D);
+    return partials_of(std::min<size_t>(kMaxSplit * rows, kMaxPartRows), D);
 }
 
-template <int D, int F>
+template <int D, int F, int R>
 int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipStream_t stream) {
     constexpr int kWave = (2 * 16 * F + 16 * F * (D + 4)) * 4;  // bytes of LDS per wave
+    static_assert(kWave >= kTile * D * (R > 1 ? 3 : 1) + (R > 1 ? 256 : 0), "the tiles fit where the join does");
     static PerDeviceOnce once;
     const int st = once.run([] {
         const hipError_t e = hipFuncSetAttribute(
-            reinterpret_cast<const void*>(&paged_attend_kernel<D, F>),
+            reinterpret_cast<const void*>(&paged_attend_kernel<D, F, R>),
             hipFuncAttributeMaxDynamicSharedMemorySize, 8 * kWave);
         if (e == hipSuccess) return (int)INT8K_OK;
         set_last_error("hipFuncSetAttribute", e);
         return (int)INT8K_ERR_HIP;
     });
     if (st != INT8K_OK) return st;
-    paged_attend_kernel<D, F><<<blocks, 64 * pl.waves, pl.waves * kWave, stream>>>(p);
+    paged_attend_kernel<D, F, R><<<blocks, 64 * kWaves, kWaves * kWave, stream>>>(p);
     return check_launch("paged_attend_kernel");
 }
 
@@ -760,8 +886,10 @@ int launch_attend(Attend p, const AttendPlan& pl, void* workspace, hipStream_t s
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           plan_partials(pl, p.B, (size_t)p.Hq * p.N, D).ml_bytes);
     const unsigned blocks = (unsigned)(ceil_div((long long)p.slots * p.Hkv, 8) * 8 * pl.groups);
-    const int st = pl.frags == 1 ? launch_instance<D, 1>(p, pl, blocks, stream)
-                                 : launch_instance<D, 2>(p, pl, blocks, stream);
+    const int st = pl.frags == 1 ? launch_instance<D, 1, 1>(p, pl, blocks, stream)
+                   : pl.share == 1 ? launch_instance<D, 2, 1>(p, pl, blocks, stream)
+                   : pl.share == 4 ? launch_instance<D, 2, 4>(p, pl, blocks, stream)
+                                   : launch_instance<D, 2, 8>(p, pl, blocks, stream);
     if (st != INT8K_OK || pl.pieces == 0) return st;
     const int blocks_each = (int)ceil_div((long long)p.Hq * p.N, kCombineRows<D>);
     paged_combine_kernel<D><<<(unsigned)(p.B * blocks_each), 256, 0, stream>>>(p, blocks_each);
@@ -777,7 +905,7 @@ int run_attend(const Attend& p, const AttendPlan& pl, int D, void* workspace, hi
 bool attend_fits(long long B, long long heads, long long kv_heads, long long nodes, int max_context,
                  const AttendPlan& pl) {
     return B * heads * nodes < (1LL << 24) && max_context <= (1 << 30) &&
-           ceil_div(pl.slots((int)B) * kv_heads, 8) * 8 * pl.groups * pl.waves < (1LL << 25);
+           ceil_div(pl.slots((int)B) * kv_heads, 8) * 8 * pl.groups * kWaves < (1LL << 25);
 }
 
 constexpr int kMaxNodes = 256;

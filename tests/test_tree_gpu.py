@@ -56,6 +56,32 @@ def test_masks_and_node_counts(ext, gpu, N, mask):
     _check(c, out)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,G,N,Hkv,longest", [
+    (33, 2, 50, 2, 300), (5, 3, 43, 12, 300), (33, 2, 50, 2, 1500), (3, 8, 50, 2, 4000),
+    (33, 3, 43, 4, 300), (12, 2, 130, 8, 300), (33, 8, 50, 1, 1500), (5, 3, 43, 12, 4000)])
+def test_many_rows_per_key_head(ext, gpu, B, G, N, Hkv, longest, D):
+    # where waves of a block share their keys: whole sequences and cut ones, rows past the last, one
+    # long sequence among short and empty ones
+    g = torch.Generator().manual_seed(B + N)
+    lens = [longest - N] + torch.randint(0, 150, (B - 2,), generator=g).tolist() + [0]
+    counts = [N] + torch.randint(0, N + 1, (B - 2,), generator=g).tolist() + [N]
+    c = tree_case(B * N + D, lens, N, G * Hkv, Hkv, D, 32, gpu, counts=counts)
+    before = capi.paged_bad_ids()
+    out = _run(ext, c)
+    _check(c, out)
+    assert capi.paged_bad_ids() == before
+    c["mask"], c["counts"] = None, None
+    c["max_context"] = longest
+    c["lens"].clamp_(max=100)
+    c["lens"][0] = longest - N
+    need = (c["lens"] + N + 31) // 32  # entries behind a sequence's pages become page 0
+    c["tables"].clamp_(min=0)
+    assert int(need.max()) <= c["tables"].shape[1]
+    _check(c, _run(ext, c))
+    assert torch.equal(_run(ext, c), _run(ext, c))
+
+
 def test_chain_is_the_mask_of_the_tokens_up_to_itself(ext, gpu):
     c = tree_case(1, [77, 500], 70, 4, 1, 128, 64, gpu, mask=None)
     want = _run(ext, c)
