@@ -588,13 +588,13 @@ int int8k_qk_norm_rope_append(const void* x, int dtype, const float* cos, const 
  * counts are 0; positions from max_context on are not attended to (context_lens are cut to it,
  * then the nodes).  A page id outside [0, num_pages) reads page num_pages-1 and is counted
  * (int8k_paged_bad_ids); entries past a sequence's last position are never read.  nodes at most
- * 256, max_context at most 2^30, B*heads*nodes below 2^24 (else INT8K_ERR_UNSUPPORTED).  Q
- * 16-byte, out 8-byte aligned.  The workspace (16-byte aligned) holds partial states: one of
- * int8k_tree_attention_paged_workspace_bytes serves every call of up to B*nodes tokens with the
- * same heads, whatever its max_context; _call_workspace_bytes is what a call of exactly these
- * sizes needs (0: none), for callers that allocate per call.  How a sequence is split, and so the
- * order of its fp32 sums, follows B, nodes, max_context and the lengths of the batch: under others
- * a result agrees within the rounding of those sums, not bit for bit. */
+ * 256, max_context at most 2^30, B*heads*nodes below 2^24, B*kv_heads below 2^21 (else
+ * INT8K_ERR_UNSUPPORTED).  Q 16-byte, out 8-byte aligned.  The workspace (16-byte aligned) holds
+ * partial states: one of int8k_tree_attention_paged_workspace_bytes serves every call of up to
+ * B*nodes tokens with the same heads, whatever its max_context; _call_workspace_bytes is what a
+ * call of exactly these sizes needs (0: none), for callers that allocate per call.  How a sequence
+ * is split, and so the order of its fp32 sums, follows B, nodes, max_context and the lengths of the
+ * batch: under others a result agrees within the rounding of those sums, not bit for bit. */
 size_t int8k_tree_attention_paged_workspace_bytes(int B, int heads, int kv_heads, int nodes,
                                                   int max_context, int head_dim);
 size_t int8k_tree_attention_paged_call_workspace_bytes(int B, int heads, int kv_heads, int nodes,
@@ -613,8 +613,8 @@ int int8k_tree_attention_forward_paged(
  * is written, so a destination may be a source of another pair of the list (the accepted path of
  * a drafted tree moves together).  A slot that one list writes must be in no other list, and the
  * destinations of a list distinct.  A pair with a negative slot is left out; one with a slot past
- * the cache too, and is counted (int8k_paged_bad_ids).  pairs at most 256 (else
- * INT8K_ERR_UNSUPPORTED). */
+ * the cache too, and is counted (int8k_paged_bad_ids).  pairs at most 256, lists*kv_heads below
+ * 2^23 (else INT8K_ERR_UNSUPPORTED). */
 int int8k_kv_cache_move_paged(int8_t* K_pages, int8_t* V_pages, float* sK_pages, float* sV_pages,
                               const int32_t* src_slots, const int32_t* dst_slots, int lists,
                               int pairs, int kv_heads, int head_dim, int num_pages, int page_size,
@@ -626,7 +626,7 @@ int int8k_kv_cache_move_paged(int8_t* K_pages, int8_t* V_pages, float* sK_pages,
  *   quantized as int8k_quantize_per_token does (a NaN in m makes the scale NaN).
  * All page_size rows enter, so a page is due once it is full.  Negative ids are skipped, ids past
  * the cache too, and counted (int8k_paged_bad_ids).  Other pages' means are left as they were.
- * K_means 16-byte aligned. */
+ * K_means 16-byte aligned; count*kv_heads below 2^23 (else INT8K_ERR_UNSUPPORTED). */
 int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages, const int32_t* page_ids,
                         int8_t* K_means, float* sK_means, int count, int kv_heads, int head_dim,
                         int num_pages, int page_size, void* stream);
@@ -644,7 +644,8 @@ int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages, const int3
  * A length of 0 gives a zero row; lengths past max_context are cut to it.  The means of a
  * sequence's last block are not read.  Page ids outside [0, num_pages) read page num_pages-1 and
  * are counted (int8k_paged_bad_ids); entries past a sequence's last block are never read.
- * max_context at most 2^30, B*kv_heads at most 65535 (else INT8K_ERR_UNSUPPORTED).  The workspace
+ * max_context at most 2^30, B*kv_heads at most 65535, B*heads below 2^24, B*kv_heads*top_pages
+ * below 2^31 (else INT8K_ERR_UNSUPPORTED).  The workspace
  * (16-byte aligned) holds scores, the selection and partial states: one of
  * int8k_decode_attention_paged_sparse_workspace_bytes serves every call of up to B sequences,
  * max_context positions and top_pages blocks with the same heads and page size;

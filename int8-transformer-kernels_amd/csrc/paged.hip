@@ -901,11 +901,10 @@ int run_attend(const Attend& p, const AttendPlan& pl, int D, void* workspace, hi
                    : launch_attend<128>(p, pl, workspace, stream);
 }
 
-// Sizes that the grid and the row indexes hold.
-bool attend_fits(long long B, long long heads, long long kv_heads, long long nodes, int max_context,
-                 const AttendPlan& pl) {
-    return B * heads * nodes < (1LL << 24) && max_context <= (1 << 30) &&
-           ceil_div(pl.slots((int)B) * kv_heads, 8) * 8 * pl.groups * kWaves < (1LL << 25);
+// Sizes that the row indexes and the grid hold: at most B * kv_heads * (rows / 16 + 1) blocks, or a
+// cut's, of 512 threads each.
+bool attend_fits(long long B, long long heads, long long kv_heads, long long nodes, int max_context) {
+    return B * heads * nodes < (1LL << 24) && B * kv_heads < (1LL << 21) && max_context <= (1 << 30);
 }
 
 constexpr int kMaxNodes = 256;
@@ -974,10 +973,9 @@ extern "C" int int8k_tree_attention_forward_paged(
         !aligned_to(block_tables, 4) || !aligned_to(context_lens, 4) || !aligned_to(out, 8) ||
         !aligned_to(tree_mask, 8) || !aligned_to(node_counts, 4))
         return INT8K_ERR_MISALIGNED;
-    if (nodes > kMaxNodes || (long long)B * heads * nodes >= (1LL << 24))
+    if (nodes > kMaxNodes || !attend_fits(B, heads, kv_heads, nodes, max_context))
         return INT8K_ERR_UNSUPPORTED;
     const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context, head_dim);
-    if (!attend_fits(B, heads, kv_heads, nodes, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
     const size_t need = plan_partials(pl, B, (size_t)heads * nodes, head_dim).bytes;
     if (need > 0) {
         if (!workspace || workspace_bytes < need) return INT8K_ERR_WORKSPACE;
@@ -1033,11 +1031,10 @@ extern "C" int int8k_decode_attention_forward_paged_sparse(
         !aligned_to(context_lens, 4) || !aligned_to(out, 8) || !aligned_to(selected, 4))
         return INT8K_ERR_MISALIGNED;
     const int context = (int)std::min<long long>(max_context, (long long)top_pages * page_size);
-    if ((long long)B * heads >= (1LL << 24) || max_context > (1 << 30) ||
-        (long long)B * kv_heads > 65535 || (long long)B * kv_heads * top_pages >= (1LL << 31))
+    if (!attend_fits(B, heads, kv_heads, 1, max_context) || (long long)B * kv_heads > 65535 ||
+        (long long)B * kv_heads * top_pages >= (1LL << 31))
         return INT8K_ERR_UNSUPPORTED;
     const AttendPlan pl = attend_plan(B, heads / kv_heads, kv_heads, context, head_dim);
-    if (!attend_fits(B, heads, kv_heads, 1, max_context, pl)) return INT8K_ERR_UNSUPPORTED;
     const SelectSpace sel = select_space(B, kv_heads, max_context, page_size, top_pages);
     if (!workspace ||
         workspace_bytes < sel.bytes + plan_partials(pl, B, (size_t)heads, head_dim).bytes)

@@ -44,7 +44,7 @@ def _tree(lib, **change):
     (dict(H=5), INVALID), (dict(H=0), INVALID), (dict(N=0), INVALID), (dict(cols=0), INVALID), (dict(top=0), INVALID),
     (dict(top=321), INVALID), (dict(flags=1), INVALID), (dict(flags=4), INVALID), (dict(words=2), INVALID),
     (dict(words=0), INVALID), (dict(N=65), INVALID), (dict(each=4), INVALID), (dict(each=-5), INVALID),
-    (dict(N=257, words=5), UNSUPPORTED), (dict(B=1 << 20, N=4), UNSUPPORTED),
+    (dict(N=257, words=5), UNSUPPORTED), (dict(B=1 << 20, N=4), UNSUPPORTED), (dict(B=1 << 21, H=1, Hkv=1, N=1), UNSUPPORTED),
     (dict(cols=1 << 27, top=(1 << 30) + 1), UNSUPPORTED), (dict(Q=ODD8), MISALIGNED), (dict(lens=ODD2), MISALIGNED),
     (dict(mask=ctypes.c_void_p(0x10004)), MISALIGNED), (dict(counts=ODD2), MISALIGNED),
     (dict(out=ctypes.c_void_p(0x10004)), MISALIGNED),
@@ -77,7 +77,7 @@ def test_means_refusals(capi, change, status):
 @pytest.mark.parametrize("change,status", CACHE + [
     (dict(Q=NULL), INVALID), (dict(M=NULL), INVALID), (dict(sel=NULL), INVALID), (dict(B=0), INVALID), (dict(H=5), INVALID),
     (dict(cols=0), INVALID), (dict(top=0), INVALID), (dict(top=321), INVALID), (dict(k=0), INVALID),
-    (dict(B=40000), UNSUPPORTED), (dict(cols=1 << 27, top=(1 << 30) + 1), UNSUPPORTED), (dict(M=ODD8), MISALIGNED),
+    (dict(B=40000), UNSUPPORTED), (dict(B=30000, H=1024), UNSUPPORTED), (dict(k=1 << 30), UNSUPPORTED), (dict(cols=1 << 27, top=(1 << 30) + 1), UNSUPPORTED), (dict(M=ODD8), MISALIGNED),
     (dict(sel=ODD2), MISALIGNED), (dict(ws=NULL), WORKSPACE), (dict(bytes=100), WORKSPACE), (dict(ws=ODD8), MISALIGNED)])
 def test_sparse_refusals(capi, change, status):
     a = dict(Q=P[0], K=P[1], M=P[2], sel=P[3], B=2, H=8, Hkv=2, D=64, NP=40, page=16, cols=20, top=300, k=4, ws=P[4],

@@ -272,6 +272,32 @@ def test_graph_replay_and_streams(ext, gpu):
         assert torch.equal(y1, eager) and torch.equal(y2, eager), lens
 
 
+@pytest.mark.parametrize("B,G,N,Hkv,longest", [(33, 2, 50, 2, 300), (33, 3, 43, 4, 300), (5, 3, 43, 12, 4000)])
+def test_replays_of_many_rows_beside_rows_that_hold_anything(ext, gpu, B, G, N, Hkv, longest):
+    g = torch.Generator().manual_seed(N)
+    lens = [longest - N] + torch.randint(0, 250, (B - 1,), generator=g).tolist()
+    c = tree_case(B + N, lens, N, G * Hkv, Hkv, 128, 32, gpu)
+    want = _run(ext, c)
+    for b, n in enumerate(lens):
+        at = torch.arange(n + N, -(-(n + N) // 32) * 32)
+        p = c["tables"][b, at // 32].long()
+        c["sK"][p, :, at % 32], c["sV"][p, :, at % 32] = float("nan"), float("inf")
+        c["K"][p, :, at % 32], c["V"][p, :, at % 32] = -128, -128
+    assert torch.isfinite(want).all() and torch.equal(_run(ext, c), want)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = _run(ext, c)
+    for shrink in (0, 100, 1):
+        c["lens"].copy_((torch.tensor(lens) - shrink).clamp(min=0))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            eager = _run(ext, c)
+        y.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager) and (shrink or torch.equal(y, want))
+
+
 def test_the_same_every_time_and_with_a_larger_workspace(ext, gpu):
     c = tree_case(15, [4000, 3000], 6, 16, 2, 64, 16, gpu)
     want = _run(ext, c)
