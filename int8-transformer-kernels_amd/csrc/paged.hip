@@ -18,15 +18,16 @@
 // into two fp16.  K passes through LDS, where a wave's loads of whole lines become that layout.
 // A wave takes one or two fragments of every 8th tile of a piece of a sequence, and the 8 waves of
 // a block are joined in LDS; or, where a key head has many rows, R = 4 or 8 waves take two
-// fragments each of the same tiles, which they load and convert in turn and share through LDS.
+// fragments each of the same tiles, which they load and convert in turn and share through LDS: two
+// such slices of a block, joined, or one, whose waves write what they hold.
 // Pieces are joined by a second kernel.
 //
 // Bound by memory with one fragment (8 sequences of 16384, one token of 4 heads on 8: 5.2 TB/s) and
 // by the issue of instructions with two: 32 rows x 32 keys take 300 vector instructions (190 with
 // R = 8: V's conversion is shared) beside 44 MFMAs, each of which keeps the SIMD from vector ones
 // for about 10 of its 16 cycles.  16 sequences of up to 8192 with trees of 16, 32 heads on 8 of
-// 128: 67 us (2.6 TB/s, 0.32 PFLOP/s); 4 of 16320 with trees of 64: 104 us (0.41 PFLOP/s; 115 without
-// R = 8).
+// 128: 67 us (2.6 TB/s, 0.32 PFLOP/s); 4 of 16320 with trees of 64: 102 us (0.42 PFLOP/s; 115 with
+// R = 1).
 //
 // p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
 // that the largest weight p sV of the tile that set it lies in [2^9, 2^10), and a tile whose
@@ -217,6 +218,15 @@ __device__ __forceinline__ void store_row(const Attend& p, size_t at, const floa
             : make_uint2(0, 0);
 }
 
+// A partial row is stored in the order in which lanes hold it, four dims at a time: four lanes (g) of
+// a row write 64 bytes.  The first dim of its float4 `at`.
+template <int D>
+__device__ __forceinline__ int part_dim(int at) {
+    constexpr int NF = D / 16;
+    const int g = at & 3, i = at / 4 % (NF / 4), c = at / NF;
+    return NF * (4 * g + c) + 4 * i;
+}
+
 template <int D>
 struct AttendTile {
     static constexpr int kV = D / 64;   // 4-byte words of a V row per lane
@@ -233,8 +243,8 @@ __device__ __forceinline__ uint32_t k_slot(int r, int c) {
     return (r / RP) * 256 + ((r % RP) * C + (c ^ (r / RP % C))) * 16;
 }
 
-template <int D, int F, int R>
-__global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
+template <int D, int F, int R, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_attend_kernel(Attend p) {
     using Tile = AttendTile<D>;
     constexpr int NF = D / 16;          // fragments of O^T
     constexpr int KI = D / 64;          // loads of 1 KiB per 16 rows
@@ -244,7 +254,7 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     extern __shared__ __align__(16) float s_merge[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int nw = kWaves;
+    constexpr int nw = W;
     const int mine = wave & (R - 1), slice = wave / R;  // which rows of the block's, which of its waves on them
     const int g = lane >> 4, m16 = lane & 15;
 
@@ -542,8 +552,8 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
         // 8 tiles at a time: every wave loads and converts one of them, and the R waves of a slice
         // read the slice's R from LDS, V as the A operands of the MFMA.  The next 8 are on their
         // way meanwhile.
-        char* s_v = reinterpret_cast<char*>(s_merge) + kWaves * kTile * D;
-        float* s_s = reinterpret_cast<float*>(s_v + kWaves * kTile * D * 2);  // [tile][sK, sV][g][j]
+        char* s_v = reinterpret_cast<char*>(s_merge) + W * kTile * D;
+        float* s_s = reinterpret_cast<float*>(s_v + W * kTile * D * 2);  // [tile][sK, sV][g][j]
         const bool any_rows = MR * mine < rows;
         // the queries have arrived: a wait for them inside the loop would be one for the next tiles'
         // loads too
@@ -609,7 +619,7 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
                         const float4 x = *reinterpret_cast<const float4*>(s_s + slot * 64 + 32 + 8 * g + j);
                         svj[j] = x.x, svj[j + 1] = x.y, svj[j + 2] = x.z, svj[j + 3] = x.w;
                     }
-                    compute(sk, svj, t0 + slot, [&]() { take_k(min(slot + 1, kWaves - 1)); }, [&](int i) {
+                    compute(sk, svj, t0 + slot, [&]() { take_k(min(slot + 1, W - 1)); }, [&](int i) {
                         if (i < NF / 2) v[i + NF / 2] = v_at(i + NF / 2);
                         return v[i];
                     });
@@ -669,6 +679,31 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     __syncthreads();  // the tiles of K give way to the join
     if (bad && lane == 0) atomicAdd(&g_attend_bad_ids, 1u);
 
+    if constexpr (R == W) {  // nothing to join: lane l holds NF dims from NF (4 g + c) on of its rows
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            const float sum = sum_groups(l[f]);
+            const int row = MR * mine + 16 * f + m16;
+            if (row >= rows) continue;
+            const int r = row0_q + row, n = r % p.N, h = kvh * (p.Hq / p.Hkv) + r / p.N;
+            const size_t at = (p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : first_row + row) * D;
+            const size_t part = ((size_t)number * p.Hkv + kvh) * all_rows + r;
+            const bool any = piece.count > 1 || attends(p, b, n, e);
+            if (piece.count > 1 && g == 0)
+                reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m[f], sum);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < NF; i += 4) {
+                    const int d = NF * (4 * g + c) + i;
+                    const float4 acc = make_float4(o[f][i][c], o[f][i + 1][c], o[f][i + 2][c], o[f][i + 3][c]);
+                    if (piece.count == 1) store_row(p, at + d, acc, sum, any);
+                    else reinterpret_cast<float4*>(p.part_acc + part * D)[c * NF + i + g] = acc;
+                }
+        }
+        return;
+    }
+
     // Join the waves: m and l of each row go to LDS, and O scaled to the rows' common maximum, which
     // are then added four dims at a time (element by element, with the factors worked out by each
     // thread, the join took 11 us of the 78 of 16 sequences with trees of 16).
@@ -700,7 +735,7 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
     __syncthreads();
     constexpr int L = D / 4;  // threads per row
     for (int x = threadIdx.x; x < rows * L; x += blockDim.x) {
-        const int row = x / L, d = x % L * 4;
+        const int row = x / L, d = part_dim<D>(x % L);
         float top = -INFINITY, sum = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         const int at = row % MR;
@@ -717,8 +752,8 @@ __global__ __launch_bounds__(512) void paged_attend_kernel(Attend p) {
             store_row(p, at * D + d, acc, sum, attends(p, b, n, e));
         } else {
             const size_t part = ((size_t)number * p.Hkv + kvh) * all_rows + row0_q + row;
-            if (d == 0) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(top, sum);
-            *reinterpret_cast<float4*>(p.part_acc + part * D + d) = acc;
+            if (x % L == 0) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(top, sum);
+            reinterpret_cast<float4*>(p.part_acc + part * D)[x % L] = acc;
         }
     }
 }
@@ -770,13 +805,13 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(Attend p, int blocks
     }
     const int h = row / p.N, n = row - h * p.N;
     const size_t at = p.bshd ? ((size_t)b * p.N + n) * p.Hq + h : (size_t)b * all_rows + row;
-    store_row(p, at * D + 4 * c, a, sum, attends(p, b, n, extent_of(p, b)));
+    store_row(p, at * D + part_dim<D>(c), a, sum, attends(p, b, n, extent_of(p, b)));
 }
 
 // ------------------------------------------------------------------ host side
 
 struct AttendPlan {
-    int frags, share, groups;
+    int frags, share, waves, groups;
     int pieces, min_tiles;  // 0: one piece per sequence
     int slots(int B) const { return pieces > 0 ? pieces : B; }
 };
@@ -788,57 +823,58 @@ constexpr int kMaxPartRows = 1 << 16;    // rows of all pieces of a cut
 // Two fragments share a tile's loads and conversions where one alone would leave a block to half of
 // the CUs anyhow (us with one / two: 16 sequences of 8192 x 32 rows x 8 heads 59 / 53; 2 of 4096 x
 // 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).  With two,
-// the waves of a block take 32 rows each of the same keys, one, four or eight of them, and a
-// sequence is cut into k pieces (on average: into B k pieces of equal tiles); both are those of
-// the least estimated time.
+// the waves of a block take the same 32 rows, or four of eight, all of four or all of eight share
+// their tiles, and a sequence is cut into k pieces (on average: into B k pieces of equal tiles); both are those
+// of the least estimated time.
 // The estimate (0.01 us), for sequences of max_context: a CU runs one block of 8 waves at a time,
-// two where a wave takes at most 128 registers (one fragment at head dim 64), and the (piece, key
-// head) pairs go to the 8 XCDs of 32 CUs in equal runs.  A round of blocks costs 7 us (12 where
-// waves share tiles) and a time per tile of a wave; the join of pieces 5 us and its bytes.
-// Measured, us, one / four / eight waves on the same keys, the best k of each: 4 sequences of 16384,
-// 256 rows, 8 heads 124 / 107 / 95; 16 of 2064, 256 rows 83 / 66 / 75; 32 of 732, 128 rows 50 / 34 / -;
-// 19 of 692, 380 rows 96 / 60 / 82; 8 of 732, 128 rows 16 / 28 / -; 4 of 3100, 800 rows, 2 heads
-// 30 / 41 / 37.  (Two lost to one or to four: 136, 80, 43, 81, 24 and 42.)  The chosen cut and the
-// other, one wave each: in one piece / cut 16 of up to 8192, 64 rows 68 / 74; 13 of up to 3001, 12
-// heads of 64 17 / 20; 1 of 1000, 20 rows 12 / 12; cut / in one piece 8 of up to 8192, 16 heads of 64
-// 29 / 36; 16 of up to 8192, 32 rows 53 / 68; 4 of up to 4096, 32 rows 19 / 27; 8 of up to 16384, 4 rows
-// 47 / 105; 1 of 2048, 4 rows 13 / 15.
+// two of 4 waves or where a wave takes at most 128 registers (one fragment at head dim 64), and the
+// (piece, key head) pairs go to the 8 XCDs of 32 CUs in equal runs.  A round of blocks costs 7 us (12
+// and 10 where waves share tiles) and a time per tile of a wave; the join of pieces 5 us and its
+// bytes.  Measured, us, no sharing / four of eight / four / eight, the best k of each: 4 sequences of
+// 16384, 256 rows, 8 heads 124 / 107 / 97 / 95; 2 of 20100, 400 rows - / - / 113 / 105; 8 of 12048, 384
+// rows, 4 heads - / - / 104 / 108; 16 of 2064, 256 rows 83 / 66 / 72 / 75; 32 of 732, 128 rows 50 / 34 /
+// 40 / -; 19 of 692, 380 rows 95 / 59 / 46 / 82; 8 of 732, 128 rows 16 / 28 / 30 / -; 4 of 3100, 800 rows,
+// 2 heads 29 / 39 / 37 / 36.  (Two of eight, 136, -, -, 80, 43, 81, 24 and 42, lost to one or the other
+// everywhere.)  The chosen cut and the other, without sharing: in one piece / cut 16 of up to 8192,
+// 64 rows 68 / 74; 13 of up to 3001, 12 heads of 64 17 / 20; 1 of 1000, 20 rows 12 / 12; cut / in one
+// piece 8 of up to 8192, 16 heads of 64 29 / 36; 16 of up to 8192, 32 rows 53 / 68; 4 of up to 4096, 32
+// rows 19 / 27; 8 of up to 16384, 4 rows 47 / 105; 1 of 2048, 4 rows 13 / 15.
 AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
     AttendPlan pl{};
     pl.min_tiles = kWaves;
     pl.frags = rows > 16 && (long long)B * Hkv * ceil_div(rows, 16) >= 128 ? 2 : 1;
     const long long tiles = ceil_div(context, kTile);
-    const bool two = D == 64 && pl.frags == 1;  // blocks per CU
-    const long long cus = two ? 64 : 32;        // blocks per XCD and round
     long long best = -1;
-    for (int share = 1; share <= 8; share *= share == 1 ? 4 : 2) {
-        if (share > 1 && (pl.frags == 1 || rows <= 16 * share)) break;
+    auto consider_all = [&](int share, int waves, long long round, bool two, long long tile, long long tile_two) {
         const long long groups = ceil_div(rows, 16 * pl.frags * share);
-        auto time_of = [&](long long k) {
-            const long long blocks = ceil_div(k * B * Hkv, 8) * groups;  // of an XCD
-            const long long t = ceil_div(tiles, k);                      // tiles of a block
-            const long long each = share == 1 ? ceil_div(t, kWaves)      // and of a wave
-                                              : t / kWaves * share + std::min<long long>(t % kWaves, share);
-            const long long tile = two ? (blocks > 32 ? 130 : 80)
-                                   : pl.frags == 1 ? 110
-                                   : share == 1 ? (D == 64 ? 130 : 190)
-                                                : (share == 4 ? 150 : 125) * (D == 64 ? 2 : 3) / 3;
-            const long long join = k == 1 ? 0 : 500 + k * B * Hkv * rows * D / 5000;
-            return ceil_div(blocks, cus) * ((share == 1 ? 700 : 1200) + each * tile) + join;
-        };
+        const long long slots = two ? 64 : 32;  // blocks of an XCD at a time
         auto consider = [&](long long k) {
-            const long long time = time_of(k);
+            const long long blocks = ceil_div(k * B * Hkv, 8) * groups;  // of an XCD
+            const long long t = ceil_div(tiles, k);                      // tiles of a block, and of a wave
+            const long long each = share == 1 ? ceil_div(t, waves) : t / waves * share + std::min<long long>(t % waves, share);
+            const long long join = k == 1 ? 0 : 500 + k * B * Hkv * rows * D / 5000;
+            const long long time = ceil_div(blocks, slots) * (round + each * (blocks > 32 ? tile_two : tile)) + join;
             if (best >= 0 && time >= best) return;
             best = time;
-            pl.share = share, pl.groups = (int)groups, pl.pieces = k == 1 ? 0 : (int)(k * B);
+            pl.share = share, pl.waves = waves, pl.groups = (int)groups, pl.pieces = k == 1 ? 0 : (int)(k * B);
         };
         consider(1);
         for (int rounds = 1; rounds <= 4; ++rounds) {
-            const long long k = std::min<long long>({kMaxSplit, rounds * cus * 8 / (B * Hkv * groups),
+            const long long k = std::min<long long>({kMaxSplit, rounds * slots * 8 / (B * Hkv * groups),
                                                      ceil_div(tiles, pl.min_tiles)});
             // (the sum of all tiles is an int)
             if (k > 1 && k * B * Hkv * rows <= kMaxPartRows && B * tiles < (1LL << 31)) consider(k);
         }
+    };
+    if (pl.frags == 1) {
+        if (D == 64) consider_all(1, kWaves, 700, true, 80, 130);
+        else consider_all(1, kWaves, 700, false, 110, 110);
+    } else {
+        const int d = D == 64 ? 2 : 3;
+        consider_all(1, kWaves, 700, false, D == 64 ? 130 : 190, D == 64 ? 130 : 190);
+        if (rows > 64) consider_all(4, kWaves, 1200, false, 50 * d, 50 * d);
+        if (rows > 64) consider_all(4, 4, 1000, true, 35 * d, 40 * d);
+        if (rows > 128) consider_all(8, kWaves, 1200, false, 37 * d, 37 * d);
     }
     return pl;
 }
@@ -861,21 +897,21 @@ Partials most_partials(size_t rows, int D) {
     return partials_of(std::min<size_t>(kMaxSplit * rows, kMaxPartRows), D);
 }
 
-template <int D, int F, int R>
+template <int D, int F, int R, int W>
 int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipStream_t stream) {
-    constexpr int kWave = (2 * 16 * F + 16 * F * (D + 4)) * 4;  // bytes of LDS per wave
-    static_assert(kWave >= kTile * D * (R > 1 ? 3 : 1) + (R > 1 ? 256 : 0), "the tiles fit where the join does");
+    constexpr int kTiles = R > 1 ? 3 * kTile * D + 256 : kTile * D;  // bytes of LDS per wave
+    constexpr int kWave = R == W ? kTiles : std::max(kTiles, (2 * 16 * F + 16 * F * (D + 4)) * 4);
     static PerDeviceOnce once;
     const int st = once.run([] {
         const hipError_t e = hipFuncSetAttribute(
-            reinterpret_cast<const void*>(&paged_attend_kernel<D, F, R>),
-            hipFuncAttributeMaxDynamicSharedMemorySize, 8 * kWave);
+            reinterpret_cast<const void*>(&paged_attend_kernel<D, F, R, W>),
+            hipFuncAttributeMaxDynamicSharedMemorySize, W * kWave);
         if (e == hipSuccess) return (int)INT8K_OK;
         set_last_error("hipFuncSetAttribute", e);
         return (int)INT8K_ERR_HIP;
     });
     if (st != INT8K_OK) return st;
-    paged_attend_kernel<D, F, R><<<blocks, 64 * kWaves, kWaves * kWave, stream>>>(p);
+    paged_attend_kernel<D, F, R, W><<<blocks, 64 * W, W * kWave, stream>>>(p);
     return check_launch("paged_attend_kernel");
 }
 
@@ -886,10 +922,11 @@ int launch_attend(Attend p, const AttendPlan& pl, void* workspace, hipStream_t s
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           plan_partials(pl, p.B, (size_t)p.Hq * p.N, D).ml_bytes);
     const unsigned blocks = (unsigned)(ceil_div((long long)p.slots * p.Hkv, 8) * 8 * pl.groups);
-    const int st = pl.frags == 1 ? launch_instance<D, 1, 1>(p, pl, blocks, stream)
-                   : pl.share == 1 ? launch_instance<D, 2, 1>(p, pl, blocks, stream)
-                   : pl.share == 4 ? launch_instance<D, 2, 4>(p, pl, blocks, stream)
-                                   : launch_instance<D, 2, 8>(p, pl, blocks, stream);
+    const int st = pl.frags == 1 ? launch_instance<D, 1, 1, kWaves>(p, pl, blocks, stream)
+                   : pl.share == 1 ? launch_instance<D, 2, 1, kWaves>(p, pl, blocks, stream)
+                   : pl.share == 8 ? launch_instance<D, 2, 8, kWaves>(p, pl, blocks, stream)
+                   : pl.waves == 4 ? launch_instance<D, 2, 4, 4>(p, pl, blocks, stream)
+                                   : launch_instance<D, 2, 4, kWaves>(p, pl, blocks, stream);
     if (st != INT8K_OK || pl.pieces == 0) return st;
     const int blocks_each = (int)ceil_div((long long)p.Hq * p.N, kCombineRows<D>);
     paged_combine_kernel<D><<<(unsigned)(p.B * blocks_each), 256, 0, stream>>>(p, blocks_each);

@@ -59,7 +59,9 @@ def test_masks_and_node_counts(ext, gpu, N, mask):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("B,G,N,Hkv,longest", [
     (33, 2, 50, 2, 300), (5, 3, 43, 12, 300), (33, 2, 50, 2, 1500), (3, 8, 50, 2, 4000),
-    (33, 3, 43, 4, 300), (12, 2, 130, 8, 300), (33, 8, 50, 1, 1500), (5, 3, 43, 12, 4000)])
+    (33, 3, 43, 4, 300), (12, 2, 130, 8, 300), (33, 8, 50, 1, 1500), (5, 3, 43, 12, 4000),
+    (5, 8, 50, 4, 1500), (12, 1, 100, 12, 700), (5, 1, 256, 8, 1500), (20, 3, 43, 8, 1500), (33, 3, 43, 2, 4000),
+    (2, 8, 50, 8, 9000)])
 def test_many_rows_per_key_head(ext, gpu, B, G, N, Hkv, longest, D):
     # where waves of a block share their keys: whole sequences and cut ones, rows past the last, one
     # long sequence among short and empty ones
@@ -272,7 +274,8 @@ def test_graph_replay_and_streams(ext, gpu):
         assert torch.equal(y1, eager) and torch.equal(y2, eager), lens
 
 
-@pytest.mark.parametrize("B,G,N,Hkv,longest", [(33, 2, 50, 2, 300), (33, 3, 43, 4, 300), (5, 3, 43, 12, 4000)])
+@pytest.mark.parametrize("B,G,N,Hkv,longest", [(33, 2, 50, 2, 300), (33, 3, 43, 4, 300), (5, 3, 43, 12, 4000),
+                                                (12, 1, 100, 12, 700), (5, 8, 50, 4, 1500), (2, 8, 50, 8, 9000)])
 def test_replays_of_many_rows_beside_rows_that_hold_anything(ext, gpu, B, G, N, Hkv, longest):
     g = torch.Generator().manual_seed(N)
     lens = [longest - N] + torch.randint(0, 250, (B - 1,), generator=g).tolist()
