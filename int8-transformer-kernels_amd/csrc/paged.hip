@@ -819,62 +819,76 @@ struct AttendPlan {
 constexpr int kMaxSplit = 64;            // pieces per sequence, on average
 constexpr int kMaxPartRows = 1 << 16;    // rows of all pieces of a cut
 
+// The kernels that a plan picks from, with what they cost in us at head dims 128 and 64: a round of
+// blocks, and a tile of a wave while few blocks run and while the GPU is full of them.
+struct AttendCost {
+    int frags, share, waves;
+    double round[2], idle[2], full[2];
+};
+constexpr AttendCost kAttendCosts[] = {
+    {1, 1, 8, {5.5, 6}, {1.3, 0.75}, {1.25, 1.4}},
+    {2, 1, 8, {8.5, 6.5}, {1.5, 0.75}, {1.65, 1.3}},
+    {2, 4, 8, {11.5, 12.5}, {1.6, 1.0}, {1.4, 1.15}},
+    {2, 4, 4, {9, 11.5}, {1.4, 1.05}, {1.25, 0.95}},
+    {2, 8, 8, {11, 12}, {1.3, 0.95}, {1.2, 0.95}}};
+
 // rows: query rows per key head.
-// Two fragments share a tile's loads and conversions where one alone would leave a block to half of
-// the CUs anyhow (us with one / two: 16 sequences of 8192 x 32 rows x 8 heads 59 / 53; 2 of 4096 x
-// 128 rows 23.3 / 22.1; 4 of 4096 x 32 rows 18.5 / 21.2; 1 of 32000 x 32 rows 26 / 29).  With two,
-// the waves of a block take the same 32 rows, or four of eight, all of four or all of eight share
-// their tiles, and a sequence is cut into k pieces (on average: into B k pieces of equal tiles); both are those
-// of the least estimated time.
-// The estimate (0.01 us), for sequences of max_context: a CU runs one block of 8 waves at a time,
-// two of 4 waves or where a wave takes at most 128 registers (one fragment at head dim 64), and the
-// (piece, key head) pairs go to the 8 XCDs of 32 CUs in equal runs.  A round of blocks costs 7 us (12
-// and 10 where waves share tiles) and a time per tile of a wave; the join of pieces 5 us and its
-// bytes.  Measured, us, no sharing / four of eight / four / eight, the best k of each: 4 sequences of
-// 16384, 256 rows, 8 heads 124 / 107 / 97 / 95; 2 of 20100, 400 rows - / - / 113 / 105; 8 of 12048, 384
-// rows, 4 heads - / - / 104 / 108; 16 of 2064, 256 rows 83 / 66 / 72 / 75; 32 of 732, 128 rows 50 / 34 /
-// 40 / -; 19 of 692, 380 rows 95 / 59 / 46 / 82; 8 of 732, 128 rows 16 / 28 / 30 / -; 4 of 3100, 800 rows,
-// 2 heads 29 / 39 / 37 / 36.  (Two of eight, 136, -, -, 80, 43, 81, 24 and 42, lost to one or the other
-// everywhere.)  The chosen cut and the other, without sharing: in one piece / cut 16 of up to 8192,
-// 64 rows 68 / 74; 13 of up to 3001, 12 heads of 64 17 / 20; 1 of 1000, 20 rows 12 / 12; cut / in one
-// piece 8 of up to 8192, 16 heads of 64 29 / 36; 16 of up to 8192, 32 rows 53 / 68; 4 of up to 4096, 32
-// rows 19 / 27; 8 of up to 16384, 4 rows 47 / 105; 1 of 2048, 4 rows 13 / 15.
+// The plan is the kernel and the number of pieces of least estimated time, for sequences of unequal
+// lengths: one of max_context, 3/4 of that in the mean.  A CU runs one block of 8 waves at a time, two
+// of 4 waves or where a wave takes at most 128 registers (one fragment at head dim 64), and the
+// (piece, key head) pairs go to the 8 XCDs of 32 CUs in equal runs.  The join of pieces costs 6 us and
+// 0.25 for a MB of partial rows.
+// The costs are fitted to every kernel at one piece per sequence and up to eight cuts, timed at 3993
+// sizes (1 to 64 sequences of 16 to 45000, 1 to 256 tokens, 1 to 16 heads on each of 1 to 12): the plan is
+// 0.8% off the fastest in the mean and 20% at the 20 worst (2% at 958 other sizes, that timed again).  Measured, us, one fragment / two / four of
+// eight waves sharing / four / eight, the best cut of each: 16 sequences of 8192 x 32 rows x 8 heads
+// 59 / 53 / - / - / -; 4 of 4096 x 32 rows 18.5 / 21 / - / - / -; 4 of 16384, 256 rows - / 124 / 107 / 97 / 95; 2 of
+// 20100, 400 rows - / 118 / 115 / 106 / 102; 8 of 12048, 384 rows, 4 heads - / 126 / 111 / 94 / 107; 16 of 2064,
+// 256 rows - / 83 / 66 / 72 / 75; 32 of 732, 128 rows - / 50 / 34 / 40 / -; 19 of 692, 380 rows - / 95 / 59 / 46 /
+// 82; 8 of 732, 128 rows - / 16 / 28 / 30 / -; 4 of 3100, 800 rows, 2 heads - / 29 / 39 / 37 / 36.  (Two of eight
+// waves sharing, 53, -, 136, -, -, 80, 43, 81, 24 and 42 of these, lost to one or the other everywhere.)
 AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
     AttendPlan pl{};
     pl.min_tiles = kWaves;
-    pl.frags = rows > 16 && (long long)B * Hkv * ceil_div(rows, 16) >= 128 ? 2 : 1;
-    const long long tiles = ceil_div(context, kTile);
-    long long best = -1;
-    auto consider_all = [&](int share, int waves, long long round, bool two, long long tile, long long tile_two) {
-        const long long groups = ceil_div(rows, 16 * pl.frags * share);
-        const long long slots = two ? 64 : 32;  // blocks of an XCD at a time
-        auto consider = [&](long long k) {
-            const long long blocks = ceil_div(k * B * Hkv, 8) * groups;  // of an XCD
-            const long long t = ceil_div(tiles, k);                      // tiles of a block, and of a wave
-            const long long each = share == 1 ? ceil_div(t, waves) : t / waves * share + std::min<long long>(t % waves, share);
-            const long long join = k == 1 ? 0 : 500 + k * B * Hkv * rows * D / 5000;
-            const long long time = ceil_div(blocks, slots) * (round + each * (blocks > 32 ? tile_two : tile)) + join;
-            if (best >= 0 && time >= best) return;
-            best = time;
-            pl.share = share, pl.waves = waves, pl.groups = (int)groups, pl.pieces = k == 1 ? 0 : (int)(k * B);
+    const int d = D == 64;
+    const long long tiles = ceil_div(context, kTile), pairs = (long long)B * Hkv;
+    double best = INFINITY;
+    for (const AttendCost& c : kAttendCosts) {
+        if (c.frags == 2 && rows <= 16 * c.share) continue;
+        const long long groups = ceil_div(rows, 16 * c.frags * c.share);
+        const long long slots = c.waves == 4 || (c.frags == 1 && D == 64) ? 64 : 32;  // blocks of an XCD at a time
+        auto wave_tiles = [&](long long t) {  // of a block's t
+            return c.share == 1 ? ceil_div(t, c.waves)
+                                : t / c.waves * c.share + std::min<long long>(t % c.waves, c.share);
         };
-        consider(1);
-        for (int rounds = 1; rounds <= 4; ++rounds) {
-            const long long k = std::min<long long>({kMaxSplit, rounds * slots * 8 / (B * Hkv * groups),
-                                                     ceil_div(tiles, pl.min_tiles)});
-            // (the sum of all tiles is an int)
-            if (k > 1 && k * B * Hkv * rows <= kMaxPartRows && B * tiles < (1LL << 31)) consider(k);
+        auto consider = [&](long long pieces) {  // 0: the sequences whole
+            const long long blocks = ceil_div(pieces > 0 ? pieces * Hkv : pairs, 8) * groups;  // of an XCD
+            const long long rounds = ceil_div(blocks, slots);
+            const double tile = c.idle[d] + (c.full[d] - c.idle[d]) * std::min(1.0, (double)blocks / slots);
+            double time;
+            if (pieces > 0) {  // (0.4 of a piece of each sequence but one is lost)
+                const double t = std::ceil(tiles * (1 + 0.75 * (B - 1)) / (pieces - 0.4 * (B - 1)));
+                time = (0.15 + 0.85 * rounds) * (c.round[d] + wave_tiles(std::min((long long)t, tiles)) * tile) +
+                       6 + 0.25e-6 * 8 * pieces * Hkv * rows * D;
+            } else {
+                time = rounds * c.round[d] + ((rounds - 1) * wave_tiles(ceil_div(4 * tiles, 5)) + wave_tiles(tiles)) * tile;
+            }
+            if (time >= best) return;
+            best = time;
+            pl.frags = c.frags, pl.share = c.share, pl.waves = c.waves, pl.groups = (int)groups;
+            pl.pieces = (int)pieces;
+        };
+        consider(0);
+        if (B * tiles >= (1LL << 31)) continue;  // (the sum of all tiles is an int)
+        const long long most = std::min(std::min<long long>(kMaxSplit, ceil_div(tiles, pl.min_tiles)) * B,
+                                        kMaxPartRows / ((long long)Hkv * rows));
+        for (int r = 1; r <= 4; ++r) {
+            const long long pieces = std::min(r * slots * 8 / (Hkv * groups), most);
+            if (pieces <= B) continue;
+            consider(pieces);
+            if (pieces % B != 0 && pieces > 2 * B) consider(pieces / B * B);
+            if (pieces == most) break;
         }
-    };
-    if (pl.frags == 1) {
-        if (D == 64) consider_all(1, kWaves, 700, true, 80, 130);
-        else consider_all(1, kWaves, 700, false, 110, 110);
-    } else {
-        const int d = D == 64 ? 2 : 3;
-        consider_all(1, kWaves, 700, false, D == 64 ? 130 : 190, D == 64 ? 130 : 190);
-        if (rows > 64) consider_all(4, kWaves, 1200, false, 50 * d, 50 * d);
-        if (rows > 64) consider_all(4, 4, 1000, true, 35 * d, 40 * d);
-        if (rows > 128) consider_all(8, kWaves, 1200, false, 37 * d, 37 * d);
     }
     return pl;
 }

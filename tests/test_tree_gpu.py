@@ -61,7 +61,8 @@ def test_masks_and_node_counts(ext, gpu, N, mask):
     (33, 2, 50, 2, 300), (5, 3, 43, 12, 300), (33, 2, 50, 2, 1500), (3, 8, 50, 2, 4000),
     (33, 3, 43, 4, 300), (12, 2, 130, 8, 300), (33, 8, 50, 1, 1500), (5, 3, 43, 12, 4000),
     (5, 8, 50, 4, 1500), (12, 1, 100, 12, 700), (5, 1, 256, 8, 1500), (20, 3, 43, 8, 1500), (33, 3, 43, 2, 4000),
-    (2, 8, 50, 8, 9000)])
+    (2, 8, 50, 8, 9000), (33, 1, 256, 4, 1000), (33, 3, 43, 2, 6000), (20, 1, 100, 4, 2000), (20, 1, 100, 8, 300),
+    (5, 8, 50, 12, 6000)])
 def test_many_rows_per_key_head(ext, gpu, B, G, N, Hkv, longest, D):
     # where waves of a block share their keys: whole sequences and cut ones, rows past the last, one
     # long sequence among short and empty ones
@@ -275,7 +276,7 @@ def test_graph_replay_and_streams(ext, gpu):
 
 
 @pytest.mark.parametrize("B,G,N,Hkv,longest", [(33, 2, 50, 2, 300), (33, 3, 43, 4, 300), (5, 3, 43, 12, 4000),
-                                                (12, 1, 100, 12, 700), (5, 8, 50, 4, 1500), (2, 8, 50, 8, 9000)])
+                                                (12, 1, 100, 12, 700), (5, 8, 50, 4, 1500), (33, 1, 256, 4, 1000), (33, 3, 43, 2, 6000)])
 def test_replays_of_many_rows_beside_rows_that_hold_anything(ext, gpu, B, G, N, Hkv, longest):
     g = torch.Generator().manual_seed(N)
     lens = [longest - N] + torch.randint(0, 250, (B - 1,), generator=g).tolist()
