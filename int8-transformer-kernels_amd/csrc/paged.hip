@@ -26,7 +26,7 @@
 // by the issue of instructions with two: 32 rows x 32 keys take 300 vector instructions (190 with
 // R = 8: V's conversion is shared) beside 44 MFMAs, each of which keeps the SIMD from vector ones
 // for about 10 of its 16 cycles.  16 sequences of up to 8192 with trees of 16, 32 heads on 8 of
-// 128: 67 us (2.6 TB/s, 0.32 PFLOP/s); 4 of 16320 with trees of 64: 102 us (0.42 PFLOP/s; 115 with
+// 128: 67 us (2.6 TB/s, 0.32 PFLOP/s); 4 of 16320 with trees of 64: 89 us (0.48 PFLOP/s; 115 with
 // R = 1).
 //
 // p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
