@@ -243,6 +243,7 @@ __device__ __forceinline__ uint32_t k_slot(int r, int c) {
     return (r / RP) * 256 + ((r % RP) * C + (c ^ (r / RP % C))) * 16;
 }
 
+// F fragments of query rows per wave, W waves per block, of which R share their tiles.
 template <int D, int F, int R, int W>
 __global__ __launch_bounds__(64 * W, 2) void paged_attend_kernel(Attend p) {
     using Tile = AttendTile<D>;
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attend_kernel(Attend p) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int nw = W;
-    const int mine = wave & (R - 1), slice = wave / R;  // which rows of the block's, which of its waves on them
+    const int mine = wave & (R - 1), slice = wave / R;  // of the block's rows, and of its waves on them
     const int g = lane >> 4, m16 = lane & 15;
 
     // Block -> piece of a sequence, key head and rows of it.  Blocks go to the 8 XCDs in turn; each
@@ -549,8 +550,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attend_kernel(Attend p) {
     };
 
     if constexpr (R > 1) {
-        // 8 tiles at a time: every wave loads and converts one of them, and the R waves of a slice
-        // read the slice's R from LDS, V as the A operands of the MFMA.  The next 8 are on their
+        // W tiles at a time: every wave loads and converts one of them, and the R waves of a slice
+        // read the slice's R from LDS, V as the A operands of the MFMA.  The next W are on their
         // way meanwhile.
         char* s_v = reinterpret_cast<char*>(s_merge) + W * kTile * D;
         float* s_s = reinterpret_cast<float*>(s_v + W * kTile * D * 2);  // [tile][sK, sV][g][j]
@@ -839,14 +840,21 @@ constexpr AttendCost kAttendCosts[] = {
 // (piece, key head) pairs go to the 8 XCDs of 32 CUs in equal runs.  The join of pieces costs 6 us and
 // 0.25 for a MB of partial rows.
 // The costs are fitted to every kernel at one piece per sequence and up to eight cuts, timed at 3993
-// sizes (1 to 64 sequences of 16 to 45000, 1 to 256 tokens, 1 to 16 heads on each of 1 to 12): the plan is
-// 0.8% off the fastest in the mean and 20% at the 20 worst (2% at 958 other sizes, that timed again).  Measured, us, one fragment / two / four of
-// eight waves sharing / four / eight, the best cut of each: 16 sequences of 8192 x 32 rows x 8 heads
-// 59 / 53 / - / - / -; 4 of 4096 x 32 rows 18.5 / 21 / - / - / -; 4 of 16384, 256 rows - / 124 / 107 / 97 / 95; 2 of
-// 20100, 400 rows - / 118 / 115 / 106 / 102; 8 of 12048, 384 rows, 4 heads - / 126 / 111 / 94 / 107; 16 of 2064,
-// 256 rows - / 83 / 66 / 72 / 75; 32 of 732, 128 rows - / 50 / 34 / 40 / -; 19 of 692, 380 rows - / 95 / 59 / 46 /
-// 82; 8 of 732, 128 rows - / 16 / 28 / 30 / -; 4 of 3100, 800 rows, 2 heads - / 29 / 39 / 37 / 36.  (Two of eight
-// waves sharing, 53, -, 136, -, -, 80, 43, 81, 24 and 42 of these, lost to one or the other everywhere.)
+// sizes (1 to 64 sequences of 16 to 45000, 1 to 256 tokens, 1 to 16 heads on each of 1 to 12): the plan
+// is 0.8% off the fastest in the mean and 20% at the 20 worst (2% at 958 other sizes, with the plan
+// timed again).  Measured, us, one fragment / two / four of eight waves sharing / four / eight, the
+// best cut of each, 8 key heads but where stated:
+//   16 sequences of 8192, 32 rows          59 / 53
+//   4 of 4096, 32 rows                     18.5 / 21
+//   32 of 732, 128 rows                    - / 50 / 34 / 40
+//   8 of 732, 128 rows                     - / 16 / 28 / 30
+//   16 of 2064, 256 rows                   - / 83 / 66 / 72 / 75
+//   4 of 16384, 256 rows                   - / 124 / 107 / 97 / 95
+//   19 of 692, 380 rows                    - / 95 / 59 / 46 / 82
+//   8 of 12048, 384 rows, 4 key heads      - / 126 / 111 / 94 / 107
+//   2 of 20100, 400 rows                   - / 118 / 115 / 106 / 102
+//   4 of 3100, 800 rows, 2 key heads       - / 29 / 39 / 37 / 36
+// (two of eight waves sharing lost to one or the other everywhere: 43, 24, 80, 136 and 81 at rows 3 to 7).
 AttendPlan attend_plan(int B, int rows, int Hkv, int context, int D) {
     AttendPlan pl{};
     pl.min_tiles = kWaves;
