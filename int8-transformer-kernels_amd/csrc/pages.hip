@@ -344,7 +344,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_blocks_kernel(Select p)
     const int taken = min(n, p.top);
     if (t == 0 && row % p.Hkv == 0)
         p.positions[b] = taken == 0 ? 0 : (taken - 1) * page + len - (n - 1) * page;
-    for (int i = taken + t; i < p.top; i += blockDim.x) selected[i] = -1;
+    // (unsigned: top may be within a step of 2^31)
+    for (unsigned i = taken + t; i < (unsigned)p.top; i += blockDim.x) selected[i] = -1;
     if (n <= p.top) {
         for (int i = t; i < n; i += blockDim.x) selected[i] = i, pages[i] = table[i];
         return;
