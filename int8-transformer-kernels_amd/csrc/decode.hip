@@ -1312,13 +1312,7 @@ extern "C" int int8k_decode_attention_paged_num_splits(int B, int H, int max_con
 extern "C" int int8k_decode_paged_bad_page_ids(unsigned int* count) {
     clear_last_error();
     if (!count) return INT8K_ERR_INVALID_ARGUMENT;
-    const hipError_t e = hipMemcpyFromSymbol(count, HIP_SYMBOL(g_paged_bad_ids),
-                                             sizeof(unsigned int), 0, hipMemcpyDeviceToHost);
-    if (e != hipSuccess) {
-        set_last_error("hipMemcpyFromSymbol(g_paged_bad_ids)", e);
-        return INT8K_ERR_HIP;
-    }
-    return INT8K_OK;
+    return read_counter(&g_paged_bad_ids, "hipMemcpyFromSymbol(g_paged_bad_ids)", count);
 }
 
 static int paged_impl(

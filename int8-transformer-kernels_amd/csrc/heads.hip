@@ -511,11 +511,5 @@ int append_bad_slots(unsigned int* count) {
 extern "C" int int8k_rope_bad_positions(unsigned int* count) {
     clear_last_error();
     if (!count) return INT8K_ERR_INVALID_ARGUMENT;
-    const hipError_t e = hipMemcpyFromSymbol(count, HIP_SYMBOL(g_rope_bad_positions),
-                                             sizeof(unsigned int), 0, hipMemcpyDeviceToHost);
-    if (e != hipSuccess) {
-        set_last_error("hipMemcpyFromSymbol(g_rope_bad_positions)", e);
-        return INT8K_ERR_HIP;
-    }
-    return INT8K_OK;
+    return read_counter(&g_rope_bad_positions, "hipMemcpyFromSymbol(g_rope_bad_positions)", count);
 }

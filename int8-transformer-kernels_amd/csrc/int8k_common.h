@@ -41,6 +41,21 @@ inline bool aligned_to(const void* p, size_t a) {
 inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
+// A device counter of this library, read with the device synchronised (the copy alone waits for the
+// null stream and those that block on it, not for streams created without blocking).
+inline int read_counter(const void* symbol, const char* name, unsigned int* count) {
+    const hipError_t sync = hipDeviceSynchronize();
+    if (sync != hipSuccess) {
+        set_last_error("hipDeviceSynchronize", sync);
+        return INT8K_ERR_HIP;
+    }
+    const hipError_t e =
+        hipMemcpyFromSymbol(count, symbol, sizeof(unsigned int), 0, hipMemcpyDeviceToHost);
+    if (e == hipSuccess) return INT8K_OK;
+    set_last_error(name, e);
+    return INT8K_ERR_HIP;
+}
+
 // Workspace sub-allocations are carved at this granularity.
 constexpr size_t kWorkspaceAlign = 256;
 

@@ -788,11 +788,5 @@ extern "C" int int8k_decode_attention_forward_kv4_paged(
 extern "C" int int8k_kv4_bad_ids(unsigned int* count) {
     clear_last_error();
     if (!count) return INT8K_ERR_INVALID_ARGUMENT;
-    const hipError_t e = hipMemcpyFromSymbol(count, HIP_SYMBOL(g_kv4_bad_ids),
-                                             sizeof(unsigned int), 0, hipMemcpyDeviceToHost);
-    if (e != hipSuccess) {
-        set_last_error("hipMemcpyFromSymbol(g_kv4_bad_ids)", e);
-        return INT8K_ERR_HIP;
-    }
-    return INT8K_OK;
+    return read_counter(&g_kv4_bad_ids, "hipMemcpyFromSymbol(g_kv4_bad_ids)", count);
 }

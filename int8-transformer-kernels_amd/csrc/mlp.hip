@@ -1579,13 +1579,7 @@ extern "C" size_t int8k_mlp_call_workspace_bytes(int T, int d_model, int d_ff, i
 extern "C" int int8k_mlp_sync_timeouts(unsigned int* count) {
     clear_last_error();
     if (!count) return INT8K_ERR_INVALID_ARGUMENT;
-    const hipError_t e = hipMemcpyFromSymbol(count, HIP_SYMBOL(g_rq_timeouts), sizeof(unsigned int),
-                                             0, hipMemcpyDeviceToHost);
-    if (e != hipSuccess) {
-        set_last_error("hipMemcpyFromSymbol(g_rq_timeouts)", e);
-        return INT8K_ERR_HIP;
-    }
-    return INT8K_OK;
+    return read_counter(&g_rq_timeouts, "hipMemcpyFromSymbol(g_rq_timeouts)", count);
 }
 
 extern "C" int int8k_mlp_forward(const int8_t* x, const int8_t* W1, const int8_t* W2, int8_t* out,

@@ -27,15 +27,6 @@ inline int check_pages(int num_pages, int page_size, int kv_heads, int head_dim)
     return INT8K_OK;
 }
 
-// A device counter of this library, read with the device synchronised.
-inline int read_counter(const void* symbol, const char* name, unsigned int* count) {
-    const hipError_t e =
-        hipMemcpyFromSymbol(count, symbol, sizeof(unsigned int), 0, hipMemcpyDeviceToHost);
-    if (e == hipSuccess) return INT8K_OK;
-    set_last_error(name, e);
-    return INT8K_ERR_HIP;
-}
-
 // Bad slots and page ids met on the current device, per translation unit (int8k_paged_bad_ids).
 int append_bad_slots(unsigned int* count);   // heads.hip
 int attend_bad_ids(unsigned int* count);     // paged.hip
