@@ -600,6 +600,17 @@ size_t int8k_tree_attention_paged_workspace_bytes(int B, int heads, int kv_heads
 size_t int8k_tree_attention_paged_call_workspace_bytes(int B, int heads, int kv_heads, int nodes,
                                                        int max_context, int head_dim);
 
+/* How a call of these sizes is split, which its lengths have no part in:
+ *   plan[0]  query rows of a wave, 16 or 32
+ *   plan[1]  waves of a block that share the keys they read, 1, 4 or 8
+ *   plan[2]  waves of a block, 4 or 8
+ *   plan[3]  pieces that the batch is cut into, or 0: every sequence is read whole
+ * The sparse decode's attention is split as the tree's of one node a sequence, max_context the
+ * smaller of its own and top_pages * page_size.  INT8K_ERR_INVALID_ARGUMENT where the workspace
+ * queries return 0. */
+int int8k_tree_attention_paged_plan(int B, int heads, int kv_heads, int nodes, int max_context,
+                                    int head_dim, int* plan);
+
 int int8k_tree_attention_forward_paged(
     const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
     const float* scale_Q, const float* sK_pages, const float* sV_pages,

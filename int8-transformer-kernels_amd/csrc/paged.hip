@@ -1007,6 +1007,16 @@ extern "C" size_t int8k_tree_attention_paged_call_workspace_bytes(int B, int hea
     return plan_partials(pl, B, (size_t)heads * nodes, head_dim).bytes;
 }
 
+extern "C" int int8k_tree_attention_paged_plan(int B, int heads, int kv_heads, int nodes,
+                                               int max_context, int head_dim, int* plan) {
+    clear_last_error();
+    if (!plan || !tree_query_ok(B, heads, kv_heads, nodes, max_context, head_dim))
+        return INT8K_ERR_INVALID_ARGUMENT;
+    const AttendPlan pl = attend_plan(B, heads / kv_heads * nodes, kv_heads, max_context, head_dim);
+    plan[0] = 16 * pl.frags, plan[1] = pl.share, plan[2] = pl.waves, plan[3] = pl.pieces;
+    return INT8K_OK;
+}
+
 extern "C" int int8k_tree_attention_forward_paged(
     const int8_t* Q, const int8_t* K_pages, const int8_t* V_pages, uint16_t* out,
     const float* scale_Q, const float* sK_pages, const float* sV_pages,

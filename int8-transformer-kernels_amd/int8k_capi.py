@@ -83,6 +83,7 @@ _SIGNATURES = {
                                   [_I] * 8 + [_P]),
     "int8k_tree_attention_paged_workspace_bytes": (_SZ, [_I] * 6),
     "int8k_tree_attention_paged_call_workspace_bytes": (_SZ, [_I] * 6),
+    "int8k_tree_attention_paged_plan": (_I, [_I] * 6 + [ctypes.POINTER(ctypes.c_int)]),
     "int8k_tree_attention_forward_paged": (_I, [_P] * 10 + [_I, _LL, _P] + [_I] * 10 +
                                            [_P, _SZ, _P]),
     "int8k_kv_cache_move_paged": (_I, [_P] * 6 + [_I] * 6 + [_P]),
@@ -723,6 +724,14 @@ def tree_attention_paged_call_workspace_bytes(B, heads, kv_heads, nodes, max_con
     """What a call of exactly these sizes needs."""
     return load().int8k_tree_attention_paged_call_workspace_bytes(B, heads, kv_heads, nodes,
                                                                   max_context, D)
+
+
+def tree_attention_paged_plan(B, heads, kv_heads, nodes, max_context, D):
+    """(query rows of a wave, waves that share their keys, waves of a block, pieces or 0)."""
+    plan = (ctypes.c_int * 4)()
+    check("int8k_tree_attention_paged_plan", load().int8k_tree_attention_paged_plan(
+        B, heads, kv_heads, nodes, max_context, D, plan))
+    return tuple(plan)
 
 
 def tree_attention_paged(Qi, K_pages, V_pages, sQ, sK_pages, sV_pages, block_tables, context_lens,
