@@ -584,6 +584,8 @@ int int8k_qk_norm_rope_append(const void* x, int dtype, const float* cos, const 
  *   out fp16 [B, heads, nodes, D], or [B, nodes, heads, D] with INT8K_ATTN_OUT_BSHD
  * Node i attends to all positions before the tree and to the nodes it sees:
  *   out = sum_j softmax_j(q . k_j sQ sK_j / sqrt(D)) v_j sV_j, q . k exact int32.
+ * A weight p sV is off by up to 2^-22 of itself and 2^-34 of its row's largest.  Value scales are
+ * taken up to 2^64 in magnitude; a row that sees an infinite or NaN one has no finite component.
  * Rows that see nothing, and rows of nodes past a sequence's, are zeros.  Negative lengths and
  * counts are 0; positions from max_context on are not attended to (context_lens are cut to it,
  * then the nodes).  A page id outside [0, num_pages) reads page num_pages-1 and is counted
@@ -660,7 +662,8 @@ int int8k_kv_page_means(const int8_t* K_pages, const float* sK_pages, const int3
  * (16-byte aligned) holds scores, the selection and partial states: one of
  * int8k_decode_attention_paged_sparse_workspace_bytes serves every call of up to B sequences,
  * max_context positions and top_pages blocks with the same heads and page size;
- * _call_workspace_bytes is what a call of exactly these sizes needs.  Splits as for the tree. */
+ * _call_workspace_bytes is what a call of exactly these sizes needs.  Weights, value scales and
+ * splits as for the tree. */
 size_t int8k_decode_attention_paged_sparse_workspace_bytes(int B, int heads, int kv_heads,
                                                            int max_context, int page_size,
                                                            int top_pages, int head_dim);

@@ -86,3 +86,21 @@ def test_no_component_is_finite_however_small_the_weight(ext, gpu, gap):
         if at != 300:
             c["sV"][p, :, off] = float("inf")
     assert not torch.isfinite(_run(ext, c)).any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,N,H,Hkv,L,at", [(3, 5, 8, 2, 333, 40), (2, 16, 4, 1, 9000, 4444), (33, 43, 12, 4, 257, 256),
+                                            (5, 50, 32, 4, 1450, 1000)])
+def test_value_scales_of_2_to_64(ext, gpu, B, N, H, Hkv, L, at, D):
+    # the largest that are taken: past fp16's range where the code is not zero, finite where it is
+    lens = [L] + [max(1, L - 40 * b) for b in range(1, B)]
+    c = tree_case(N + L, lens, N, H, Hkv, D, 32, gpu)
+    p, off = int(c["tables"][0, at // 32]), at % 32
+    c["V"][p, :, off, ::5] = 0
+    c["sV"][p, :, off] = 2.0 ** 64
+    out = _run(ext, c)
+    for h in range(Hkv):
+        v = c["V"][p, h, off]
+        rows = out[0, h * (H // Hkv):(h + 1) * (H // Hkv)]
+        assert torch.isfinite(rows[..., v == 0]).all()
+        assert (rows[..., v != 0].double() == torch.sign(v[v != 0].double()) * float("inf")).all()
