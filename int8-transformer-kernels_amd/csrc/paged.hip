@@ -22,12 +22,15 @@
 // such slices of a block, joined, or one, whose waves write what they hold.
 // Pieces are joined by a second kernel.
 //
-// Bound by memory with one fragment (8 sequences of 16384, one token of 4 heads on 8: 5.2 TB/s) and
-// by the issue of instructions with two: 32 rows x 32 keys take 300 vector instructions (190 with
-// R = 8: V's conversion is shared) beside 44 MFMAs, each of which keeps the SIMD from vector ones
-// for about 10 of its 16 cycles.  16 sequences of up to 8192 with trees of 16, 32 heads on 8 of
-// 128: 67 us (2.6 TB/s, 0.32 PFLOP/s); 4 of 16320 with trees of 64: 89 us (0.48 PFLOP/s; 115 with
-// R = 1).
+// With one fragment it reads 5.2 TB/s (8 sequences of 16384, one token of 4 heads on 8), as fast as a
+// copy moves data here and three quarters of what a kernel that only reads reaches.  With two, a CU
+// that has work is bound by the issue of instructions: 32 rows x 32 keys take 300 vector instructions
+// (190 with R = 8: V's conversion is shared) beside 44 MFMAs, each of which keeps the SIMD from
+// vector ones for about 10 of its 16 cycles.  Unequal lengths come on top: 16 sequences of up to
+// 8192 with trees of 16, 32 heads on 8 of 128, take 65 to 67 us (2.7 TB/s, 0.32 PFLOP/s), one whole
+// sequence of a key head and 32 rows per block, and a CU is busy for 66% of that; 16 that are all of
+// 8192 take 71.  4 of up to 16320 with trees of 64: 89 to 99 us on different cards (0.43 to 0.48
+// PFLOP/s; 115 with R = 1), 9 of them the join.
 //
 // p_j = 2^(s_j - m) with a reference m per query that is not the running maximum: it is set so
 // that the largest weight p sV of the tile that set it lies in [2^9, 2^10), and a tile whose
@@ -126,10 +129,12 @@ __device__ __forceinline__ bool attends(const Attend& p, int b, int node, const 
     return any != 0;
 }
 
-// How the sequences are cut.  Their lengths are on the device, so every wave works the cut out from
-// them: into p.pieces pieces over all sequences, at least one each, whose largest is about as small
-// as can be, but p.min_tiles.  The host takes as many pieces as the GPU holds at a time, so all
-// blocks run at once and end together however unequal the lengths are.
+// How the sequences are cut, where the plan cuts them.  Their lengths are on the device, so every wave
+// works the cut out from them: into p.pieces pieces over all sequences, at least one each, whose
+// largest is about as small as can be, but p.min_tiles.  The host takes as many pieces as the GPU
+// holds at a time, so all blocks run at once and end about together.  A plan that does not cut (it
+// knows max_context only) takes as long as its longest sequence: one of 8192 beside 15 of 256, with
+// trees of 16, 58 us where 16 of up to 8192 take 65.
 struct Piece {
     int b, index, count, first;  // sequence, which of its pieces, how many, number of its first
     int tiles;                   // of a piece
@@ -261,7 +266,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attend_kernel(Attend p) {
 
     // Block -> piece of a sequence, key head and rows of it.  Blocks go to the 8 XCDs in turn; each
     // XCD takes a run of the (piece, key head) pairs, and the blocks of one pair, which read the same
-    // rows, one after the other.
+    // rows, one after the other.  (Whole sequences that lie in the batch by length load the XCDs
+    // unequally: 64 of up to 4096 with trees of 16, 117 us shuffled, 137 with the longest first.)
     const int units = p.slots * p.Hkv, each_xcd = (units + 7) / 8;
     const int local = (int)blockIdx.x / 8 / p.groups;
     const int unit = (int)blockIdx.x % 8 * each_xcd + local;
@@ -835,15 +841,18 @@ constexpr AttendCost kAttendCosts[] = {
 
 // rows: query rows per key head.
 // The plan is the kernel and the number of pieces of least estimated time, for sequences of unequal
-// lengths: one of max_context, 3/4 of that in the mean.  A CU runs one block of 8 waves at a time, two
+// lengths: one of max_context, 3/4 of that in the mean.  So a max_context far above the lengths, as a
+// captured graph's may be, costs what the plan for such lengths costs: 16 sequences of up to 8192 with
+// trees of 16, 66 us at 8208, 63 at 16384, 74 at 32768, 75 at 131072 (64 pieces).  A CU runs one block of 8 waves at a time, two
 // of 4 waves or where a wave takes at most 128 registers (one fragment at head dim 64), and the
 // (piece, key head) pairs go to the 8 XCDs of 32 CUs in equal runs.  The join of pieces costs 6 us and
 // 0.25 for a MB of partial rows.
 // The costs are fitted to every kernel at one piece per sequence and up to eight cuts, timed at 3993
-// sizes (1 to 64 sequences of 16 to 45000, 1 to 256 tokens, 1 to 16 heads on each of 1 to 12): the plan
-// is 0.8% off the fastest in the mean and 20% at the 20 worst (2% at 958 other sizes, with the plan
-// timed again).  Measured, us, one fragment / two / four of eight waves sharing / four / eight, the
-// best cut of each, 8 key heads but where stated:
+// sizes (1 to 64 sequences of 16 to 45000, 1 to 256 tokens, 1 to 16 heads on each of 1 to 12, lengths
+// drawn evenly from a quarter of max_context up), by the smallest mean loss against the fastest: the
+// plan is 0.8% off it in the mean, 20% at the 20 worst and 43% at the worst size of a run (2% at 958
+// other sizes, with the plan timed again).  Measured, us, one fragment / two / four of eight waves
+// sharing / four / eight, the best cut of each, 8 key heads but where stated:
 //   16 sequences of 8192, 32 rows          59 / 53
 //   4 of 4096, 32 rows                     18.5 / 21
 //   32 of 732, 128 rows                    - / 50 / 34 / 40
@@ -920,7 +929,7 @@ Partials most_partials(size_t rows, int D) {
 }
 
 template <int D, int F, int R, int W>
-int launch_instance(const Attend& p, const AttendPlan& pl, unsigned blocks, hipStream_t stream) {
+int launch_instance(const Attend& p, unsigned blocks, hipStream_t stream) {
     constexpr int kTiles = R > 1 ? 3 * kTile * D + 256 : kTile * D;  // bytes of LDS per wave
     constexpr int kWave = R == W ? kTiles : std::max(kTiles, (2 * 16 * F + 16 * F * (D + 4)) * 4);
     static PerDeviceOnce once;
@@ -944,11 +953,11 @@ int launch_attend(Attend p, const AttendPlan& pl, void* workspace, hipStream_t s
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           plan_partials(pl, p.B, (size_t)p.Hq * p.N, D).ml_bytes);
     const unsigned blocks = (unsigned)(ceil_div((long long)p.slots * p.Hkv, 8) * 8 * pl.groups);
-    const int st = pl.frags == 1 ? launch_instance<D, 1, 1, kWaves>(p, pl, blocks, stream)
-                   : pl.share == 1 ? launch_instance<D, 2, 1, kWaves>(p, pl, blocks, stream)
-                   : pl.share == 8 ? launch_instance<D, 2, 8, kWaves>(p, pl, blocks, stream)
-                   : pl.waves == 4 ? launch_instance<D, 2, 4, 4>(p, pl, blocks, stream)
-                                   : launch_instance<D, 2, 4, kWaves>(p, pl, blocks, stream);
+    const int st = pl.frags == 1 ? launch_instance<D, 1, 1, kWaves>(p, blocks, stream)
+                   : pl.share == 1 ? launch_instance<D, 2, 1, kWaves>(p, blocks, stream)
+                   : pl.share == 8 ? launch_instance<D, 2, 8, kWaves>(p, blocks, stream)
+                   : pl.waves == 4 ? launch_instance<D, 2, 4, 4>(p, blocks, stream)
+                                   : launch_instance<D, 2, 4, kWaves>(p, blocks, stream);
     if (st != INT8K_OK || pl.pieces == 0) return st;
     const int blocks_each = (int)ceil_div((long long)p.Hq * p.N, kCombineRows<D>);
     paged_combine_kernel<D><<<(unsigned)(p.B * blocks_each), 256, 0, stream>>>(p, blocks_each);

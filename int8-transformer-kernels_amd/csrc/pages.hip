@@ -219,7 +219,7 @@ __device__ __forceinline__ uint64_t score_key(double s) {
 
 // A group of D / 16 lanes, which hold 16 dims each, scores kEach blocks.  (In the selection's block,
 // which spares a launch: 40.2 against 41.4 us for 32 sequences of 512 blocks, 27.5 against 23.9 for one
-// of 1024, 42 against 22 for one of 4096.)
+// of 1024, 42 against 22 for one of 4096; fewer blocks were not timed so.)
 template <int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(Select p) {
     constexpr int L = D / 16, kRows = 256 / L, kEach = 2;
